@@ -39,6 +39,34 @@ class ca_chunk_job(C.Structure):
 
 
 CA_MAX_CHUNK_JOBS = 32
+CA_F16 = 3
+CA_MAX_AXES = 4
+
+
+class ca_seq_view(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("head", C.c_int64), ("token", C.c_int64), ("batch", C.c_int64)]
+
+
+class ca_page_view(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token", C.c_int64), ("head", C.c_int64), ("page", C.c_int64)]
+
+
+class ca_pages(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("starts", C.c_void_p), ("lengths", C.c_void_p), ("width", C.c_int32),
+                ("page", C.c_int32), ("pages", C.c_int32), ("sequences", C.c_int32)]
+
+
+class ca_rotary_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("dim", C.c_int32), ("pairs", C.c_int32), ("interleaved", C.c_int32),
+                ("inverse", C.c_int32), ("axes", C.c_int32), ("sections", C.c_int32 * CA_MAX_AXES),
+                ("tokens", C.c_int32), ("batch", C.c_int32), ("positions", C.c_void_p), ("axis_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("batch_stride", C.c_int64), ("turns", C.c_void_p)]
+
+
+class ca_seq_desc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("dim", C.c_int32), ("heads_q", C.c_int32), ("heads_kv", C.c_int32),
+                ("tokens", C.c_int32), ("batch", C.c_int32), ("left", C.c_int32), ("right", C.c_int32),
+                ("sinks", C.c_int32), ("scale", C.c_float)]
 
 
 def _load():
@@ -53,6 +81,8 @@ lib = _load()
 
 _p = C.c_void_p
 _D = C.POINTER(ca_desc)
+_V, _G = C.POINTER(ca_seq_view), C.POINTER(ca_page_view)
+_R, _S, _P = C.POINTER(ca_rotary_desc), C.POINTER(ca_seq_desc), C.POINTER(ca_pages)
 _i32, _i64, _f32 = C.c_int32, C.c_int64, C.c_float
 
 PROTOTYPES = {
@@ -89,6 +119,12 @@ PROTOTYPES = {
     "ca_sum_batch": (C.c_int, [_i64, _i32, _i32, _i32, _i32, _p, _p, _p]),
     "ca_sum_rows": (C.c_int, [_D, _p, _p, _p]),
     "ca_sum_cols": (C.c_int, [_D, _p, _p, _p]),
+    "ca_rotary": (C.c_int, [_R, _V, _V, _i32, _V, _V, _i32, _p]),
+    "ca_rotary_append": (C.c_int, [_R, _V, _V, _i32, _V, _V, _i32, _G, _G, _P, _p]),
+    "ca_window_fwd": (C.c_int, [_S, _V, _V, _V, _p, _V, _V, _p, _p]),
+    "ca_window_bwd_workspace": (C.c_size_t, [_S]),
+    "ca_window_bwd": (C.c_int, [_S] + [_V] * 6 + [_p, _p] + [_V] * 3 + [_p, _p]),
+    "ca_paged_window": (C.c_int, [_S, _V, _G, _G, _P, _V, _p]),
     "ca_probe_launch_count": (C.c_int64, []),
     "ca_probe_tiled_launch_count": (C.c_int64, []),
     "ca_probe_tensor_launch_count": (C.c_int64, []),

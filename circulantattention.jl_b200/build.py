@@ -8,14 +8,16 @@ import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
+INCLUDE = os.path.join(PKG_DIR, "..", "include")
 OUT = os.path.join(PKG_DIR, "libcircatt_b200.so")
 SOURCES = ["fwd_exact.cu", "fwd_any.cu", "fwd_values_exact.cu", "fwd_values_any.cu", "bwd_exact.cu", "bwd_any.cu", "emit_exact.cu", "emit_any.cu",
-           "apply_exact.cu", "apply_any.cu", "operators.cu", "tiled.cu", "pack.cu", "split_pack.cu", "split_fwd.cu", "split_bwd.cu", "line.cu", "api.cu", "static_scratch.cu", "comm.cu"]
+           "apply_exact.cu", "apply_any.cu", "operators.cu", "tiled.cu", "pack.cu", "split_pack.cu", "split_fwd.cu", "split_bwd.cu", "line.cu", "api.cu", "static_scratch.cu", "comm.cu",
+           "rotary.cu", "seq_api.cu", "seq_fma.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--use_fast_math", "-Xcompiler", "-fPIC"]
 
 
-HOST_SRC = os.path.join(CSRC, "host.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_tokens.cpp")]
 HOST_OUT = os.path.join(PKG_DIR, "_circatt_host.so")
 
 
@@ -28,7 +30,7 @@ def _stale():
         return True
     t = os.path.getmtime(OUT)
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h"))]
-    deps.append(os.path.join(PKG_DIR, "..", "include", "circatt_b200.h"))
+    deps += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
     return any(os.path.getmtime(d) > t for d in deps)
 
 
@@ -37,9 +39,8 @@ def _obj_stale(src_path: str, obj: str) -> bool:
     if not os.path.exists(obj):
         return True
     t = os.path.getmtime(obj)
-    inc = os.path.join(PKG_DIR, "..", "include")
     deps = [src_path] + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    deps += [os.path.join(inc, f) for f in os.listdir(inc) if f.endswith(".h")]
+    deps += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
     return any(os.path.getmtime(d) > t for d in deps)
 
 
@@ -51,7 +52,7 @@ def _host_command():
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], cuda]
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"] + ["-I" + d for d in include] +
-            [HOST_SRC, "-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
+            HOST_SRCS + ["-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
              "-ltorch_python"])
 
 
@@ -59,7 +60,7 @@ def _host_stale():
     if not os.path.exists(HOST_OUT):
         return True
     t = os.path.getmtime(HOST_OUT)
-    return any(os.path.getmtime(d) > t for d in (HOST_SRC, os.path.join(PKG_DIR, "..", "include", "circatt_b200.h")))
+    return any(os.path.getmtime(d) > t for d in (*HOST_SRCS, os.path.join(CSRC, "host_common.h"), *(os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE))))
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -68,7 +69,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return _build_library(force, verbose)
     finally:
         if host is not None and host.wait() != 0:
-            raise RuntimeError("g++ failed on host.cpp")
+            raise RuntimeError("g++ failed on the host extension")
 
 
 def _build_library(force, verbose):
