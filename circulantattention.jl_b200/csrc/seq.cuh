@@ -30,6 +30,7 @@ struct SeqArgs {
     int N, B;                       // dense: tokens and batch; paged: packed tokens and 1
     int left, right, sinks;         // left: kNoLeft without a left end
     float scale, scale_log2;        // scale_log2 = scale * log2(e)
+    float mag_log2;                 // its magnitude, never 0 (0 * -inf of a masked score would be NaN): the sign goes to q
     const int* lengths;             // dense: nullable; paged: tokens in the cache
     ca_seq_view q, k, v, y, rest, dy, dq, dk, dv;   // rest.data nullable: what rounding took from y
     ca_page_view kp, vp;

@@ -1,5 +1,5 @@
 // C ABI of the attention on token sequences: argument checks and dispatch.
-#include "seq.cuh"
+#include "seq_umma.cuh"
 
 namespace ca {
 
@@ -63,7 +63,9 @@ static int fill(const ca_seq_desc* d, SeqArgs* a) {
     a->right = d->right > kNoLeft ? kNoLeft : d->right;
     a->sinks = d->sinks;
     a->scale = d->scale;
+    if (!isfinite(d->scale)) { set_error("scale is not finite"); return CA_ERR_BAD_DESC; }
     a->scale_log2 = d->scale * kLog2e;
+    a->mag_log2 = fmaxf(fabsf(a->scale_log2), 1e-30f);
     a->status = status_word();
     return CA_OK;
 }
@@ -87,7 +89,7 @@ int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     if (y_rest) a.rest = *y_rest;
     a.lengths = lengths;
     a.lse = lse;
-    return fma_window_fwd(a, d->dtype, as_stream(stream));
+    return d->dtype == CA_F32 ? fma_window_fwd(a, d->dtype, as_stream(stream)) : umma_window_fwd(a, d->dtype, as_stream(stream));
 }
 
 size_t ca_window_bwd_workspace(const ca_seq_desc* d) {
@@ -130,7 +132,7 @@ int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_vi
     a.q = *q; a.y = *y;
     a.kp = *k_pages; a.vp = *v_pages;
     a.pages = *pages;
-    return fma_paged(a, d->dtype, as_stream(stream));
+    return d->dtype == CA_F32 ? fma_paged(a, d->dtype, as_stream(stream)) : umma_paged(a, d->dtype, as_stream(stream));
 }
 
 }  // extern "C"

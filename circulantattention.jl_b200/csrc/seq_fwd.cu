@@ -1,0 +1,463 @@
+// Attention on token sequences, forward, on the tensor cores (tcgen05): dense tensors and a paged cache, 16-bit types.
+//
+// A CTA takes tiles of 128 query rows of one key head and walks the tiles of 128 keys that they see, with a running maximum
+// and sum per row.  Scores of a tile come into tensor memory (128 lanes = rows, 128 columns = keys); the thread that owns the
+// row reads them, turns them into weights, and writes those back over the scores as 16-bit pairs, from where the second
+// product takes them as its A operand: the weights never see shared memory.
+//
+// Roles: two groups of four warps do the softmax, one warp copies keys and values by TMA into a ring of tiles, one thread
+// issues the products.  The two groups are two streams that share the tensor cores: while one turns its scores into weights,
+// the products of the other run.  With PAIR the streams are two row tiles that share every key tile; without, they take
+// the even and the odd key tiles of one row tile and are joined at the end (few rows: decoding).
+//
+// The accumulator is rescaled only where a row's maximum grew by more than 2^8 since its reference: the weights stay below
+// 2^8, and the products and sums are held in Float32.
+#include "seq_umma.cuh"
+
+namespace ca {
+namespace {
+
+// Two warpgroups of softmax, one whose first warp copies and whose second issues the products.  384 threads are launched with
+// 168 registers each: 64512, of which 2 x 128 x 216 + 128 x 64 = 63488 are used.
+constexpr int kThreads = 384, kSoftmaxWarps = 8;
+
+template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
+template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
+template <int DM> constexpr size_t kFwdSmem = (size_t)(2 + kSlots<DM>) * kTileBytes<DM> + 1024;
+
+struct FwdMaps {
+    CUtensorMap k, v;
+    int box;            // paged: keys of a box
+    int* timeouts;
+};
+
+template <typename T, int DM, bool PAIR, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ FwdMaps maps) {
+    constexpr int S = kSlots<DM>;
+    constexpr uint32_t TILE = kTileBytes<DM>;
+    constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
+    extern __shared__ char raw[];
+    __shared__ uint64_t kv_full[S], kv_empty[S], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    __shared__ uint32_t tmem_slot, valid[S];
+    __shared__ int stop_flag;
+    __shared__ float merge_m[128], merge_l[128];
+    volatile int* stop = &stop_flag;
+
+    const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
+    char* const smem = raw + (base_at - raw_at);
+    const uint32_t q_at = base_at, kv_at = base_at + 2 * TILE;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+    int tile = (int)(gridDim.x - 1 - blockIdx.x);       // the last rows see the most keys: first
+    Seq s;
+    if (PAGED) {
+        if (!paged_seq(a, PAIR ? 256 : 128, tile, &s)) return;
+    } else {
+        s = dense_seq(a, blockIdx.z);
+    }
+    const int rows = s.T * a.G, R0 = tile * (PAIR ? 256 : 128);
+    const int p_lo = max(0, s.base + R0 / a.G), p_hi = min(s.n - 1, s.base + (min(R0 + (PAIR ? 256 : 128), rows) - 1) / a.G);
+    const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, 128);
+
+    // Which key tiles a stream needs: both streams see nearly the same, but each leaves out what all of its rows are blind to.
+    int u_lo[2], u_hi[2];                               // positions of its rows that exist; lo > hi: none
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int r = R0 + (PAIR ? 128 * u : 0);
+        u_lo[u] = max(0, s.base + r / a.G);
+        u_hi[u] = r < rows ? min(s.n - 1, s.base + (min(r + 128, rows) - 1) / a.G) : -1;
+    }
+    auto need = [&](int u, int i) {
+        if (!PAIR) return (i & 1) == u;
+        if (u_hi[u] < u_lo[u]) return false;
+        const int key0 = kt.key(i, 128);
+        return key0 <= u_hi[u] + a.right && (key0 + 127 >= u_lo[u] - a.left || key0 < a.sinks);
+    };
+    auto next = [&](int u, int i) {
+        do ++i; while (i < kt.count && !need(u, i));
+        return i;
+    };
+
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
+        for (int u = 0; u < 2; ++u) {
+            mbar_init(&q_full[u], PAIR ? 4 : 8);
+            mbar_init(&s_full[u], 1);
+            mbar_init(&p_full[u], 4);
+            mbar_init(&o_full[u], 1);
+        }
+        mbar_init(&drained, 1);
+        stop_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    const uint32_t s_col = tmem, o_col = tmem + 256;
+
+    if (warp < kSoftmaxWarps) {
+        // ------------------------------------------------------------ softmax: thread = row
+        more_registers<216>();
+        const int u = warp >> 2, r = tid & 127, R = R0 + (PAIR ? 128 * u : 0) + r;
+        const int pos = s.base + R / a.G;
+        const bool have = R < rows, live = have && pos >= 0 && pos < s.n;
+        {
+            const T* src = live ? seq_row<T>(a.q, a, s, h, R) : nullptr;
+            stage_row<T, DM>(smem + (PAIR ? u : 0) * TILE, r, src, a.D, PAIR ? 0 : u, PAIR ? 1 : 2, a.scale < 0.f);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&q_full[PAIR ? u : 0]));
+        }
+        const uint32_t lane_off = (uint32_t)(warp & 3) << 21;              // lane 32 * (warp % 4) in bits 16..
+        const uint32_t S_at = s_col + u * 128 + lane_off, O_at = o_col + u * DM + lane_off;
+        const float sl2 = a.mag_log2;
+        const int c_lo = p_lo - a.left, c_hi = min(p_hi + a.right, s.n - 1);   // keys that any row of the CTA sees (or < sinks)
+        float m = -INFINITY, l = 0.f;
+        int done = 0;
+        bool ok = true;
+        for (int i = next(u, -1); i < kt.count; i = next(u, i)) {
+            const int key0 = kt.key(i, 128), vslot = (2 * i + 1) % S;
+            const uint32_t vpar = ((2 * i + 1) / S) & 1;
+            if (!warp_wait(smem_u32(&s_full[u]), done & 1, stop)) { ok = false; break; }
+            fence_after();
+            uint32_t x[128];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) tmem_ld32(S_at + 32 * g, x + 32 * g);
+            uint32_t there = 0xff;
+            if (PAGED) {                                                   // which pages exist is known when their copy has landed
+                if (!warp_wait(smem_u32(&kv_full[vslot]), vpar, stop)) { ok = false; break; }
+                there = *(volatile uint32_t*)&valid[vslot];
+            }
+            tmem_wait_ld();
+#pragma unroll
+            for (int g = 0; g < 4; ++g) settled32(x + 32 * g);
+            const int far = key0 + 127;
+            if (!(far <= u_lo[u] + a.right && far < s.n && u_lo[u] == s.base + (R - r) / a.G && u_hi[u] == s.base + (min(R - r + 128, rows) - 1) / a.G &&
+                  (key0 >= u_hi[u] - a.left || far < a.sinks) && there == 0xff)) {
+                const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t mk = seen_bits(lo - 32 * g, hi - 32 * g, sk - 32 * g);
+                    if (PAGED) mk &= ((there >> (2 * g)) & 1 ? 0xffffu : 0u) | ((there >> (2 * g + 1)) & 1 ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) x[32 * g + c] = (mk >> c) & 1 ? x[32 * g + c] : 0xff800000u;
+                }
+            }
+            // values that no row sees may be anything (a page that was freed, tokens behind the length): zeros
+            const bool all_used = (key0 >= c_lo || far < a.sinks) && far <= c_hi && there == 0xff;
+            if (!all_used) {
+                if (!PAGED && !warp_wait(smem_u32(&kv_full[vslot]), vpar, stop)) { ok = false; break; }
+                const int j = key0 + r;
+                if (!(j <= c_hi && (j >= c_lo || j < a.sinks) && (there >> (r >> 4) & 1))) {
+#pragma unroll
+                    for (int p = 0; p < DM / 64; ++p)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            *reinterpret_cast<uint4*>(smem + (2 + vslot) * TILE + p * kPanel + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 128; c += 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(x[c + e]));
+            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl2;
+            float f = 1.f;
+            const bool grew = mx > m + 8.f;                                // also from -inf
+            if (grew) {
+                f = fast_exp2(m - mx);
+                m = mx;
+            }
+            if (done && __any_sync(~0u, grew)) {
+                // the scores came after the previous weighted sum, which is therefore complete
+#pragma unroll
+                for (int c = 0; c < DM; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(O_at + c, o);
+                    tmem_wait_ld();
+                    settled32(o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_st32(O_at + c, o);
+                }
+            }
+            l *= f;
+            const float ref = m == -INFINITY ? 0.f : m;                    // a row that has seen nothing yet
+            const f32x2 sc2 = pack2(sl2, sl2), ref2 = pack2(-ref, -ref);
+            f32x2 sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                uint32_t w[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    float e0, e1;
+                    unpack2(fma2(pack2(__uint_as_float(x[64 * g + 2 * c]), __uint_as_float(x[64 * g + 2 * c + 1])), sc2, ref2), e0, e1);
+                    e0 = fast_exp2(e0);
+                    e1 = fast_exp2(e1);
+                    sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
+                    w[c] = pack16<T>(e0, e1);
+                }
+                tmem_st32(S_at + 32 * g, w);
+            }
+            float a0, a1;
+            unpack2(add2(sum2[0], sum2[1]), a0, a1);
+            l += a0 + a1;
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&p_full[u]));
+            ++done;
+        }
+        if (done && ok) ok = warp_wait(smem_u32(&o_full[u]), 0, stop);
+        fence_after();
+
+        // ------------------------------------------------------------ results
+        float inv, f0 = 1.f, f1 = 0.f;
+        float* const other = reinterpret_cast<float*>(smem + 2 * TILE);    // [column][row] of the odd stream, in the ring's place
+        if (!PAIR) {
+            asm volatile("bar.sync 1, 256;" ::: "memory");                 // both streams are through with the ring
+            if (u == 1) {
+                merge_m[r] = m;
+                merge_l[r] = l;
+                if (done && ok) {
+#pragma unroll
+                    for (int c = 0; c < DM; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(O_at + c, o);
+                        tmem_wait_ld();
+                        settled32(o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) other[(c + e) * 128 + r] = __uint_as_float(o[e]);
+                    }
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float m1 = merge_m[r], l1 = merge_l[r], M = fmaxf(m, m1), ref = M == -INFINITY ? 0.f : M;
+            f0 = fast_exp2(m - ref);
+            f1 = fast_exp2(m1 - ref);
+            l = l * f0 + l1 * f1;
+            m = M;
+        }
+        if (PAIR || u == 0) {
+            inv = l > 0.f ? 1.f / l : 0.f;
+            if (!ok || *stop) inv = __int_as_float(0x7fffffff);            // a wait ran out: NaN, never a wrong number
+            const bool both = !PAIR && kt.count > 1;
+            T* dst = seq_row<T>(a.y, a, s, h, have ? R : R0);
+            T* rest = !PAGED && a.rest.data ? seq_row<T>(a.rest, a, s, h, have ? R : R0) : nullptr;
+            if (!PAGED && a.lse && have) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = l > 0.f ? m + log2f(l) : -INFINITY;
+            const float w0 = f0 * inv, w1 = f1 * inv;
+#pragma unroll
+            for (int c = 0; c < DM; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(O_at + c, o);
+                tmem_wait_ld();
+                settled32(o);
+                float y[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    y[e] = done ? __uint_as_float(o[e]) * w0 : 0.f * inv;
+                    if (both) y[e] = fmaf(other[(c + e) * 128 + r], w1, y[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (c + e >= a.D || !have) continue;
+                    uint4 w = make_uint4(pack16<T>(y[e], y[e + 1]), pack16<T>(y[e + 2], y[e + 3]), pack16<T>(y[e + 4], y[e + 5]), pack16<T>(y[e + 6], y[e + 7]));
+                    *reinterpret_cast<uint4*>(dst + c + e) = w;
+                    if (rest) {
+                        const uint32_t* ww = &w.x;
+                        uint4 q;
+                        uint32_t* qq = &q.x;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) qq[k] = pack16<T>(y[e + 2 * k] - low16<T>(ww[k]), y[e + 2 * k + 1] - high16<T>(ww[k]));
+                        *reinterpret_cast<uint4*>(rest + c + e) = q;
+                    }
+                }
+            }
+        }
+    } else {
+        fewer_registers<64>();
+    }
+    if (warp == 8) {
+        // ------------------------------------------------------------ copies
+        bool ok = true;
+        int issued = 0;
+        if (!PAGED) {
+            if (lane == 0) {
+                for (; issued < 2 * kt.count; ++issued) {
+                    const int slot = issued % S;
+                    if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
+                    const uint32_t bar = smem_u32(&kv_full[slot]), dst = kv_at + slot * TILE;
+                    mbar_arrive_expect_tx(bar, TILE);
+#pragma unroll
+                    for (int p = 0; p < DM / 64; ++p)
+                        tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.v : &maps.k, 64 * p, kt.key(issued >> 1, 128), h, s.b, bar);
+                }
+            }
+        } else {
+            const int box = maps.box, chunks = 128 / box;
+            for (int i = 0; i < kt.count && ok; ++i) {
+                const int j = kt.key(i, 128) + lane * box;
+                const int page = lane < chunks && j < s.n ? page_of(a, s.b, j) : -1;
+                const unsigned has = __ballot_sync(~0u, page >= 0);
+                uint32_t bits = 0;                                         // per 16 keys
+                for (int c = 0; c < 8; ++c) bits |= (has >> (c * 16 / box) & 1) << c;
+                for (int kv = 0; kv < 2; ++kv, ++issued) {
+                    const int slot = issued % S;
+                    int go = 1;
+                    if (lane == 0) go = wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop);
+                    if (!__shfl_sync(~0u, go, 0)) { ok = false; break; }
+                    const uint32_t bar = smem_u32(&kv_full[slot]), dst = kv_at + slot * TILE;
+                    if (lane == 0) {
+                        *(volatile uint32_t*)&valid[slot] = bits;
+                        mbar_arrive_expect_tx(bar, (uint32_t)__popc(has) * box * DM * 2);
+                    }
+                    __syncwarp();
+                    if (page >= 0) {
+#pragma unroll
+                        for (int p = 0; p < DM / 64; ++p)
+                            tma_load_4d(dst + p * kPanel + lane * box * 128, kv ? &maps.v : &maps.k, 64 * p, j % a.pages.page, h, page, bar);
+                    }
+                }
+            }
+        }
+        if (!ok && lane == 0)                                              // copies in flight land before the memory goes away
+            for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
+    } else if (warp == 9 && lane == 0) {
+        // ------------------------------------------------------------ products
+        bool ok = true;
+        uint32_t scored = 0;                                               // slots whose keys one of two streams has used
+        int started[2] = {0, 0}, weighted[2] = {0, 0};
+        auto scores = [&](int u, int i) {
+            const int slot = (2 * i) % S;
+            if (!started[u]++ && !wait_or_stop(smem_u32(&q_full[PAIR ? u : 0]), 0, stop)) return false;
+            if (!wait_or_stop(smem_u32(&kv_full[slot]), ((2 * i) / S) & 1, stop)) return false;
+            fence_after();
+            mma_dot<DM>(s_col + u * 128, q_at + (PAIR ? u : 0) * TILE, kv_at + slot * TILE, kPanel, IDESC_S);
+            mma_commit(smem_u32(&s_full[u]));
+            if (!PAIR || !need(1 - u, i) || (scored >> slot & 1)) {
+                scored &= ~(1u << slot);
+                mma_commit(smem_u32(&kv_empty[slot]));
+            } else {
+                scored |= 1u << slot;
+            }
+            return true;
+        };
+        for (int u = 0; u < 2 && ok; ++u) {
+            const int i = next(u, -1);
+            if (i < kt.count) ok = scores(u, i);
+        }
+        for (int i = 0; i < kt.count && ok; ++i) {
+            for (int u = 0; u < 2 && ok; ++u) {
+                if (!need(u, i)) continue;
+                const int slot = (2 * i + 1) % S;
+                ok = wait_or_stop(smem_u32(&p_full[u]), weighted[u] & 1, stop) && wait_or_stop(smem_u32(&kv_full[slot]), ((2 * i + 1) / S) & 1, stop);
+                if (!ok) break;
+                fence_after();
+                mma_weighted<128>(o_col + u * DM, s_col + u * 128, kv_at + slot * TILE, IDESC_O, weighted[u]++ != 0);
+                if (!PAIR || u == 1 || !need(1, i)) mma_commit(smem_u32(&kv_empty[slot]));
+                const int nx = next(u, i);
+                if (nx < kt.count) ok = scores(u, nx);
+                else mma_commit(smem_u32(&o_full[u]));
+            }
+        }
+        if (!ok) {                                                         // products in flight end before tensor memory is freed
+            mma_commit(smem_u32(&drained));
+            mbar_wait(smem_u32(&drained), 0, 1u << 14);
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_free(tmem, 512);
+    if (tid == 0 && stop_flag) report_stop(maps.timeouts, a.status);
+}
+
+template <typename T, int DM, bool PAIR, bool PAGED>
+int launch(const SeqArgs& a, const FwdMaps& maps, dim3 grid, cudaStream_t st) {
+    const cudaError_t e = cudaFuncSetAttribute(umma_fwd_kernel<T, DM, PAIR, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFwdSmem<DM>);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    umma_fwd_kernel<T, DM, PAIR, PAGED><<<grid, kThreads, kFwdSmem<DM>, st>>>(a, maps);
+    count_tensor_launch();
+    CA_CHECK_LAUNCH("window forward kernel (tensor cores)");
+    return CA_OK;
+}
+
+template <bool PAGED>
+int launch_any(const SeqArgs& a, const FwdMaps& maps, int dtype, bool pair, dim3 grid, cudaStream_t st) {
+    const bool wide = a.D > 64;
+#define CA_FWD(T)                                                                                                             \
+    return wide ? (pair ? launch<T, 128, true, PAGED>(a, maps, grid, st) : launch<T, 128, false, PAGED>(a, maps, grid, st))   \
+                : (pair ? launch<T, 64, true, PAGED>(a, maps, grid, st) : launch<T, 64, false, PAGED>(a, maps, grid, st))
+    if (dtype == CA_BF16) CA_FWD(__nv_bfloat16);
+    CA_FWD(__half);
+#undef CA_FWD
+}
+
+}  // namespace
+
+int encode_swizzled_map(CUtensorMap* map, bool bf16, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                        const uint32_t* box) {
+    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static std::atomic<EncodeFn> cache{nullptr};
+    EncodeFn fn = cache.load(std::memory_order_relaxed);
+    if (!fn) {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q);
+        if (e != cudaSuccess || !sym) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return CA_ERR_CUDA; }
+        fn = reinterpret_cast<EncodeFn>(sym);
+        cache.store(fn, std::memory_order_relaxed);
+    }
+    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base),
+                          dims, strides_bytes, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return CA_ERR_CUDA; }
+    return CA_OK;
+}
+
+int encode_tokens(CUtensorMap* m, bool bf16, const ca_seq_view& v, int D, int heads, int tokens, int batch, int box_tokens) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)tokens, (uint64_t)heads, (uint64_t)batch};
+    const uint64_t strides[3] = {(uint64_t)v.token * 2, (uint64_t)v.head * 2, (uint64_t)v.batch * 2};
+    const uint32_t box[4] = {64, (uint32_t)box_tokens, 1, 1};
+    return encode_swizzled_map(m, bf16, v.data, 4, dims, strides, box);
+}
+
+// Two row tiles a CTA share the key tiles; where that leaves SMs idle, one row tile and two streams over its keys.
+int umma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st) {
+    FwdMaps maps{};
+    const bool bf16 = dtype == CA_BF16;
+    int rc;
+    if ((rc = encode_tokens(&maps.k, bf16, a.k, a.D, a.Hkv, a.N, a.B, 128)) || (rc = encode_tokens(&maps.v, bf16, a.v, a.D, a.Hkv, a.N, a.B, 128))) return rc;
+    if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
+    const int64_t rows = (int64_t)a.N * a.G;
+    const bool pair = (rows + 255) / 256 * a.Hkv * a.B >= sm_count();
+    return launch_any<false>(a, maps, dtype, pair, dim3((unsigned)((rows + (pair ? 255 : 127)) / (pair ? 256 : 128)), a.Hkv, a.B), st);
+}
+
+int umma_paged(const SeqArgs& a, int dtype, cudaStream_t st) {
+    FwdMaps maps{};
+    const bool bf16 = dtype == CA_BF16;
+    int box = 16;
+    while (box < 128 && a.pages.page % (2 * box) == 0) box *= 2;
+    maps.box = box;
+    const ca_page_view* pools[2] = {&a.kp, &a.vp};
+    for (int i = 0; i < 2; ++i) {
+        const ca_page_view& p = *pools[i];
+        const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)a.pages.page, (uint64_t)a.Hkv, (uint64_t)(a.pages.pages > 0 ? a.pages.pages : 1)};
+        const uint64_t strides[3] = {(uint64_t)p.token * 2, (uint64_t)p.head * 2, (uint64_t)p.page * 2};
+        const uint32_t b[4] = {64, (uint32_t)box, 1, 1};
+        const int rc = encode_swizzled_map(i ? &maps.v : &maps.k, bf16, p.data, 4, dims, strides, b);
+        if (rc) return rc;
+    }
+    if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
+    const bool pair = paged_tiles(a.N, a.G, a.pages.sequences, 256) * a.Hkv >= sm_count() && (int64_t)a.N * a.G > 128LL * a.pages.sequences;
+    const int64_t tiles = paged_tiles(a.N, a.G, a.pages.sequences, pair ? 256 : 128);
+    return launch_any<true>(a, maps, dtype, pair, dim3((unsigned)tiles, a.Hkv, 1), st);
+}
+
+}  // namespace ca
