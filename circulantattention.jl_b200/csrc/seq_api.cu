@@ -70,6 +70,9 @@ static int fill(const ca_seq_desc* d, SeqArgs* a) {
     return CA_OK;
 }
 
+// delta, one float a row, padded so that what follows is aligned
+static size_t delta_bytes(const SeqArgs& a) { return ((size_t)a.N * a.B * a.Hq * sizeof(float) + 255) & ~(size_t)255; }
+
 }  // namespace ca
 
 using namespace ca;
@@ -95,7 +98,7 @@ int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
 size_t ca_window_bwd_workspace(const ca_seq_desc* d) {
     SeqArgs a{};
     if (fill(d, &a)) return 0;
-    return (size_t)a.N * a.B * a.Hq * sizeof(float);
+    return delta_bytes(a) + (d->dtype == CA_F32 ? 0 : umma_bwd_parts(a));
 }
 
 int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
@@ -115,7 +118,8 @@ int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     a.lengths = lengths;
     a.lse = const_cast<float*>(lse);
     a.delta = static_cast<float*>(workspace);
-    return fma_window_bwd(a, d->dtype, as_stream(stream));
+    if (d->dtype == CA_F32) return fma_window_bwd(a, d->dtype, as_stream(stream));
+    return umma_window_bwd(a, d->dtype, reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a)), as_stream(stream));
 }
 
 int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_view* k_pages, const ca_page_view* v_pages,

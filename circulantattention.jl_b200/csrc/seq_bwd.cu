@@ -1,0 +1,586 @@
+// Attention on token sequences, backward, on the tensor cores (tcgen05), 16-bit types, no atomics.
+//
+// With P = 2^(scale log2(e) q.k - lse), dP = dy.v and delta = dy.y:  dS = P (dP - delta),
+//     dq = scale dS k,   dk = scale dS^T q,   dv = P^T dy.
+// dq needs the sum over keys, dk and dv the sum over queries.  One sweep that did both would add one of the two into
+// memory from many CTAs, in an order that changes; two sweeps recompute two of seven products instead and stay exact in
+// their order: the first owns 128 query rows, the second 128 keys.
+//
+// In both, two warpgroups share each 128 x 128 tile: a thread owns one lane (row / key) and 64 of the columns.  The
+// weights return to tensor memory as 16-bit pairs over the columns that the same warpgroup has read, and are the A operand
+// of the next product from there.
+#include "seq_umma.cuh"
+
+#include <limits.h>
+#include <algorithm>
+
+namespace ca {
+namespace {
+
+constexpr int kThreads = 384;       // two warpgroups that compute, one that copies and issues; registers as in the forward
+template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
+template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
+template <int DM> constexpr size_t kBwdSmem = (size_t)(2 + kSlots<DM>) * kTileBytes<DM> + 1024;
+
+struct BwdMaps {
+    CUtensorMap k, v, q, dy;
+    int* timeouts;
+    float* partial;         // [b][key head][tile][segment][dk, dv][feature][128 keys]
+    int split_tiles;        // the first key tiles, whose queries are dealt to
+    int segments;           // so many CTAs
+};
+
+// A operand whose two halves of 64 contracted elements lie 64 columns apart.
+__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    mma_weighted<64>(d, a, b, idesc, add);
+    mma_weighted<64>(d, a + 64, b + 64 * 128, idesc, true);
+}
+
+__device__ __forceinline__ void read64(uint32_t at, uint32_t* x) {
+    tmem_ld32(at, x);
+    tmem_ld32(at + 32, x + 32);
+    tmem_wait_ld();
+    settled32(x);
+    settled32(x + 32);
+}
+
+template <typename T>
+__device__ __forceinline__ void store32(T* dst, const uint32_t* o, float f, int first, int D) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+        if (first + e >= D) continue;
+        float y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(o[e + k]) * f;
+        *reinterpret_cast<uint4*>(dst + first + e) = make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
+    }
+}
+
+template <int DM>
+__device__ __forceinline__ void clear_row(char* tile, int r) {
+#pragma unroll
+    for (int p = 0; p < DM / 64; ++p)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + p * kPanel + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------- dq
+// Tensor memory: scores 0..127, dP twice 128..383, dq from 384.  While the warpgroups turn tile i into dS, the products of
+// tile i + 1 run.
+template <typename T, int DM>
+__global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ BwdMaps maps) {
+    constexpr int S = kSlots<DM>;
+    constexpr uint32_t TILE = kTileBytes<DM>;
+    constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
+    extern __shared__ char raw[];
+    __shared__ uint64_t kv_full[S], kv_empty[S], q_full, s_full, s_free, dp_full[2], ds_full[2], o_full, drained;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int stop_flag;
+    __shared__ float part[2][128];
+    volatile int* stop = &stop_flag;
+    const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
+    char* const smem = raw + (base_at - raw_at);
+    const uint32_t kv_at = base_at + 2 * TILE;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+    const Seq s = dense_seq(a, blockIdx.z);
+    const int rows = s.T * a.G, R0 = (int)(gridDim.x - 1 - blockIdx.x) * 128;
+    const int f_lo = R0 / a.G, f_hi = (min(R0 + 128, rows) - 1) / a.G;      // tokens of the tile
+    const int p_hi = min(s.n - 1, f_hi);
+    const KeyTiles kt = key_tiles(a, s, f_lo, f_hi, 128);
+
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
+        mbar_init(&q_full, 8);
+        mbar_init(&s_full, 1);
+        mbar_init(&s_free, 8);
+        for (int i = 0; i < 2; ++i) { mbar_init(&dp_full[i], 1); mbar_init(&ds_full[i], 8); }
+        mbar_init(&o_full, 1);
+        mbar_init(&drained, 1);
+        stop_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot, o_col = tmem + 384;
+
+    if (warp < 8) {
+        more_registers<216>();
+        const int u = warp >> 2, r = tid & 127, R = R0 + r, pos = R / a.G;
+        const bool have = R < rows, live = have && pos < s.n;
+        const int64_t stat = ((int64_t)s.b * a.Hkv + h) * rows + R;
+        stage_row<T, DM>(smem, r, live ? seq_row<T>(a.q, a, s, h, R) : nullptr, a.D, u, 2, false);
+        const T* dyr = live ? seq_row<T>(a.dy, a, s, h, R) : nullptr;
+        stage_row<T, DM>(smem + TILE, r, dyr, a.D, u, 2, false);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&q_full));
+        float d = 0.f;
+        if (live) {
+            const T* yr = seq_row<T>(a.y, a, s, h, R);
+            const T* rr = a.rest.data ? seq_row<T>(a.rest, a, s, h, R) : nullptr;
+#pragma unroll 2
+            for (int c = u * 8; c < a.D; c += 16) {
+                const uint4 w = *reinterpret_cast<const uint4*>(dyr + c), y = *reinterpret_cast<const uint4*>(yr + c);
+                const uint4 e = rr ? *reinterpret_cast<const uint4*>(rr + c) : make_uint4(0, 0, 0, 0);
+                const uint32_t *pw = &w.x, *py = &y.x, *pe = &e.x;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    d = fmaf(low16<T>(pw[k]), low16<T>(py[k]) + low16<T>(pe[k]), d);
+                    d = fmaf(high16<T>(pw[k]), high16<T>(py[k]) + high16<T>(pe[k]), d);
+                }
+            }
+        }
+        part[u][r] = d;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float delta = part[0][r] + part[1][r];
+        if (u == 0 && have) a.delta[stat] = delta;
+        const float lse = live ? a.lse[stat] : 0.f;
+        const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta, -delta);
+        const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
+        const uint32_t S_at = tmem + 64 * u + lane_off;
+        bool ok = true;
+        for (int i = 0; i < kt.count; ++i) {
+            const int key0 = kt.key(i, 128), far = key0 + 127;
+            if (!warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
+            fence_after();
+            uint32_t x[64];
+            read64(S_at, x);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_free));
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+                float e0, e1;
+                unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, lse2), e0, e1);
+                x[c] = __float_as_uint(fast_exp2(e0));
+                x[c + 1] = __float_as_uint(fast_exp2(e1));
+            }
+            uint32_t mk[2] = {~0u, ~0u};
+            const bool edge = !(far <= f_lo + a.right && far < s.n && f_hi == p_hi && (key0 >= p_hi - a.left || far < a.sinks));
+            if (edge) {
+                const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) mk[g] = seen_bits(lo - 64 * u - 32 * g, hi - 64 * u - 32 * g, sk - 64 * u - 32 * g);
+                if (far >= s.n && u == 0) {                    // keys behind the length may be anything: zeros
+                    const int slot = (2 * i) % S;              // the scores are there, so the keys are
+                    if (key0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
+                    fence_async_smem();
+                }
+            }
+            if (!warp_wait(smem_u32(&dp_full[i & 1]), (i >> 1) & 1, stop)) { ok = false; break; }
+            fence_after();
+            const uint32_t dp_at = tmem + 128 + (i & 1) * 128 + 64 * u + lane_off;
+            uint32_t y[64], w[32];
+            read64(dp_at, y);
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+                float e0, e1;
+                unpack2(mul2(add2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), dl2), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e0, e1);
+                if (edge) {
+                    e0 = (mk[c >> 5] >> (c & 31)) & 1 ? e0 : 0.f;
+                    e1 = (mk[c >> 5] >> (c & 31)) & 2 ? e1 : 0.f;
+                }
+                w[c >> 1] = pack16<T>(e0, e1);
+            }
+            tmem_st32(dp_at, w);
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ds_full[i & 1]));
+        }
+        if (kt.count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
+        fence_after();
+        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : a.scale;
+        T* dst = seq_row<T>(a.dq, a, s, h, have ? R : R0);
+#pragma unroll
+        for (int c = 0; c < DM / 2; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_col + lane_off + u * (DM / 2) + c, o);
+            tmem_wait_ld();
+            settled32(o);
+            if (!kt.count)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0;
+            if (have) store32<T>(dst, o, f, u * (DM / 2) + c, a.D);
+        }
+    } else {
+        fewer_registers<64>();
+    }
+    if (warp == 8 && lane == 0) {
+        bool ok = true;
+        int issued = 0;
+        for (; issued < 2 * kt.count; ++issued) {
+            const int slot = issued % S;
+            if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
+            const uint32_t bar = smem_u32(&kv_full[slot]), dst = kv_at + slot * TILE;
+            mbar_arrive_expect_tx(bar, TILE);
+#pragma unroll
+            for (int p = 0; p < DM / 64; ++p)
+                tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.v : &maps.k, 64 * p, kt.key(issued >> 1, 128), h, s.b, bar);
+        }
+        if (!ok)                                               // copies in flight land before the memory goes away
+            for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
+    } else if (warp == 9 && lane == 0 && kt.count) {
+        auto products = [&](int i) {                           // scores and dP of tile i
+            const int ks = (2 * i) % S, vs = (2 * i + 1) % S;
+            if (!wait_or_stop(smem_u32(&kv_full[ks]), ((2 * i) / S) & 1, stop)) return false;
+            fence_after();
+            mma_dot<DM>(tmem, base_at, kv_at + ks * TILE, kPanel, IDESC_S);
+            mma_commit(smem_u32(&s_full));
+            if (!wait_or_stop(smem_u32(&kv_full[vs]), ((2 * i + 1) / S) & 1, stop)) return false;
+            fence_after();
+            mma_dot<DM>(tmem + 128 + (i & 1) * 128, base_at + TILE, kv_at + vs * TILE, kPanel, IDESC_S);
+            mma_commit(smem_u32(&dp_full[i & 1]));
+            mma_commit(smem_u32(&kv_empty[vs]));
+            return true;
+        };
+        bool ok = wait_or_stop(smem_u32(&q_full), 0, stop) && products(0);
+        for (int i = 0; i < kt.count && ok; ++i) {
+            if (i + 1 < kt.count) {
+                ok = wait_or_stop(smem_u32(&s_free), i & 1, stop) && products(i + 1);
+                if (!ok) break;
+            }
+            ok = wait_or_stop(smem_u32(&ds_full[i & 1]), (i >> 1) & 1, stop);
+            if (!ok) break;
+            fence_after();
+            const int ks = (2 * i) % S;
+            mma_halves(o_col, tmem + 128 + (i & 1) * 128, kv_at + ks * TILE, IDESC_O, i != 0);
+            mma_commit(smem_u32(&kv_empty[ks]));
+        }
+        if (ok) {
+            mma_commit(smem_u32(&o_full));
+        } else {                                               // products in flight end before tensor memory is freed
+            mma_commit(smem_u32(&drained));
+            mbar_wait(smem_u32(&drained), 0, 1u << 14);
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_free(tmem, 512);
+    if (tid == 0 && stop_flag) report_stop(maps.timeouts, a.status);
+}
+
+// ---------------------------------------------------------------- dk, dv
+// Tiles are transposed: lanes are the CTA's 128 keys, columns 128 tokens of one query head.  Tensor memory: scores 0..127, dP
+// 128..255, dv from 256, dk behind it.  The order of the products keeps them running: dv(i), scores(i+1), dk(i), dP(i+1);
+// the weights of i + 1 are made during the last two, dS(i) during the first two.
+//
+// Keys that stay visible to every later token would give their CTA all queries of the sequence; the queries of such tiles are
+// dealt to `segments` CTAs, which store Float32 parts for join_kernel to add up in order.
+template <typename T, int DM>
+__global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ BwdMaps maps) {
+    constexpr int S = kSlots<DM>;
+    constexpr uint32_t TILE = kTileBytes<DM>;
+    constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
+    extern __shared__ char raw[];
+    __shared__ uint64_t q_full[S], q_empty[S], kv_full, s_full, dp_full, p_full, ds_full, st_full[2], st_empty[2], dl_full, dl_empty, o_full, drained;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int stop_flag;
+    __shared__ __align__(16) float s_lse[2][128], s_delta[128];       // delta once: the tiles take all but 2 KB
+    volatile int* stop = &stop_flag;
+    const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
+    char* const smem = raw + (base_at - raw_at);
+    const uint32_t ring_at = base_at + 2 * TILE;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+    const Seq s = dense_seq(a, blockIdx.z);
+    const int dealt = maps.split_tiles * maps.segments;
+    const bool split = (int)blockIdx.x < dealt;
+    const int tile = split ? (int)blockIdx.x / maps.segments : maps.split_tiles + (int)blockIdx.x - dealt;
+    const int seg = split ? (int)blockIdx.x % maps.segments : 0;
+    const int k0 = tile * 128;
+    const int t_lo = max(0, k0 - a.right);
+    const int t_hi = k0 >= s.n ? t_lo : k0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)k0 + 128 + a.left);
+    const int all = max(0, t_hi - t_lo + 127) / 128 * a.G;          // steps: token tiles outside, query heads inside
+    const int first = split ? (int)((int64_t)all * seg / maps.segments) : 0;
+    const int count = (split ? (int)((int64_t)all * (seg + 1) / maps.segments) : all) - first;
+
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
+        mbar_init(&kv_full, 1);
+        mbar_init(&s_full, 1);
+        mbar_init(&dp_full, 1);
+        mbar_init(&p_full, 8);
+        mbar_init(&ds_full, 8);
+        for (int i = 0; i < 2; ++i) { mbar_init(&st_full[i], 1); mbar_init(&st_empty[i], 8); }
+        mbar_init(&dl_full, 1);
+        mbar_init(&dl_empty, 8);
+        mbar_init(&o_full, 1);
+        mbar_init(&drained, 1);
+        stop_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot, dv_col = tmem + 256, dk_col = tmem + 256 + DM;
+
+    if (warp < 8) {
+        more_registers<216>();
+        const int u = warp >> 2, r = tid & 127, j = k0 + r;
+        const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
+        const uint32_t S_at = tmem + 64 * u + lane_off, dp_at = S_at + 128;
+        const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
+        const f32x2 minus2 = pack2(-1.f, -1.f);
+        bool ok = true;
+        for (int i = 0; i < count; ++i) {
+            const int step = first + i, q0 = t_lo + step / a.G * 128, b = i & 1;
+            const bool edge = !(k0 + 127 <= q0 + a.right && (q0 + 127 <= k0 + a.left || k0 + 127 < a.sinks) && q0 + 127 < s.n && k0 + 127 < s.n);
+            if (!warp_wait(smem_u32(&st_full[b]), (i >> 1) & 1, stop) || !warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
+            fence_after();
+            uint32_t x[64], w[32];
+            read64(S_at, x);
+            uint32_t mk[2] = {~0u, ~0u};
+            if (edge) {
+                const int hi = j >= s.n ? -1 : (j < a.sinks ? s.n - 1 : min(j + a.left, s.n - 1)) - q0, lo = j - a.right - q0;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) mk[g] = seen_bits(lo - 64 * u - 32 * g, hi - 64 * u - 32 * g, INT_MIN + 1);
+            }
+            const float4* lse4 = reinterpret_cast<const float4*>(&s_lse[b][64 * u]);
+            const float4* del4 = reinterpret_cast<const float4*>(&s_delta[64 * u]);
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                const float4 z = lse4[c >> 2];
+                float e[4];
+                unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack2(z.x, z.y)), e[0], e[1]);
+                unpack2(fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), sc2, pack2(z.z, z.w)), e[2], e[3]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    e[k] = fast_exp2(e[k]);
+                    if (edge) e[k] = (mk[c >> 5] >> ((c & 31) + k)) & 1 ? e[k] : 0.f;
+                    x[c + k] = __float_as_uint(e[k]);
+                }
+                w[c >> 1] = pack16<T>(e[0], e[1]);
+                w[(c >> 1) + 1] = pack16<T>(e[2], e[3]);
+            }
+            tmem_st32(S_at, w);
+            if (q0 + 127 >= s.n) {                              // queries behind the length may be anything: zeros
+                const int slot = (2 * i + u) % S;               // one warpgroup clears q, the other dy
+                if (!warp_wait(smem_u32(&q_full[slot]), ((2 * i + u) / S) & 1, stop)) { ok = false; break; }
+                if (q0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
+                fence_async_smem();
+            }
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&p_full));
+                mbar_arrive(smem_u32(&st_empty[b]));
+            }
+            if (!warp_wait(smem_u32(&dl_full), i & 1, stop) || !warp_wait(smem_u32(&dp_full), i & 1, stop)) { ok = false; break; }
+            fence_after();
+            uint32_t y[64];
+            read64(dp_at, y);
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                const float4 z = del4[c >> 2];
+                float e[4];
+                unpack2(mul2(fma2(pack2(z.x, z.y), minus2, pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1]))), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e[0], e[1]);
+                unpack2(mul2(fma2(pack2(z.z, z.w), minus2, pack2(__uint_as_float(y[c + 2]), __uint_as_float(y[c + 3]))), pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3]))), e[2], e[3]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (edge) e[k] = (mk[c >> 5] >> ((c & 31) + k)) & 1 ? e[k] : 0.f;
+                w[c >> 1] = pack16<T>(e[0], e[1]);
+                w[(c >> 1) + 1] = pack16<T>(e[2], e[3]);
+            }
+            tmem_st32(dp_at, w);
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&ds_full));
+                mbar_arrive(smem_u32(&dl_empty));
+            }
+        }
+        if (count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
+        fence_after();
+        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : u ? a.scale : 1.f;       // the first warpgroup stores dv, the second dk
+        const ca_seq_view& out = u ? a.dk : a.dv;
+        T* dst = (T*)out.data + h * out.head + (int64_t)min(j, a.N - 1) * out.token + s.b * out.batch;
+        float* part = maps.partial + (((((int64_t)s.b * a.Hkv + h) * maps.split_tiles + tile) * maps.segments + seg) * 2 + 1 - u) * (DM * 128) + r;
+#pragma unroll
+        for (int c = 0; c < DM; c += 32) {
+            uint32_t o[32];
+            tmem_ld32((u ? dk_col : dv_col) + lane_off + c, o);
+            tmem_wait_ld();
+            settled32(o);
+            if (!count)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0;
+            if (split) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) part[(c + e) * 128] = __uint_as_float(o[e]) * f;
+            } else if (j < a.N) {
+                store32<T>(dst, o, f, c, a.D);
+            }
+        }
+    } else {
+        fewer_registers<64>();
+    }
+    if (warp == 8 && lane == 0 && count) {
+        bool ok = true;
+        int issued = 0;
+        mbar_arrive_expect_tx(smem_u32(&kv_full), 2 * TILE);
+#pragma unroll
+        for (int p = 0; p < DM / 64; ++p) {
+            tma_load_4d(base_at + p * kPanel, &maps.k, 64 * p, k0, h, s.b, smem_u32(&kv_full));
+            tma_load_4d(base_at + TILE + p * kPanel, &maps.v, 64 * p, k0, h, s.b, smem_u32(&kv_full));
+        }
+        for (; issued < 2 * count; ++issued) {
+            const int slot = issued % S, step = first + (issued >> 1), q0 = t_lo + step / a.G * 128;
+            if (!wait_or_stop(smem_u32(&q_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
+            const uint32_t bar = smem_u32(&q_full[slot]), dst = ring_at + slot * TILE;
+            mbar_arrive_expect_tx(bar, TILE);
+#pragma unroll
+            for (int p = 0; p < DM / 64; ++p)
+                tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.dy : &maps.q, 64 * p, q0, h * a.G + step % a.G, s.b, bar);
+        }
+        if (!ok) {                                             // copies in flight land before the memory goes away
+            mbar_wait(smem_u32(&kv_full), 0, 1u << 12);
+            for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&q_full[i % S]), (i / S) & 1, 1u << 12);
+        }
+    } else if (warp == 9 && lane == 0 && count) {
+        auto scores = [&](int i) {
+            const int qs = (2 * i) % S;
+            if (!wait_or_stop(smem_u32(&q_full[qs]), ((2 * i) / S) & 1, stop)) return false;
+            fence_after();
+            mma_dot<DM>(tmem, base_at, ring_at + qs * TILE, kPanel, IDESC_S);
+            mma_commit(smem_u32(&s_full));
+            return true;
+        };
+        auto dprobs = [&](int i) {
+            const int ds = (2 * i + 1) % S;
+            if (!wait_or_stop(smem_u32(&q_full[ds]), ((2 * i + 1) / S) & 1, stop)) return false;
+            fence_after();
+            mma_dot<DM>(tmem + 128, base_at + TILE, ring_at + ds * TILE, kPanel, IDESC_S);
+            mma_commit(smem_u32(&dp_full));
+            return true;
+        };
+        bool ok = wait_or_stop(smem_u32(&kv_full), 0, stop) && scores(0) && dprobs(0);
+        for (int i = 0; i < count && ok; ++i) {
+            const int qs = (2 * i) % S, ds = (2 * i + 1) % S;
+            ok = wait_or_stop(smem_u32(&p_full), i & 1, stop);
+            if (!ok) break;
+            fence_after();
+            mma_halves(dv_col, tmem, ring_at + ds * TILE, IDESC_O, i != 0);
+            mma_commit(smem_u32(&q_empty[ds]));
+            if (i + 1 < count && !(ok = scores(i + 1))) break;
+            ok = wait_or_stop(smem_u32(&ds_full), i & 1, stop);
+            if (!ok) break;
+            fence_after();
+            mma_halves(dk_col, tmem + 128, ring_at + qs * TILE, IDESC_O, i != 0);
+            mma_commit(smem_u32(&q_empty[qs]));
+            if (i + 1 < count) ok = dprobs(i + 1);
+        }
+        if (ok) {
+            mma_commit(smem_u32(&o_full));
+        } else {                                               // products in flight end before tensor memory is freed
+            mma_commit(smem_u32(&drained));
+            mbar_wait(smem_u32(&drained), 0, 1u << 14);
+        }
+    } else if (warp == 10) {
+        // minus the rows' sums, and their delta
+        const int rows = s.T * a.G;
+        const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
+        for (int i = 0; i < count; ++i) {
+            const int step = first + i, q0 = t_lo + step / a.G * 128, b = i & 1;
+            float z[4], d[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = q0 + lane + 32 * k;
+                const bool in = t < s.n;
+                z[k] = in ? -a.lse[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
+                d[k] = in ? a.delta[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
+            }
+            if (!warp_wait(smem_u32(&st_empty[b]), ((i >> 1) & 1) ^ 1, stop)) break;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s_lse[b][lane + 32 * k] = z[k];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&st_full[b]));
+            if (!warp_wait(smem_u32(&dl_empty), (i & 1) ^ 1, stop)) break;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s_delta[lane + 32 * k] = d[k];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&dl_full));
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_free(tmem, 512);
+    if (tid == 0 && stop_flag) report_stop(maps.timeouts, a.status);
+}
+
+// Adds the parts of a split key tile in order: thread = key, eight features of dk or dv a block.
+template <typename T, int DM>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ SeqArgs a, const float* __restrict__ partial, int split_tiles, int segments) {
+    const int r = threadIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const int c = blockIdx.x % (DM / 8) * 8, which = blockIdx.x / (DM / 8) & 1, tile = blockIdx.x / (DM / 4), j = tile * 128 + r;
+    const float* p = partial + ((((int64_t)b * a.Hkv + h) * split_tiles + tile) * segments * 2 + which) * (DM * 128) + c * 128 + r;
+    float sum[8] = {};
+    for (int seg = 0; seg < segments; ++seg, p += 2 * DM * 128)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += p[e * 128];
+    if (j >= a.N || c >= a.D) return;
+    const ca_seq_view& out = which ? a.dv : a.dk;
+    T* dst = (T*)out.data + h * out.head + (int64_t)j * out.token + b * out.batch + c;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack16<T>(sum[0], sum[1]), pack16<T>(sum[2], sum[3]), pack16<T>(sum[4], sum[5]), pack16<T>(sum[6], sum[7]));
+}
+
+// Key tiles of first tokens have every later query; they are dealt out in pieces of about an ordinary tile's work.
+void split_rule(const SeqArgs& a, int* tiles, int* segments) {
+    const int64_t all = (a.N + 127) / 128, window = ((int64_t)a.left + a.right + 255) / 128;
+    *tiles = (int)((std::min(a.sinks, a.N) + 127) / 128);
+    *segments = (int)std::min<int64_t>(64, (all + window - 1) / window);
+    if (*segments < 2 || *tiles == 0) { *tiles = 0; *segments = 1; }
+}
+
+template <typename T, int DM>
+int launch(const SeqArgs& a, const BwdMaps& maps, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(umma_dq_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(umma_dkdv_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    umma_dq_kernel<T, DM><<<dim3((unsigned)(((int64_t)a.N * a.G + 127) / 128), a.Hkv, a.B), kThreads, kBwdSmem<DM>, st>>>(a, maps);
+    count_tensor_launch();
+    CA_CHECK_LAUNCH("window dq kernel (tensor cores)");
+    const int tiles = (a.N + 127) / 128;
+    umma_dkdv_kernel<T, DM><<<dim3(tiles - maps.split_tiles + maps.split_tiles * maps.segments, a.Hkv, a.B), kThreads, kBwdSmem<DM>, st>>>(a, maps);
+    count_tensor_launch();
+    CA_CHECK_LAUNCH("window dk/dv kernel (tensor cores)");
+    if (maps.split_tiles) {
+        join_kernel<T, DM><<<dim3(maps.split_tiles * (DM / 4), a.Hkv, a.B), 128, 0, st>>>(a, maps.partial, maps.split_tiles, maps.segments);
+        CA_CHECK_LAUNCH("window dk/dv join kernel");
+    }
+    return CA_OK;
+}
+
+}  // namespace
+
+// Float32 parts of the dealt key tiles, behind the rows' delta.
+size_t umma_bwd_parts(const SeqArgs& a) {
+    int tiles, segments;
+    split_rule(a, &tiles, &segments);
+    return (size_t)tiles * segments * 2 * (a.D > 64 ? 128 : 64) * 128 * a.Hkv * a.B * sizeof(float);
+}
+
+int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) {
+    BwdMaps maps{};
+    const bool bf16 = dtype == CA_BF16;
+    int rc;
+    if ((rc = encode_tokens(&maps.k, bf16, a.k, a.D, a.Hkv, a.N, a.B, 128)) || (rc = encode_tokens(&maps.v, bf16, a.v, a.D, a.Hkv, a.N, a.B, 128)) ||
+        (rc = encode_tokens(&maps.q, bf16, a.q, a.D, a.Hq, a.N, a.B, 128)) || (rc = encode_tokens(&maps.dy, bf16, a.dy, a.D, a.Hq, a.N, a.B, 128)))
+        return rc;
+    if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
+    maps.partial = parts;
+    split_rule(a, &maps.split_tiles, &maps.segments);
+    const bool wide = a.D > 64;
+    if (bf16) return wide ? launch<__nv_bfloat16, 128>(a, maps, st) : launch<__nv_bfloat16, 64>(a, maps, st);
+    return wide ? launch<__half, 128>(a, maps, st) : launch<__half, 64>(a, maps, st);
+}
+
+}  // namespace ca

@@ -68,6 +68,7 @@ int encode_tokens(CUtensorMap* m, bool bf16, const ca_seq_view& v, int D, int he
 int umma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st);
 int umma_paged(const SeqArgs& a, int dtype, cudaStream_t st);
 // seq_bwd.cu
-int umma_window_bwd(const SeqArgs& a, int dtype, cudaStream_t st);
+size_t umma_bwd_parts(const SeqArgs& a);
+int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st);
 
 }  // namespace ca
