@@ -25,10 +25,27 @@ template <int DM> constexpr size_t kBwdSmem = (size_t)(2 + kSlots<DM>) * kTileBy
 struct BwdMaps {
     CUtensorMap k, v, q, dy;
     int* timeouts;
+    float *dy_peak, *v_peak;    // half: largest magnitudes of each tile of 128 query rows / keys, [b][key head][tile]
     float* partial;         // [b][key head][tile][segment][dk, dv][feature][128 keys]
     int split_tiles;        // the first key tiles, whose queries are dealt to
     int segments;           // so many CTAs
 };
+
+// Half precision has too few exponents for the weights of long windows and for dS of scaled losses.  P is at most 1 and goes
+// into its product as 2^8 P.  dS goes in as c dS with c = 2^(7 - floor(log2 max|dy|) - floor(log2 max|v|)): since
+// P_j |v_j - sum P v| <= max|v| / 2, |dS| is at most 128 max|dy| max|v| / 2 for 128 features, and |c dS| < 2^15; and where dP
+// is of the usual size, weights down to 2^-20 still give normal numbers.  Both factors are powers of two and leave with the
+// results.  The peaks cost one pass over v (5 us for 32 MB).  bfloat16 has the exponents of Float32 and needs none of this.
+constexpr float kPScale = 256.f, kPLog2 = 8.f;
+__device__ __forceinline__ int exponent(float x) { return x > 0.f && !isinf(x) ? (int)(__float_as_uint(x) >> 23) - 127 : 0; }
+__device__ __forceinline__ float ds_factor(float dy_peak, float v_peak) {
+    return __uint_as_float((uint32_t)(127 + 7 - exponent(dy_peak) - exponent(v_peak)) << 23);      // halves: -24 <= exponents <= 15
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+    return x;
+}
 
 // A operand whose two halves of 64 contracted elements lie 64 columns apart.
 __device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
@@ -64,6 +81,29 @@ __device__ __forceinline__ void clear_row(char* tile, int r) {
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + p * kPanel + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
 }
 
+__global__ void __launch_bounds__(256) peak_kernel(const __grid_constant__ SeqArgs a, float* __restrict__ peaks) {
+    __shared__ float part[8];
+    const Seq s = dense_seq(a, blockIdx.z);
+    const int pieces = a.D / 8, key0 = blockIdx.x * 128;
+    const __half* v = (const __half*)a.v.data + blockIdx.y * a.v.head + s.b * a.v.batch;
+    float peak = 0.f;
+    for (int i = threadIdx.x; i < 128 * pieces; i += 256) {
+        const int j = key0 + i / pieces;
+        if (j >= s.n) break;
+        const uint4 w = *reinterpret_cast<const uint4*>(v + (int64_t)j * a.v.token + i % pieces * 8);
+        const uint32_t* p = &w.x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) peak = fmaxf(peak, fmaxf(fabsf(low16<__half>(p[k])), fabsf(high16<__half>(p[k]))));
+    }
+    peak = warp_max(peak);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = peak;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        peak = warp_max(threadIdx.x < 8 ? part[threadIdx.x] : 0.f);
+        if (threadIdx.x == 0) peaks[((int64_t)s.b * a.Hkv + blockIdx.y) * gridDim.x + blockIdx.x] = peak;
+    }
+}
+
 // ---------------------------------------------------------------- dq
 // Tensor memory: scores 0..127, dP twice 128..383, dq from 384.  While the warpgroups turn tile i into dS, the products of
 // tile i + 1 run.
@@ -76,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     __shared__ uint64_t kv_full[S], kv_empty[S], q_full, s_full, s_free, dp_full[2], ds_full[2], o_full, drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int stop_flag;
-    __shared__ float part[2][128];
+    __shared__ float part[2][128], warp_peak[4];
     volatile int* stop = &stop_flag;
     const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
     char* const smem = raw + (base_at - raw_at);
@@ -117,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&q_full));
-        float d = 0.f;
+        float d = 0.f, peak = 0.f;
         if (live) {
             const T* yr = seq_row<T>(a.y, a, s, h, R);
             const T* rr = a.rest.data ? seq_row<T>(a.rest, a, s, h, R) : nullptr;
@@ -130,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 for (int k = 0; k < 4; ++k) {
                     d = fmaf(low16<T>(pw[k]), low16<T>(py[k]) + low16<T>(pe[k]), d);
                     d = fmaf(high16<T>(pw[k]), high16<T>(py[k]) + high16<T>(pe[k]), d);
+                    if (!kIsBf16<T>) peak = fmaxf(peak, fmaxf(fabsf(low16<T>(pw[k])), fabsf(high16<T>(pw[k]))));
                 }
             }
         }
@@ -137,8 +178,21 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         asm volatile("bar.sync 1, 256;" ::: "memory");
         const float delta = part[0][r] + part[1][r];
         if (u == 0 && have) a.delta[stat] = delta;
+        float c = 1.f;
+        if (!kIsBf16<T>) {
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            part[u][r] = peak;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            peak = fmaxf(part[0][r], part[1][r]);
+            const float* p = maps.v_peak + ((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128);
+            float v_peak = 0.f;
+            for (int i = lane; i < kt.count; i += 32) v_peak = fmaxf(v_peak, p[kt.key(i, 128) / 128]);
+            c = ds_factor(peak, warp_max(v_peak));
+            peak = warp_max(peak);
+            if (u == 0 && lane == 0) warp_peak[warp] = peak;
+        }
         const float lse = live ? a.lse[stat] : 0.f;
-        const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta, -delta);
+        const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta * c, -delta * c), c2 = pack2(c, c);
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
         const uint32_t S_at = tmem + 64 * u + lane_off;
         bool ok = true;
@@ -178,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
 #pragma unroll
             for (int c = 0; c < 64; c += 2) {
                 float e0, e1;
-                unpack2(mul2(add2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), dl2), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e0, e1);
+                unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, dl2), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e0, e1);
                 if (edge) {
                     e0 = (mk[c >> 5] >> (c & 31)) & 1 ? e0 : 0.f;
                     e1 = (mk[c >> 5] >> (c & 31)) & 2 ? e1 : 0.f;
@@ -193,7 +247,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         }
         if (kt.count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
         fence_after();
-        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : a.scale;
+        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : a.scale / c;
+        if (!kIsBf16<T>) {
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (tid == 0)
+                maps.dy_peak[((int64_t)s.b * a.Hkv + h) * gridDim.x + R0 / 128] = fmaxf(fmaxf(warp_peak[0], warp_peak[1]), fmaxf(warp_peak[2], warp_peak[3]));
+        }
         T* dst = seq_row<T>(a.dq, a, s, h, have ? R : R0);
 #pragma unroll
         for (int c = 0; c < DM / 2; c += 32) {
@@ -319,6 +378,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot, dv_col = tmem + 256, dk_col = tmem + 256 + DM;
+    float c = 1.f;                                                  // factor of dS
+    if (!kIsBf16<T> && count) {
+        const int tiles = (int)(((int64_t)s.T * a.G + 127) / 128);
+        const float* p = maps.dy_peak + ((int64_t)s.b * a.Hkv + h) * tiles;
+        float peak = 0.f;
+        for (int i = (int)((int64_t)t_lo * a.G / 128) + lane; i <= (int)(((int64_t)t_hi * a.G - 1) / 128); i += 32) peak = fmaxf(peak, p[i]);
+        c = ds_factor(warp_max(peak), maps.v_peak[((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128) + tile]);
+    }
 
     if (warp < 8) {
         more_registers<216>();
@@ -326,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
         const uint32_t S_at = tmem + 64 * u + lane_off, dp_at = S_at + 128;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
-        const f32x2 minus2 = pack2(-1.f, -1.f);
+        const f32x2 c2 = kIsBf16<T> ? pack2(1.f, 1.f) : pack2(c / kPScale, c / kPScale);
         bool ok = true;
         for (int i = 0; i < count; ++i) {
             const int step = first + i, q0 = t_lo + step / a.G * 128, b = i & 1;
@@ -380,8 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             for (int c = 0; c < 64; c += 4) {
                 const float4 z = del4[c >> 2];
                 float e[4];
-                unpack2(mul2(fma2(pack2(z.x, z.y), minus2, pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1]))), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e[0], e[1]);
-                unpack2(mul2(fma2(pack2(z.z, z.w), minus2, pack2(__uint_as_float(y[c + 2]), __uint_as_float(y[c + 3]))), pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3]))), e[2], e[3]);
+                unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, pack2(z.x, z.y)), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e[0], e[1]);
+                unpack2(mul2(fma2(pack2(__uint_as_float(y[c + 2]), __uint_as_float(y[c + 3])), c2, pack2(z.z, z.w)), pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3]))), e[2], e[3]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     if (edge) e[k] = (mk[c >> 5] >> ((c & 31) + k)) & 1 ? e[k] : 0.f;
@@ -399,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         }
         if (count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
         fence_after();
-        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : u ? a.scale : 1.f;       // the first warpgroup stores dv, the second dk
+        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : u ? a.scale / c : kIsBf16<T> ? 1.f : 1.f / kPScale;       // the first warpgroup stores dv, the second dk
         const ca_seq_view& out = u ? a.dk : a.dv;
         T* dst = (T*)out.data + h * out.head + (int64_t)min(j, a.N - 1) * out.token + s.b * out.batch;
         float* part = maps.partial + (((((int64_t)s.b * a.Hkv + h) * maps.split_tiles + tile) * maps.segments + seg) * 2 + 1 - u) * (DM * 128) + r;
@@ -484,7 +551,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             mbar_wait(smem_u32(&drained), 0, 1u << 14);
         }
     } else if (warp == 10) {
-        // minus the rows' sums, and their delta
+        // minus the rows' sums, and minus their delta, with the factors of half precision
+        const float shift = kIsBf16<T> ? 0.f : kPLog2, minus = kIsBf16<T> ? -1.f : -c / kPScale;
         const int rows = s.T * a.G;
         const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
         for (int i = 0; i < count; ++i) {
@@ -494,8 +562,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             for (int k = 0; k < 4; ++k) {
                 const int t = q0 + lane + 32 * k;
                 const bool in = t < s.n;
-                z[k] = in ? -a.lse[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
-                d[k] = in ? a.delta[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
+                z[k] = in ? shift - a.lse[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
+                d[k] = in ? minus * a.delta[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
             }
             if (!warp_wait(smem_u32(&st_empty[b]), ((i >> 1) & 1) ^ 1, stop)) break;
 #pragma unroll
@@ -545,6 +613,10 @@ int launch(const SeqArgs& a, const BwdMaps& maps, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(umma_dq_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(umma_dkdv_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    if (!kIsBf16<T>) {
+        peak_kernel<<<dim3((a.N + 127) / 128, a.Hkv, a.B), 256, 0, st>>>(a, maps.v_peak);
+        CA_CHECK_LAUNCH("window peak kernel");
+    }
     umma_dq_kernel<T, DM><<<dim3((unsigned)(((int64_t)a.N * a.G + 127) / 128), a.Hkv, a.B), kThreads, kBwdSmem<DM>, st>>>(a, maps);
     count_tensor_launch();
     CA_CHECK_LAUNCH("window dq kernel (tensor cores)");
@@ -561,11 +633,14 @@ int launch(const SeqArgs& a, const BwdMaps& maps, cudaStream_t st) {
 
 }  // namespace
 
-// Float32 parts of the dealt key tiles, behind the rows' delta.
+static size_t dy_peaks(const SeqArgs& a) { return ((size_t)a.N * a.G + 127) / 128 * a.Hkv * a.B; }
+static size_t peak_floats(const SeqArgs& a) { return (dy_peaks(a) + ((size_t)a.N + 127) / 128 * a.Hkv * a.B + 63) & ~(size_t)63; }
+
+// Behind the rows' delta: the peaks of dy, and the Float32 parts of the dealt key tiles.
 size_t umma_bwd_parts(const SeqArgs& a) {
     int tiles, segments;
     split_rule(a, &tiles, &segments);
-    return (size_t)tiles * segments * 2 * (a.D > 64 ? 128 : 64) * 128 * a.Hkv * a.B * sizeof(float);
+    return (peak_floats(a) + (size_t)tiles * segments * 2 * (a.D > 64 ? 128 : 64) * 128 * a.Hkv * a.B) * sizeof(float);
 }
 
 int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) {
@@ -576,7 +651,9 @@ int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) 
         (rc = encode_tokens(&maps.q, bf16, a.q, a.D, a.Hq, a.N, a.B, 128)) || (rc = encode_tokens(&maps.dy, bf16, a.dy, a.D, a.Hq, a.N, a.B, 128)))
         return rc;
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
-    maps.partial = parts;
+    maps.dy_peak = parts;
+    maps.v_peak = parts + dy_peaks(a);
+    maps.partial = parts + peak_floats(a);
     split_rule(a, &maps.split_tiles, &maps.segments);
     const bool wide = a.D > 64;
     if (bf16) return wide ? launch<__nv_bfloat16, 128>(a, maps, st) : launch<__nv_bfloat16, 64>(a, maps, st);

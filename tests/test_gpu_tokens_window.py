@@ -118,6 +118,25 @@ def test_flat_and_peaked_rows(ca, dtype, size):
     assert u >= 0
 
 
+@pytest.mark.parametrize("size", [2.0 ** -12, 1.0, 4096.0])
+def test_range_of_half_precision(ca, size):
+    """Scaled losses and vanishing gradients, and rows whose weights are all below the smallest normal half: the products'
+    operands stay inside the type's range."""
+    D, N = 64, 900
+    q, k, v, dy = problem(D, 2, 1, N, 1, torch.float64)
+    q = q * 0.01                                        # flat rows: weights of about 1/900
+    v = v * (1.0 / size if size > 1 else 1.0)           # gradients of k and q stay inside the type
+    dy = dy * size
+    q, k, v, dy = (t.to(torch.float16) for t in (q, k, v, dy))
+    got = run(ca, q, k, v, dy, None, 899, 0)
+    want = ref.window(q.double(), k.double(), v.double(), None, 899, 0, None, None, dy.double(), ref.UNIT[torch.float16])
+    for name, (x, e) in want.items():
+        # results below the smallest normal half are rounded to multiples of 2^-24
+        ref.check(got[name], x, e + 2.0 ** -24, name)
+        norm = float((got[name].double().cpu() - x).norm() / x.norm())
+        assert norm < 2.0 ** -11 or float(x.abs().amax()) < 2.0 ** -9, (name, norm)
+
+
 def test_gradients_against_differences(ca):
     q, k, v, dy = problem(24, 4, 2, 90, 2, torch.float32)
     args = dict(left=17, right=2, sinks=3, lengths=[90, 55])
