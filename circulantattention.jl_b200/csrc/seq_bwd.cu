@@ -48,9 +48,9 @@ __device__ __forceinline__ float warp_max(float x) {
 }
 
 // A operand whose two halves of 64 contracted elements lie 64 columns apart.
-__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
     mma_weighted<64>(d, a, b, idesc, add);
-    mma_weighted<64>(d, a + 64, b + 64 * 128, idesc, true);
+    mma_weighted<64>(d, a + 64, b + 4 * 128, idesc, true);
 }
 
 __device__ __forceinline__ void read64(uint32_t at, uint32_t* x) {
@@ -282,39 +282,44 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         }
         if (!ok)                                               // copies in flight land before the memory goes away
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
-    } else if (warp == 9 && lane == 0 && kt.count) {
-        auto products = [&](int i) {                           // scores and dP of tile i
-            const int ks = (2 * i) % S, vs = (2 * i + 1) % S;
-            if (!wait_or_stop(smem_u32(&kv_full[ks]), ((2 * i) / S) & 1, stop)) return false;
+    } else if (warp == 9 && kt.count) {
+        const bool leader = elect_one();
+        const uint64_t q_desc = desc_features(base_at), dy_desc = desc_features(base_at + TILE), f_desc = desc_features(kv_at), r_desc = desc_rows(kv_at);
+        auto products = [&](uint32_t i) {                      // scores and dP of tile i
+            const uint32_t ks = (2 * i) % S, vs = (2 * i + 1) % S;
+            if (!warp_wait(smem_u32(&kv_full[ks]), ((2 * i) / S) & 1, stop)) return false;
             fence_after();
-            mma_dot<DM>(tmem, base_at, kv_at + ks * TILE, kPanel, IDESC_S);
-            mma_commit(smem_u32(&s_full));
-            if (!wait_or_stop(smem_u32(&kv_full[vs]), ((2 * i + 1) / S) & 1, stop)) return false;
+            if (leader) {
+                mma_dot<DM>(tmem, q_desc, f_desc + ks * (TILE >> 4), IDESC_S);
+                mma_commit(smem_u32(&s_full));
+            }
+            if (!warp_wait(smem_u32(&kv_full[vs]), ((2 * i + 1) / S) & 1, stop)) return false;
             fence_after();
-            mma_dot<DM>(tmem + 128 + (i & 1) * 128, base_at + TILE, kv_at + vs * TILE, kPanel, IDESC_S);
-            mma_commit(smem_u32(&dp_full[i & 1]));
-            mma_commit(smem_u32(&kv_empty[vs]));
+            if (leader) {
+                mma_dot<DM>(tmem + 128 + (i & 1) * 128, dy_desc, f_desc + vs * (TILE >> 4), IDESC_S);
+                mma_commit(smem_u32(&dp_full[i & 1]));
+                mma_commit(smem_u32(&kv_empty[vs]));
+            }
             return true;
         };
-        bool ok = wait_or_stop(smem_u32(&q_full), 0, stop) && products(0);
-        for (int i = 0; i < kt.count && ok; ++i) {
-            if (i + 1 < kt.count) {
-                ok = wait_or_stop(smem_u32(&s_free), i & 1, stop) && products(i + 1);
+        const uint32_t count = kt.count;
+        bool ok = warp_wait(smem_u32(&q_full), 0, stop) && products(0);
+        for (uint32_t i = 0; i < count && ok; ++i) {
+            if (i + 1 < count) {
+                ok = warp_wait(smem_u32(&s_free), i & 1, stop) && products(i + 1);
                 if (!ok) break;
             }
-            ok = wait_or_stop(smem_u32(&ds_full[i & 1]), (i >> 1) & 1, stop);
+            ok = warp_wait(smem_u32(&ds_full[i & 1]), (i >> 1) & 1, stop);
             if (!ok) break;
             fence_after();
-            const int ks = (2 * i) % S;
-            mma_halves(o_col, tmem + 128 + (i & 1) * 128, kv_at + ks * TILE, IDESC_O, i != 0);
-            mma_commit(smem_u32(&kv_empty[ks]));
+            const uint32_t ks = (2 * i) % S;
+            if (leader) {
+                mma_halves(o_col, tmem + 128 + (i & 1) * 128, r_desc + ks * (TILE >> 4), IDESC_O, i != 0);
+                mma_commit(smem_u32(&kv_empty[ks]));
+            }
         }
-        if (ok) {
-            mma_commit(smem_u32(&o_full));
-        } else {                                               // products in flight end before tensor memory is freed
-            mma_commit(smem_u32(&drained));
-            mbar_wait(smem_u32(&drained), 0, 1u << 14);
-        }
+        if (leader) mma_commit(smem_u32(ok ? &o_full : &drained));
+        if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
     }
     __syncwarp();
     fence_before();
@@ -511,45 +516,50 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             mbar_wait(smem_u32(&kv_full), 0, 1u << 12);
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&q_full[i % S]), (i / S) & 1, 1u << 12);
         }
-    } else if (warp == 9 && lane == 0 && count) {
-        auto scores = [&](int i) {
-            const int qs = (2 * i) % S;
-            if (!wait_or_stop(smem_u32(&q_full[qs]), ((2 * i) / S) & 1, stop)) return false;
+    } else if (warp == 9 && count) {
+        const bool leader = elect_one();
+        const uint64_t k_desc = desc_features(base_at), v_desc = desc_features(base_at + TILE), f_desc = desc_features(ring_at), r_desc = desc_rows(ring_at);
+        const uint32_t steps = count;
+        auto scores = [&](uint32_t i) {
+            const uint32_t qs = (2 * i) % S;
+            if (!warp_wait(smem_u32(&q_full[qs]), ((2 * i) / S) & 1, stop)) return false;
             fence_after();
-            mma_dot<DM>(tmem, base_at, ring_at + qs * TILE, kPanel, IDESC_S);
-            mma_commit(smem_u32(&s_full));
+            if (leader) {
+                mma_dot<DM>(tmem, k_desc, f_desc + qs * (TILE >> 4), IDESC_S);
+                mma_commit(smem_u32(&s_full));
+            }
             return true;
         };
-        auto dprobs = [&](int i) {
-            const int ds = (2 * i + 1) % S;
-            if (!wait_or_stop(smem_u32(&q_full[ds]), ((2 * i + 1) / S) & 1, stop)) return false;
+        auto dprobs = [&](uint32_t i) {
+            const uint32_t ds = (2 * i + 1) % S;
+            if (!warp_wait(smem_u32(&q_full[ds]), ((2 * i + 1) / S) & 1, stop)) return false;
             fence_after();
-            mma_dot<DM>(tmem + 128, base_at + TILE, ring_at + ds * TILE, kPanel, IDESC_S);
-            mma_commit(smem_u32(&dp_full));
+            if (leader) {
+                mma_dot<DM>(tmem + 128, v_desc, f_desc + ds * (TILE >> 4), IDESC_S);
+                mma_commit(smem_u32(&dp_full));
+            }
             return true;
         };
-        bool ok = wait_or_stop(smem_u32(&kv_full), 0, stop) && scores(0) && dprobs(0);
-        for (int i = 0; i < count && ok; ++i) {
-            const int qs = (2 * i) % S, ds = (2 * i + 1) % S;
-            ok = wait_or_stop(smem_u32(&p_full), i & 1, stop);
-            if (!ok) break;
+        bool ok = warp_wait(smem_u32(&kv_full), 0, stop) && scores(0) && dprobs(0);
+        for (uint32_t i = 0; i < steps && ok; ++i) {
+            const uint32_t qs = (2 * i) % S, ds = (2 * i + 1) % S;
+            if (!(ok = warp_wait(smem_u32(&p_full), i & 1, stop))) break;
             fence_after();
-            mma_halves(dv_col, tmem, ring_at + ds * TILE, IDESC_O, i != 0);
-            mma_commit(smem_u32(&q_empty[ds]));
-            if (i + 1 < count && !(ok = scores(i + 1))) break;
-            ok = wait_or_stop(smem_u32(&ds_full), i & 1, stop);
-            if (!ok) break;
+            if (leader) {
+                mma_halves(dv_col, tmem, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
+                mma_commit(smem_u32(&q_empty[ds]));
+            }
+            if (i + 1 < steps && !(ok = scores(i + 1))) break;
+            if (!(ok = warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
             fence_after();
-            mma_halves(dk_col, tmem + 128, ring_at + qs * TILE, IDESC_O, i != 0);
-            mma_commit(smem_u32(&q_empty[qs]));
-            if (i + 1 < count) ok = dprobs(i + 1);
+            if (leader) {
+                mma_halves(dk_col, tmem + 128, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
+                mma_commit(smem_u32(&q_empty[qs]));
+            }
+            if (i + 1 < steps) ok = dprobs(i + 1);
         }
-        if (ok) {
-            mma_commit(smem_u32(&o_full));
-        } else {                                               // products in flight end before tensor memory is freed
-            mma_commit(smem_u32(&drained));
-            mbar_wait(smem_u32(&drained), 0, 1u << 14);
-        }
+        if (leader) mma_commit(smem_u32(ok ? &o_full : &drained));
+        if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
     } else if (warp == 10) {
         // minus the rows' sums, and minus their delta, with the factors of half precision
         const float shift = kIsBf16<T> ? 0.f : kPLog2, minus = kIsBf16<T> ? -1.f : -c / kPScale;

@@ -31,6 +31,46 @@ struct FwdMaps {
     int* timeouts;
 };
 
+// A stream's tiles: those of first tokens below `first`, then from..upto, in steps of one (PAIR) or two.
+struct Stream {
+    int lo, hi;             // positions of its rows that exist; lo > hi: none
+    int first, from, upto, step;
+    __device__ __forceinline__ bool takes(int i) const { return step == 2 ? (i & 1) == (from & 1) && i <= upto : i < first || (i >= from && i <= upto); }
+    __device__ __forceinline__ int begin() const { return first > 0 ? 0 : from; }
+    __device__ __forceinline__ int next(int i) const {
+        i += step;
+        return i >= first && i < from ? from : i;
+    }
+};
+
+template <bool PAIR>
+__device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, const KeyTiles& kt, int u, int r, int rows) {
+    Stream t;
+    t.lo = max(0, s.base + r / a.G);
+    t.hi = r < rows ? min(s.n - 1, s.base + (min(r + 128, rows) - 1) / a.G) : -1;
+    if (!PAIR) {
+        t.first = 0;
+        t.from = u;
+        t.upto = kt.count - 1;
+        t.step = 2;
+        return t;
+    }
+    t.step = 1;
+    if (t.hi < t.lo) {
+        t.first = 0;
+        t.from = 0;
+        t.upto = -1;
+        return t;
+    }
+    // the window's tiles begin at kt.lo; those of first tokens lie before it, and beyond it only up to the window
+    const int begin = max(0, t.lo - a.left), end = (int)min((int64_t)s.n - 1, (int64_t)t.hi + a.right);
+    t.from = kt.first + (begin - kt.lo) / 128;
+    t.upto = kt.first + (end - kt.lo) / 128;
+    t.first = kt.first;
+    if (a.sinks > kt.lo) t.first = max(t.first, min(t.from, kt.first + (min(a.sinks, s.n) - kt.lo + 127) / 128));
+    return t;
+}
+
 template <typename T, int DM, bool PAIR, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ FwdMaps maps) {
     constexpr int S = kSlots<DM>;
@@ -59,24 +99,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     const int p_lo = max(0, s.base + R0 / a.G), p_hi = min(s.n - 1, s.base + (min(R0 + (PAIR ? 256 : 128), rows) - 1) / a.G);
     const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, 128);
 
-    // Which key tiles a stream needs: both streams see nearly the same, but each leaves out what all of its rows are blind to.
-    int u_lo[2], u_hi[2];                               // positions of its rows that exist; lo > hi: none
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int r = R0 + (PAIR ? 128 * u : 0);
-        u_lo[u] = max(0, s.base + r / a.G);
-        u_hi[u] = r < rows ? min(s.n - 1, s.base + (min(r + 128, rows) - 1) / a.G) : -1;
-    }
-    auto need = [&](int u, int i) {
-        if (!PAIR) return (i & 1) == u;
-        if (u_hi[u] < u_lo[u]) return false;
-        const int key0 = kt.key(i, 128);
-        return key0 <= u_hi[u] + a.right && (key0 + 127 >= u_lo[u] - a.left || key0 < a.sinks);
-    };
-    auto next = [&](int u, int i) {
-        do ++i; while (i < kt.count && !need(u, i));
-        return i;
-    };
+    // Which key tiles a stream takes: with PAIR both see nearly the same, but each leaves out what all of its rows are blind to.
+    const Stream st0 = stream_of<PAIR>(a, s, kt, 0, R0, rows), st1 = stream_of<PAIR>(a, s, kt, 1, PAIR ? R0 + 128 : R0, rows);
 
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
@@ -100,7 +124,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax: thread = row
         more_registers<216>();
-        const int u = warp >> 2, r = tid & 127, R = R0 + (PAIR ? 128 * u : 0) + r;
+        const int u = warp >> 2, r = tid & 127;
+        const Stream st = u ? st1 : st0;
+        const int R = R0 + (PAIR ? 128 * u : 0) + r;
         const int pos = s.base + R / a.G;
         const bool have = R < rows, live = have && pos >= 0 && pos < s.n;
         {
@@ -117,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         float m = -INFINITY, l = 0.f;
         int done = 0;
         bool ok = true;
-        for (int i = next(u, -1); i < kt.count; i = next(u, i)) {
+        for (int i = st.begin(); i <= st.upto; i = st.next(i)) {
             const int key0 = kt.key(i, 128), vslot = (2 * i + 1) % S;
             const uint32_t vpar = ((2 * i + 1) / S) & 1;
             if (!warp_wait(smem_u32(&s_full[u]), done & 1, stop)) { ok = false; break; }
@@ -134,8 +160,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
 #pragma unroll
             for (int g = 0; g < 4; ++g) settled32(x + 32 * g);
             const int far = key0 + 127;
-            if (!(far <= u_lo[u] + a.right && far < s.n && u_lo[u] == s.base + (R - r) / a.G && u_hi[u] == s.base + (min(R - r + 128, rows) - 1) / a.G &&
-                  (key0 >= u_hi[u] - a.left || far < a.sinks) && there == 0xff)) {
+            if (!(far <= st.lo + a.right && far < s.n && st.lo == s.base + (R - r) / a.G && st.hi == s.base + (min(R - r + 128, rows) - 1) / a.G &&
+                  (key0 >= st.hi - a.left || far < a.sinks) && there == 0xff)) {
                 const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
@@ -325,46 +351,49 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         }
         if (!ok && lane == 0)                                              // copies in flight land before the memory goes away
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
-    } else if (warp == 9 && lane == 0) {
-        // ------------------------------------------------------------ products
+    } else if (warp == 9) {
+        // ------------------------------------------------------------ products: the warp in step, one lane issues
+        const bool leader = elect_one();
+        const uint64_t q_desc = desc_features(q_at), k_desc = desc_features(kv_at), v_desc = desc_rows(kv_at);
         bool ok = true;
         uint32_t scored = 0;                                               // slots whose keys one of two streams has used
-        int started[2] = {0, 0}, weighted[2] = {0, 0};
-        auto scores = [&](int u, int i) {
-            const int slot = (2 * i) % S;
-            if (!started[u]++ && !wait_or_stop(smem_u32(&q_full[PAIR ? u : 0]), 0, stop)) return false;
-            if (!wait_or_stop(smem_u32(&kv_full[slot]), ((2 * i) / S) & 1, stop)) return false;
+        uint32_t n0 = 0, n1 = 0;                                           // tiles whose values each stream has added
+        auto scores = [&](int u, int i, bool first_of_stream) {
+            const uint32_t item = 2 * i, slot = item % S;
+            if (first_of_stream && !warp_wait(smem_u32(&q_full[PAIR ? u : 0]), 0, stop)) return false;
+            if (!warp_wait(smem_u32(&kv_full[slot]), (item / S) & 1, stop)) return false;
             fence_after();
-            mma_dot<DM>(s_col + u * 128, q_at + (PAIR ? u : 0) * TILE, kv_at + slot * TILE, kPanel, IDESC_S);
-            mma_commit(smem_u32(&s_full[u]));
-            if (!PAIR || !need(1 - u, i) || (scored >> slot & 1)) {
-                scored &= ~(1u << slot);
-                mma_commit(smem_u32(&kv_empty[slot]));
-            } else {
-                scored |= 1u << slot;
+            const bool last = !PAIR || !(u ? st0 : st1).takes(i) || (scored >> slot & 1);
+            if (leader) {
+                mma_dot<DM>(s_col + u * 128, q_desc + (PAIR ? u : 0) * (TILE >> 4), k_desc + slot * (TILE >> 4), IDESC_S);
+                mma_commit(smem_u32(&s_full[u]));
+                if (last) mma_commit(smem_u32(&kv_empty[slot]));
             }
+            scored = last ? scored & ~(1u << slot) : scored | 1u << slot;
             return true;
         };
-        for (int u = 0; u < 2 && ok; ++u) {
-            const int i = next(u, -1);
-            if (i < kt.count) ok = scores(u, i);
-        }
-        for (int i = 0; i < kt.count && ok; ++i) {
-            for (int u = 0; u < 2 && ok; ++u) {
-                if (!need(u, i)) continue;
-                const int slot = (2 * i + 1) % S;
-                ok = wait_or_stop(smem_u32(&p_full[u]), weighted[u] & 1, stop) && wait_or_stop(smem_u32(&kv_full[slot]), ((2 * i + 1) / S) & 1, stop);
-                if (!ok) break;
-                fence_after();
-                mma_weighted<128>(o_col + u * DM, s_col + u * 128, kv_at + slot * TILE, IDESC_O, weighted[u]++ != 0);
-                if (!PAIR || u == 1 || !need(1, i)) mma_commit(smem_u32(&kv_empty[slot]));
-                const int nx = next(u, i);
-                if (nx < kt.count) ok = scores(u, nx);
-                else mma_commit(smem_u32(&o_full[u]));
+        auto weighted = [&](int u, int i, uint32_t& n) {
+            const Stream& st = u ? st1 : st0;
+            const uint32_t item = 2 * i + 1, slot = item % S;
+            if (!warp_wait(smem_u32(&p_full[u]), n & 1, stop) || !warp_wait(smem_u32(&kv_full[slot]), (item / S) & 1, stop)) return false;
+            fence_after();
+            const int nx = st.next(i);
+            if (leader) {
+                mma_weighted<128>(o_col + u * DM, s_col + u * 128, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
+                if (!PAIR || u == 1 || !st1.takes(i)) mma_commit(smem_u32(&kv_empty[slot]));
+                if (nx > st.upto) mma_commit(smem_u32(&o_full[u]));
             }
+            ++n;
+            return nx > st.upto || scores(u, nx, false);
+        };
+        if (st0.begin() <= st0.upto) ok = scores(0, st0.begin(), true);
+        if (ok && st1.begin() <= st1.upto) ok = scores(1, st1.begin(), true);
+        for (int i = 0; i < kt.count && ok; ++i) {
+            if (st0.takes(i)) ok = weighted(0, i, n0);
+            if (ok && st1.takes(i)) ok = weighted(1, i, n1);
         }
         if (!ok) {                                                         // products in flight end before tensor memory is freed
-            mma_commit(smem_u32(&drained));
+            if (leader) mma_commit(smem_u32(&drained));
             mbar_wait(smem_u32(&drained), 0, 1u << 14);
         }
     }

@@ -27,6 +27,14 @@ __host__ __device__ constexpr uint32_t instr_desc(bool bf16, int N, bool rows_b)
 }
 
 // ---------------------------------------------------------------- instructions (one thread)
+// The warp that issues products runs as a whole, and one elected lane does the issuing: what all lanes compute alike stays
+// in uniform registers, where the instructions want their descriptors.  As a branch of lane 0 alone the same code took
+// 84 cycles an instruction, more than the product itself (64).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
@@ -42,20 +50,18 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// Tile times tile: D[128, N] (+)= A[128 rows] . B[N rows]^T over DM features.
+// Tile times tile: D[128, 128] = A[128 rows] . B[128 rows]^T over DM features; desc_features of both.
 template <int DM>
-__device__ __forceinline__ void mma_dot(uint32_t d, uint32_t a, uint32_t b, uint32_t b_panel, uint32_t idesc) {
+__device__ __forceinline__ void mma_dot(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
-    for (int k = 0; k < DM / 16; ++k) {
-        const uint32_t off = (k & 3) * 32;
-        mma_ss(d, desc_features(a + (k >> 2) * kPanel + off), desc_features(b + (k >> 2) * b_panel + off), idesc, k != 0);
-    }
+    for (int k = 0; k < DM / 16; ++k)         // addresses stand in units of 16 bytes in a descriptor's lowest bits
+        mma_ss(d, a + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, b + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, idesc, k != 0);
 }
-// D[128, N] (+)= A[128, KEYS] in tensor memory (16-bit pairs) . B[KEYS rows, N].
+// D[128, N] (+)= A[128, KEYS] in tensor memory (16-bit pairs) . B[KEYS rows, N]; desc_rows of B.
 template <int KEYS>
-__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
 #pragma unroll
-    for (int k = 0; k < KEYS / 16; ++k) mma_ts(d, a + k * 8, desc_rows(b + k * 2048), idesc, add || k != 0);
+    for (int k = 0; k < KEYS / 16; ++k) mma_ts(d, a + k * 8, b + k * 128, idesc, add || k != 0);
 }
 
 // ---------------------------------------------------------------- tensor memory (whole warps)
