@@ -17,7 +17,7 @@
 namespace ca {
 namespace {
 
-constexpr int kThreads = 384;       // two warpgroups that compute, one that copies and issues; registers as in the forward
+constexpr int kThreads = 352;       // two warpgroups that compute, and warps that copy, issue products and fetch the rows' sums
 template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
 template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
 template <int DM> constexpr size_t kBwdSmem = (size_t)(2 + kSlots<DM>) * kTileBytes<DM> + 1024;
@@ -48,9 +48,9 @@ __device__ __forceinline__ float warp_max(float x) {
 }
 
 // A operand whose two halves of 64 contracted elements lie 64 columns apart.
-__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    mma_weighted<64>(d, a, b, idesc, add);
-    mma_weighted<64>(d, a + 64, b + 4 * 128, idesc, true);
+__device__ __forceinline__ void mma_halves(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    mma_weighted<64>(lead, d, a, b, idesc, add);
+    mma_weighted<64>(lead, d, a + 64, b + 4 * 128, idesc, true);
 }
 
 __device__ __forceinline__ void read64(uint32_t at, uint32_t* x) {
@@ -147,7 +147,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     const uint32_t tmem = tmem_slot, o_col = tmem + 384;
 
     if (warp < 8) {
-        more_registers<216>();
         const int u = warp >> 2, r = tid & 127, R = R0 + r, pos = R / a.G;
         const bool have = R < rows, live = have && pos < s.n;
         const int64_t stat = ((int64_t)s.b * a.Hkv + h) * rows + R;
@@ -265,10 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 for (int e = 0; e < 32; ++e) o[e] = 0;
             if (have) store32<T>(dst, o, f, u * (DM / 2) + c, a.D);
         }
-    } else {
-        fewer_registers<64>();
-    }
-    if (warp == 8 && lane == 0) {
+    } else if (warp == 8 && lane == 0) {
         bool ok = true;
         int issued = 0;
         for (; issued < 2 * kt.count; ++issued) {
@@ -283,23 +279,19 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         if (!ok)                                               // copies in flight land before the memory goes away
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
     } else if (warp == 9 && kt.count) {
-        const bool leader = elect_one();
+        const uint32_t lead = elect_one();
         const uint64_t q_desc = desc_features(base_at), dy_desc = desc_features(base_at + TILE), f_desc = desc_features(kv_at), r_desc = desc_rows(kv_at);
         auto products = [&](uint32_t i) {                      // scores and dP of tile i
             const uint32_t ks = (2 * i) % S, vs = (2 * i + 1) % S;
             if (!warp_wait(smem_u32(&kv_full[ks]), ((2 * i) / S) & 1, stop)) return false;
             fence_after();
-            if (leader) {
-                mma_dot<DM>(tmem, q_desc, f_desc + ks * (TILE >> 4), IDESC_S);
-                mma_commit(smem_u32(&s_full));
-            }
+            mma_dot<DM>(lead, tmem, q_desc, f_desc + ks * (TILE >> 4), IDESC_S);
+            mma_commit(lead, smem_u32(&s_full));
             if (!warp_wait(smem_u32(&kv_full[vs]), ((2 * i + 1) / S) & 1, stop)) return false;
             fence_after();
-            if (leader) {
-                mma_dot<DM>(tmem + 128 + (i & 1) * 128, dy_desc, f_desc + vs * (TILE >> 4), IDESC_S);
-                mma_commit(smem_u32(&dp_full[i & 1]));
-                mma_commit(smem_u32(&kv_empty[vs]));
-            }
+            mma_dot<DM>(lead, tmem + 128 + (i & 1) * 128, dy_desc, f_desc + vs * (TILE >> 4), IDESC_S);
+            mma_commit(lead, smem_u32(&dp_full[i & 1]));
+            mma_commit(lead, smem_u32(&kv_empty[vs]));
             return true;
         };
         const uint32_t count = kt.count;
@@ -313,12 +305,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             if (!ok) break;
             fence_after();
             const uint32_t ks = (2 * i) % S;
-            if (leader) {
-                mma_halves(o_col, tmem + 128 + (i & 1) * 128, r_desc + ks * (TILE >> 4), IDESC_O, i != 0);
-                mma_commit(smem_u32(&kv_empty[ks]));
-            }
+            mma_halves(lead, o_col, tmem + 128 + (i & 1) * 128, r_desc + ks * (TILE >> 4), IDESC_O, i != 0);
+            mma_commit(lead, smem_u32(&kv_empty[ks]));
         }
-        if (leader) mma_commit(smem_u32(ok ? &o_full : &drained));
+        mma_commit(lead, smem_u32(ok ? &o_full : &drained));
         if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
     }
     __syncwarp();
@@ -393,7 +383,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     }
 
     if (warp < 8) {
-        more_registers<216>();
         const int u = warp >> 2, r = tid & 127, j = k0 + r;
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
         const uint32_t S_at = tmem + 64 * u + lane_off, dp_at = S_at + 128;
@@ -491,10 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 store32<T>(dst, o, f, c, a.D);
             }
         }
-    } else {
-        fewer_registers<64>();
-    }
-    if (warp == 8 && lane == 0 && count) {
+    } else if (warp == 8 && lane == 0 && count) {
         bool ok = true;
         int issued = 0;
         mbar_arrive_expect_tx(smem_u32(&kv_full), 2 * TILE);
@@ -517,27 +503,23 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&q_full[i % S]), (i / S) & 1, 1u << 12);
         }
     } else if (warp == 9 && count) {
-        const bool leader = elect_one();
+        const uint32_t lead = elect_one();
         const uint64_t k_desc = desc_features(base_at), v_desc = desc_features(base_at + TILE), f_desc = desc_features(ring_at), r_desc = desc_rows(ring_at);
         const uint32_t steps = count;
         auto scores = [&](uint32_t i) {
             const uint32_t qs = (2 * i) % S;
             if (!warp_wait(smem_u32(&q_full[qs]), ((2 * i) / S) & 1, stop)) return false;
             fence_after();
-            if (leader) {
-                mma_dot<DM>(tmem, k_desc, f_desc + qs * (TILE >> 4), IDESC_S);
-                mma_commit(smem_u32(&s_full));
-            }
+            mma_dot<DM>(lead, tmem, k_desc, f_desc + qs * (TILE >> 4), IDESC_S);
+            mma_commit(lead, smem_u32(&s_full));
             return true;
         };
         auto dprobs = [&](uint32_t i) {
             const uint32_t ds = (2 * i + 1) % S;
             if (!warp_wait(smem_u32(&q_full[ds]), ((2 * i + 1) / S) & 1, stop)) return false;
             fence_after();
-            if (leader) {
-                mma_dot<DM>(tmem + 128, v_desc, f_desc + ds * (TILE >> 4), IDESC_S);
-                mma_commit(smem_u32(&dp_full));
-            }
+            mma_dot<DM>(lead, tmem + 128, v_desc, f_desc + ds * (TILE >> 4), IDESC_S);
+            mma_commit(lead, smem_u32(&dp_full));
             return true;
         };
         bool ok = warp_wait(smem_u32(&kv_full), 0, stop) && scores(0) && dprobs(0);
@@ -545,20 +527,16 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             const uint32_t qs = (2 * i) % S, ds = (2 * i + 1) % S;
             if (!(ok = warp_wait(smem_u32(&p_full), i & 1, stop))) break;
             fence_after();
-            if (leader) {
-                mma_halves(dv_col, tmem, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
-                mma_commit(smem_u32(&q_empty[ds]));
-            }
+            mma_halves(lead, dv_col, tmem, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
+            mma_commit(lead, smem_u32(&q_empty[ds]));
             if (i + 1 < steps && !(ok = scores(i + 1))) break;
             if (!(ok = warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
             fence_after();
-            if (leader) {
-                mma_halves(dk_col, tmem + 128, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
-                mma_commit(smem_u32(&q_empty[qs]));
-            }
+            mma_halves(lead, dk_col, tmem + 128, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
+            mma_commit(lead, smem_u32(&q_empty[qs]));
             if (i + 1 < steps) ok = dprobs(i + 1);
         }
-        if (leader) mma_commit(smem_u32(ok ? &o_full : &drained));
+        mma_commit(lead, smem_u32(ok ? &o_full : &drained));
         if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
     } else if (warp == 10) {
         // minus the rows' sums, and minus their delta, with the factors of half precision

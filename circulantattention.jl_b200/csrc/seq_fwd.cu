@@ -14,12 +14,13 @@
 // 2^8, and the products and sums are held in Float32.
 #include "seq_umma.cuh"
 
+#include <limits.h>
+
 namespace ca {
 namespace {
 
-// Two warpgroups of softmax, one whose first warp copies and whose second issues the products.  384 threads are launched with
-// 168 registers each: 64512, of which 2 x 128 x 216 + 128 x 64 = 63488 are used.
-constexpr int kThreads = 384, kSoftmaxWarps = 8;
+// Two warpgroups of softmax, a warp that copies and one that issues the products.
+constexpr int kThreads = 320, kSoftmaxWarps = 8;
 
 template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
 template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
@@ -123,7 +124,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
 
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax: thread = row
-        more_registers<216>();
         const int u = warp >> 2, r = tid & 127;
         const Stream st = u ? st1 : st0;
         const int R = R0 + (PAIR ? 128 * u : 0) + r;
@@ -140,6 +140,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         const uint32_t S_at = s_col + u * 128 + lane_off, O_at = o_col + u * DM + lane_off;
         const float sl2 = a.mag_log2;
         const int c_lo = p_lo - a.left, c_hi = min(p_hi + a.right, s.n - 1);   // keys that any row of the CTA sees (or < sinks)
+        // tiles from in_lo (or below in_sink) to in_hi need no mask
+        const bool whole = st.lo == s.base + (R - r) / a.G && st.hi == s.base + (min(R - r + 128, rows) - 1) / a.G;
+        const int in_hi = whole ? min(st.lo + a.right, s.n - 1) - 127 : INT_MIN, in_lo = st.hi - a.left, in_sink = a.sinks - 127;
         float m = -INFINITY, l = 0.f;
         int done = 0;
         bool ok = true;
@@ -148,49 +151,58 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             const uint32_t vpar = ((2 * i + 1) / S) & 1;
             if (!warp_wait(smem_u32(&s_full[u]), done & 1, stop)) { ok = false; break; }
             fence_after();
-            uint32_t x[128];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) tmem_ld32(S_at + 32 * g, x + 32 * g);
             uint32_t there = 0xff;
             if (PAGED) {                                                   // which pages exist is known when their copy has landed
                 if (!warp_wait(smem_u32(&kv_full[vslot]), vpar, stop)) { ok = false; break; }
                 there = *(volatile uint32_t*)&valid[vslot];
             }
-            tmem_wait_ld();
-#pragma unroll
-            for (int g = 0; g < 4; ++g) settled32(x + 32 * g);
             const int far = key0 + 127;
-            if (!(far <= st.lo + a.right && far < s.n && st.lo == s.base + (R - r) / a.G && st.hi == s.base + (min(R - r + 128, rows) - 1) / a.G &&
-                  (key0 >= st.hi - a.left || far < a.sinks) && there == 0xff)) {
-                const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
+            const bool edge = !(key0 <= in_hi && (key0 >= in_lo || key0 < in_sink) && there == 0xff);
+            const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
+            // the columns 64 g .. 64 g + 63 of the scores, -inf where the row does not see the key
+            auto scores = [&](int g, uint32_t* x) {
+                tmem_ld32(S_at + 64 * g, x);
+                tmem_ld32(S_at + 64 * g + 32, x + 32);
+                tmem_wait_ld();
+                settled32(x);
+                settled32(x + 32);
+                if (edge) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint32_t mk = seen_bits(lo - 32 * g, hi - 32 * g, sk - 32 * g);
-                    if (PAGED) mk &= ((there >> (2 * g)) & 1 ? 0xffffu : 0u) | ((there >> (2 * g + 1)) & 1 ? 0xffff0000u : 0u);
+                    for (int q = 0; q < 2; ++q) {
+                        const int at = 64 * g + 32 * q;
+                        uint32_t mk = seen_bits(lo - at, hi - at, sk - at);
+                        if (PAGED) mk &= ((there >> (at / 16)) & 1 ? 0xffffu : 0u) | ((there >> (at / 16 + 1)) & 1 ? 0xffff0000u : 0u);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) x[32 * g + c] = (mk >> c) & 1 ? x[32 * g + c] : 0xff800000u;
+                        for (int c = 0; c < 32; ++c) x[32 * q + c] = (mk >> c) & 1 ? x[32 * q + c] : 0xff800000u;
+                    }
                 }
-            }
+            };
             // values that no row sees may be anything (a page that was freed, tokens behind the length): zeros
-            const bool all_used = (key0 >= c_lo || far < a.sinks) && far <= c_hi && there == 0xff;
-            if (!all_used) {
+            if (!((key0 >= c_lo || far < a.sinks) && far <= c_hi && there == 0xff)) {
                 if (!PAGED && !warp_wait(smem_u32(&kv_full[vslot]), vpar, stop)) { ok = false; break; }
                 const int j = key0 + r;
                 if (!(j <= c_hi && (j >= c_lo || j < a.sinks) && (there >> (r >> 4) & 1))) {
-#pragma unroll
+#pragma unroll 1
                     for (int p = 0; p < DM / 64; ++p)
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
-                            *reinterpret_cast<uint4*>(smem + (2 + vslot) * TILE + p * kPanel + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(smem + (2 + vslot) * TILE + p * kPanel + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                 }
                 fence_async_smem();
             }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int g = 0; g < 2; ++g) {
+                uint32_t x[64];
+                scores(g, x);
+                float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 128; c += 4)
+                for (int c = 0; c < 64; c += 8)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(x[c + e]));
-            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl2;
+                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]));
+                mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            }
+            mx *= sl2;
             float f = 1.f;
             const bool grew = mx > m + 8.f;                                // also from -inf
             if (grew) {
@@ -199,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             }
             if (done && __any_sync(~0u, grew)) {
                 // the scores came after the previous weighted sum, which is therefore complete
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < DM; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(O_at + c, o);
@@ -210,27 +222,27 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     tmem_st32(O_at + c, o);
                 }
             }
-            l *= f;
             const float ref = m == -INFINITY ? 0.f : m;                    // a row that has seen nothing yet
             const f32x2 sc2 = pack2(sl2, sl2), ref2 = pack2(-ref, -ref);
-            f32x2 sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-#pragma unroll
+            f32x2 sum2 = pack2(l * f, 0.f);
+#pragma unroll 1
             for (int g = 0; g < 2; ++g) {
-                uint32_t w[32];
+                uint32_t x[64], w[32];
+                scores(g, x);
 #pragma unroll
                 for (int c = 0; c < 32; ++c) {
                     float e0, e1;
-                    unpack2(fma2(pack2(__uint_as_float(x[64 * g + 2 * c]), __uint_as_float(x[64 * g + 2 * c + 1])), sc2, ref2), e0, e1);
+                    unpack2(fma2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), sc2, ref2), e0, e1);
                     e0 = fast_exp2(e0);
                     e1 = fast_exp2(e1);
-                    sum2[c & 1] = add2(sum2[c & 1], pack2(e0, e1));
+                    sum2 = add2(sum2, pack2(e0, e1));
                     w[c] = pack16<T>(e0, e1);
                 }
-                tmem_st32(S_at + 32 * g, w);
+                tmem_st32(S_at + 32 * g, w);                               // over scores that this warp has read twice
             }
             float a0, a1;
-            unpack2(add2(sum2[0], sum2[1]), a0, a1);
-            l += a0 + a1;
+            unpack2(sum2, a0, a1);
+            l = a0 + a1;
             tmem_wait_st();
             fence_before();
             __syncwarp();
@@ -249,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 merge_m[r] = m;
                 merge_l[r] = l;
                 if (done && ok) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < DM; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(O_at + c, o);
@@ -275,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             T* rest = !PAGED && a.rest.data ? seq_row<T>(a.rest, a, s, h, have ? R : R0) : nullptr;
             if (!PAGED && a.lse && have) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = l > 0.f ? m + log2f(l) : -INFINITY;
             const float w0 = f0 * inv, w1 = f1 * inv;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < DM; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(O_at + c, o);
@@ -303,10 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 }
             }
         }
-    } else {
-        fewer_registers<64>();
-    }
-    if (warp == 8) {
+    } else if (warp == 8) {
         // ------------------------------------------------------------ copies
         bool ok = true;
         int issued = 0;
@@ -353,47 +362,50 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
     } else if (warp == 9) {
         // ------------------------------------------------------------ products: the warp in step, one lane issues
-        const bool leader = elect_one();
+        const uint32_t lead = elect_one();
         const uint64_t q_desc = desc_features(q_at), k_desc = desc_features(kv_at), v_desc = desc_rows(kv_at);
         bool ok = true;
         uint32_t scored = 0;                                               // slots whose keys one of two streams has used
         uint32_t n0 = 0, n1 = 0;                                           // tiles whose values each stream has added
-        auto scores = [&](int u, int i, bool first_of_stream) {
-            const uint32_t item = 2 * i, slot = item % S;
-            if (first_of_stream && !warp_wait(smem_u32(&q_full[PAIR ? u : 0]), 0, stop)) return false;
-            if (!warp_wait(smem_u32(&kv_full[slot]), (item / S) & 1, stop)) return false;
-            fence_after();
+        auto landed = [&](uint32_t item) { return warp_wait(smem_u32(&kv_full[item % S]), (item / S) & 1, stop); };
+        auto scores = [&](int u, int i) {
+            const uint32_t slot = (2 * i) % S;
             const bool last = !PAIR || !(u ? st0 : st1).takes(i) || (scored >> slot & 1);
-            if (leader) {
-                mma_dot<DM>(s_col + u * 128, q_desc + (PAIR ? u : 0) * (TILE >> 4), k_desc + slot * (TILE >> 4), IDESC_S);
-                mma_commit(smem_u32(&s_full[u]));
-                if (last) mma_commit(smem_u32(&kv_empty[slot]));
-            }
+            mma_dot<DM>(lead, s_col + u * 128, q_desc + (PAIR ? u : 0) * (TILE >> 4), k_desc + slot * (TILE >> 4), IDESC_S);
+            mma_commit(lead, smem_u32(&s_full[u]));
+            if (last) mma_commit(lead, smem_u32(&kv_empty[slot]));
             scored = last ? scored & ~(1u << slot) : scored | 1u << slot;
-            return true;
         };
         auto weighted = [&](int u, int i, uint32_t& n) {
             const Stream& st = u ? st1 : st0;
-            const uint32_t item = 2 * i + 1, slot = item % S;
-            if (!warp_wait(smem_u32(&p_full[u]), n & 1, stop) || !warp_wait(smem_u32(&kv_full[slot]), (item / S) & 1, stop)) return false;
-            fence_after();
+            const uint32_t slot = (2 * i + 1) % S;
             const int nx = st.next(i);
-            if (leader) {
-                mma_weighted<128>(o_col + u * DM, s_col + u * 128, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
-                if (!PAIR || u == 1 || !st1.takes(i)) mma_commit(smem_u32(&kv_empty[slot]));
-                if (nx > st.upto) mma_commit(smem_u32(&o_full[u]));
-            }
+            // the weights are what is late: everything else is waited for first.  The next keys' slot was freed by products
+            // that came before (a stream is at most two tiles ahead, and the ring holds five).
+            if (!landed(2 * i + 1) || (nx <= st.upto && !landed(2 * nx)) || !warp_wait(smem_u32(&p_full[u]), n & 1, stop)) return false;
+            fence_after();
+            mma_weighted<128>(lead, o_col + u * DM, s_col + u * 128, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
+            if (!PAIR || u == 1 || !st1.takes(i)) mma_commit(lead, smem_u32(&kv_empty[slot]));
+            if (nx > st.upto) mma_commit(lead, smem_u32(&o_full[u]));
             ++n;
-            return nx > st.upto || scores(u, nx, false);
+            if (nx <= st.upto) scores(u, nx);
+            return true;
         };
-        if (st0.begin() <= st0.upto) ok = scores(0, st0.begin(), true);
-        if (ok && st1.begin() <= st1.upto) ok = scores(1, st1.begin(), true);
+        auto begin = [&](int u) {
+            const int i = (u ? st1 : st0).begin();
+            if (i > (u ? st1 : st0).upto) return true;
+            if (!warp_wait(smem_u32(&q_full[PAIR ? u : 0]), 0, stop) || !landed(2 * i)) return false;
+            fence_after();
+            scores(u, i);
+            return true;
+        };
+        ok = begin(0) && begin(1);
         for (int i = 0; i < kt.count && ok; ++i) {
             if (st0.takes(i)) ok = weighted(0, i, n0);
             if (ok && st1.takes(i)) ok = weighted(1, i, n1);
         }
         if (!ok) {                                                         // products in flight end before tensor memory is freed
-            if (leader) mma_commit(smem_u32(&drained));
+            mma_commit(lead, smem_u32(&drained));
             mbar_wait(smem_u32(&drained), 0, 1u << 14);
         }
     }

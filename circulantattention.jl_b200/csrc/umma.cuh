@@ -26,42 +26,43 @@ __host__ __device__ constexpr uint32_t instr_desc(bool bf16, int N, bool rows_b)
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (rows_b ? 1u << 16 : 0u) | (uint32_t)(N >> 3) << 17 | (128u >> 4) << 24;
 }
 
-// ---------------------------------------------------------------- instructions (one thread)
-// The warp that issues products runs as a whole, and one elected lane does the issuing: what all lanes compute alike stays
-// in uniform registers, where the instructions want their descriptors.  As a branch of lane 0 alone the same code took
-// 84 cycles an instruction, more than the product itself (64).
-__device__ __forceinline__ bool elect_one() {
+// ---------------------------------------------------------------- instructions (a warp in step, one lane issues)
+// The warp that issues products runs as a whole; `lead` is set in one elected lane and guards the instruction itself, not a
+// branch: control flow stays uniform, and descriptors are computed in the uniform registers that the instruction reads.
+// As a branch of one lane the same code took 56 to 104 cycles an instruction, more than the product itself (64).
+__device__ __forceinline__ uint32_t elect_one() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(lead) : "memory");
 }
-// The barrier gets one arrival when everything that this thread has issued so far is complete.
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The barrier gets one arrival when everything that the lane has issued so far is complete.
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
 
 // Tile times tile: D[128, 128] = A[128 rows] . B[128 rows]^T over DM features; desc_features of both.
 template <int DM>
-__device__ __forceinline__ void mma_dot(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_dot(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
 #pragma unroll
     for (int k = 0; k < DM / 16; ++k)         // addresses stand in units of 16 bytes in a descriptor's lowest bits
-        mma_ss(d, a + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, b + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, idesc, k != 0);
+        mma_ss(lead, d, a + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, b + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, idesc, k != 0);
 }
 // D[128, N] (+)= A[128, KEYS] in tensor memory (16-bit pairs) . B[KEYS rows, N]; desc_rows of B.
 template <int KEYS>
-__device__ __forceinline__ void mma_weighted(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_weighted(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
 #pragma unroll
-    for (int k = 0; k < KEYS / 16; ++k) mma_ts(d, a + k * 8, b + k * 128, idesc, add || k != 0);
+    for (int k = 0; k < KEYS / 16; ++k) mma_ts(lead, d, a + k * 8, b + k * 128, idesc, add || k != 0);
 }
 
 // ---------------------------------------------------------------- tensor memory (whole warps)
@@ -105,7 +106,8 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
 
 // ---------------------------------------------------------------- bounded waits of a CTA with several roles
 // A wait that runs out raises the CTA's flag, and every other wait of the CTA gives up when it sees it.
-__device__ __forceinline__ bool wait_or_stop(uint32_t bar, uint32_t parity, volatile int* stop) {
+// The loop stands outside the callers' code: inlined, a wait for a barrier that is long complete took 300 cycles, not 100.
+static __device__ __noinline__ bool keep_waiting(uint32_t bar, uint32_t parity, volatile int* stop) {
     for (int i = 0; i < 64; ++i) {
         if (mbar_wait(bar, parity, 1u << 14)) return true;
         if (*stop) return false;
@@ -113,18 +115,17 @@ __device__ __forceinline__ bool wait_or_stop(uint32_t bar, uint32_t parity, vola
     *stop = 1;
     return false;
 }
+__device__ __forceinline__ bool wait_or_stop(uint32_t bar, uint32_t parity, volatile int* stop) {
+    return mbar_wait(bar, parity, 1) || keep_waiting(bar, parity, stop);
+}
 // The same for a whole warp, which then goes on or gives up together.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop) {
-    return __all_sync(~0u, wait_or_stop(bar, parity, stop));
+    if (__all_sync(~0u, mbar_wait(bar, parity, 1))) return true;
+    return __all_sync(~0u, keep_waiting(bar, parity, stop));
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-
-// Registers move from the warps that issue copies and products to those that compute; N is a multiple of 8, and the shares of
-// all warpgroups together stay within what the block was launched with.
-template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // ---------------------------------------------------------------- pairs of Float32
 typedef unsigned long long f32x2;
