@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     constexpr uint32_t TILE = kTileBytes<DM>;
     constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
     extern __shared__ char raw[];
-    __shared__ uint64_t kv_full[S], kv_empty[S], q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    __shared__ uint64_t kv_full[S], kv_empty[S], q_full[2], s_full[2], p_full[2][2], o_full[2], drained;
     __shared__ uint32_t tmem_slot, valid[S];
     __shared__ int stop_flag;
     __shared__ float merge_m[128], merge_l[128];
@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         for (int u = 0; u < 2; ++u) {
             mbar_init(&q_full[u], PAIR ? 4 : 8);
             mbar_init(&s_full[u], 1);
-            mbar_init(&p_full[u], 4);
+            mbar_init(&p_full[u][0], 4);
+            mbar_init(&p_full[u][1], 4);
             mbar_init(&o_full[u], 1);
         }
         mbar_init(&drained, 1);
@@ -239,14 +240,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     w[c] = pack16<T>(e0, e1);
                 }
                 tmem_st32(S_at + 32 * g, w);                               // over scores that this warp has read twice
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&p_full[u][g]));       // the product with the first half may start
             }
             float a0, a1;
             unpack2(sum2, a0, a1);
             l = a0 + a1;
-            tmem_wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&p_full[u]));
             ++done;
         }
         if (done && ok) ok = warp_wait(smem_u32(&o_full[u]), 0, stop);
@@ -367,7 +368,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         bool ok = true;
         uint32_t scored = 0;                                               // slots whose keys one of two streams has used
         uint32_t n0 = 0, n1 = 0;                                           // tiles whose values each stream has added
-        auto landed = [&](uint32_t item) { return warp_wait(smem_u32(&kv_full[item % S]), (item / S) & 1, stop); };
+        int have = -1;                                                     // keys and values land in order: each is waited for once
+        auto landed = [&](int item) {
+            while (have < item) {
+                ++have;
+                if (!warp_wait(smem_u32(&kv_full[(uint32_t)have % S]), ((uint32_t)have / S) & 1, stop)) return false;
+            }
+            return true;
+        };
         auto scores = [&](int u, int i) {
             const uint32_t slot = (2 * i) % S;
             const bool last = !PAIR || !(u ? st0 : st1).takes(i) || (scored >> slot & 1);
@@ -382,9 +390,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             const int nx = st.next(i);
             // the weights are what is late: everything else is waited for first.  The next keys' slot was freed by products
             // that came before (a stream is at most two tiles ahead, and the ring holds five).
-            if (!landed(2 * i + 1) || (nx <= st.upto && !landed(2 * nx)) || !warp_wait(smem_u32(&p_full[u]), n & 1, stop)) return false;
+            if (!landed(nx <= st.upto ? 2 * nx : 2 * i + 1) || !warp_wait(smem_u32(&p_full[u][0]), n & 1, stop)) return false;
             fence_after();
-            mma_weighted<128>(lead, o_col + u * DM, s_col + u * 128, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
+            mma_weighted<64>(lead, o_col + u * DM, s_col + u * 128, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
+            if (!warp_wait(smem_u32(&p_full[u][1]), n & 1, stop)) return false;
+            fence_after();
+            mma_weighted<64>(lead, o_col + u * DM, s_col + u * 128 + 32, v_desc + slot * (TILE >> 4) + 4 * 128, IDESC_O, true);
             if (!PAIR || u == 1 || !st1.takes(i)) mma_commit(lead, smem_u32(&kv_empty[slot]));
             if (nx > st.upto) mma_commit(lead, smem_u32(&o_full[u]));
             ++n;
