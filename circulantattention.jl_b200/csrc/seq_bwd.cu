@@ -61,18 +61,6 @@ __device__ __forceinline__ void read64(uint32_t at, uint32_t* x) {
     settled32(x + 32);
 }
 
-template <typename T>
-__device__ __forceinline__ void store32(T* dst, const uint32_t* o, float f, int first, int D) {
-#pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-        if (first + e >= D) continue;
-        float y[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(o[e + k]) * f;
-        *reinterpret_cast<uint4*>(dst + first + e) = make_uint4(pack16<T>(y[0], y[1]), pack16<T>(y[2], y[3]), pack16<T>(y[4], y[5]), pack16<T>(y[6], y[7]));
-    }
-}
-
 template <int DM>
 __device__ __forceinline__ void clear_row(char* tile, int r) {
 #pragma unroll
@@ -129,6 +117,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     const int p_hi = min(s.n - 1, f_hi);
     const KeyTiles kt = key_tiles(a, s, f_lo, f_hi, 128);
 
+    if (warp == 8 && lane == 0) {
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
+    }
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
         mbar_init(&q_full, 8);
@@ -150,45 +142,54 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         const int u = warp >> 2, r = tid & 127, R = R0 + r, pos = R / a.G;
         const bool have = R < rows, live = have && pos < s.n;
         const int64_t stat = ((int64_t)s.b * a.Hkv + h) * rows + R;
-        stage_row<T, DM>(smem, r, live ? seq_row<T>(a.q, a, s, h, R) : nullptr, a.D, u, 2, false);
-        const T* dyr = live ? seq_row<T>(a.dy, a, s, h, R) : nullptr;
-        stage_row<T, DM>(smem + TILE, r, dyr, a.D, u, 2, false);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&q_full));
-        float d = 0.f, peak = 0.f;
-        if (live) {
-            const T* yr = seq_row<T>(a.y, a, s, h, R);
-            const T* rr = a.rest.data ? seq_row<T>(a.rest, a, s, h, R) : nullptr;
-#pragma unroll 2
-            for (int c = u * 8; c < a.D; c += 16) {
-                const uint4 w = *reinterpret_cast<const uint4*>(dyr + c), y = *reinterpret_cast<const uint4*>(yr + c);
-                const uint4 e = rr ? *reinterpret_cast<const uint4*>(rr + c) : make_uint4(0, 0, 0, 0);
-                const uint32_t *pw = &w.x, *py = &y.x, *pe = &e.x;
+        float delta, c = 1.f;
+        {
+            typedef TileCopy<DM, 256> C;
+            auto row = [&](const ca_seq_view& v) {
+                return [&](int rr) -> const T* { return R0 + rr < rows && (R0 + rr) / a.G < s.n ? seq_row<T>(v, a, s, h, R0 + rr) : nullptr; };
+            };
+            uint4 w[C::kCount], y[C::kCount], e[C::kCount];
+            fetch_tile<T, DM, 256>(y, row(a.q), a.D, tid);
+            fetch_tile<T, DM, 256>(w, row(a.dy), a.D, tid);
+            put_tile<DM, 256>(smem, y, tid);
+            put_tile<DM, 256>(smem + TILE, w, tid);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&q_full));
+            fetch_tile<T, DM, 256>(y, row(a.y), a.D, tid);
+            if (a.rest.data) fetch_tile<T, DM, 256>(e, row(a.rest), a.D, tid);
+#pragma unroll
+            for (int i = 0; i < C::kCount; ++i) {
+                if (!a.rest.data) e[i] = make_uint4(0, 0, 0, 0);
+                const uint32_t *pw = &w[i].x, *py = &y[i].x, *pe = &e[i].x;
+                float d = 0.f, peak = 0.f;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     d = fmaf(low16<T>(pw[k]), low16<T>(py[k]) + low16<T>(pe[k]), d);
                     d = fmaf(high16<T>(pw[k]), high16<T>(py[k]) + high16<T>(pe[k]), d);
                     if (!kIsBf16<T>) peak = fmaxf(peak, fmaxf(fabsf(low16<T>(pw[k])), fabsf(high16<T>(pw[k]))));
                 }
+#pragma unroll
+                for (int o = C::kPieces / 2; o; o >>= 1) {
+                    d += __shfl_xor_sync(~0u, d, o);
+                    if (!kIsBf16<T>) peak = fmaxf(peak, __shfl_xor_sync(~0u, peak, o));
+                }
+                if (C::piece(tid) == 0) {
+                    part[0][C::row(tid, i)] = d;
+                    part[1][C::row(tid, i)] = peak;
+                }
             }
-        }
-        part[u][r] = d;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float delta = part[0][r] + part[1][r];
-        if (u == 0 && have) a.delta[stat] = delta;
-        float c = 1.f;
-        if (!kIsBf16<T>) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            part[u][r] = peak;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            peak = fmaxf(part[0][r], part[1][r]);
-            const float* p = maps.v_peak + ((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128);
-            float v_peak = 0.f;
-            for (int i = lane; i < kt.count; i += 32) v_peak = fmaxf(v_peak, p[kt.key(i, 128) / 128]);
-            c = ds_factor(peak, warp_max(v_peak));
-            peak = warp_max(peak);
-            if (u == 0 && lane == 0) warp_peak[warp] = peak;
+            group_sync<256>(1);
+            delta = part[0][r];
+            if (u == 0 && have) a.delta[stat] = delta;
+            if (!kIsBf16<T>) {
+                float peak = part[1][r], v_peak = 0.f;
+                const float* p = maps.v_peak + ((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128);
+                for (int i = lane; i < kt.count; i += 32) v_peak = fmaxf(v_peak, p[kt.key(i, 128) / 128]);
+                c = ds_factor(peak, warp_max(v_peak));
+                peak = warp_max(peak);
+                if (u == 0 && lane == 0) warp_peak[warp] = peak;
+            }
         }
         const float lse = live ? a.lse[stat] : 0.f;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta * c, -delta * c), c2 = pack2(c, c);
@@ -248,22 +249,23 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         fence_after();
         const float f = !ok || *stop ? __int_as_float(0x7fffffff) : a.scale / c;
         if (!kIsBf16<T>) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            group_sync<256>(1);
             if (tid == 0)
                 maps.dy_peak[((int64_t)s.b * a.Hkv + h) * gridDim.x + R0 / 128] = fmaxf(fmaxf(warp_peak[0], warp_peak[1]), fmaxf(warp_peak[2], warp_peak[3]));
         }
-        T* dst = seq_row<T>(a.dq, a, s, h, have ? R : R0);
-#pragma unroll
-        for (int c = 0; c < DM / 2; c += 32) {
+#pragma unroll 1
+        for (int col = u * (DM / 2); col < (u + 1) * (DM / 2); col += 32) {
             uint32_t o[32];
-            tmem_ld32(o_col + lane_off + u * (DM / 2) + c, o);
+            tmem_ld32(o_col + lane_off + col, o);
             tmem_wait_ld();
             settled32(o);
-            if (!kt.count)
+            float y[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0;
-            if (have) store32<T>(dst, o, f, u * (DM / 2) + c, a.D);
+            for (int e = 0; e < 32; ++e) y[e] = kt.count ? __uint_as_float(o[e]) * f : 0.f * f;
+            put_row32<T>(smem, r, col, y);                         // the queries' place: their last scores are done
         }
+        group_sync<256>(1);
+        store_tile<T, DM, 256>(smem, [&](int rr) -> T* { return R0 + rr < rows ? seq_row<T>(a.dq, a, s, h, R0 + rr) : nullptr; }, a.D, tid);
     } else if (warp == 8 && lane == 0) {
         bool ok = true;
         int issued = 0;
@@ -353,6 +355,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     const int first = split ? (int)((int64_t)all * seg / maps.segments) : 0;
     const int count = (split ? (int)((int64_t)all * (seg + 1) / maps.segments) : all) - first;
 
+    if (warp == 8 && lane == 0) {
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
+        prefetch_map(&maps.q);
+        prefetch_map(&maps.dy);
+    }
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
         mbar_init(&kv_full, 1);
@@ -462,23 +470,27 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         fence_after();
         const float f = !ok || *stop ? __int_as_float(0x7fffffff) : u ? a.scale / c : kIsBf16<T> ? 1.f : 1.f / kPScale;       // the first warpgroup stores dv, the second dk
         const ca_seq_view& out = u ? a.dk : a.dv;
-        T* dst = (T*)out.data + h * out.head + (int64_t)min(j, a.N - 1) * out.token + s.b * out.batch;
         float* part = maps.partial + (((((int64_t)s.b * a.Hkv + h) * maps.split_tiles + tile) * maps.segments + seg) * 2 + 1 - u) * (DM * 128) + r;
-#pragma unroll
-        for (int c = 0; c < DM; c += 32) {
+        char* const stage = smem + u * TILE;                       // the keys' and values' place
+#pragma unroll 1
+        for (int col = 0; col < DM; col += 32) {
             uint32_t o[32];
-            tmem_ld32((u ? dk_col : dv_col) + lane_off + c, o);
+            tmem_ld32((u ? dk_col : dv_col) + lane_off + col, o);
             tmem_wait_ld();
             settled32(o);
-            if (!count)
+            float y[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0;
+            for (int e = 0; e < 32; ++e) y[e] = count ? __uint_as_float(o[e]) * f : 0.f * f;
             if (split) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) part[(c + e) * 128] = __uint_as_float(o[e]) * f;
-            } else if (j < a.N) {
-                store32<T>(dst, o, f, c, a.D);
+                for (int e = 0; e < 32; ++e) part[(col + e) * 128] = y[e];
+            } else {
+                put_row32<T>(stage, r, col, y);
             }
+        }
+        if (!split) {
+            group_sync<128>(2 + u);
+            store_tile<T, DM, 128>(stage, [&](int rr) -> T* { return k0 + rr < a.N ? (T*)out.data + h * out.head + (int64_t)(k0 + rr) * out.token + s.b * out.batch : nullptr; }, a.D, r);
         }
     } else if (warp == 8 && lane == 0 && count) {
         bool ok = true;

@@ -103,6 +103,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     // Which key tiles a stream takes: with PAIR both see nearly the same, but each leaves out what all of its rows are blind to.
     const Stream st0 = stream_of<PAIR>(a, s, kt, 0, R0, rows), st1 = stream_of<PAIR>(a, s, kt, 1, PAIR ? R0 + 128 : R0, rows);
 
+    if (warp == 8 && lane == 0) {
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
+    }
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
         for (int u = 0; u < 2; ++u) {
@@ -131,8 +135,18 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         const int pos = s.base + R / a.G;
         const bool have = R < rows, live = have && pos >= 0 && pos < s.n;
         {
-            const T* src = live ? seq_row<T>(a.q, a, s, h, R) : nullptr;
-            stage_row<T, DM>(smem + (PAIR ? u : 0) * TILE, r, src, a.D, PAIR ? 0 : u, PAIR ? 1 : 2, a.scale < 0.f);
+            const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;        // scores use the scale's magnitude
+            auto row = [&](int rr) -> const T* {
+                const int Rr = R - r + rr, p = s.base + Rr / a.G;
+                return Rr < rows && p >= 0 && p < s.n ? seq_row<T>(a.q, a, s, h, Rr) : nullptr;
+            };
+            constexpr int THREADS = PAIR ? 128 : 256;
+            const int t = PAIR ? r : tid;
+            uint4 w[TileCopy<DM, THREADS>::kCount];
+            fetch_tile<T, DM, THREADS>(w, row, a.D, t);
+#pragma unroll
+            for (int i = 0; i < TileCopy<DM, THREADS>::kCount; ++i) { w[i].x ^= sign; w[i].y ^= sign; w[i].z ^= sign; w[i].w ^= sign; }
+            put_tile<DM, THREADS>(smem + (PAIR ? u : 0) * TILE, w, t);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&q_full[PAIR ? u : 0]));
@@ -284,36 +298,29 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             inv = l > 0.f ? 1.f / l : 0.f;
             if (!ok || *stop) inv = __int_as_float(0x7fffffff);            // a wait ran out: NaN, never a wrong number
             const bool both = !PAIR && kt.count > 1;
-            T* dst = seq_row<T>(a.y, a, s, h, have ? R : R0);
-            T* rest = !PAGED && a.rest.data ? seq_row<T>(a.rest, a, s, h, have ? R : R0) : nullptr;
             if (!PAGED && a.lse && have) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = l > 0.f ? m + log2f(l) : -INFINITY;
             const float w0 = f0 * inv, w1 = f1 * inv;
+            char* const out = smem + (PAIR ? u : 0) * TILE;                // the queries' place: their last scores are done
+            for (int pass = 0; pass < (!PAGED && a.rest.data ? 2 : 1); ++pass) {
+                if (pass) group_sync<128>(2 + u);
 #pragma unroll 1
-            for (int c = 0; c < DM; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(O_at + c, o);
-                tmem_wait_ld();
-                settled32(o);
-                float y[32];
+                for (int c = 0; c < DM; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(O_at + c, o);
+                    tmem_wait_ld();
+                    settled32(o);
+                    float y[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    y[e] = done ? __uint_as_float(o[e]) * w0 : 0.f * inv;
-                    if (both) y[e] = fmaf(other[(c + e) * 128 + r], w1, y[e]);
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    if (c + e >= a.D || !have) continue;
-                    uint4 w = make_uint4(pack16<T>(y[e], y[e + 1]), pack16<T>(y[e + 2], y[e + 3]), pack16<T>(y[e + 4], y[e + 5]), pack16<T>(y[e + 6], y[e + 7]));
-                    *reinterpret_cast<uint4*>(dst + c + e) = w;
-                    if (rest) {
-                        const uint32_t* ww = &w.x;
-                        uint4 q;
-                        uint32_t* qq = &q.x;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) qq[k] = pack16<T>(y[e + 2 * k] - low16<T>(ww[k]), y[e + 2 * k + 1] - high16<T>(ww[k]));
-                        *reinterpret_cast<uint4*>(rest + c + e) = q;
+                    for (int e = 0; e < 32; ++e) {
+                        y[e] = done ? __uint_as_float(o[e]) * w0 : 0.f * inv;
+                        if (both) y[e] = fmaf(other[(c + e) * 128 + r], w1, y[e]);
+                        if (pass) y[e] -= to_float(from_float<T>(y[e]));   // what rounding took
                     }
+                    put_row32<T>(out, r, c, y);
                 }
+                group_sync<128>(2 + u);
+                const ca_seq_view& view = pass ? a.rest : a.y;
+                store_tile<T, DM, 128>(out, [&](int rr) -> T* { return R - r + rr < rows ? seq_row<T>(view, a, s, h, R - r + rr) : nullptr; }, a.D, r);
             }
         }
     } else if (warp == 8) {

@@ -30,19 +30,57 @@ __device__ __forceinline__ void settled32(uint32_t* r) {
         asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-// One row of D elements into a swizzled tile of DM features, zeros behind D and where `src` is null; pieces from `first` on,
-// every `step`-th.  `flip`: the sign is turned.
-template <typename T, int DM>
-__device__ __forceinline__ void stage_row(char* tile, int r, const T* src, int D, int first, int step, bool flip) {
-    const uint32_t sign = flip ? 0x80008000u : 0u;
-#pragma unroll 8
-    for (int c = first; c < DM / 8; c += step) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (src && c * 8 < D) w = *reinterpret_cast<const uint4*>(src + c * 8);
-        w.x ^= sign; w.y ^= sign; w.z ^= sign; w.w ^= sign;
-        *reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = w;
+// Tiles between global and shared memory: consecutive threads take consecutive 16-byte pieces of a row, so that a warp covers
+// two to four whole rows at a time (a thread for each row would touch 32 lines an instruction: 4096 cycles a tile of 128 rows,
+// and three such tiles made the prologue of dq 10 us).  `row(r)`: address of row r, or null (zeros / not stored).
+template <int DM, int THREADS> struct TileCopy {
+    static constexpr int kPieces = DM / 8, kStep = THREADS / kPieces, kCount = 128 / kStep;
+    static __device__ __forceinline__ int piece(int tid) { return tid % kPieces; }
+    static __device__ __forceinline__ int row(int tid, int i) { return tid / kPieces + i * kStep; }
+    static __device__ __forceinline__ uint32_t at(int r, int c) { return (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+};
+
+template <typename T, int DM, int THREADS, typename Row>
+__device__ __forceinline__ void fetch_tile(uint4 (&w)[TileCopy<DM, THREADS>::kCount], Row row, int D, int tid) {
+    typedef TileCopy<DM, THREADS> C;
+    const int c = C::piece(tid);
+#pragma unroll
+    for (int i = 0; i < C::kCount; ++i) {
+        const T* src = row(C::row(tid, i));
+        w[i] = src && c * 8 < D ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
     }
 }
+template <int DM, int THREADS>
+__device__ __forceinline__ void put_tile(char* tile, const uint4 (&w)[TileCopy<DM, THREADS>::kCount], int tid) {
+    typedef TileCopy<DM, THREADS> C;
+#pragma unroll
+    for (int i = 0; i < C::kCount; ++i) *reinterpret_cast<uint4*>(tile + C::at(C::row(tid, i), C::piece(tid))) = w[i];
+}
+template <typename T, int DM, int THREADS, typename Row>
+__device__ __forceinline__ void store_tile(const char* tile, Row row, int D, int tid) {
+    typedef TileCopy<DM, THREADS> C;
+    const int c = C::piece(tid);
+#pragma unroll 4
+    for (int i = 0; i < C::kCount; ++i) {
+        const int r = C::row(tid, i);
+        T* dst = row(r);
+        if (dst && c * 8 < D) *reinterpret_cast<uint4*>(dst + c * 8) = *reinterpret_cast<const uint4*>(tile + C::at(r, c));
+    }
+}
+// 32 results of row r, columns first .. first + 31, into a tile that store_tile takes.
+template <typename T>
+__device__ __forceinline__ void put_row32(char* tile, int r, int first, const float* y) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+        const int c = (first + e) >> 3;
+        *reinterpret_cast<uint4*>(tile + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pack16<T>(y[e], y[e + 1]), pack16<T>(y[e + 2], y[e + 3]), pack16<T>(y[e + 4], y[e + 5]), pack16<T>(y[e + 6], y[e + 7]));
+    }
+}
+// All threads of one or two warpgroups (named barrier `id`); every one of them gets here on every path.
+template <int THREADS> __device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory"); }
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
 
 // Bits 0..31 of the columns c with lo <= c <= hi or c < sk, c <= hi.
 __device__ __forceinline__ uint32_t bits_upto(int h) { return h < 0 ? 0u : h >= 31 ? ~0u : (2u << h) - 1u; }
