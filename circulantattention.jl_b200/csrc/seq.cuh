@@ -27,6 +27,7 @@ int check_pages(const ca_pages* p, int tokens);
 // the query heads that share a key head share its tiles.
 struct SeqArgs {
     int D, Hq, Hkv, G;
+    uint32_t g_mul, g_shift;        // R / G = R * g_mul >> g_shift for 0 <= R < 2^31
     int N, B;                       // dense: tokens and batch; paged: packed tokens and 1
     int left, right, sinks;         // left: kNoLeft without a left end
     float scale, scale_log2;        // scale_log2 = scale * log2(e)
@@ -40,6 +41,9 @@ struct SeqArgs {
     int* status;
 };
 constexpr int kNoLeft = 1 << 30;
+
+// Token of row R.  A division by a number that the compiler does not know costs some forty instructions.
+__device__ __forceinline__ int token_of(const SeqArgs& a, int R) { return (int)((uint64_t)(uint32_t)R * a.g_mul >> a.g_shift); }
 
 // The sequence that a tile works on.
 struct Seq {

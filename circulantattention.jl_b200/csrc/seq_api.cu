@@ -57,6 +57,11 @@ static int fill(const ca_seq_desc* d, SeqArgs* a) {
         set_error("tokens=%d heads=%d/%d batch=%d exceed 2^31 rows per key head or the grid limit 65535", d->tokens, d->heads_q, d->heads_kv, d->batch);
         return CA_ERR_TOO_LARGE;
     }
+    // ceil(2^(31 + s) / G) with 2^s >= G: off by less than 2^s / 2^(31 + s) = 2^-31 of a unit per row, so the quotient is exact
+    int shift = 0;
+    while ((1LL << shift) < a->G) ++shift;
+    a->g_shift = 31 + shift;
+    a->g_mul = (uint32_t)(((1ULL << (31 + shift)) + a->G - 1) / a->G);
     a->D = d->dim; a->Hq = d->heads_q; a->Hkv = d->heads_kv;
     a->N = d->tokens; a->B = d->batch;
     a->left = d->left < 0 || d->left > kNoLeft ? kNoLeft : d->left;

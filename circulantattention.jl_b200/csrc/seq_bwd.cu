@@ -139,25 +139,26 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     const uint32_t tmem = tmem_slot, o_col = tmem + 384;
 
     if (warp < 8) {
-        const int u = warp >> 2, r = tid & 127, R = R0 + r, pos = R / a.G;
+        const int u = warp >> 2, r = tid & 127, R = R0 + r, pos = token_of(a, R);
         const bool have = R < rows, live = have && pos < s.n;
         const int64_t stat = ((int64_t)s.b * a.Hkv + h) * rows + R;
         float delta, c = 1.f;
         {
             typedef TileCopy<DM, 256> C;
             auto row = [&](const ca_seq_view& v) {
-                return [&](int rr) -> const T* { return R0 + rr < rows && (R0 + rr) / a.G < s.n ? seq_row<T>(v, a, s, h, R0 + rr) : nullptr; };
+                return [&](int rr) { return seq_row<T>(v, a, s, h, min(R0 + rr, rows - 1)); };
             };
+            const int to = (int)min((int64_t)rows, (int64_t)s.n * a.G) - R0;
             uint4 w[C::kCount], y[C::kCount], e[C::kCount];
-            fetch_tile<T, DM, 256>(y, row(a.q), a.D, tid);
-            fetch_tile<T, DM, 256>(w, row(a.dy), a.D, tid);
+            fetch_tile<T, DM, 256>(y, row(a.q), 0, to, a.D, tid);
+            fetch_tile<T, DM, 256>(w, row(a.dy), 0, to, a.D, tid);
             put_tile<DM, 256>(smem, y, tid);
             put_tile<DM, 256>(smem + TILE, w, tid);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&q_full));
-            fetch_tile<T, DM, 256>(y, row(a.y), a.D, tid);
-            if (a.rest.data) fetch_tile<T, DM, 256>(e, row(a.rest), a.D, tid);
+            fetch_tile<T, DM, 256>(y, row(a.y), 0, to, a.D, tid);
+            if (a.rest.data) fetch_tile<T, DM, 256>(e, row(a.rest), 0, to, a.D, tid);
 #pragma unroll
             for (int i = 0; i < C::kCount; ++i) {
                 if (!a.rest.data) e[i] = make_uint4(0, 0, 0, 0);
@@ -213,12 +214,15 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 x[c + 1] = __float_as_uint(fast_exp2(e1));
             }
             uint32_t mk[2] = {~0u, ~0u};
+            const bool ragged = far >= s.n;
             const bool edge = !(far <= f_lo + a.right && far < s.n && f_hi == p_hi && (key0 >= p_hi - a.left || far < a.sinks));
             if (edge) {
                 const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
 #pragma unroll
                 for (int g = 0; g < 2; ++g) mk[g] = seen_bits(lo - 64 * u - 32 * g, hi - 64 * u - 32 * g, sk - 64 * u - 32 * g);
-                if (far >= s.n && u == 0) {                    // keys behind the length may be anything: zeros
+#pragma unroll
+                for (int c = 0; c < 64; ++c) x[c] = (mk[c >> 5] >> (c & 31)) & 1 ? x[c] : 0u;
+                if (ragged && u == 0) {                        // keys behind the length may be anything: zeros
                     const int slot = (2 * i) % S;              // the scores are there, so the keys are
                     if (key0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
                     fence_async_smem();
@@ -233,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             for (int c = 0; c < 64; c += 2) {
                 float e0, e1;
                 unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, dl2), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e0, e1);
-                if (edge) {
+                if (ragged) {                                  // dP of such keys may be anything
                     e0 = (mk[c >> 5] >> (c & 31)) & 1 ? e0 : 0.f;
                     e1 = (mk[c >> 5] >> (c & 31)) & 2 ? e1 : 0.f;
                 }
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             put_row32<T>(smem, r, col, y);                         // the queries' place: their last scores are done
         }
         group_sync<256>(1);
-        store_tile<T, DM, 256>(smem, [&](int rr) -> T* { return R0 + rr < rows ? seq_row<T>(a.dq, a, s, h, R0 + rr) : nullptr; }, a.D, tid);
+        store_tile<T, DM, 256>(smem, [&](int rr) { return seq_row<T>(a.dq, a, s, h, R0 + rr); }, rows - R0, a.D, tid);
     } else if (warp == 8 && lane == 0) {
         bool ok = true;
         int issued = 0;
@@ -283,13 +287,18 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     } else if (warp == 9 && kt.count) {
         const uint32_t lead = elect_one();
         const uint64_t q_desc = desc_features(base_at), dy_desc = desc_features(base_at + TILE), f_desc = desc_features(kv_at), r_desc = desc_rows(kv_at);
+        uint32_t have = 0;                                     // keys and values land in order: each is waited for once
+        auto landed = [&](uint32_t items) {
+            for (; have < items; ++have)
+                if (!warp_wait(smem_u32(&kv_full[have % S]), (have / S) & 1, stop)) return false;
+            return true;
+        };
         auto products = [&](uint32_t i) {                      // scores and dP of tile i
             const uint32_t ks = (2 * i) % S, vs = (2 * i + 1) % S;
-            if (!warp_wait(smem_u32(&kv_full[ks]), ((2 * i) / S) & 1, stop)) return false;
             fence_after();
             mma_dot<DM>(lead, tmem, q_desc, f_desc + ks * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&s_full));
-            if (!warp_wait(smem_u32(&kv_full[vs]), ((2 * i + 1) / S) & 1, stop)) return false;
+            if (!landed(2 * i + 2)) return false;
             fence_after();
             mma_dot<DM>(lead, tmem + 128 + (i & 1) * 128, dy_desc, f_desc + vs * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&dp_full[i & 1]));
@@ -297,11 +306,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             return true;
         };
         const uint32_t count = kt.count;
-        bool ok = warp_wait(smem_u32(&q_full), 0, stop) && products(0);
+        bool ok = warp_wait(smem_u32(&q_full), 0, stop) && landed(1) && products(0);
         for (uint32_t i = 0; i < count && ok; ++i) {
             if (i + 1 < count) {
-                ok = warp_wait(smem_u32(&s_free), i & 1, stop) && products(i + 1);
-                if (!ok) break;
+                if (!(ok = landed(2 * i + 3) && warp_wait(smem_u32(&s_free), i & 1, stop) && products(i + 1))) break;
             }
             ok = warp_wait(smem_u32(&ds_full[i & 1]), (i >> 1) & 1, stop);
             if (!ok) break;
@@ -399,6 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         bool ok = true;
         for (int i = 0; i < count; ++i) {
             const int step = first + i, q0 = t_lo + step / a.G * 128, b = i & 1;
+            const bool ragged = q0 + 127 >= s.n || k0 + 127 >= s.n;
             const bool edge = !(k0 + 127 <= q0 + a.right && (q0 + 127 <= k0 + a.left || k0 + 127 < a.sinks) && q0 + 127 < s.n && k0 + 127 < s.n);
             if (!warp_wait(smem_u32(&st_full[b]), (i >> 1) & 1, stop) || !warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
             fence_after();
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 w[(c >> 1) + 1] = pack16<T>(e[2], e[3]);
             }
             tmem_st32(S_at, w);
-            if (q0 + 127 >= s.n) {                              // queries behind the length may be anything: zeros
+            if (ragged && q0 + 127 >= s.n) {                    // queries behind the length may be anything: zeros
                 const int slot = (2 * i + u) % S;               // one warpgroup clears q, the other dy
                 if (!warp_wait(smem_u32(&q_full[slot]), ((2 * i + u) / S) & 1, stop)) { ok = false; break; }
                 if (q0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
@@ -453,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 unpack2(mul2(fma2(pack2(__uint_as_float(y[c + 2]), __uint_as_float(y[c + 3])), c2, pack2(z.z, z.w)), pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3]))), e[2], e[3]);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (edge) e[k] = (mk[c >> 5] >> ((c & 31) + k)) & 1 ? e[k] : 0.f;
+                    if (ragged) e[k] = (mk[c >> 5] >> ((c & 31) + k)) & 1 ? e[k] : 0.f;    // dP of such pairs may be anything
                 w[c >> 1] = pack16<T>(e[0], e[1]);
                 w[(c >> 1) + 1] = pack16<T>(e[2], e[3]);
             }
@@ -490,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         }
         if (!split) {
             group_sync<128>(2 + u);
-            store_tile<T, DM, 128>(stage, [&](int rr) -> T* { return k0 + rr < a.N ? (T*)out.data + h * out.head + (int64_t)(k0 + rr) * out.token + s.b * out.batch : nullptr; }, a.D, r);
+            store_tile<T, DM, 128>(stage, [&](int rr) { return (T*)out.data + h * out.head + (int64_t)(k0 + rr) * out.token + s.b * out.batch; }, a.N - k0, a.D, r);
         }
     } else if (warp == 8 && lane == 0 && count) {
         bool ok = true;
@@ -518,35 +527,39 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         const uint32_t lead = elect_one();
         const uint64_t k_desc = desc_features(base_at), v_desc = desc_features(base_at + TILE), f_desc = desc_features(ring_at), r_desc = desc_rows(ring_at);
         const uint32_t steps = count;
-        auto scores = [&](uint32_t i) {
-            const uint32_t qs = (2 * i) % S;
-            if (!warp_wait(smem_u32(&q_full[qs]), ((2 * i) / S) & 1, stop)) return false;
-            fence_after();
-            mma_dot<DM>(lead, tmem, k_desc, f_desc + qs * (TILE >> 4), IDESC_S);
-            mma_commit(lead, smem_u32(&s_full));
+        uint32_t have = 0;                                     // queries and cotangents land in order: each is waited for once
+        auto landed = [&](uint32_t items) {
+            for (; have < items; ++have)
+                if (!warp_wait(smem_u32(&q_full[have % S]), (have / S) & 1, stop)) return false;
             return true;
+        };
+        auto scores = [&](uint32_t i) {
+            mma_dot<DM>(lead, tmem, k_desc, f_desc + (2 * i) % S * (TILE >> 4), IDESC_S);
+            mma_commit(lead, smem_u32(&s_full));
         };
         auto dprobs = [&](uint32_t i) {
-            const uint32_t ds = (2 * i + 1) % S;
-            if (!warp_wait(smem_u32(&q_full[ds]), ((2 * i + 1) / S) & 1, stop)) return false;
-            fence_after();
-            mma_dot<DM>(lead, tmem + 128, v_desc, f_desc + ds * (TILE >> 4), IDESC_S);
+            mma_dot<DM>(lead, tmem + 128, v_desc, f_desc + (2 * i + 1) % S * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&dp_full));
-            return true;
         };
-        bool ok = warp_wait(smem_u32(&kv_full), 0, stop) && scores(0) && dprobs(0);
+        bool ok = warp_wait(smem_u32(&kv_full), 0, stop) && landed(2);
+        fence_after();
+        if (ok) {
+            scores(0);
+            dprobs(0);
+        }
         for (uint32_t i = 0; i < steps && ok; ++i) {
             const uint32_t qs = (2 * i) % S, ds = (2 * i + 1) % S;
-            if (!(ok = warp_wait(smem_u32(&p_full), i & 1, stop))) break;
+            const bool more = i + 1 < steps;
+            if (!(ok = (!more || landed(2 * i + 3)) && warp_wait(smem_u32(&p_full), i & 1, stop))) break;
             fence_after();
             mma_halves(lead, dv_col, tmem, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&q_empty[ds]));
-            if (i + 1 < steps && !(ok = scores(i + 1))) break;
-            if (!(ok = warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
+            if (more) scores(i + 1);
+            if (!(ok = (!more || landed(2 * i + 4)) && warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
             fence_after();
             mma_halves(lead, dk_col, tmem + 128, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&q_empty[qs]));
-            if (i + 1 < steps) ok = dprobs(i + 1);
+            if (more) dprobs(i + 1);
         }
         mma_commit(lead, smem_u32(ok ? &o_full : &drained));
         if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed

@@ -132,18 +132,19 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         const int u = warp >> 2, r = tid & 127;
         const Stream st = u ? st1 : st0;
         const int R = R0 + (PAIR ? 128 * u : 0) + r;
-        const int pos = s.base + R / a.G;
+        const int pos = s.base + token_of(a, R);
         const bool have = R < rows, live = have && pos >= 0 && pos < s.n;
         {
             const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;        // scores use the scale's magnitude
-            auto row = [&](int rr) -> const T* {
-                const int Rr = R - r + rr, p = s.base + Rr / a.G;
-                return Rr < rows && p >= 0 && p < s.n ? seq_row<T>(a.q, a, s, h, Rr) : nullptr;
-            };
+            // rows of the tile that exist: those of positions 0 .. n - 1
+            const int tile0 = R - r;
+            const int from = (int)min((int64_t)128, max((int64_t)0, -(int64_t)s.base * a.G - tile0));
+            const int to = (int)min((int64_t)rows, ((int64_t)s.n - s.base) * a.G) - tile0;
+            auto row = [&](int rr) { return seq_row<T>(a.q, a, s, h, min(tile0 + rr, rows - 1)); };
             constexpr int THREADS = PAIR ? 128 : 256;
             const int t = PAIR ? r : tid;
             uint4 w[TileCopy<DM, THREADS>::kCount];
-            fetch_tile<T, DM, THREADS>(w, row, a.D, t);
+            fetch_tile<T, DM, THREADS>(w, row, from, to, a.D, t);
 #pragma unroll
             for (int i = 0; i < TileCopy<DM, THREADS>::kCount; ++i) { w[i].x ^= sign; w[i].y ^= sign; w[i].z ^= sign; w[i].w ^= sign; }
             put_tile<DM, THREADS>(smem + (PAIR ? u : 0) * TILE, w, t);
@@ -174,13 +175,16 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             const int far = key0 + 127;
             const bool edge = !(key0 <= in_hi && (key0 >= in_lo || key0 < in_sink) && there == 0xff);
             const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
-            // the columns 64 g .. 64 g + 63 of the scores, -inf where the row does not see the key
-            auto scores = [&](int g, uint32_t* x) {
+            auto scores = [&](int g, uint32_t* x) {                        // the columns 64 g .. 64 g + 63
                 tmem_ld32(S_at + 64 * g, x);
                 tmem_ld32(S_at + 64 * g + 32, x + 32);
                 tmem_wait_ld();
                 settled32(x);
                 settled32(x + 32);
+            };
+            // The same for the maximum: -inf where the row does not see the key, written back for the exponentials
+            auto masked_scores = [&](int g, uint32_t* x) {
+                scores(g, x);
                 if (edge) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
@@ -189,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                         if (PAGED) mk &= ((there >> (at / 16)) & 1 ? 0xffffu : 0u) | ((there >> (at / 16 + 1)) & 1 ? 0xffff0000u : 0u);
 #pragma unroll
                         for (int c = 0; c < 32; ++c) x[32 * q + c] = (mk >> c) & 1 ? x[32 * q + c] : 0xff800000u;
+                        tmem_st32(S_at + at, x + 32 * q);
                     }
                 }
             };
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
 #pragma unroll 1
             for (int g = 0; g < 2; ++g) {
                 uint32_t x[64];
-                scores(g, x);
+                masked_scores(g, x);
                 float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < 64; c += 8)
@@ -217,6 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     for (int e = 0; e < 4; ++e) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]));
                 mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             }
+            tmem_wait_st();
             mx *= sl2;
             float f = 1.f;
             const bool grew = mx > m + 8.f;                                // also from -inf
@@ -311,16 +317,24 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     settled32(o);
                     float y[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        y[e] = done ? __uint_as_float(o[e]) * w0 : 0.f * inv;
-                        if (both) y[e] = fmaf(other[(c + e) * 128 + r], w1, y[e]);
-                        if (pass) y[e] -= to_float(from_float<T>(y[e]));   // what rounding took
+                    for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * w0;
+                    if (!done) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y[e] = 0.f * inv;
+                    }
+                    if (both) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y[e] = fmaf(other[(c + e) * 128 + r], w1, y[e]);
+                    }
+                    if (pass) {                                            // what rounding took
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) y[e] -= to_float(from_float<T>(y[e]));
                     }
                     put_row32<T>(out, r, c, y);
                 }
                 group_sync<128>(2 + u);
                 const ca_seq_view& view = pass ? a.rest : a.y;
-                store_tile<T, DM, 128>(out, [&](int rr) -> T* { return R - r + rr < rows ? seq_row<T>(view, a, s, h, R - r + rr) : nullptr; }, a.D, r);
+                store_tile<T, DM, 128>(out, [&](int rr) { return seq_row<T>(view, a, s, h, max(R - r + rr, 0)); }, rows - (R - r), a.D, r);
             }
         }
     } else if (warp == 8) {

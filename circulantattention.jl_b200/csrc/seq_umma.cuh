@@ -32,7 +32,8 @@ __device__ __forceinline__ void settled32(uint32_t* r) {
 
 // Tiles between global and shared memory: consecutive threads take consecutive 16-byte pieces of a row, so that a warp covers
 // two to four whole rows at a time (a thread for each row would touch 32 lines an instruction: 4096 cycles a tile of 128 rows,
-// and three such tiles made the prologue of dq 10 us).  `row(r)`: address of row r, or null (zeros / not stored).
+// and three such tiles made the prologue of dq 10 us).  `row(r)`: address of row r.  Rows
+// from..to-1 exist; others are zeros, or not stored.  Addresses are computed without branches, so that they overlap.
 template <int DM, int THREADS> struct TileCopy {
     static constexpr int kPieces = DM / 8, kStep = THREADS / kPieces, kCount = 128 / kStep;
     static __device__ __forceinline__ int piece(int tid) { return tid % kPieces; }
@@ -41,13 +42,15 @@ template <int DM, int THREADS> struct TileCopy {
 };
 
 template <typename T, int DM, int THREADS, typename Row>
-__device__ __forceinline__ void fetch_tile(uint4 (&w)[TileCopy<DM, THREADS>::kCount], Row row, int D, int tid) {
+__device__ __forceinline__ void fetch_tile(uint4 (&w)[TileCopy<DM, THREADS>::kCount], Row row, int from, int to, int D, int tid) {
     typedef TileCopy<DM, THREADS> C;
     const int c = C::piece(tid);
 #pragma unroll
     for (int i = 0; i < C::kCount; ++i) {
-        const T* src = row(C::row(tid, i));
-        w[i] = src && c * 8 < D ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+        const int r = C::row(tid, i);
+        const T* src = row(min(max(r, from), max(to - 1, from)));
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (r >= from && r < to && c * 8 < D) w[i] = *reinterpret_cast<const uint4*>(src + c * 8);
     }
 }
 template <int DM, int THREADS>
@@ -57,14 +60,17 @@ __device__ __forceinline__ void put_tile(char* tile, const uint4 (&w)[TileCopy<D
     for (int i = 0; i < C::kCount; ++i) *reinterpret_cast<uint4*>(tile + C::at(C::row(tid, i), C::piece(tid))) = w[i];
 }
 template <typename T, int DM, int THREADS, typename Row>
-__device__ __forceinline__ void store_tile(const char* tile, Row row, int D, int tid) {
+__device__ __forceinline__ void store_tile(const char* tile, Row row, int to, int D, int tid) {
     typedef TileCopy<DM, THREADS> C;
     const int c = C::piece(tid);
-#pragma unroll 4
+    uint4 w[C::kCount];
+#pragma unroll
+    for (int i = 0; i < C::kCount; ++i) w[i] = *reinterpret_cast<const uint4*>(tile + C::at(C::row(tid, i), c));
+#pragma unroll
     for (int i = 0; i < C::kCount; ++i) {
         const int r = C::row(tid, i);
-        T* dst = row(r);
-        if (dst && c * 8 < D) *reinterpret_cast<uint4*>(dst + c * 8) = *reinterpret_cast<const uint4*>(tile + C::at(r, c));
+        T* dst = row(min(r, to - 1));
+        if (r < to && c * 8 < D) *reinterpret_cast<uint4*>(dst + c * 8) = w[i];
     }
 }
 // 32 results of row r, columns first .. first + 31, into a tile that store_tile takes.
@@ -89,7 +95,7 @@ __device__ __forceinline__ uint32_t seen_bits(int lo, int hi, int sk) { return b
 
 template <typename T>
 __device__ __forceinline__ T* seq_row(const ca_seq_view& v, const SeqArgs& a, const Seq& s, int h, int R) {
-    const int t = R / a.G, g = R - t * a.G;
+    const int t = token_of(a, R), g = R - t * a.G;
     return (T*)v.data + (h * a.G + g) * v.head + (int64_t)(s.t0 + t) * v.token + (a.pages.table ? 0 : s.b * v.batch);
 }
 
