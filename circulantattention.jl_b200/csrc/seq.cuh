@@ -136,8 +136,8 @@ __device__ __forceinline__ int page_of(const SeqArgs& a, int b, int j) {
 }
 
 // seq_fma.cu: Float32 on the FMA pipe
-int fma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st);
-int fma_window_bwd(const SeqArgs& a, int dtype, cudaStream_t st);
-int fma_paged(const SeqArgs& a, int dtype, cudaStream_t st);
+int fma_fwd(const SeqArgs& a, cudaStream_t st);               // dense or paged
+size_t fma_bwd_parts(const SeqArgs& a);
+int fma_bwd(const SeqArgs& a, float* parts, cudaStream_t st);
 
 }  // namespace ca

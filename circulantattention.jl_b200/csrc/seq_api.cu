@@ -97,13 +97,13 @@ int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     if (y_rest) a.rest = *y_rest;
     a.lengths = lengths;
     a.lse = lse;
-    return d->dtype == CA_F32 ? fma_window_fwd(a, d->dtype, as_stream(stream)) : umma_window_fwd(a, d->dtype, as_stream(stream));
+    return d->dtype == CA_F32 ? fma_fwd(a, as_stream(stream)) : umma_window_fwd(a, d->dtype, as_stream(stream));
 }
 
 size_t ca_window_bwd_workspace(const ca_seq_desc* d) {
     SeqArgs a{};
     if (fill(d, &a)) return 0;
-    return delta_bytes(a) + (d->dtype == CA_F32 ? 0 : umma_bwd_parts(a));
+    return delta_bytes(a) + (d->dtype == CA_F32 ? fma_bwd_parts(a) : umma_bwd_parts(a));
 }
 
 int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
@@ -123,8 +123,8 @@ int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     a.lengths = lengths;
     a.lse = const_cast<float*>(lse);
     a.delta = static_cast<float*>(workspace);
-    if (d->dtype == CA_F32) return fma_window_bwd(a, d->dtype, as_stream(stream));
-    return umma_window_bwd(a, d->dtype, reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a)), as_stream(stream));
+    float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a));
+    return d->dtype == CA_F32 ? fma_bwd(a, parts, as_stream(stream)) : umma_window_bwd(a, d->dtype, parts, as_stream(stream));
 }
 
 int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_view* k_pages, const ca_page_view* v_pages,
@@ -141,7 +141,7 @@ int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_vi
     a.q = *q; a.y = *y;
     a.kp = *k_pages; a.vp = *v_pages;
     a.pages = *pages;
-    return d->dtype == CA_F32 ? fma_paged(a, d->dtype, as_stream(stream)) : umma_paged(a, d->dtype, as_stream(stream));
+    return d->dtype == CA_F32 ? fma_fwd(a, as_stream(stream)) : umma_paged(a, d->dtype, as_stream(stream));
 }
 
 }  // extern "C"

@@ -1,33 +1,41 @@
-// Attention on token sequences on the FMA pipe, in Float32.
+// Attention on token sequences in Float32, on the FMA pipe: dense tensors and a paged cache.
+//
+// The tensor cores round Float32 operands; pairs of rounded numbers would bring the products back, but their sums are cut
+// rather than rounded, which shows at the 1e-6 that Float32 users get here.  So every product is an FMA, two at a time
+// (fma.rn.f32x2).
 //
 // Tiles of 64 rows and 64 columns in shared memory, features fastest and rows padded by 4 floats, so that the 16-byte
 // reads of eight lanes (rows 1 apart) fall into different banks.  A thread (ty, tx) of 16 x 16 holds the products of rows
-// ty + 16i with columns tx + 16j (i, j < 4): 64 FMA for 8 reads of 16 bytes.
+// ty + 16i with columns tx + 16j (i, j < 4): 32 packed FMA for 8 reads of 16 bytes.  The next tile is copied (cp.async)
+// while this one is worked on.
+#include <algorithm>
+
 #include "seq.cuh"
+#include "umma.cuh"
 
 namespace ca {
 namespace {
 
 constexpr int kTile = 64, kThreads = 256, kPPitch = kTile + 4;
-
 template <int DM> constexpr int kPitch = DM + 4;
+template <int DM> constexpr int kTileFloats = kTile * kPitch<DM>;
 
-// One row of D elements -> Float32 in shared memory, zeros behind D and where `src` is null; four threads a row.
-template <typename T, int DM>
-__device__ __forceinline__ void load_row(float* dst, const T* src, int D, int part) {
-#pragma unroll 4
-    for (int f = part * 4; f < DM; f += 16) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (src && f < D) {
-            if (sizeof(T) == 4) {
-                x = *(const float4*)(src + f);
-            } else {
-                const uint2 w = *(const uint2*)(src + f);
-                const T* e = (const T*)&w;
-                x = make_float4(to_float(e[0]), to_float(e[1]), to_float(e[2]), to_float(e[3]));
-            }
-        }
-        *(float4*)(dst + f) = x;
+__device__ __forceinline__ void copy16(float* dst, const float* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 64 rows of D features; `row(r, on)` gives the address of row r and clears `on` where the row counts as zeros.
+template <int DM, typename Row>
+__device__ __forceinline__ void fetch(float* dst, Row row, const float* any, int D, int tid) {
+    constexpr int PIECES = DM / 4, STEP = kThreads / PIECES;
+    const int c = tid % PIECES;
+#pragma unroll
+    for (int r = tid / PIECES; r < kTile; r += STEP) {
+        bool on = c * 4 < D;
+        const float* src = row(r, on);
+        copy16(dst + r * kPitch<DM> + c * 4, on ? src + c * 4 : any, on);
     }
 }
 
@@ -35,28 +43,36 @@ __device__ __forceinline__ void load_row(float* dst, const T* src, int D, int pa
 template <int DM>
 __device__ __forceinline__ void dot_tile(const float* A, const float* B, int ty, int tx, float (&s)[4][4]) {
     constexpr int P = kPitch<DM>;
+    f32x2 acc[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0;
 #pragma unroll 4
     for (int d = 0; d < DM; d += 4) {
-        float4 x[4], y[4];
+        ulonglong2 x[4], y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = *(const float4*)(A + (ty + 16 * i) * P + d);
+        for (int i = 0; i < 4; ++i) x[i] = *(const ulonglong2*)(A + (ty + 16 * i) * P + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = *(const float4*)(B + (tx + 16 * j) * P + d);
+        for (int j = 0; j < 4; ++j) y[j] = *(const ulonglong2*)(B + (tx + 16 * j) * P + d);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                s[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, s[i][j]))));
+            for (int j = 0; j < 4; ++j) acc[i][j] = fma2(x[i].y, y[j].y, fma2(x[i].x, y[j].x, acc[i][j]));
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float lo, hi;
+            unpack2(acc[i][j], lo, hi);
+            s[i][j] = lo + hi;
+        }
 }
 
-// o[i][c] += row ty+16i of P times column (tx*4 + 64*(c/4) + c%4) of B.
+// o[i][2c], o[i][2c+1]: += row ty+16i of P times columns (tx*4 + 64*(c/2) + 2*(c%2)) and the next pair of B.
 template <int DM>
-__device__ __forceinline__ void acc_tile(const float* Pm, const float* B, int ty, int tx, float (&o)[4][DM / 16]) {
+__device__ __forceinline__ void acc_tile(const float* Pm, const float* B, int ty, int tx, f32x2 (&o)[4][DM / 32]) {
     constexpr int P = kPitch<DM>;
 #pragma unroll 2
     for (int k = 0; k < kTile; k += 4) {
@@ -64,19 +80,23 @@ __device__ __forceinline__ void acc_tile(const float* Pm, const float* B, int ty
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[i] = *(const float4*)(Pm + (ty + 16 * i) * kPPitch + k);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+        for (int kk = 0; kk < 4; ++kk) {
+            f32x2 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w;
+                w[i] = pack2(e, e);
+            }
 #pragma unroll
             for (int c = 0; c < DM / 64; ++c) {
-                const float4 v = *(const float4*)(B + (k + kk) * P + tx * 4 + 64 * c);
+                const ulonglong2 v = *(const ulonglong2*)(B + (k + kk) * P + tx * 4 + 64 * c);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float w = kk == 0 ? p[i].x : kk == 1 ? p[i].y : kk == 2 ? p[i].z : p[i].w;
-                    o[i][4 * c + 0] = fmaf(w, v.x, o[i][4 * c + 0]);
-                    o[i][4 * c + 1] = fmaf(w, v.y, o[i][4 * c + 1]);
-                    o[i][4 * c + 2] = fmaf(w, v.z, o[i][4 * c + 2]);
-                    o[i][4 * c + 3] = fmaf(w, v.w, o[i][4 * c + 3]);
+                    o[i][2 * c] = fma2(w[i], v.x, o[i][2 * c]);
+                    o[i][2 * c + 1] = fma2(w[i], v.y, o[i][2 * c + 1]);
                 }
             }
+        }
     }
 }
 
@@ -91,42 +111,41 @@ __device__ __forceinline__ float sum16(float x) {
     return x;
 }
 
-template <typename T, int DM>
-__device__ __forceinline__ void store_row(T* dst, const float (&o)[DM / 16], float f, int D, int tx) {
+template <int DM>
+__device__ __forceinline__ void store_row(float* dst, const f32x2 (&o)[DM / 32], float f, int D, int tx) {
+    const f32x2 f2 = pack2(f, f);
 #pragma unroll
     for (int c = 0; c < DM / 64; ++c) {
         const int at = tx * 4 + 64 * c;
         if (at >= D) continue;
-        if (sizeof(T) == 4) {
-            *(float4*)(dst + at) = make_float4(o[4 * c] * f, o[4 * c + 1] * f, o[4 * c + 2] * f, o[4 * c + 3] * f);
-        } else {
-            T e[4] = {from_float<T>(o[4 * c] * f), from_float<T>(o[4 * c + 1] * f), from_float<T>(o[4 * c + 2] * f), from_float<T>(o[4 * c + 3] * f)};
-            *(uint2*)(dst + at) = *(const uint2*)e;
-        }
+        ulonglong2 w;
+        w.x = mul2(o[2 * c], f2);
+        w.y = mul2(o[2 * c + 1], f2);
+        *(ulonglong2*)(dst + at) = w;
     }
 }
 
-template <typename T>
-__device__ __forceinline__ T* row_ptr(const ca_seq_view& v, const SeqArgs& a, const Seq& s, int h, int R) {
-    const int t = R / a.G, g = R - t * a.G;
-    return (T*)v.data + (h * a.G + g) * v.head + (int64_t)(s.t0 + t) * v.token + (a.pages.table ? 0 : s.b * v.batch);
+__device__ __forceinline__ float* row_ptr(const ca_seq_view& v, const SeqArgs& a, const Seq& s, int h, int R) {
+    const int t = token_of(a, R), g = R - t * a.G;
+    return (float*)v.data + (h * a.G + g) * v.head + (int64_t)(s.t0 + t) * v.token + (a.pages.table ? 0 : s.b * v.batch);
 }
-// Key row j, or null where it does not exist.
-template <typename T>
-__device__ __forceinline__ const T* key_ptr(const ca_seq_view& v, const ca_page_view& pv, const SeqArgs& a, const Seq& s, int h, int j) {
-    if (j >= s.n) return nullptr;
-    if (!a.pages.table) return (const T*)v.data + h * v.head + (int64_t)j * v.token + s.b * v.batch;
-    const int p = page_of(a, s.b, j);
-    return p < 0 ? nullptr : (const T*)pv.data + h * pv.head + (int64_t)(j % a.pages.page) * pv.token + p * pv.page;
+// Key row j; clears `on` where it does not exist.
+__device__ __forceinline__ const float* key_ptr(const ca_seq_view& v, const ca_page_view& pv, const SeqArgs& a, const Seq& s, int h, int j, bool& on) {
+    on = on && j < s.n;
+    if (!a.pages.table) return (const float*)v.data + h * v.head + (int64_t)j * v.token + s.b * v.batch;
+    const int p = on ? page_of(a, s.b, j) : -1;
+    on = on && p >= 0;
+    return (const float*)pv.data + h * pv.head + (int64_t)(j % a.pages.page) * pv.token + p * pv.page;
 }
 
 // ---------------------------------------------------------------- forward
-template <typename T, int DM>
+template <int DM> constexpr size_t kFwdSmem = (5 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
+
+template <int DM>
 __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
-    constexpr int P = kPitch<DM>;
-    float *Q = (float*)smem4, *K = Q + kTile * P, *V = K + kTile * P, *Pm = V + kTile * P;
-    __shared__ unsigned char gone[kTile];
+    float *Q = (float*)smem4, *KV = Q + kTileFloats<DM>, *Pm = KV + 4 * kTileFloats<DM>;      // K, V, K, V
+    __shared__ unsigned char gone[2][kTile];
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
     int tile = blockIdx.x;
     Seq s;
@@ -137,42 +156,61 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
     }
     const int rows = s.T * a.G, R0 = tile * kTile;
     const int p_lo = s.base + R0 / a.G, p_hi = s.base + (min(R0 + kTile, rows) - 1) / a.G;
-    {
-        const int r = tid >> 2, R = R0 + r, pos = s.base + R / a.G;
-        load_row<T, DM>(Q + r * P, R < rows && pos >= 0 && pos < s.n ? row_ptr<T>(a.q, a, s, h, R) : nullptr, a.D, tid & 3);
-    }
+    const float* any = (const float*)a.q.data;
+    fetch<DM>(Q, [&](int r, bool& on) {
+        const int R = min(R0 + r, rows - 1), pos = s.base + token_of(a, R);
+        on = on && R0 + r < rows && pos >= 0 && pos < s.n;
+        return row_ptr(a.q, a, s, h, R);
+    }, any, a.D, tid);
     const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kTile);
-    float m[4], l[4], o[4][DM / 16];
+    auto prefetch = [&](int it) {
+        const int j0 = kt.key(it, kTile), b = it & 1;
+        float* K = KV + 2 * b * kTileFloats<DM>;
+        fetch<DM>(K, [&](int r, bool& on) {
+            const bool whole = on;
+            const float* p = key_ptr(a.k, a.kp, a, s, h, j0 + r, on);
+            if (tid % (DM / 4) == 0 && whole) gone[b][r] = !on;
+            return p;
+        }, any, a.D, tid);
+        // rows of v that no query of this tile sees may hold anything: they count as zeros
+        fetch<DM>(K + kTileFloats<DM>, [&](int r, bool& on) {
+            const int j = j0 + r;
+            on = on && (j >= p_lo - a.left || j < a.sinks) && j <= (int64_t)p_hi + a.right;
+            return key_ptr(a.v, a.vp, a, s, h, j, on);
+        }, any, a.D, tid);
+    };
+    int pos[4];
+    float m[4], l[4];
+    f32x2 o[4][DM / 32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        const int R = R0 + ty + 16 * i;
+        pos[i] = R < rows ? s.base + token_of(a, R) : -1;
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < DM / 16; ++c) o[i][c] = 0.f;
+        for (int c = 0; c < DM / 32; ++c) o[i][c] = 0;
     }
+    if (kt.count) prefetch(0);
+    copies_commit();
     for (int it = 0; it < kt.count; ++it) {
-        const int j0 = kt.key(it, kTile);
+        if (it + 1 < kt.count) prefetch(it + 1);
+        copies_commit();
+        copies_wait<1>();
         __syncthreads();
-        {
-            const int r = tid >> 2, j = j0 + r;
-            const T* kr = key_ptr<T>(a.k, a.kp, a, s, h, j);
-            load_row<T, DM>(K + r * P, kr, a.D, tid & 3);
-            // rows of v that no query of this tile sees may hold anything: they count as zeros
-            const bool used = kr && (j >= p_lo - a.left || j < a.sinks) && j <= (int64_t)p_hi + a.right;
-            load_row<T, DM>(V + r * P, used ? key_ptr<T>(a.v, a.vp, a, s, h, j) : nullptr, a.D, tid & 3);
-            if (!(tid & 3)) gone[r] = !kr;
-        }
-        __syncthreads();
+        const int j0 = kt.key(it, kTile), b = it & 1;
+        const float* K = KV + 2 * b * kTileFloats<DM>;
         float sc[4][4];
         dot_tile<DM>(Q, K, ty, tx, sc);
+        const bool edge = !(p_lo >= 0 && p_hi < s.n && j0 + kTile - 1 <= (int64_t)p_lo + a.right && j0 + kTile <= s.n &&
+                            (j0 >= p_hi - a.left || j0 + kTile <= a.sinks)) || a.pages.table;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int R = R0 + ty + 16 * i, pos = s.base + R / a.G;
             float top = m[i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bool see = R < rows && sees(a, s.n, pos, j0 + tx + 16 * j) && !gone[tx + 16 * j];
-                sc[i][j] = see ? sc[i][j] * a.scale_log2 : -INFINITY;
+                sc[i][j] *= a.scale_log2;
+                if (edge && (!sees(a, s.n, pos[i], j0 + tx + 16 * j) || gone[b][tx + 16 * j])) sc[i][j] = -INFINITY;
                 top = fmaxf(top, sc[i][j]);
             }
             top = max16(top);
@@ -187,158 +225,235 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
                 Pm[(ty + 16 * i) * kPPitch + tx + 16 * j] = p;
             }
             l[i] = l[i] * f + sum;
+            const f32x2 f2 = pack2(f, f);
 #pragma unroll
-            for (int c = 0; c < DM / 16; ++c) o[i][c] *= f;
+            for (int c = 0; c < DM / 32; ++c) o[i][c] = mul2(o[i][c], f2);
         }
         __syncwarp();                                             // rows ty + 16i are written and read by one half warp
-        acc_tile<DM>(Pm, V, ty, tx, o);
+        acc_tile<DM>(Pm, K + kTileFloats<DM>, ty, tx, o);
+        __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int R = R0 + ty + 16 * i;
-        if (R >= rows) continue;
         const float sum = sum16(l[i]);
-        store_row<T, DM>(row_ptr<T>(a.y, a, s, h, R), o[i], sum > 0.f ? 1.f / sum : 0.f, a.D, tx);
-        if (sizeof(T) == 2 && a.rest.data) {
-            const float f = sum > 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-            for (int c = 0; c < DM / 16; ++c) o[i][c] = o[i][c] * f - to_float(from_float<T>(o[i][c] * f));
-            store_row<T, DM>(row_ptr<T>(a.rest, a, s, h, R), o[i], 1.f, a.D, tx);
-        }
+        if (R >= rows) continue;
+        store_row<DM>(row_ptr(a.y, a, s, h, R), o[i], sum > 0.f ? 1.f / sum : 0.f, a.D, tx);
         if (a.lse && tx == 0) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = sum > 0.f ? m[i] + log2f(sum) : -INFINITY;
     }
 }
 
 // ---------------------------------------------------------------- backward
 // P = 2^(scale q.k log2 e - lse), dP = dy.v, dS = P (dP - delta), delta = dy.y; dq = scale dS k.
-template <typename T, int DM>
+template <int DM> constexpr size_t kDqSmem = (6 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
+
+template <int DM>
 __global__ void __launch_bounds__(kThreads) fma_dq_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
-    constexpr int P = kPitch<DM>;
-    float *Q = (float*)smem4, *O = Q + kTile * P, *K = O + kTile * P, *V = K + kTile * P, *Pm = V + kTile * P;
+    float *Q = (float*)smem4, *O = Q + kTileFloats<DM>, *KV = O + kTileFloats<DM>, *Pm = KV + 4 * kTileFloats<DM>;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
     const Seq s = dense_seq(a, blockIdx.z);
     const int rows = s.T * a.G, R0 = blockIdx.x * kTile;
     const int p_lo = R0 / a.G, p_hi = (min(R0 + kTile, rows) - 1) / a.G;
     const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
-    float *yrow = K, *rest = V;                                   // y passes through the keys' place
-    {
-        const int r = tid >> 2, R = R0 + r;
-        const bool live = R < rows && R / a.G < s.n;
-        load_row<T, DM>(Q + r * P, live ? row_ptr<T>(a.q, a, s, h, R) : nullptr, a.D, tid & 3);
-        load_row<T, DM>(O + r * P, live ? row_ptr<T>(a.dy, a, s, h, R) : nullptr, a.D, tid & 3);
-        load_row<T, DM>(yrow + r * P, live ? row_ptr<T>(a.y, a, s, h, R) : nullptr, a.D, tid & 3);
-        load_row<T, DM>(rest + r * P, live && a.rest.data ? row_ptr<T>(a.rest, a, s, h, R) : nullptr, a.D, tid & 3);
-    }
+    const float* any = (const float*)a.q.data;
+    auto from = [&](const ca_seq_view& v) {
+        return [&](int r, bool& on) {
+            const int R = min(R0 + r, rows - 1);
+            on = on && R0 + r < rows && token_of(a, R) < s.n;
+            return (const float*)row_ptr(v, a, s, h, R);
+        };
+    };
+    fetch<DM>(Q, from(a.q), any, a.D, tid);
+    fetch<DM>(O, from(a.dy), any, a.D, tid);
+    float* yrow = KV + 2 * kTileFloats<DM>;                       // y passes through the place of the second tile
+    fetch<DM>(yrow, from(a.y), any, a.D, tid);
+    copies_commit();
+    const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kTile);
+    auto prefetch = [&](int it) {
+        const int j0 = kt.key(it, kTile);
+        float* K = KV + 2 * (it & 1) * kTileFloats<DM>;
+        fetch<DM>(K, [&](int r, bool& on) { return key_ptr(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
+        fetch<DM>(K + kTileFloats<DM>, [&](int r, bool& on) { return key_ptr(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
+    };
+    if (kt.count) prefetch(0);
+    copies_commit();
+    copies_wait<1>();
     __syncthreads();
-    float lse[4], delta[4], o[4][DM / 16];
+    int pos[4];
+    float lse[4], delta[4];
+    f32x2 o[4][DM / 32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i, R = R0 + r;
         float d = 0.f;
-        for (int f = tx; f < DM; f += 16) d = fmaf(O[r * P + f], yrow[r * P + f] + rest[r * P + f], d);
+        for (int f = tx; f < DM; f += 16) d = fmaf(O[r * kPitch<DM> + f], yrow[r * kPitch<DM> + f], d);
         delta[i] = sum16(d);
-        lse[i] = R < rows ? a.lse[stat0 + R] : -INFINITY;
+        pos[i] = R < rows ? token_of(a, R) : -1;
+        lse[i] = R < rows ? a.lse[stat0 + R] : 0.f;
         if (R < rows && tx == 0) a.delta[stat0 + R] = delta[i];
 #pragma unroll
-        for (int c = 0; c < DM / 16; ++c) o[i][c] = 0.f;
+        for (int c = 0; c < DM / 32; ++c) o[i][c] = 0;
     }
-    const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kTile);
+    __syncthreads();
     for (int it = 0; it < kt.count; ++it) {
+        if (it + 1 < kt.count) prefetch(it + 1);
+        copies_commit();
+        copies_wait<1>();
+        __syncthreads();
         const int j0 = kt.key(it, kTile);
-        __syncthreads();
-        {
-            const int r = tid >> 2, j = j0 + r;
-            load_row<T, DM>(K + r * P, key_ptr<T>(a.k, a.kp, a, s, h, j), a.D, tid & 3);
-            load_row<T, DM>(V + r * P, key_ptr<T>(a.v, a.vp, a, s, h, j), a.D, tid & 3);
-        }
-        __syncthreads();
+        const float* K = KV + 2 * (it & 1) * kTileFloats<DM>;
+        const bool edge = !(p_hi < s.n && j0 + kTile - 1 <= (int64_t)p_lo + a.right && j0 + kTile <= s.n && (j0 >= p_hi - a.left || j0 + kTile <= a.sinks));
         float sc[4][4], dp[4][4];
         dot_tile<DM>(Q, K, ty, tx, sc);
-        dot_tile<DM>(O, V, ty, tx, dp);
+        dot_tile<DM>(O, K + kTileFloats<DM>, ty, tx, dp);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int R = R0 + ty + 16 * i;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bool see = R < rows && sees(a, s.n, R / a.G, j0 + tx + 16 * j);
-                const float p = see ? fast_exp2(sc[i][j] * a.scale_log2 - lse[i]) : 0.f;
-                Pm[(ty + 16 * i) * kPPitch + tx + 16 * j] = see ? p * (dp[i][j] - delta[i]) : 0.f;
+                const bool see = !edge || sees(a, s.n, pos[i], j0 + tx + 16 * j);
+                Pm[(ty + 16 * i) * kPPitch + tx + 16 * j] = see ? fast_exp2(sc[i][j] * a.scale_log2 - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
             }
-        }
         __syncwarp();
         acc_tile<DM>(Pm, K, ty, tx, o);
+        __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int R = R0 + ty + 16 * i;
-        if (R < rows) store_row<T, DM>(row_ptr<T>(a.dq, a, s, h, R), o[i], a.scale, a.D, tx);
+        if (R < rows) store_row<DM>(row_ptr(a.dq, a, s, h, R), o[i], a.scale, a.D, tx);
     }
 }
 
-// A block owns 64 keys and walks the query rows that see any of them: dv = P^T dy, dk = scale dS^T q, no atomics.
-template <typename T, int DM>
-__global__ void __launch_bounds__(kThreads) fma_dkdv_kernel(const __grid_constant__ SeqArgs a) {
+// A block owns 64 keys and walks the query rows that see any of them: dv = P^T dy, dk = scale dS^T q, no atomics.  The rows of
+// key tiles that hold first tokens are dealt to `segments` blocks, whose parts fma_join_kernel adds up in order.
+// Two stages of q and dy beside k, v and both weights; at 128 features only one fits.
+template <int DM> constexpr int kStages = DM == 64 ? 2 : 1;
+template <int DM> constexpr size_t kDkdvSmem = ((2 + 2 * kStages<DM>) * kTileFloats<DM> + 2 * kTile * kPPitch) * sizeof(float);
+
+struct Parts {
+    float* data;            // [b][key head][tile][segment][dk, dv][64 keys][DM]
+    int tiles, segments;
+};
+
+template <int DM>
+__global__ void __launch_bounds__(kThreads) fma_dkdv_kernel(const __grid_constant__ SeqArgs a, const Parts parts) {
     extern __shared__ float4 smem4[];
-    constexpr int P = kPitch<DM>;
-    float *K = (float*)smem4, *V = K + kTile * P, *Q = V + kTile * P, *O = Q + kTile * P, *Pm = O + kTile * P, *Sm = Pm + kTile * kPPitch;
-    __shared__ float s_lse[kTile], s_delta[kTile];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y, j0 = blockIdx.x * kTile;
+    constexpr int STAGES = kStages<DM>;
+    float *K = (float*)smem4, *V = K + kTileFloats<DM>, *QO = V + kTileFloats<DM>, *Pm = QO + 2 * STAGES * kTileFloats<DM>, *Sm = Pm + kTile * kPPitch;
+    __shared__ float s_lse[2][kTile], s_delta[2][kTile];
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
+    const int dealt = parts.tiles * parts.segments;
+    const bool split = (int)blockIdx.x < dealt;
+    const int tile = split ? (int)blockIdx.x / parts.segments : parts.tiles + (int)blockIdx.x - dealt, seg = split ? (int)blockIdx.x % parts.segments : 0;
+    const int j0 = tile * kTile;
     const Seq s = dense_seq(a, blockIdx.z);
     const int rows = s.T * a.G;
     const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
-    {
-        const int r = tid >> 2;
-        load_row<T, DM>(K + r * P, key_ptr<T>(a.k, a.kp, a, s, h, j0 + r), a.D, tid & 3);
-        load_row<T, DM>(V + r * P, key_ptr<T>(a.v, a.vp, a, s, h, j0 + r), a.D, tid & 3);
-    }
-    float dk[4][DM / 16], dv[4][DM / 16];
+    const float* any = (const float*)a.q.data;
+    fetch<DM>(K, [&](int r, bool& on) { return key_ptr(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
+    fetch<DM>(V, [&](int r, bool& on) { return key_ptr(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
+    f32x2 dk[4][DM / 32], dv[4][DM / 32];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int c = 0; c < DM / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
+        for (int c = 0; c < DM / 32; ++c) dk[i][c] = dv[i][c] = 0;
     const int t_lo = max(0, j0 - a.right);
-    const int t_hi = j0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)j0 + kTile + a.left);
-    for (int R0 = t_lo * a.G; R0 < t_hi * a.G && j0 < s.n; R0 += kTile) {
-        __syncthreads();
-        {
-            const int r = tid >> 2, R = R0 + r;
-            const bool live = R < t_hi * a.G;
-            load_row<T, DM>(Q + r * P, live ? row_ptr<T>(a.q, a, s, h, R) : nullptr, a.D, tid & 3);
-            load_row<T, DM>(O + r * P, live ? row_ptr<T>(a.dy, a, s, h, R) : nullptr, a.D, tid & 3);
-            if (tid < kTile) {
-                const bool have = R0 + tid < t_hi * a.G;
-                s_lse[tid] = have ? a.lse[stat0 + R0 + tid] : 0.f;
-                s_delta[tid] = have ? a.delta[stat0 + R0 + tid] : 0.f;
-            }
+    const int t_hi = j0 >= s.n ? t_lo : j0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)j0 + kTile + a.left);
+    const int lo = t_lo * a.G, hi = max(t_lo, t_hi) * a.G, all = (hi - lo + kTile - 1) / kTile;
+    const int first = split ? (int)((int64_t)all * seg / parts.segments) : 0;
+    const int count = (split ? (int)((int64_t)all * (seg + 1) / parts.segments) : all) - first;
+    auto prefetch = [&](int it) {
+        const int R0 = lo + (first + it) * kTile, b = it % STAGES;
+        float* Q = QO + 2 * b * kTileFloats<DM>;
+        auto from = [&](const ca_seq_view& v) {
+            return [&](int r, bool& on) {
+                on = on && R0 + r < hi;
+                return (const float*)row_ptr(v, a, s, h, min(R0 + r, hi - 1));
+            };
+        };
+        fetch<DM>(Q, from(a.q), any, a.D, tid);
+        fetch<DM>(Q + kTileFloats<DM>, from(a.dy), any, a.D, tid);
+        if (tid < kTile) {
+            const bool have = R0 + tid < hi;
+            s_lse[it & 1][tid] = have ? a.lse[stat0 + R0 + tid] : 0.f;
+            s_delta[it & 1][tid] = have ? a.delta[stat0 + R0 + tid] : 0.f;
+        }
+    };
+    if (count) prefetch(0);
+    copies_commit();
+    for (int it = 0; it < count; ++it) {
+        if (STAGES == 2) {
+            if (it + 1 < count) prefetch(it + 1);
+            copies_commit();
+            copies_wait<1>();
+        } else {
+            copies_wait<0>();
         }
         __syncthreads();
+        const int R0 = lo + (first + it) * kTile, b = it & 1;
+        const float *Q = QO + 2 * (it % STAGES) * kTileFloats<DM>, *O = Q + kTileFloats<DM>;
         float sc[4][4], dp[4][4];
         dot_tile<DM>(K, Q, ty, tx, sc);
         dot_tile<DM>(V, O, ty, tx, dp);
+        const int t0 = R0 / a.G, t1 = min(R0 + kTile, hi) - 1 < R0 ? t0 : (min(R0 + kTile, hi) - 1) / a.G;
+        const bool edge = !(R0 + kTile <= hi && t1 < s.n && j0 + kTile <= s.n && j0 + kTile - 1 <= (int64_t)t0 + a.right && (j0 >= t1 - a.left || j0 + kTile <= a.sinks));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int j = j0 + ty + 16 * i;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int R = R0 + tx + 16 * c;
-                const bool see = R < t_hi * a.G && sees(a, s.n, R / a.G, j);
-                const float p = see ? fast_exp2(sc[i][c] * a.scale_log2 - s_lse[tx + 16 * c]) : 0.f;
+                const bool see = !edge || (R < hi && sees(a, s.n, token_of(a, R), j0 + ty + 16 * i));
+                const float p = see ? fast_exp2(sc[i][c] * a.scale_log2 - s_lse[b][tx + 16 * c]) : 0.f;
                 Pm[(ty + 16 * i) * kPPitch + tx + 16 * c] = p;
-                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? p * (dp[i][c] - s_delta[tx + 16 * c]) : 0.f;
+                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? p * (dp[i][c] - s_delta[b][tx + 16 * c]) : 0.f;
             }
-        }
         __syncwarp();
         acc_tile<DM>(Pm, O, ty, tx, dv);
         acc_tile<DM>(Sm, Q, ty, tx, dk);
+        __syncthreads();
+        if (STAGES == 1) {
+            if (it + 1 < count) prefetch(it + 1);
+            copies_commit();
+        }
     }
+    copies_wait<0>();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int j = j0 + ty + 16 * i;
-        if (j >= a.N) continue;
-        store_row<T, DM>((T*)a.dk.data + h * a.dk.head + (int64_t)j * a.dk.token + s.b * a.dk.batch, dk[i], a.scale, a.D, tx);
-        store_row<T, DM>((T*)a.dv.data + h * a.dv.head + (int64_t)j * a.dv.token + s.b * a.dv.batch, dv[i], 1.f, a.D, tx);
+        const int r = ty + 16 * i, j = j0 + r;
+        if (split) {
+            float* p = parts.data + ((((int64_t)s.b * a.Hkv + h) * parts.tiles + tile) * parts.segments + seg) * 2 * kTile * DM + r * DM;
+            store_row<DM>(p, dk[i], a.scale, DM, tx);
+            store_row<DM>(p + kTile * DM, dv[i], 1.f, DM, tx);
+        } else if (j < a.N) {
+            store_row<DM>((float*)a.dk.data + h * a.dk.head + (int64_t)j * a.dk.token + s.b * a.dk.batch, dk[i], a.scale, a.D, tx);
+            store_row<DM>((float*)a.dv.data + h * a.dv.head + (int64_t)j * a.dv.token + s.b * a.dv.batch, dv[i], 1.f, a.D, tx);
+        }
     }
+}
+
+template <int DM>
+__global__ void __launch_bounds__(256) fma_join_kernel(const __grid_constant__ SeqArgs a, const Parts parts) {
+    const int which = blockIdx.x & 1, tile = blockIdx.x >> 1, h = blockIdx.y, b = blockIdx.z;
+    const float* p = parts.data + (((int64_t)b * a.Hkv + h) * parts.tiles + tile) * parts.segments * 2 * kTile * DM + which * kTile * DM;
+    const ca_seq_view& out = which ? a.dv : a.dk;
+    for (int i = threadIdx.x; i < kTile * DM / 4; i += 256) {
+        const int r = i / (DM / 4), c = i % (DM / 4) * 4, j = tile * kTile + r;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int seg = 0; seg < parts.segments; ++seg) {
+            const float4 x = *(const float4*)(p + (int64_t)seg * 2 * kTile * DM + r * DM + c);
+            sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+        }
+        if (j < a.N && c < a.D) *(float4*)((float*)out.data + h * out.head + (int64_t)j * out.token + b * out.batch + c) = sum;
+    }
+}
+
+// Key tiles of first tokens have every later row; they are dealt out in pieces of about an ordinary tile's work.
+Parts split_rule(const SeqArgs& a, float* data) {
+    const int64_t all = (a.N + kTile - 1) / kTile, window = ((int64_t)a.left + a.right + 2 * kTile - 1) / kTile;
+    Parts p{data, (int)((std::min(a.sinks, a.N) + kTile - 1) / kTile), (int)std::min<int64_t>(64, (all + window - 1) / window)};
+    if (p.segments < 2 || p.tiles == 0) { p.tiles = 0; p.segments = 1; }
+    return p;
 }
 
 template <typename K>
@@ -347,42 +462,41 @@ int raise_smem(K kernel, size_t bytes) {
     return e == cudaSuccess ? CA_OK : cuda_fail(e, "cudaFuncSetAttribute");
 }
 
-template <typename T, int DM>
+template <int DM>
 int launch_fwd(const SeqArgs& a, cudaStream_t st) {
-    const size_t smem = (3 * kTile * kPitch<DM> + kTile * kPPitch) * sizeof(float);
-    const int rc = raise_smem(fma_fwd_kernel<T, DM>, smem);
+    const int rc = raise_smem(fma_fwd_kernel<DM>, kFwdSmem<DM>);
     if (rc) return rc;
     const int64_t tiles = a.pages.table ? paged_tiles(a.N, a.G, a.pages.sequences, kTile) : ((int64_t)a.N * a.G + kTile - 1) / kTile;
-    const dim3 grid((unsigned)tiles, a.Hkv, a.B);
-    fma_fwd_kernel<T, DM><<<grid, kThreads, smem, st>>>(a);
+    fma_fwd_kernel<DM><<<dim3((unsigned)tiles, a.Hkv, a.B), kThreads, kFwdSmem<DM>, st>>>(a);
     CA_CHECK_LAUNCH("window forward kernel");
     return CA_OK;
 }
 
-template <typename T, int DM>
-int launch_bwd(const SeqArgs& a, cudaStream_t st) {
-    const size_t smem_q = (4 * kTile * kPitch<DM> + kTile * kPPitch) * sizeof(float), smem_k = smem_q + kTile * kPPitch * sizeof(float);
-    int rc = raise_smem(fma_dq_kernel<T, DM>, smem_q);
-    if (rc || (rc = raise_smem(fma_dkdv_kernel<T, DM>, smem_k))) return rc;
-    fma_dq_kernel<T, DM><<<dim3((unsigned)(((int64_t)a.N * a.G + kTile - 1) / kTile), a.Hkv, a.B), kThreads, smem_q, st>>>(a);
+template <int DM>
+int launch_bwd(const SeqArgs& a, float* data, cudaStream_t st) {
+    int rc = raise_smem(fma_dq_kernel<DM>, kDqSmem<DM>);
+    if (rc || (rc = raise_smem(fma_dkdv_kernel<DM>, kDkdvSmem<DM>))) return rc;
+    const Parts parts = split_rule(a, data);
+    fma_dq_kernel<DM><<<dim3((unsigned)(((int64_t)a.N * a.G + kTile - 1) / kTile), a.Hkv, a.B), kThreads, kDqSmem<DM>, st>>>(a);
     CA_CHECK_LAUNCH("window dq kernel");
-    fma_dkdv_kernel<T, DM><<<dim3((a.N + kTile - 1) / kTile, a.Hkv, a.B), kThreads, smem_k, st>>>(a);
+    const int tiles = (a.N + kTile - 1) / kTile;
+    fma_dkdv_kernel<DM><<<dim3(tiles - parts.tiles + parts.tiles * parts.segments, a.Hkv, a.B), kThreads, kDkdvSmem<DM>, st>>>(a, parts);
     CA_CHECK_LAUNCH("window dk/dv kernel");
+    if (parts.tiles) {
+        fma_join_kernel<DM><<<dim3(2 * parts.tiles, a.Hkv, a.B), 256, 0, st>>>(a, parts);
+        CA_CHECK_LAUNCH("window dk/dv join kernel");
+    }
     return CA_OK;
 }
 
 }  // namespace
 
-#define CA_SEQ_DISPATCH(dtype, D, FN, ...)                                                                            \
-    do {                                                                                                             \
-        const bool wide = (D) > 64;                                                                                  \
-        if ((dtype) == CA_F32) return wide ? FN<float, 128>(__VA_ARGS__) : FN<float, 64>(__VA_ARGS__);               \
-        if ((dtype) == CA_BF16) return wide ? FN<__nv_bfloat16, 128>(__VA_ARGS__) : FN<__nv_bfloat16, 64>(__VA_ARGS__); \
-        return wide ? FN<__half, 128>(__VA_ARGS__) : FN<__half, 64>(__VA_ARGS__);                                    \
-    } while (0)
+size_t fma_bwd_parts(const SeqArgs& a) {
+    const Parts p = split_rule(a, nullptr);
+    return (size_t)p.tiles * p.segments * 2 * kTile * (a.D > 64 ? 128 : 64) * a.Hkv * a.B * sizeof(float);
+}
 
-int fma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st) { CA_SEQ_DISPATCH(dtype, a.D, launch_fwd, a, st); }
-int fma_window_bwd(const SeqArgs& a, int dtype, cudaStream_t st) { CA_SEQ_DISPATCH(dtype, a.D, launch_bwd, a, st); }
-int fma_paged(const SeqArgs& a, int dtype, cudaStream_t st) { CA_SEQ_DISPATCH(dtype, a.D, launch_fwd, a, st); }
+int fma_fwd(const SeqArgs& a, cudaStream_t st) { return a.D > 64 ? launch_fwd<128>(a, st) : launch_fwd<64>(a, st); }
+int fma_bwd(const SeqArgs& a, float* parts, cudaStream_t st) { return a.D > 64 ? launch_bwd<128>(a, parts, st) : launch_bwd<64>(a, parts, st); }
 
 }  // namespace ca
