@@ -111,6 +111,8 @@ int encode_tokens(CUtensorMap* m, bool bf16, const ca_seq_view& v, int D, int he
 // seq_fwd.cu
 int umma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st);
 int umma_paged(const SeqArgs& a, int dtype, cudaStream_t st);
+// seq_decode.cu: few rows a key head, every type
+int decode_paged(const SeqArgs& a, int dtype, cudaStream_t st);
 // seq_bwd.cu
 size_t umma_bwd_parts(const SeqArgs& a);
 int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st);

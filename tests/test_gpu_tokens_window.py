@@ -209,6 +209,23 @@ def test_repeated_calls_and_other_streams(ca, dtype):
     ca.ops.check_status()
 
 
+def test_a_host_thread_of_its_own(ca):
+    """The first CUDA call of a thread: tensor maps are made through the driver, which needs the device's context there."""
+    import threading
+    q, k, v, dy = (t.cuda() for t in problem(64, 4, 2, 300, 1, torch.bfloat16))
+    base = run(ca, q, k, v, dy, 60, 0, 4)["y"].detach()
+    got = []
+
+    def work():
+        with torch.no_grad():
+            got.append(ca.window_attention(q, k, v, 60, sinks=4))
+    for _ in range(3):
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+    assert len(got) == 3 and all(torch.equal(g, base) for g in got)
+
+
 def test_in_a_graph(ca):
     q, k, v, dy = (t.cuda() for t in problem(64, 4, 2, 300, 1, torch.bfloat16))
     base = run(ca, q, k, v, dy, 60, 0, 4)
