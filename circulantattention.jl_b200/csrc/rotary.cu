@@ -24,6 +24,7 @@ struct RotaryTensor {
 struct RotaryArgs {
     RotaryTensor t[3];
     int nt, total_heads;
+    uint32_t heads_inv;                   // ceil(2^32 / total_heads): exact quotients of items below 2^32 / total_heads
     int D, R, axes, ends[CA_MAX_AXES];    // ends: first pair behind each section
     const int* pos;
     int64_t p_axis, p_token, p_batch;
@@ -43,14 +44,21 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
 template <typename T, int V, bool INTER>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
     extern __shared__ float2 cs[];                    // [token][p % V][p / V]: lanes of consecutive chunks read consecutive words
-    __shared__ int s_page[kRotaryTokens], s_off[kRotaryTokens];
+    __shared__ int s_page[kRotaryTokens], s_off[kRotaryTokens], s_batch[kRotaryTokens], s_token[kRotaryTokens];
     const int R = a.R, nc = R / V;
     const int64_t tok0 = (int64_t)blockIdx.x * a.per_block;
     const int ntok = (int)min((int64_t)a.per_block, a.tokens - tok0);
+    // Quotients are taken once a token: as part of every piece they were more than half of the instructions.
+    if (threadIdx.x < ntok) {
+        const uint32_t tok = (uint32_t)tok0 + threadIdx.x, b = tok / (uint32_t)a.N;
+        s_batch[threadIdx.x] = (int)b;
+        s_token[threadIdx.x] = (int)(tok - b * (uint32_t)a.N);
+    }
+    __syncthreads();
 
     for (int i = threadIdx.x; i < ntok * R; i += kRotaryThreads) {
         const int t = i / R, p = i - t * R;
-        const int64_t tok = tok0 + t, b = tok / a.N, n = tok - b * a.N;
+        const int64_t b = s_batch[t], n = s_token[t];
         int axis = 0;
         while (axis + 1 < a.axes && p >= a.ends[axis]) ++axis;
         const int x = a.pos[axis * a.p_axis + n * a.p_token + b * a.p_batch];
@@ -81,15 +89,15 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     // A group of nv threads takes one head of one token: R/V chunks of pairs, then the features that pass.
     const int nv = nc + (a.D - 2 * R) / V;
     const int groups = max(1, kRotaryThreads / nv);
-    const int g0 = threadIdx.x / nv;
+    const int g0 = (int)threadIdx.x / nv;
     if (g0 >= groups) return;
     for (int c = threadIdx.x - g0 * nv; c < nv; c += groups == 1 ? kRotaryThreads : nv) {
         for (int item = g0; item < ntok * a.total_heads; item += groups) {
-            const int t = item / a.total_heads;
+            const int t = a.total_heads == 1 ? item : (int)__umulhi((uint32_t)item, a.heads_inv);
             int h = item - t * a.total_heads, which = 0;
             while (which + 1 < a.nt && h >= a.t[which].heads) h -= a.t[which++].heads;
             const RotaryTensor& x = a.t[which];
-            const int64_t tok = tok0 + t, b = tok / a.N, n = tok - b * a.N;
+            const int64_t b = s_batch[t], n = s_token[t];
             const T* src = (const T*)x.src + h * x.s_head + n * x.s_token + b * x.s_batch;
             T* dst;
             if (x.paged) {
@@ -194,7 +202,9 @@ RotaryTensor tensor(const ca_seq_view* x, const ca_seq_view* y, int heads, int t
 
 int run(RotaryArgs& a, int dtype, int interleaved, cudaStream_t st) {
     for (int i = 0; i < a.nt; ++i) a.total_heads += a.t[i].heads;
-    if (!a.tokens || !a.total_heads) return CA_OK;
+    if (a.total_heads > 16384) { set_error("heads=%d: up to 16384 in one call are supported", a.total_heads); return CA_ERR_TOO_LARGE; }
+    if (!a.tokens) return CA_OK;
+    a.heads_inv = (uint32_t)(((1ULL << 32) + a.total_heads - 1) / a.total_heads);
     // Tokens of a block: as many as keep two blocks for every SM, so that the sines fill the threads of a long call and
     // a short one still spreads over the chip.
     a.per_block = kRotaryTokens;
