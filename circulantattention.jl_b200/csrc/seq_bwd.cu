@@ -24,6 +24,8 @@ template <int DM> constexpr size_t kBwdSmem = (size_t)(2 + kSlots<DM>) * kTileBy
 
 struct BwdMaps {
     CUtensorMap k, v, q, dy;
+    CUtensorMap q_rows, dy_rows, dq_rows, dk, dv;
+    int rows;               // q, dy and dq of the first sweep move by tiles of rows (maps), else by threads
     int* timeouts;
     float *dy_peak, *v_peak;    // half: largest magnitudes of each tile of 128 query rows / keys, [b][key head][tile]
     float* partial;         // [b][key head][tile][segment][dk, dv][feature][128 keys]
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     }
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
-        mbar_init(&q_full, 8);
+        mbar_init(&q_full, maps.rows ? 1 : 8);
         mbar_init(&s_full, 1);
         mbar_init(&s_free, 8);
         for (int i = 0; i < 2; ++i) { mbar_init(&dp_full[i], 1); mbar_init(&ds_full[i], 8); }
@@ -150,15 +152,25 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             };
             const int to = (int)min((int64_t)rows, (int64_t)s.n * a.G) - R0;
             uint4 w[C::kCount], y[C::kCount], e[C::kCount];
-            fetch_tile<T, DM, 256>(y, row(a.q), 0, to, a.D, tid);
-            fetch_tile<T, DM, 256>(w, row(a.dy), 0, to, a.D, tid);
-            put_tile<DM, 256>(smem, y, tid);
-            put_tile<DM, 256>(smem + TILE, w, tid);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&q_full));
+            if (!maps.rows) {
+                fetch_tile<T, DM, 256>(y, row(a.q), 0, to, a.D, tid);
+                fetch_tile<T, DM, 256>(w, row(a.dy), 0, to, a.D, tid);
+                put_tile<DM, 256>(smem, y, tid);
+                put_tile<DM, 256>(smem + TILE, w, tid);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&q_full));
+            }
             fetch_tile<T, DM, 256>(y, row(a.y), 0, to, a.D, tid);
             if (a.rest.data) fetch_tile<T, DM, 256>(e, row(a.rest), 0, to, a.D, tid);
+            if (maps.rows) {
+                warp_wait(smem_u32(&q_full), 0, stop);                         // a wait that ran out shows at the next one
+#pragma unroll
+                for (int i = 0; i < C::kCount; ++i) {
+                    w[i] = *reinterpret_cast<const uint4*>(smem + TILE + C::at(C::row(tid, i), C::piece(tid)));
+                    if (C::row(tid, i) >= to) w[i] = make_uint4(0, 0, 0, 0);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < C::kCount; ++i) {
                 if (!a.rest.data) e[i] = make_uint4(0, 0, 0, 0);
@@ -214,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 x[c + 1] = __float_as_uint(fast_exp2(e1));
             }
             uint32_t mk[2] = {~0u, ~0u};
-            const bool ragged = far >= s.n;
+            const bool ragged = far >= s.n || f_hi != p_hi;      // the tile holds keys or rows that may be anything
             const bool edge = !(far <= f_lo + a.right && far < s.n && f_hi == p_hi && (key0 >= p_hi - a.left || far < a.sinks));
             if (edge) {
                 const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
@@ -222,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 for (int g = 0; g < 2; ++g) mk[g] = seen_bits(lo - 64 * u - 32 * g, hi - 64 * u - 32 * g, sk - 64 * u - 32 * g);
 #pragma unroll
                 for (int c = 0; c < 64; ++c) x[c] = (mk[c >> 5] >> (c & 31)) & 1 ? x[c] : 0u;
-                if (ragged && u == 0) {                        // keys behind the length may be anything: zeros
+                if (far >= s.n && u == 0) {                    // keys behind the length may be anything: zeros
                     const int slot = (2 * i) % S;              // the scores are there, so the keys are
                     if (key0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
                     fence_async_smem();
@@ -268,11 +280,26 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             for (int e = 0; e < 32; ++e) y[e] = kt.count ? __uint_as_float(o[e]) * f : 0.f * f;
             put_row32<T>(smem, r, col, y);                         // the queries' place: their last scores are done
         }
+        fence_async_smem();
         group_sync<256>(1);
-        store_tile<T, DM, 256>(smem, [&](int rr) { return seq_row<T>(a.dq, a, s, h, R0 + rr); }, rows - R0, a.D, tid);
+        if (!maps.rows) {
+            store_tile<T, DM, 256>(smem, [&](int rr) { return seq_row<T>(a.dq, a, s, h, R0 + rr); }, rows - R0, a.D, tid);
+        } else if (tid == 0) {
+#pragma unroll
+            for (int p = 0; p < DM / 64; ++p) tma_store_4d(&maps.dq_rows, base_at + p * kPanel, 64 * p, h * a.G, R0 / a.G, s.b);
+            tma_stores_read();
+        }
     } else if (warp == 8 && lane == 0) {
         bool ok = true;
         int issued = 0;
+        if (maps.rows) {
+            mbar_arrive_expect_tx(smem_u32(&q_full), 2 * TILE);
+#pragma unroll
+            for (int p = 0; p < DM / 64; ++p) {
+                tma_load_4d(base_at + p * kPanel, &maps.q_rows, 64 * p, h * a.G, R0 / a.G, s.b, smem_u32(&q_full));
+                tma_load_4d(base_at + TILE + p * kPanel, &maps.dy_rows, 64 * p, h * a.G, R0 / a.G, s.b, smem_u32(&q_full));
+            }
+        }
         for (; issued < 2 * kt.count; ++issued) {
             const int slot = issued % S;
             if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
@@ -478,7 +505,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         if (count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
         fence_after();
         const float f = !ok || *stop ? __int_as_float(0x7fffffff) : u ? a.scale / c : kIsBf16<T> ? 1.f : 1.f / kPScale;       // the first warpgroup stores dv, the second dk
-        const ca_seq_view& out = u ? a.dk : a.dv;
         float* part = maps.partial + (((((int64_t)s.b * a.Hkv + h) * maps.split_tiles + tile) * maps.segments + seg) * 2 + 1 - u) * (DM * 128) + r;
         char* const stage = smem + u * TILE;                       // the keys' and values' place
 #pragma unroll 1
@@ -498,8 +524,13 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             }
         }
         if (!split) {
+            fence_async_smem();
             group_sync<128>(2 + u);
-            store_tile<T, DM, 128>(stage, [&](int rr) { return (T*)out.data + h * out.head + (int64_t)(k0 + rr) * out.token + s.b * out.batch; }, a.N - k0, a.D, r);
+            if (r == 0) {
+#pragma unroll
+                for (int p = 0; p < DM / 64; ++p) tma_store_4d(u ? &maps.dk : &maps.dv, smem_u32(stage) + p * kPanel, 64 * p, k0, h, s.b);
+                tma_stores_read();
+            }
         }
     } else if (warp == 8 && lane == 0 && count) {
         bool ok = true;
@@ -660,8 +691,13 @@ int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) 
     BwdMaps maps{};
     const bool bf16 = dtype == CA_BF16;
     int rc;
-    if ((rc = encode_tokens(&maps.k, bf16, a.k, a.D, a.Hkv, a.N, a.B, 128)) || (rc = encode_tokens(&maps.v, bf16, a.v, a.D, a.Hkv, a.N, a.B, 128)) ||
-        (rc = encode_tokens(&maps.q, bf16, a.q, a.D, a.Hq, a.N, a.B, 128)) || (rc = encode_tokens(&maps.dy, bf16, a.dy, a.D, a.Hq, a.N, a.B, 128)))
+    if ((rc = encode_tokens(&maps.k, bf16, a.k, a.D, a.Hkv, a.N, a.B)) || (rc = encode_tokens(&maps.v, bf16, a.v, a.D, a.Hkv, a.N, a.B)) ||
+        (rc = encode_tokens(&maps.q, bf16, a.q, a.D, a.Hq, a.N, a.B)) || (rc = encode_tokens(&maps.dy, bf16, a.dy, a.D, a.Hq, a.N, a.B)))
+        return rc;
+    if ((rc = encode_tokens(&maps.dk, bf16, a.dk, a.D, a.Hkv, a.N, a.B)) || (rc = encode_tokens(&maps.dv, bf16, a.dv, a.D, a.Hkv, a.N, a.B))) return rc;
+    maps.rows = rows_fit(a);
+    if (maps.rows && ((rc = encode_rows(&maps.q_rows, bf16, a.q, a)) || (rc = encode_rows(&maps.dy_rows, bf16, a.dy, a)) ||
+                      (rc = encode_rows(&maps.dq_rows, bf16, a.dq, a))))
         return rc;
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
     maps.dy_peak = parts;

@@ -27,7 +27,8 @@ template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
 template <int DM> constexpr size_t kFwdSmem = (size_t)(2 + kSlots<DM>) * kTileBytes<DM> + 1024;
 
 struct FwdMaps {
-    CUtensorMap k, v;
+    CUtensorMap k, v, q, y, rest;
+    int rows;           // q, y and rest move by tiles of rows (maps), else by threads
     int box;            // paged: keys of a box
     int* timeouts;
 };
@@ -104,13 +105,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     const Stream st0 = stream_of<PAIR>(a, s, kt, 0, R0, rows), st1 = stream_of<PAIR>(a, s, kt, 1, PAIR ? R0 + 128 : R0, rows);
 
     if (warp == 8 && lane == 0) {
+        if (maps.rows) prefetch_map(&maps.q);
         prefetch_map(&maps.k);
         prefetch_map(&maps.v);
     }
     if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
         for (int u = 0; u < 2; ++u) {
-            mbar_init(&q_full[u], PAIR ? 4 : 8);
+            mbar_init(&q_full[u], maps.rows ? 1 : PAIR ? 4 : 8);
             mbar_init(&s_full[u], 1);
             mbar_init(&p_full[u][0], 4);
             mbar_init(&p_full[u][1], 4);
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         const int R = R0 + (PAIR ? 128 * u : 0) + r;
         const int pos = s.base + token_of(a, R);
         const bool have = R < rows, live = have && pos >= 0 && pos < s.n;
-        {
+        if (!maps.rows) {
             const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;        // scores use the scale's magnitude
             // rows of the tile that exist: those of positions 0 .. n - 1
             const int tile0 = R - r;
@@ -274,10 +276,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         fence_after();
 
         // ------------------------------------------------------------ results
-        float inv, f0 = 1.f, f1 = 0.f;
+        float f0 = 1.f, f1 = 0.f;
         float* const other = reinterpret_cast<float*>(smem + 2 * TILE);    // [column][row] of the odd stream, in the ring's place
+        const bool keep_rest = !PAGED && a.rest.data;
+        if (!PAIR || keep_rest) group_sync<256>(1);                        // both streams are through with the ring
         if (!PAIR) {
-            asm volatile("bar.sync 1, 256;" ::: "memory");                 // both streams are through with the ring
             if (u == 1) {
                 merge_m[r] = m;
                 merge_l[r] = l;
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     }
                 }
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            group_sync<256>(1);
             const float m1 = merge_m[r], l1 = merge_l[r], M = fmaxf(m, m1), ref = M == -INFINITY ? 0.f : M;
             f0 = fast_exp2(m - ref);
             f1 = fast_exp2(m1 - ref);
@@ -301,46 +304,71 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             m = M;
         }
         if (PAIR || u == 0) {
-            inv = l > 0.f ? 1.f / l : 0.f;
+            float inv = l > 0.f ? 1.f / l : 0.f;
             if (!ok || *stop) inv = __int_as_float(0x7fffffff);            // a wait ran out: NaN, never a wrong number
             const bool both = !PAIR && kt.count > 1;
             if (!PAGED && a.lse && have) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = l > 0.f ? m + log2f(l) : -INFINITY;
             const float w0 = f0 * inv, w1 = f1 * inv;
-            char* const out = smem + (PAIR ? u : 0) * TILE;                // the queries' place: their last scores are done
-            for (int pass = 0; pass < (!PAGED && a.rest.data ? 2 : 1); ++pass) {
-                if (pass) group_sync<128>(2 + u);
+            // y goes to the queries' place (their last scores are done), what rounding took to a slot of the ring
+            const int tile0 = R - r;
+            char *const out = smem + (PAIR ? u : 0) * TILE, *const out_rest = smem + (2 + (PAIR ? u : 2)) * TILE;
 #pragma unroll 1
-                for (int c = 0; c < DM; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(O_at + c, o);
-                    tmem_wait_ld();
-                    settled32(o);
-                    float y[32];
+            for (int c = 0; c < DM; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(O_at + c, o);
+                tmem_wait_ld();
+                settled32(o);
+                float y[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * w0;
-                    if (!done) {
+                for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * w0;
+                if (!done) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] = 0.f * inv;
-                    }
-                    if (both) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] = fmaf(other[(c + e) * 128 + r], w1, y[e]);
-                    }
-                    if (pass) {                                            // what rounding took
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) y[e] -= to_float(from_float<T>(y[e]));
-                    }
-                    put_row32<T>(out, r, c, y);
+                    for (int e = 0; e < 32; ++e) y[e] = 0.f * inv;
                 }
-                group_sync<128>(2 + u);
-                const ca_seq_view& view = pass ? a.rest : a.y;
-                store_tile<T, DM, 128>(out, [&](int rr) { return seq_row<T>(view, a, s, h, max(R - r + rr, 0)); }, rows - (R - r), a.D, r);
+                if (both) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) y[e] = fmaf(other[(c + e) * 128 + r], w1, y[e]);
+                }
+                put_row32<T>(out, r, c, y);
+                if (keep_rest) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) y[e] -= to_float(from_float<T>(y[e]));
+                    put_row32<T>(out_rest, r, c, y);
+                }
+            }
+            fence_async_smem();
+            group_sync<128>(2 + u);
+            // by maps, which leave out tokens behind the tensor's; a cache's packed rows go on with the next sequence
+            if (maps.rows && (!PAGED || tile0 + 128 <= rows)) {
+                if (r == 0 && tile0 < rows) {
+                    const int token = s.t0 + tile0 / a.G, b = PAGED ? 0 : s.b;
+#pragma unroll
+                    for (int p = 0; p < DM / 64; ++p) {
+                        tma_store_4d(&maps.y, smem_u32(out) + p * kPanel, 64 * p, h * a.G, token, b);
+                        if (keep_rest) tma_store_4d(&maps.rest, smem_u32(out_rest) + p * kPanel, 64 * p, h * a.G, token, b);
+                    }
+                    tma_stores_read();
+                }
+            } else {
+                auto row = [&](const ca_seq_view& v) { return [&](int rr) { return seq_row<T>(v, a, s, h, max(tile0 + rr, 0)); }; };
+                store_tile<T, DM, 128>(out, row(a.y), rows - tile0, a.D, r);
+                if (keep_rest) store_tile<T, DM, 128>(out_rest, row(a.rest), rows - tile0, a.D, r);
             }
         }
     } else if (warp == 8) {
         // ------------------------------------------------------------ copies
         bool ok = true;
         int issued = 0;
+        if (maps.rows && lane == 0) {
+            for (int u = 0; u < (PAIR ? 2 : 1); ++u) {
+                if (R0 + 128 * u >= rows) break;
+                mbar_arrive_expect_tx(smem_u32(&q_full[u]), TILE);
+#pragma unroll
+                for (int p = 0; p < DM / 64; ++p)
+                    tma_load_4d(q_at + u * TILE + p * kPanel, &maps.q, 64 * p, h * a.G, s.t0 + (R0 + 128 * u) / a.G, PAGED ? 0 : s.b, smem_u32(&q_full[u]));
+            }
+        }
+        __syncwarp();
         if (!PAGED) {
             if (lane == 0) {
                 for (; issued < 2 * kt.count; ++issued) {
@@ -380,6 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 }
             }
         }
+        if (maps.rows && lane == 0)                                        // also where no key tile waits for them
+            for (int u = 0; u < (PAIR ? 2 : 1) && R0 + 128 * u < rows; ++u) mbar_wait(smem_u32(&q_full[u]), 0, 1u << 12);
         if (!ok && lane == 0)                                              // copies in flight land before the memory goes away
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
     } else if (warp == 9) {
@@ -498,11 +528,28 @@ int encode_swizzled_map(CUtensorMap* map, bool bf16, const void* base, int rank,
     return CA_OK;
 }
 
-int encode_tokens(CUtensorMap* m, bool bf16, const ca_seq_view& v, int D, int heads, int tokens, int batch, int box_tokens) {
+int encode_tokens(CUtensorMap* m, bool bf16, const ca_seq_view& v, int D, int heads, int tokens, int batch) {
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)tokens, (uint64_t)heads, (uint64_t)batch};
     const uint64_t strides[3] = {(uint64_t)v.token * 2, (uint64_t)v.head * 2, (uint64_t)v.batch * 2};
-    const uint32_t box[4] = {64, (uint32_t)box_tokens, 1, 1};
+    const uint32_t box[4] = {64, 128, 1, 1};
     return encode_swizzled_map(m, bf16, v.data, 4, dims, strides, box);
+}
+
+int encode_rows(CUtensorMap* m, bool bf16, const ca_seq_view& v, const SeqArgs& a) {
+    const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)a.Hq, (uint64_t)a.N, (uint64_t)a.B};
+    const uint64_t strides[3] = {(uint64_t)v.head * 2, (uint64_t)v.token * 2, (uint64_t)(a.pages.table ? 16 : v.batch * 2)};
+    const uint32_t box[4] = {64, (uint32_t)a.G, (uint32_t)(128 / a.G), 1};
+    return encode_swizzled_map(m, bf16, v.data, 4, dims, strides, box);
+}
+
+// Maps of q, y and what rounding took, where tiles of rows are boxes; a negative scale turns the signs of q on the way.
+static int encode_row_maps(FwdMaps* maps, bool bf16, const SeqArgs& a) {
+    maps->rows = rows_fit(a) && !(a.scale < 0.f);
+    if (!maps->rows) return CA_OK;
+    int rc = encode_rows(&maps->q, bf16, a.q, a);
+    if (!rc) rc = encode_rows(&maps->y, bf16, a.y, a);
+    if (!rc && a.rest.data) rc = encode_rows(&maps->rest, bf16, a.rest, a);
+    return rc;
 }
 
 // Two row tiles a CTA share the key tiles; where that leaves SMs idle, one row tile and two streams over its keys.
@@ -510,7 +557,9 @@ int umma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st) {
     FwdMaps maps{};
     const bool bf16 = dtype == CA_BF16;
     int rc;
-    if ((rc = encode_tokens(&maps.k, bf16, a.k, a.D, a.Hkv, a.N, a.B, 128)) || (rc = encode_tokens(&maps.v, bf16, a.v, a.D, a.Hkv, a.N, a.B, 128))) return rc;
+    if ((rc = encode_tokens(&maps.k, bf16, a.k, a.D, a.Hkv, a.N, a.B)) || (rc = encode_tokens(&maps.v, bf16, a.v, a.D, a.Hkv, a.N, a.B)) ||
+        (rc = encode_row_maps(&maps, bf16, a)))
+        return rc;
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
     const int64_t rows = (int64_t)a.N * a.G;
     const bool pair = (rows + 255) / 256 * a.Hkv * a.B >= sm_count();
@@ -532,6 +581,8 @@ int umma_paged(const SeqArgs& a, int dtype, cudaStream_t st) {
         const int rc = encode_swizzled_map(i ? &maps.v : &maps.k, bf16, p.data, 4, dims, strides, b);
         if (rc) return rc;
     }
+    const int rc = encode_row_maps(&maps, bf16, a);
+    if (rc) return rc;
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
     const bool pair = paged_tiles(a.N, a.G, a.pages.sequences, 256) * a.Hkv >= sm_count() && (int64_t)a.N * a.G > 128LL * a.pages.sequences;
     const int64_t tiles = paged_tiles(a.N, a.G, a.pages.sequences, pair ? 256 : 128);

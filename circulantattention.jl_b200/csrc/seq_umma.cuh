@@ -105,8 +105,23 @@ __device__ __forceinline__ void report_stop(int* timeouts, int* status) {
     if (status) atomicOr(status, 1);
 }
 
-// Dense keys (D, tokens, heads, batch), boxes of 64 features and 128 tokens.
-int encode_tokens(CUtensorMap* m, bool bf16, const ca_seq_view& v, int D, int heads, int tokens, int batch, int box_tokens);
+// One head's tokens, (D, tokens, heads, batch): boxes of 64 features and 128 tokens, coordinates (feature, token, head, batch).
+int encode_tokens(CUtensorMap* m, bool bf16, const ca_seq_view& v, int D, int heads, int tokens, int batch);
+// Tiles of 128 packed rows, (D, heads, tokens, batch): boxes of 64 features, the G heads of a group and 128 / G tokens.
+// G divides 128 (rows_fit); with other groups rows are copied by threads.
+static inline bool rows_fit(const SeqArgs& a) { return 128 % a.G == 0; }
+int encode_rows(CUtensorMap* m, bool bf16, const ca_seq_view& v, const SeqArgs& a);
+
+// Stores a tile (as put_row32 leaves it) through a map; one thread, after fence_async_smem and a barrier of the writers.
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+                 ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+// The stores of this thread have read their shared memory.
+__device__ __forceinline__ void tma_stores_read() {
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
 
 // seq_fwd.cu
 int umma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st);
