@@ -63,6 +63,13 @@ __device__ __forceinline__ void read64(uint32_t at, uint32_t* x) {
     settled32(x + 32);
 }
 
+// Zeros where the bit is not set.  Always in a block of its own behind one uniform branch: as a condition on each element the
+// selects ran for every tile and took as long as the arithmetic.
+__device__ __forceinline__ void clear_unseen(uint32_t* x, const uint32_t* mk) {
+#pragma unroll
+    for (int c = 0; c < 64; ++c) x[c] = (mk[c >> 5] >> (c & 31)) & 1 ? x[c] : 0u;
+}
+
 template <int DM>
 __device__ __forceinline__ void clear_row(char* tile, int r) {
 #pragma unroll
@@ -232,8 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
 #pragma unroll
                 for (int g = 0; g < 2; ++g) mk[g] = seen_bits(lo - 64 * u - 32 * g, hi - 64 * u - 32 * g, sk - 64 * u - 32 * g);
-#pragma unroll
-                for (int c = 0; c < 64; ++c) x[c] = (mk[c >> 5] >> (c & 31)) & 1 ? x[c] : 0u;
+                clear_unseen(x, mk);
                 if (far >= s.n && u == 0) {                    // keys behind the length may be anything: zeros
                     const int slot = (2 * i) % S;              // the scores are there, so the keys are
                     if (key0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
@@ -249,12 +255,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             for (int c = 0; c < 64; c += 2) {
                 float e0, e1;
                 unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, dl2), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e0, e1);
-                if (ragged) {                                  // dP of such keys may be anything
-                    e0 = (mk[c >> 5] >> (c & 31)) & 1 ? e0 : 0.f;
-                    e1 = (mk[c >> 5] >> (c & 31)) & 2 ? e1 : 0.f;
-                }
-                w[c >> 1] = pack16<T>(e0, e1);
+                y[c] = __float_as_uint(e0);
+                y[c + 1] = __float_as_uint(e1);
             }
+            if (ragged) clear_unseen(y, mk);                   // dP of such pairs may be anything
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
             tmem_st32(dp_at, w);
             tmem_wait_st();
             fence_before();
@@ -356,6 +362,15 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
 }
 
 // ---------------------------------------------------------------- dk, dv
+// The steps of a key tile: token tiles outside, query heads of the group inside.
+struct Steps {
+    int q0, g;
+    __device__ __forceinline__ Steps(const SeqArgs& a, int t_lo, int first) : q0(t_lo + first / a.G * 128), g(first % a.G) {}
+    __device__ __forceinline__ void next(const SeqArgs& a) {
+        if (++g == a.G) g = 0, q0 += 128;
+    }
+};
+
 // Tiles are transposed: lanes are the CTA's 128 keys, columns 128 tokens of one query head.  Tensor memory: scores 0..127, dP
 // 128..255, dv from 256, dk behind it.  The order of the products keeps them running: dv(i), scores(i+1), dk(i), dP(i+1);
 // the weights of i + 1 are made during the last two, dS(i) during the first two.
@@ -432,8 +447,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
         const f32x2 c2 = kIsBf16<T> ? pack2(1.f, 1.f) : pack2(c / kPScale, c / kPScale);
         bool ok = true;
-        for (int i = 0; i < count; ++i) {
-            const int step = first + i, q0 = t_lo + step / a.G * 128, b = i & 1;
+        Steps at(a, t_lo, first);
+        for (int i = 0; i < count; ++i, at.next(a)) {
+            const int q0 = at.q0, b = i & 1;
             const bool ragged = q0 + 127 >= s.n || k0 + 127 >= s.n;
             const bool edge = !(k0 + 127 <= q0 + a.right && (q0 + 127 <= k0 + a.left || k0 + 127 < a.sinks) && q0 + 127 < s.n && k0 + 127 < s.n);
             if (!warp_wait(smem_u32(&st_full[b]), (i >> 1) & 1, stop) || !warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
@@ -455,14 +471,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack2(z.x, z.y)), e[0], e[1]);
                 unpack2(fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), sc2, pack2(z.z, z.w)), e[2], e[3]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    e[k] = fast_exp2(e[k]);
-                    if (edge) e[k] = (mk[c >> 5] >> ((c & 31) + k)) & 1 ? e[k] : 0.f;
-                    x[c + k] = __float_as_uint(e[k]);
-                }
-                w[c >> 1] = pack16<T>(e[0], e[1]);
-                w[(c >> 1) + 1] = pack16<T>(e[2], e[3]);
+                for (int k = 0; k < 4; ++k) x[c + k] = __float_as_uint(fast_exp2(e[k]));
             }
+            if (edge) clear_unseen(x, mk);
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(x[c]), __uint_as_float(x[c + 1]));
             tmem_st32(S_at, w);
             if (ragged && q0 + 127 >= s.n) {                    // queries behind the length may be anything: zeros
                 const int slot = (2 * i + u) % S;               // one warpgroup clears q, the other dy
@@ -488,11 +501,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, pack2(z.x, z.y)), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e[0], e[1]);
                 unpack2(mul2(fma2(pack2(__uint_as_float(y[c + 2]), __uint_as_float(y[c + 3])), c2, pack2(z.z, z.w)), pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3]))), e[2], e[3]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (ragged) e[k] = (mk[c >> 5] >> ((c & 31) + k)) & 1 ? e[k] : 0.f;    // dP of such pairs may be anything
-                w[c >> 1] = pack16<T>(e[0], e[1]);
-                w[(c >> 1) + 1] = pack16<T>(e[2], e[3]);
+                for (int k = 0; k < 4; ++k) y[c + k] = __float_as_uint(e[k]);
             }
+            if (ragged) clear_unseen(y, mk);                    // dP of such pairs may be anything
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
             tmem_st32(dp_at, w);
             tmem_wait_st();
             fence_before();
@@ -541,14 +554,16 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             tma_load_4d(base_at + p * kPanel, &maps.k, 64 * p, k0, h, s.b, smem_u32(&kv_full));
             tma_load_4d(base_at + TILE + p * kPanel, &maps.v, 64 * p, k0, h, s.b, smem_u32(&kv_full));
         }
+        Steps at(a, t_lo, first);
         for (; issued < 2 * count; ++issued) {
-            const int slot = issued % S, step = first + (issued >> 1), q0 = t_lo + step / a.G * 128;
+            const int slot = issued % S;
             if (!wait_or_stop(smem_u32(&q_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
             const uint32_t bar = smem_u32(&q_full[slot]), dst = ring_at + slot * TILE;
             mbar_arrive_expect_tx(bar, TILE);
 #pragma unroll
             for (int p = 0; p < DM / 64; ++p)
-                tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.dy : &maps.q, 64 * p, q0, h * a.G + step % a.G, s.b, bar);
+                tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.dy : &maps.q, 64 * p, at.q0, h * a.G + at.g, s.b, bar);
+            if (issued & 1) at.next(a);
         }
         if (!ok) {                                             // copies in flight land before the memory goes away
             mbar_wait(smem_u32(&kv_full), 0, 1u << 12);
@@ -599,15 +614,16 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         const float shift = kIsBf16<T> ? 0.f : kPLog2, minus = kIsBf16<T> ? -1.f : -c / kPScale;
         const int rows = s.T * a.G;
         const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
-        for (int i = 0; i < count; ++i) {
-            const int step = first + i, q0 = t_lo + step / a.G * 128, b = i & 1;
+        Steps at(a, t_lo, first);
+        for (int i = 0; i < count; ++i, at.next(a)) {
+            const int b = i & 1;
             float z[4], d[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int t = q0 + lane + 32 * k;
+                const int t = at.q0 + lane + 32 * k;
                 const bool in = t < s.n;
-                z[k] = in ? shift - a.lse[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
-                d[k] = in ? minus * a.delta[stat0 + (int64_t)t * a.G + step % a.G] : 0.f;
+                z[k] = in ? shift - a.lse[stat0 + (int64_t)t * a.G + at.g] : 0.f;
+                d[k] = in ? minus * a.delta[stat0 + (int64_t)t * a.G + at.g] : 0.f;
             }
             if (!warp_wait(smem_u32(&st_empty[b]), ((i >> 1) & 1) ^ 1, stop)) break;
 #pragma unroll
