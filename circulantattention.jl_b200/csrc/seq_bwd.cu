@@ -49,10 +49,10 @@ __device__ __forceinline__ float warp_max(float x) {
     return x;
 }
 
-// A operand whose two halves of 64 contracted elements lie 64 columns apart.
-__device__ __forceinline__ void mma_halves(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+// A operand whose two halves of 64 contracted elements lie `apart` columns apart.
+__device__ __forceinline__ void mma_halves(uint32_t lead, uint32_t d, uint32_t a, uint32_t apart, uint64_t b, uint32_t idesc, bool add) {
     mma_weighted<64>(lead, d, a, b, idesc, add);
-    mma_weighted<64>(lead, d, a + 64, b + 4 * 128, idesc, true);
+    mma_weighted<64>(lead, d, a + apart, b + 4 * 128, idesc, true);
 }
 
 __device__ __forceinline__ void read64(uint32_t at, uint32_t* x) {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     constexpr uint32_t TILE = kTileBytes<DM>;
     constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
     extern __shared__ char raw[];
-    __shared__ uint64_t kv_full[S], kv_empty[S], q_full, s_full, s_free, dp_full[2], ds_full[2], o_full, drained;
+    __shared__ uint64_t kv_full[S], kv_empty[S], q_full, s_full, s_free, dp_full[2], ds_full[2], dq_done, o_full, drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int stop_flag;
     __shared__ float part[2][128], warp_peak[4];
@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         mbar_init(&s_full, 1);
         mbar_init(&s_free, 8);
         for (int i = 0; i < 2; ++i) { mbar_init(&dp_full[i], 1); mbar_init(&ds_full[i], 8); }
+        mbar_init(&dq_done, 1);
         mbar_init(&o_full, 1);
         mbar_init(&drained, 1);
         stop_flag = 0;
@@ -331,7 +332,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             fence_after();
             mma_dot<DM>(lead, tmem, q_desc, f_desc + ks * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&s_full));
-            if (!landed(2 * i + 2)) return false;
+            // dP goes where dS of two tiles before is; with 64 features the product that reads it has another shape than this one,
+            // and products of different shapes need not keep their order
+            if (!landed(2 * i + 2) || (DM == 64 && i > 1 && !warp_wait(smem_u32(&dq_done), i & 1, stop))) return false;
             fence_after();
             mma_dot<DM>(lead, tmem + 128 + (i & 1) * 128, dy_desc, f_desc + vs * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&dp_full[i & 1]));
@@ -348,8 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             if (!ok) break;
             fence_after();
             const uint32_t ks = (2 * i) % S;
-            mma_halves(lead, o_col, tmem + 128 + (i & 1) * 128, r_desc + ks * (TILE >> 4), IDESC_O, i != 0);
+            mma_halves(lead, o_col, tmem + 128 + (i & 1) * 128, 64, r_desc + ks * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&kv_empty[ks]));
+            if (DM == 64) mma_commit(lead, smem_u32(&dq_done));
         }
         mma_commit(lead, smem_u32(ok ? &o_full : &drained));
         if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
@@ -431,6 +435,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot, dv_col = tmem + 256, dk_col = tmem + 256 + DM;
+    // At 64 features the weights and dS have columns of their own; at 128 they overlay what they are made of, and the products of
+    // one shape (all 128 x 128 x 16 there) are carried out in the order of their issue.
+    const uint32_t p_col = DM == 64 ? tmem + 384 : tmem, ds_col = p_col + (DM == 64 ? 64 : 128), apart = DM == 64 ? 32 : 64;
     float c = 1.f;                                                  // factor of dS
     if (!kIsBf16<T> && count) {
         const int tiles = (int)(((int64_t)s.T * a.G + 127) / 128);
@@ -443,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     if (warp < 8) {
         const int u = warp >> 2, r = tid & 127, j = k0 + r;
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
-        const uint32_t S_at = tmem + 64 * u + lane_off, dp_at = S_at + 128;
+        const uint32_t S_at = tmem + 64 * u + lane_off, dp_at = S_at + 128, P_at = p_col + apart * u + lane_off, ds_at = ds_col + apart * u + lane_off;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
         const f32x2 c2 = kIsBf16<T> ? pack2(1.f, 1.f) : pack2(c / kPScale, c / kPScale);
         bool ok = true;
@@ -476,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             if (edge) clear_unseen(x, mk);
 #pragma unroll
             for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(x[c]), __uint_as_float(x[c + 1]));
-            tmem_st32(S_at, w);
+            tmem_st32(P_at, w);
             if (ragged && q0 + 127 >= s.n) {                    // queries behind the length may be anything: zeros
                 const int slot = (2 * i + u) % S;               // one warpgroup clears q, the other dy
                 if (!warp_wait(smem_u32(&q_full[slot]), ((2 * i + u) / S) & 1, stop)) { ok = false; break; }
@@ -506,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             if (ragged) clear_unseen(y, mk);                    // dP of such pairs may be anything
 #pragma unroll
             for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
-            tmem_st32(dp_at, w);
+            tmem_st32(ds_at, w);
             tmem_wait_st();
             fence_before();
             __syncwarp();
@@ -598,12 +605,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             const bool more = i + 1 < steps;
             if (!(ok = (!more || landed(2 * i + 3)) && warp_wait(smem_u32(&p_full), i & 1, stop))) break;
             fence_after();
-            mma_halves(lead, dv_col, tmem, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
+            mma_halves(lead, dv_col, p_col, apart, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&q_empty[ds]));
             if (more) scores(i + 1);
             if (!(ok = (!more || landed(2 * i + 4)) && warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
             fence_after();
-            mma_halves(lead, dk_col, tmem + 128, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
+            mma_halves(lead, dk_col, ds_col, apart, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&q_empty[qs]));
             if (more) dprobs(i + 1);
         }

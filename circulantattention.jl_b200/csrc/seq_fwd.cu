@@ -127,7 +127,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;
-    const uint32_t s_col = tmem, o_col = tmem + 256;
+    // Scores of both streams, then their accumulators.  At 64 features there is room for weights beside the scores; at 128 they
+    // overlay them, which needs the next scores to be written after the product with the weights has read them: products of
+    // one shape (both 128 x 128 x 16 there) are carried out in the order of their issue.
+    const uint32_t s_col = tmem, o_col = tmem + 256, p_col = DM == 64 ? tmem + 384 : s_col, p_step = DM == 64 ? 64 : 128;
 
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax: thread = row
@@ -155,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             if (lane == 0) mbar_arrive(smem_u32(&q_full[PAIR ? u : 0]));
         }
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;              // lane 32 * (warp % 4) in bits 16..
-        const uint32_t S_at = s_col + u * 128 + lane_off, O_at = o_col + u * DM + lane_off;
+        const uint32_t S_at = s_col + u * 128 + lane_off, P_at = p_col + u * p_step + lane_off, O_at = o_col + u * DM + lane_off;
         const float sl2 = a.mag_log2;
         const int c_lo = p_lo - a.left, c_hi = min(p_hi + a.right, s.n - 1);   // keys that any row of the CTA sees (or < sinks)
         // tiles from in_lo (or below in_sink) to in_hi need no mask
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     sum2 = add2(sum2, pack2(e0, e1));
                     w[c] = pack16<T>(e0, e1);
                 }
-                tmem_st32(S_at + 32 * g, w);                               // over scores that this warp has read twice
+                tmem_st32(P_at + 32 * g, w);                               // at 128 features over scores that this warp has read twice
                 tmem_wait_st();
                 fence_before();
                 __syncwarp();
@@ -443,10 +446,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             // that came before (a stream is at most two tiles ahead, and the ring holds five).
             if (!landed(nx <= st.upto ? 2 * nx : 2 * i + 1) || !warp_wait(smem_u32(&p_full[u][0]), n & 1, stop)) return false;
             fence_after();
-            mma_weighted<64>(lead, o_col + u * DM, s_col + u * 128, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
+            mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
             if (!warp_wait(smem_u32(&p_full[u][1]), n & 1, stop)) return false;
             fence_after();
-            mma_weighted<64>(lead, o_col + u * DM, s_col + u * 128 + 32, v_desc + slot * (TILE >> 4) + 4 * 128, IDESC_O, true);
+            mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step + 32, v_desc + slot * (TILE >> 4) + 4 * 128, IDESC_O, true);
             if (!PAIR || u == 1 || !st1.takes(i)) mma_commit(lead, smem_u32(&kv_empty[slot]));
             if (nx > st.upto) mma_commit(lead, smem_u32(&o_full[u]));
             ++n;
