@@ -63,7 +63,7 @@ template <typename T, int DM>
 __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_constant__ SeqArgs a) {
     typedef Decode<T, DM> L;
     extern __shared__ __align__(128) char smem[];
-    __shared__ float part_m[kWarps][kRows], part_l[kWarps][kRows];
+    __shared__ float part_m[kWarps][kRows], part_l[kWarps][kRows], row_m[kRows], row_l[kRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -78,57 +78,62 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
 
     // ------------------------------------------------------------ copies: tile i of this warp into stage `st`
     const uint32_t ring = smem_u32(smem) + warp * L::kStages * L::kStageBytes;
-    const int piece = lane % L::kPieces, row0 = lane / L::kPieces;
+    const int piece = lane % L::kPieces, row0 = lane / L::kPieces, feature = piece * (16 / (int)sizeof(T));
     constexpr int STEP = 32 / L::kPieces > 0 ? 32 / L::kPieces : 1;
-    auto page_at = [&](int i) { return i < last ? page_of(a, s.b, kt.key(i, kKeys)) : -1; };
+    const char* const k_lane = (const char*)((const T*)a.kp.data + h * a.kp.head + row0 * a.kp.token + feature);
+    const char* const v_lane = (const char*)((const T*)a.vp.data + h * a.vp.head + row0 * a.vp.token + feature);
+    const int64_t k_step = STEP * a.kp.token * (int64_t)sizeof(T), v_step = STEP * a.vp.token * (int64_t)sizeof(T);
     auto copy_tile = [&](int i, int st, int page) {
         if (page >= 0) {
             const int key0 = kt.key(i, kKeys), off = key0 % a.pages.page;
-            const T* k = (const T*)a.kp.data + h * a.kp.head + off * a.kp.token + page * a.kp.page;
-            const T* v = (const T*)a.vp.data + h * a.vp.head + off * a.vp.token + page * a.vp.page;
+            const char* k = k_lane + (off * a.kp.token + page * a.kp.page) * (int64_t)sizeof(T);
+            const char* v = v_lane + (off * a.vp.token + page * a.vp.page) * (int64_t)sizeof(T);
             const uint32_t to = ring + st * L::kStageBytes;
-            const int f = piece * (16 / (int)sizeof(T));
+            const bool all = feature < a.D && key0 + kKeys - 1 <= c_hi && (key0 >= c_lo || key0 + kKeys <= a.sinks);
 #pragma unroll
-            for (int r = 0; r < kKeys; r += STEP) {
+            for (int r = 0; r < kKeys; r += STEP, k += k_step, v += v_step) {
                 const int j = key0 + r + row0;
-                const bool on = f < a.D && j <= c_hi && (j >= c_lo || j < a.sinks);      // what no row sees counts as zeros
-                copy16(to + L::at(r + row0, piece), on ? k + (r + row0) * a.kp.token + f : (const T*)a.kp.data, on);
-                copy16(to + kKeys * L::kRowBytes + L::at(r + row0, piece), on ? v + (r + row0) * a.vp.token + f : (const T*)a.vp.data, on);
+                const bool on = all || (feature < a.D && j <= c_hi && (j >= c_lo || j < a.sinks));      // what no row sees counts as zeros
+                copy16(to + L::at(r + row0, piece), on ? k : (const char*)a.kp.data, on);
+                copy16(to + kKeys * L::kRowBytes + L::at(r + row0, piece), on ? v : (const char*)a.vp.data, on);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // pages of the tiles whose copies are under way, and of the one behind them, which is looked up a step early
-    int pages[L::kStages];
-    {
-        int i = first + warp;
+    // Pages of the warp's tiles, 32 at a time: lane k has that of tile first + warp + 4 (32 c + k), and those of the next 32
+    // are on their way.
+    auto page_at = [&](int n) {
+        const int i = first + warp + kWarps * n;
+        return i < last ? page_of(a, s.b, kt.key(i, kKeys)) : -1;
+    };
+    int page_now = page_at(lane), page_next = page_at(32 + lane);
+    auto page = [&](int n) { return __shfl_sync(~0u, n & 32 ? page_next : page_now, n & 31); };      // n is at most 31 behind the first of now
 #pragma unroll
-        for (int st = 0; st < L::kStages - 1; ++st, i += kWarps) {
-            pages[st] = page_at(i);
-            copy_tile(i, st, pages[st]);
-        }
-        pages[L::kStages - 1] = page_at(i);
-    }
+    for (int st = 0; st < L::kStages - 1; ++st) copy_tile(first + warp + kWarps * st, st, page(st));
 
     float m[sizeof(T) == 4 ? 8 : 2], l[sizeof(T) == 4 ? 8 : 2];
     constexpr int STATS = sizeof(T) == 4 ? 8 : 2;
 #pragma unroll
     for (int i = 0; i < STATS; ++i) m[i] = -INFINITY, l[i] = 0.f;
-    // f(keys, values, key0) for each of the warp's tiles that exists
+    // body(tile in shared memory, key0) for each of the warp's tiles that exists
     auto for_tiles = [&](auto body) {
-        int st = 0, ahead = L::kStages - 1;
+        int st = 0, ahead = L::kStages - 1, n = 0, first32 = 0;
         for (int i = first + warp; i < last; i += kWarps) {
-            const int next = i + (L::kStages - 1) * kWarps, behind = page_at(next + kWarps);
-            copy_tile(next, ahead, pages[L::kStages - 1]);
+            const int next = n + L::kStages - 1;
+            copy_tile(first + warp + kWarps * (first32 + next), ahead, page(next));
+            const int now = page(n);
             asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
             __syncwarp();
-            if (pages[0] >= 0) body(smem + warp * L::kStages * L::kStageBytes + st * L::kStageBytes, kt.key(i, kKeys));
+            if (now >= 0) body(smem + warp * L::kStages * L::kStageBytes + st * L::kStageBytes, kt.key(i, kKeys));
             __syncwarp();
-#pragma unroll
-            for (int k = 0; k + 1 < L::kStages; ++k) pages[k] = pages[k + 1];
-            pages[L::kStages - 1] = behind;
             st = st + 1 == L::kStages ? 0 : st + 1;
             ahead = ahead + 1 == L::kStages ? 0 : ahead + 1;
+            if (++n == 32) {                                    // numbers count from the first of these 32 tiles
+                n = 0;
+                first32 += 32;
+                page_now = page_next;
+                page_next = page_at(first32 + 32 + lane);
+            }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     };
@@ -318,40 +323,56 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
             for (int c = 0; c < C; ++c) parts[r * DM + lane * C + c] = o[r][c];
     }
 
-    // ------------------------------------------------------------ join the warps of all CTAs: four features a thread
+    // ------------------------------------------------------------ join: the CTA's warps, then the CTAs; four features a thread
+    __syncthreads();
+    auto put = [&](int r, int f, float4 y, float inv) {
+        if (f >= a.D) return;
+        T* dst = seq_row<T>(a.y, a, s, h, R0 + r) + f;
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(y.x * inv, y.y * inv), pack16<T>(y.z * inv, y.w * inv));
+        else
+            *reinterpret_cast<float4*>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    };
+    auto add = [](float4& y, float4 x, float g) { y.x = fmaf(x.x, g, y.x); y.y = fmaf(x.y, g, y.y); y.z = fmaf(x.z, g, y.z); y.w = fmaf(x.w, g, y.w); };
+    const int items = nrows * (DM / 4);
+    float* const all = reinterpret_cast<float*>(smem);          // [warp][row][feature]; the sum takes the first warp's place
+    for (int i = tid; i < items; i += 32 * kWarps) {
+        const int r = i / (DM / 4), f = i % (DM / 4) * 4;
+        float M = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, part_m[w][r]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float g = fast_exp2(part_m[w][r] - ref);
+            sum = fmaf(part_l[w][r], g, sum);
+            add(y, *reinterpret_cast<const float4*>(all + (w * kRows + r) * DM + f), g);
+        }
+        if (ranks == 1) {
+            put(r, f, y, sum > 0.f ? 1.f / sum : 0.f);
+        } else {
+            *reinterpret_cast<float4*>(all + r * DM + f) = y;
+            if (f == 0) { row_m[r] = M; row_l[r] = sum; }
+        }
+    }
+    if (ranks == 1) return;
     cluster.sync();
-    const int items = nrows * (DM / 4), begin = items * rank / ranks, end = items * (rank + 1) / ranks;
+    const int begin = items * rank / ranks, end = items * (rank + 1) / ranks;
     for (int i = begin + tid; i < end; i += 32 * kWarps) {
         const int r = i / (DM / 4), f = i % (DM / 4) * 4;
-        float M = -INFINITY;
-        for (int c = 0; c < ranks; ++c) {
-            const float* pm = cluster.map_shared_rank(&part_m[0][0], c);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, pm[w * kRows + r]);
-        }
+        float M = -INFINITY, sum = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < ranks; ++c) M = fmaxf(M, *cluster.map_shared_rank(&row_m[r], c));
         const float ref = M == -INFINITY ? 0.f : M;
-        float sum = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int c = 0; c < ranks; ++c) {
-            const float* pm = cluster.map_shared_rank(&part_m[0][0], c);
-            const float* pl = cluster.map_shared_rank(&part_l[0][0], c);
-            const float* po = cluster.map_shared_rank(reinterpret_cast<float*>(smem), c);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float g = fast_exp2(pm[w * kRows + r] - ref);
-                const float4 x = *reinterpret_cast<const float4*>(po + (w * kRows + r) * DM + f);
-                sum = fmaf(pl[w * kRows + r], g, sum);
-                y.x = fmaf(x.x, g, y.x); y.y = fmaf(x.y, g, y.y); y.z = fmaf(x.z, g, y.z); y.w = fmaf(x.w, g, y.w);
-            }
+            const float g = fast_exp2(*cluster.map_shared_rank(&row_m[r], c) - ref);
+            sum = fmaf(*cluster.map_shared_rank(&row_l[r], c), g, sum);
+            add(y, *reinterpret_cast<const float4*>(cluster.map_shared_rank(all + r * DM + f, c)), g);
         }
-        if (f < a.D) {
-            const float inv = sum > 0.f ? 1.f / sum : 0.f;
-            T* dst = seq_row<T>(a.y, a, s, h, R0 + r) + f;
-            if constexpr (sizeof(T) == 2)
-                *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(y.x * inv, y.y * inv), pack16<T>(y.z * inv, y.w * inv));
-            else
-                *reinterpret_cast<float4*>(dst) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-        }
+        put(r, f, y, sum > 0.f ? 1.f / sum : 0.f);
     }
     cluster.sync();                                             // nobody leaves while its part is read
 }
