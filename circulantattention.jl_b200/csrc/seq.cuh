@@ -109,16 +109,22 @@ struct KeyTiles {
     __device__ __forceinline__ int key(int i, int keys) const { return i < first ? i * keys : lo + (i - first) * keys; }
 };
 
+// Keys that can exist: a cache holds no more than its table has places for, whatever the length says.
+__device__ __forceinline__ int key_limit(const SeqArgs& a, const Seq& s) {
+    return a.pages.table ? (int)min((int64_t)min(s.n, 1 << 30), (int64_t)a.pages.width * a.pages.page) : s.n;
+}
+
 __device__ __forceinline__ KeyTiles key_tiles(const SeqArgs& a, const Seq& s, int p_lo, int p_hi, int keys) {
     KeyTiles k;
     p_lo = max(p_lo, 0);
     p_hi = min(p_hi, s.n - 1);
     if (p_hi < p_lo) return KeyTiles{0, 0, 0};
+    const int limit = key_limit(a, s);
     const int lo = max(0, p_lo - a.left);                                  // left <= 2^30
-    const int hi = (int)min((int64_t)s.n, (int64_t)p_hi + a.right + 1);    // > lo: it holds p_hi
-    k.lo = lo / keys * keys;
-    k.first = (min(min(a.sinks, k.lo), s.n) + keys - 1) / keys;
-    k.count = k.first + (hi - k.lo + keys - 1) / keys;
+    const int hi = (int)min((int64_t)limit, (int64_t)p_hi + a.right + 1);  // > lo where nothing is cut off: it holds p_hi
+    k.lo = min(lo, limit) / keys * keys;
+    k.first = (min(a.sinks, k.lo) + keys - 1) / keys;
+    k.count = k.first + max(0, hi - k.lo + keys - 1) / keys;
     return k;
 }
 

@@ -97,9 +97,6 @@ int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     if (y_rest) a.rest = *y_rest;
     a.lengths = lengths;
     a.lse = lse;
-    // Few rows a key head, on average: the keys are what counts.  More than one tile of 16 rows reads them again, from L2; beyond
-    // four the tiles of 128 (64) rows win.
-    if ((int64_t)a.N * a.G <= 64LL * a.pages.sequences) return decode_paged(a, d->dtype, as_stream(stream));
     return d->dtype == CA_F32 ? fma_fwd(a, as_stream(stream)) : umma_window_fwd(a, d->dtype, as_stream(stream));
 }
 
@@ -146,7 +143,7 @@ int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_vi
     a.pages = *pages;
     // Few rows a key head, on average: the keys are what counts.  More than one tile of 16 rows reads them again, from L2; beyond
     // four the tiles of 128 (64) rows win.
-    if ((int64_t)a.N * a.G <= 64LL * a.pages.sequences) return decode_paged(a, d->dtype, as_stream(stream));
+    if ((int64_t)a.N * a.G <= 64LL * a.pages.sequences || !a.pages.pages) return decode_paged(a, d->dtype, as_stream(stream));
     return d->dtype == CA_F32 ? fma_fwd(a, as_stream(stream)) : umma_paged(a, d->dtype, as_stream(stream));
 }
 

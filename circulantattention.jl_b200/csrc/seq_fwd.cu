@@ -65,11 +65,11 @@ __device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, cons
         return t;
     }
     // the window's tiles begin at kt.lo; those of first tokens lie before it, and beyond it only up to the window
-    const int begin = max(0, t.lo - a.left), end = (int)min((int64_t)s.n - 1, (int64_t)t.hi + a.right);
-    t.from = kt.first + (begin - kt.lo) / 128;
-    t.upto = kt.first + (end - kt.lo) / 128;
+    const int begin = max(0, t.lo - a.left), end = (int)min((int64_t)key_limit(a, s) - 1, (int64_t)t.hi + a.right);
+    t.from = kt.first + max(0, begin - kt.lo) / 128;
+    t.upto = end >= kt.lo ? kt.first + (end - kt.lo) / 128 : kt.first - 1;
     t.first = kt.first;
-    if (a.sinks > kt.lo) t.first = max(t.first, min(t.from, kt.first + (min(a.sinks, s.n) - kt.lo + 127) / 128));
+    if (a.sinks > kt.lo) t.first = max(t.first, min(min(t.from, t.upto + 1), kt.first + (min(a.sinks, s.n) - kt.lo + 127) / 128));
     return t;
 }
 
@@ -276,6 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             ++done;
         }
         if (done && ok) ok = warp_wait(smem_u32(&o_full[u]), 0, stop);
+        // without key tiles nothing has waited for the queries, whose place the results take
+        if (!done && maps.rows && (PAIR || u == 0) && R - r < rows) ok = warp_wait(smem_u32(&q_full[PAIR ? u : 0]), 0, stop) && ok;
         fence_after();
 
         // ------------------------------------------------------------ results

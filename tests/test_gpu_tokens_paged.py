@@ -120,6 +120,26 @@ def test_missing_pages_and_impossible_lengths(ca, dtype):
     assert not y[:, :, 1].any() and not y[:, :, 62:64].any() and y[:, :, 64:].any()
 
 
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+def test_lengths_beyond_the_table(ca, dtype, new):
+    """Tokens for which the table has no place count as missing pages: the rows still see what there is, also where a length
+    is absurd, and where the window holds nothing that exists."""
+    chunks = [(new, 200), (new, 160)]
+    q = make(9, (64, 4, 3 * new), dtype, 1.5)
+    kp, vp, table = cache(64, 2, 16, chunks, dtype, None, 0, junk=0.25)
+    table = [row[:7] for row in table] + [[0] * 7]                     # places for 112 tokens each
+    starts, lengths = [0, new, 2 * new, 3 * new], [200, 160, 2 ** 31 - 1]
+    for left, sinks in ((None, 0), (60, 20)):
+        y = ca.paged_window_attention(q.cuda(), kp.cuda(), vp.cuda(), ints(table).t(), ints(starts), ints(lengths), left, sinks=sinks)
+        for s in (0, 1):
+            cut = slice(starts[s], starts[s + 1])
+            want, bound = ref.paged(q[:, :, cut].double(), kp.double(), vp.double(), [table[s]], [0, new], [lengths[s]], left, sinks, u=ref.UNIT[dtype])
+            ref.check(y[:, :, cut], want, bound)
+        assert torch.isfinite(y).all() and (left is None or sinks or not y[:, :, 2 * new:].any())
+    ca.ops.check_status()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=lambda d: str(d)[6:])
 def test_offsets_beyond_32_bits(ca, dtype):
     """A cache of more than 2^32 elements: the pages in use are its last ones."""

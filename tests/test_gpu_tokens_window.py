@@ -97,6 +97,17 @@ def test_whatever_lies_behind_the_length_has_no_effect(ca, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+def test_empty_sequences_give_zeros_every_time(ca, dtype):
+    """Tiles that see no key at all, next to some that do, many times over: nothing that was on its way lands in the results."""
+    q, k, v, dy = (t.cuda() for t in problem(128, 4, 2, 300, 4, dtype))
+    n = torch.tensor([0, 300, 0, 7], dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        for _ in range(100):
+            y = ca.window_attention(q, k, v, 50, sinks=3, lengths=n)
+            assert not y[..., 0].any() and not y[..., 2].any() and not y[:, :, 7:, 3].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
 @pytest.mark.parametrize("size", [1e-3, 40.0])
 def test_flat_and_peaked_rows(ca, dtype, size):
     """Scores that all are nearly equal, and scores of some hundreds that grow along the sequence, so that every tile
