@@ -658,6 +658,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ SeqAr
     const int c = blockIdx.x % (DM / 8) * 8, which = blockIdx.x / (DM / 8) & 1, tile = blockIdx.x / (DM / 4), j = tile * 128 + r;
     const float* p = partial + ((((int64_t)b * a.Hkv + h) * split_tiles + tile) * segments * 2 + which) * (DM * 128) + c * 128 + r;
     float sum[8] = {};
+#pragma unroll 4
     for (int seg = 0; seg < segments; ++seg, p += 2 * DM * 128)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += p[e * 128];

@@ -7,7 +7,8 @@
 // Tiles of 64 rows and 64 columns in shared memory, features fastest and rows padded by 4 floats, so that the 16-byte
 // reads of eight lanes (rows 1 apart) fall into different banks.  A thread (ty, tx) of 16 x 16 holds the products of rows
 // ty + 16i with columns tx + 16j (i, j < 4): 32 packed FMA for 8 reads of 16 bytes.  The next tile is copied (cp.async)
-// while this one is worked on.
+// while this one is worked on (forward), or another block works (backward: two blocks on an SM with one stage each beat one
+// with two, 274 us against 311 for dq).
 #include <algorithm>
 
 #include "seq.cuh"
@@ -245,12 +246,12 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
 
 // ---------------------------------------------------------------- backward
 // P = 2^(scale q.k log2 e - lse), dP = dy.v, dS = P (dP - delta), delta = dy.y; dq = scale dS k.
-template <int DM> constexpr size_t kDqSmem = (6 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
+template <int DM> constexpr size_t kDqSmem = (4 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
 
 template <int DM>
-__global__ void __launch_bounds__(kThreads) fma_dq_kernel(const __grid_constant__ SeqArgs a) {
+__global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
-    float *Q = (float*)smem4, *O = Q + kTileFloats<DM>, *KV = O + kTileFloats<DM>, *Pm = KV + 4 * kTileFloats<DM>;
+    float *Q = (float*)smem4, *O = Q + kTileFloats<DM>, *K = O + kTileFloats<DM>, *V = K + kTileFloats<DM>, *Pm = V + kTileFloats<DM>;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
     const Seq s = dense_seq(a, blockIdx.z);
     const int rows = s.T * a.G, R0 = blockIdx.x * kTile;
@@ -266,19 +267,16 @@ __global__ void __launch_bounds__(kThreads) fma_dq_kernel(const __grid_constant_
     };
     fetch<DM>(Q, from(a.q), any, a.D, tid);
     fetch<DM>(O, from(a.dy), any, a.D, tid);
-    float* yrow = KV + 2 * kTileFloats<DM>;                       // y passes through the place of the second tile
+    float* yrow = V;                                              // y passes through the values' place
     fetch<DM>(yrow, from(a.y), any, a.D, tid);
     copies_commit();
     const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kTile);
     auto prefetch = [&](int it) {
         const int j0 = kt.key(it, kTile);
-        float* K = KV + 2 * (it & 1) * kTileFloats<DM>;
         fetch<DM>(K, [&](int r, bool& on) { return key_ptr(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
-        fetch<DM>(K + kTileFloats<DM>, [&](int r, bool& on) { return key_ptr(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
+        fetch<DM>(V, [&](int r, bool& on) { return key_ptr(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
     };
-    if (kt.count) prefetch(0);
-    copies_commit();
-    copies_wait<1>();
+    copies_wait<0>();
     __syncthreads();
     int pos[4];
     float lse[4], delta[4];
@@ -297,16 +295,15 @@ __global__ void __launch_bounds__(kThreads) fma_dq_kernel(const __grid_constant_
     }
     __syncthreads();
     for (int it = 0; it < kt.count; ++it) {
-        if (it + 1 < kt.count) prefetch(it + 1);
+        prefetch(it);
         copies_commit();
-        copies_wait<1>();
+        copies_wait<0>();
         __syncthreads();
         const int j0 = kt.key(it, kTile);
-        const float* K = KV + 2 * (it & 1) * kTileFloats<DM>;
         const bool edge = !(p_hi < s.n && j0 + kTile - 1 <= (int64_t)p_lo + a.right && j0 + kTile <= s.n && (j0 >= p_hi - a.left || j0 + kTile <= a.sinks));
         float sc[4][4], dp[4][4];
         dot_tile<DM>(Q, K, ty, tx, sc);
-        dot_tile<DM>(O, K + kTileFloats<DM>, ty, tx, dp);
+        dot_tile<DM>(O, V, ty, tx, dp);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -327,9 +324,7 @@ __global__ void __launch_bounds__(kThreads) fma_dq_kernel(const __grid_constant_
 
 // A block owns 64 keys and walks the query rows that see any of them: dv = P^T dy, dk = scale dS^T q, no atomics.  The rows of
 // key tiles that hold first tokens are dealt to `segments` blocks, whose parts fma_join_kernel adds up in order.
-// Two stages of q and dy beside k, v and both weights; at 128 features only one fits.
-template <int DM> constexpr int kStages = DM == 64 ? 2 : 1;
-template <int DM> constexpr size_t kDkdvSmem = ((2 + 2 * kStages<DM>) * kTileFloats<DM> + 2 * kTile * kPPitch) * sizeof(float);
+template <int DM> constexpr size_t kDkdvSmem = (4 * kTileFloats<DM> + 2 * kTile * kPPitch) * sizeof(float);
 
 struct Parts {
     float* data;            // [b][key head][tile][segment][dk, dv][64 keys][DM]
@@ -337,11 +332,10 @@ struct Parts {
 };
 
 template <int DM>
-__global__ void __launch_bounds__(kThreads) fma_dkdv_kernel(const __grid_constant__ SeqArgs a, const Parts parts) {
+__global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(const __grid_constant__ SeqArgs a, const Parts parts) {
     extern __shared__ float4 smem4[];
-    constexpr int STAGES = kStages<DM>;
-    float *K = (float*)smem4, *V = K + kTileFloats<DM>, *QO = V + kTileFloats<DM>, *Pm = QO + 2 * STAGES * kTileFloats<DM>, *Sm = Pm + kTile * kPPitch;
-    __shared__ float s_lse[2][kTile], s_delta[2][kTile];
+    float *K = (float*)smem4, *V = K + kTileFloats<DM>, *Q = V + kTileFloats<DM>, *O = Q + kTileFloats<DM>, *Pm = O + kTileFloats<DM>, *Sm = Pm + kTile * kPPitch;
+    __shared__ float s_lse[kTile], s_delta[kTile];
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
     const int dealt = parts.tiles * parts.segments;
     const bool split = (int)blockIdx.x < dealt;
@@ -364,8 +358,7 @@ __global__ void __launch_bounds__(kThreads) fma_dkdv_kernel(const __grid_constan
     const int first = split ? (int)((int64_t)all * seg / parts.segments) : 0;
     const int count = (split ? (int)((int64_t)all * (seg + 1) / parts.segments) : all) - first;
     auto prefetch = [&](int it) {
-        const int R0 = lo + (first + it) * kTile, b = it % STAGES;
-        float* Q = QO + 2 * b * kTileFloats<DM>;
+        const int R0 = lo + (first + it) * kTile;
         auto from = [&](const ca_seq_view& v) {
             return [&](int r, bool& on) {
                 on = on && R0 + r < hi;
@@ -373,26 +366,19 @@ __global__ void __launch_bounds__(kThreads) fma_dkdv_kernel(const __grid_constan
             };
         };
         fetch<DM>(Q, from(a.q), any, a.D, tid);
-        fetch<DM>(Q + kTileFloats<DM>, from(a.dy), any, a.D, tid);
+        fetch<DM>(O, from(a.dy), any, a.D, tid);
         if (tid < kTile) {
             const bool have = R0 + tid < hi;
-            s_lse[it & 1][tid] = have ? a.lse[stat0 + R0 + tid] : 0.f;
-            s_delta[it & 1][tid] = have ? a.delta[stat0 + R0 + tid] : 0.f;
+            s_lse[tid] = have ? a.lse[stat0 + R0 + tid] : 0.f;
+            s_delta[tid] = have ? a.delta[stat0 + R0 + tid] : 0.f;
         }
     };
     if (count) prefetch(0);
     copies_commit();
     for (int it = 0; it < count; ++it) {
-        if (STAGES == 2) {
-            if (it + 1 < count) prefetch(it + 1);
-            copies_commit();
-            copies_wait<1>();
-        } else {
-            copies_wait<0>();
-        }
+        copies_wait<0>();
         __syncthreads();
-        const int R0 = lo + (first + it) * kTile, b = it & 1;
-        const float *Q = QO + 2 * (it % STAGES) * kTileFloats<DM>, *O = Q + kTileFloats<DM>;
+        const int R0 = lo + (first + it) * kTile;
         float sc[4][4], dp[4][4];
         dot_tile<DM>(K, Q, ty, tx, sc);
         dot_tile<DM>(V, O, ty, tx, dp);
@@ -404,18 +390,16 @@ __global__ void __launch_bounds__(kThreads) fma_dkdv_kernel(const __grid_constan
             for (int c = 0; c < 4; ++c) {
                 const int R = R0 + tx + 16 * c;
                 const bool see = !edge || (R < hi && sees(a, s.n, token_of(a, R), j0 + ty + 16 * i));
-                const float p = see ? fast_exp2(sc[i][c] * a.scale_log2 - s_lse[b][tx + 16 * c]) : 0.f;
+                const float p = see ? fast_exp2(sc[i][c] * a.scale_log2 - s_lse[tx + 16 * c]) : 0.f;
                 Pm[(ty + 16 * i) * kPPitch + tx + 16 * c] = p;
-                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? p * (dp[i][c] - s_delta[b][tx + 16 * c]) : 0.f;
+                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? p * (dp[i][c] - s_delta[tx + 16 * c]) : 0.f;
             }
         __syncwarp();
         acc_tile<DM>(Pm, O, ty, tx, dv);
         acc_tile<DM>(Sm, Q, ty, tx, dk);
         __syncthreads();
-        if (STAGES == 1) {
-            if (it + 1 < count) prefetch(it + 1);
-            copies_commit();
-        }
+        if (it + 1 < count) prefetch(it + 1);
+        copies_commit();
     }
     copies_wait<0>();
 #pragma unroll
@@ -434,12 +418,13 @@ __global__ void __launch_bounds__(kThreads) fma_dkdv_kernel(const __grid_constan
 
 template <int DM>
 __global__ void __launch_bounds__(256) fma_join_kernel(const __grid_constant__ SeqArgs a, const Parts parts) {
-    const int which = blockIdx.x & 1, tile = blockIdx.x >> 1, h = blockIdx.y, b = blockIdx.z;
+    const int which = blockIdx.x & 1, piece = blockIdx.x >> 1 & 3, tile = blockIdx.x >> 3, h = blockIdx.y, b = blockIdx.z;
     const float* p = parts.data + (((int64_t)b * a.Hkv + h) * parts.tiles + tile) * parts.segments * 2 * kTile * DM + which * kTile * DM;
     const ca_seq_view& out = which ? a.dv : a.dk;
-    for (int i = threadIdx.x; i < kTile * DM / 4; i += 256) {
+    for (int i = piece * 256 + threadIdx.x; i < kTile * DM / 4; i += 4 * 256) {
         const int r = i / (DM / 4), c = i % (DM / 4) * 4, j = tile * kTile + r;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int seg = 0; seg < parts.segments; ++seg) {
             const float4 x = *(const float4*)(p + (int64_t)seg * 2 * kTile * DM + r * DM + c);
             sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
@@ -483,7 +468,7 @@ int launch_bwd(const SeqArgs& a, float* data, cudaStream_t st) {
     fma_dkdv_kernel<DM><<<dim3(tiles - parts.tiles + parts.tiles * parts.segments, a.Hkv, a.B), kThreads, kDkdvSmem<DM>, st>>>(a, parts);
     CA_CHECK_LAUNCH("window dk/dv kernel");
     if (parts.tiles) {
-        fma_join_kernel<DM><<<dim3(2 * parts.tiles, a.Hkv, a.B), 256, 0, st>>>(a, parts);
+        fma_join_kernel<DM><<<dim3(8 * parts.tiles, a.Hkv, a.B), 256, 0, st>>>(a, parts);
         CA_CHECK_LAUNCH("window dk/dv join kernel");
     }
     return CA_OK;
