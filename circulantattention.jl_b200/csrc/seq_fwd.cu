@@ -37,6 +37,10 @@ struct FwdMaps {
 struct Stream {
     int lo, hi;             // positions of its rows that exist; lo > hi: none
     int first, from, upto, step;
+    int begin_key, end_key;     // its rows' windows together
+    // Whether any row sees a key of the half tile from `key0`.  What a tile costs is its exponentials, so halves outside the
+    // windows (the tiles at their ends, a few first tokens) are left out.
+    __device__ __forceinline__ bool sees_half(const SeqArgs& a, int key0) const { return key0 <= end_key && (key0 + 63 >= begin_key || key0 < a.sinks); }
     __device__ __forceinline__ bool takes(int i) const { return step == 2 ? (i & 1) == (from & 1) && i <= upto : i < first || (i >= from && i <= upto); }
     __device__ __forceinline__ int begin() const { return first > 0 ? 0 : from; }
     __device__ __forceinline__ int next(int i) const {
@@ -50,6 +54,8 @@ __device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, cons
     Stream t;
     t.lo = max(0, s.base + r / a.G);
     t.hi = r < rows ? min(s.n - 1, s.base + (min(r + 128, rows) - 1) / a.G) : -1;
+    t.begin_key = max(0, t.lo - a.left);
+    t.end_key = (int)min((int64_t)key_limit(a, s) - 1, (int64_t)t.hi + a.right);
     if (!PAIR) {
         t.first = 0;
         t.from = u;
@@ -65,7 +71,7 @@ __device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, cons
         return t;
     }
     // the window's tiles begin at kt.lo; those of first tokens lie before it, and beyond it only up to the window
-    const int begin = max(0, t.lo - a.left), end = (int)min((int64_t)key_limit(a, s) - 1, (int64_t)t.hi + a.right);
+    const int begin = t.begin_key, end = t.end_key;
     t.from = kt.first + max(0, begin - kt.lo) / 128;
     t.upto = end >= kt.lo ? kt.first + (end - kt.lo) / 128 : kt.first - 1;
     t.first = kt.first;
@@ -218,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             float mx = -INFINITY;
 #pragma unroll 1
             for (int g = 0; g < 2; ++g) {
+                if (!st.sees_half(a, key0 + 64 * g)) continue;
                 uint32_t x[64];
                 masked_scores(g, x);
                 float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
@@ -253,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             f32x2 sum2 = pack2(l * f, 0.f);
 #pragma unroll 1
             for (int g = 0; g < 2; ++g) {
+                if (!st.sees_half(a, key0 + 64 * g)) continue;
                 uint32_t x[64], w[32];
                 scores(g, x);
 #pragma unroll
@@ -423,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         const uint64_t q_desc = desc_features(q_at), k_desc = desc_features(kv_at), v_desc = desc_rows(kv_at);
         bool ok = true;
         uint32_t scored = 0;                                               // slots whose keys one of two streams has used
-        uint32_t n0 = 0, n1 = 0;                                           // tiles whose values each stream has added
+        struct Added { uint32_t low, high; } n0{0, 0}, n1{0, 0};           // halves of tiles whose values each stream has added
         int have = -1;                                                     // keys and values land in order: each is waited for once
         auto landed = [&](int item) {
             while (have < item) {
@@ -440,21 +448,27 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             if (last) mma_commit(lead, smem_u32(&kv_empty[slot]));
             scored = last ? scored & ~(1u << slot) : scored | 1u << slot;
         };
-        auto weighted = [&](int u, int i, uint32_t& n) {
+        auto weighted = [&](int u, int i, Added& n) {
             const Stream& st = u ? st1 : st0;
             const uint32_t slot = (2 * i + 1) % S;
-            const int nx = st.next(i);
+            const int nx = st.next(i), key0 = kt.key(i, 128);
             // the weights are what is late: everything else is waited for first.  The next keys' slot was freed by products
             // that came before (a stream is at most two tiles ahead, and the ring holds five).
-            if (!landed(nx <= st.upto ? 2 * nx : 2 * i + 1) || !warp_wait(smem_u32(&p_full[u][0]), n & 1, stop)) return false;
-            fence_after();
-            mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step, v_desc + slot * (TILE >> 4), IDESC_O, n != 0);
-            if (!warp_wait(smem_u32(&p_full[u][1]), n & 1, stop)) return false;
-            fence_after();
-            mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step + 32, v_desc + slot * (TILE >> 4) + 4 * 128, IDESC_O, true);
+            if (!landed(nx <= st.upto ? 2 * nx : 2 * i + 1)) return false;
+            if (st.sees_half(a, key0)) {
+                if (!warp_wait(smem_u32(&p_full[u][0]), n.low & 1, stop)) return false;
+                fence_after();
+                mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step, v_desc + slot * (TILE >> 4), IDESC_O, n.low + n.high != 0);
+                ++n.low;
+            }
+            if (st.sees_half(a, key0 + 64)) {
+                if (!warp_wait(smem_u32(&p_full[u][1]), n.high & 1, stop)) return false;
+                fence_after();
+                mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step + 32, v_desc + slot * (TILE >> 4) + 4 * 128, IDESC_O, n.low + n.high != 0);
+                ++n.high;
+            }
             if (!PAIR || u == 1 || !st1.takes(i)) mma_commit(lead, smem_u32(&kv_empty[slot]));
             if (nx > st.upto) mma_commit(lead, smem_u32(&o_full[u]));
-            ++n;
             if (nx <= st.upto) scores(u, nx);
             return true;
         };
