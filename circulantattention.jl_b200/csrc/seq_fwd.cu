@@ -267,8 +267,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 for (int c = 0; c < 32; ++c) {
                     float e0, e1;
                     unpack2(fma2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), sc2, ref2), e0, e1);
-                    e0 = fast_exp2(e0);
-                    e1 = fast_exp2(e1);
+                    // The exponential unit and the tensor pipe take the same 2048 cycles a pair of tiles; a quarter of the
+                    // exponentials as polynomials: 443 -> 418 us for a sequence of 16384 (an eighth: 431, a half: 430).
+                    if (c % 4 == 3) {
+                        unpack2(exp2_fma<T>(e0, e1), e0, e1);
+                    } else {
+                        e0 = fast_exp2(e0);
+                        e1 = fast_exp2(e1);
+                    }
                     sum2 = add2(sum2, pack2(e0, e1));
                     w[c] = pack16<T>(e0, e1);
                 }

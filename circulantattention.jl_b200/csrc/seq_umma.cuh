@@ -23,6 +23,39 @@ template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float h
 template <typename T> __device__ __forceinline__ float low16(uint32_t w) { return to_float(reinterpret_cast<const T*>(&w)[0]); }
 template <typename T> __device__ __forceinline__ float high16(uint32_t w) { return to_float(reinterpret_cast<const T*>(&w)[1]); }
 
+// The larger of two numbers; not a number if one of them is not
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// 2^x for two numbers below 2^7 on the FMA pipe: x = n + f with n the nearest integer (the low bits of x + 1.5 2^23), a
+// polynomial for 2^f on [-1/2, 1/2], times 2^n; 0 below 2^-126.  The coefficients minimise the largest relative error (Lawson's
+// iteration): 7.5e-5 with degree 3, below the rounding to bfloat16 that follows by a factor of 26; 2.6e-6 with degree 4 for
+// half.  A number that is not one stays so, as in the other exponentials.
+template <typename T>
+__device__ __forceinline__ f32x2 exp2_fma(float x0, float x1) {
+    const f32x2 magic = pack2(12582912.f, 12582912.f), unmagic = pack2(-12582912.f, -12582912.f), minus = pack2(-1.f, -1.f);
+    const f32x2 x = pack2(max_nan(x0, -127.f), max_nan(x1, -127.f));
+    const f32x2 t = add2(x, magic);
+    const f32x2 f = fma2(add2(t, unmagic), minus, x);
+    f32x2 p;
+    if (kIsBf16<T>) {
+        p = fma2(f, pack2(0.055171494f, 0.055171494f), pack2(0.242610938f, 0.242610938f));
+        p = fma2(f, p, pack2(0.693260994f, 0.693260994f));
+        p = fma2(f, p, pack2(0.999928085f, 0.999928085f));
+    } else {
+        p = fma2(f, pack2(0.00957008612f, 0.00957008612f), pack2(0.055917851f, 0.055917851f));
+        p = fma2(f, p, pack2(0.240247451f, 0.240247451f));
+        p = fma2(f, p, pack2(0.693121816f, 0.693121816f));
+        p = fma2(f, p, pack2(0.999999261f, 0.999999261f));
+    }
+    float t0, t1;
+    unpack2(t, t0, t1);
+    return mul2(p, pack2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u)));
+}
+
 // The registers of a tensor-memory load are complete behind its wait: nothing that uses them may move before it.
 __device__ __forceinline__ void settled32(uint32_t* r) {
 #pragma unroll
