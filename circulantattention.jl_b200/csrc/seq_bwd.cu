@@ -17,7 +17,10 @@
 namespace ca {
 namespace {
 
-constexpr int kThreads = 352;       // two warpgroups that compute, and warps that copy, issue products and fetch the rows' sums
+// Four warpgroups that compute, each for a quarter of a tile's columns, and warps that copy, issue products and fetch the rows'
+// sums.
+constexpr int kGroups = 4, kCols = 128 / kGroups, kWork = 128 * kGroups, kWarps = 4 * kGroups, kThreads = kWork + 96;
+constexpr int kCopier = kWarps, kIssuer = kWarps + 1, kFetcher = kWarps + 2;
 template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
 template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
 template <int DM> constexpr size_t kBwdSmem = (size_t)(2 + kSlots<DM>) * kTileBytes<DM> + 1024;
@@ -49,25 +52,23 @@ __device__ __forceinline__ float warp_max(float x) {
     return x;
 }
 
-// A operand whose two halves of 64 contracted elements lie `apart` columns apart.
-__device__ __forceinline__ void mma_halves(uint32_t lead, uint32_t d, uint32_t a, uint32_t apart, uint64_t b, uint32_t idesc, bool add) {
-    mma_weighted<64>(lead, d, a, b, idesc, add);
-    mma_weighted<64>(lead, d, a + apart, b + 4 * 128, idesc, true);
+// A operand whose pieces of 32 contracted elements (a warpgroup's columns as 16-bit pairs) lie `apart` columns apart.
+__device__ __forceinline__ void mma_pieces(uint32_t lead, uint32_t d, uint32_t a, uint32_t apart, uint64_t b, uint32_t idesc, bool add) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mma_ts(lead, d, a + (k >> 1) * apart + (k & 1) * 8, b + k * 128, idesc, add || k != 0);
 }
 
-__device__ __forceinline__ void read64(uint32_t at, uint32_t* x) {
+__device__ __forceinline__ void read_columns(uint32_t at, uint32_t* x) {
     tmem_ld32(at, x);
-    tmem_ld32(at + 32, x + 32);
     tmem_wait_ld();
     settled32(x);
-    settled32(x + 32);
 }
 
 // Zeros where the bit is not set.  Always in a block of its own behind one uniform branch: as a condition on each element the
 // selects ran for every tile and took as long as the arithmetic.
-__device__ __forceinline__ void clear_unseen(uint32_t* x, const uint32_t* mk) {
+__device__ __forceinline__ void clear_unseen(uint32_t* x, uint32_t mk) {
 #pragma unroll
-    for (int c = 0; c < 64; ++c) x[c] = (mk[c >> 5] >> (c & 31)) & 1 ? x[c] : 0u;
+    for (int c = 0; c < kCols; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0u;
 }
 
 template <int DM>
@@ -102,22 +103,27 @@ __global__ void __launch_bounds__(256) peak_kernel(const __grid_constant__ SeqAr
 }
 
 // ---------------------------------------------------------------- dq
-// Tensor memory: scores 0..127, dP twice 128..383, dq from 384.  While the warpgroups turn tile i into dS, the products of
-// tile i + 1 run.
+// Tensor memory: scores 0..127, dP 128..255, dS 256..319, the queries 320..383, dq from 384.  While the warpgroups turn tile i
+// into dS, the products of tile i + 1 run.
+//
+// The queries move into tensor memory, and their place becomes one more slot of the ring: a tile of keys stays until its product
+// with dS, two steps behind its scores, so that with five slots the values of every tile came late (2450 cycles a tile; 1536
+// are products).
 template <typename T, int DM>
 __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ BwdMaps maps) {
-    constexpr int S = kSlots<DM>;
+    constexpr int S = kSlots<DM> + 1;
     constexpr uint32_t TILE = kTileBytes<DM>;
     constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
     extern __shared__ char raw[];
-    __shared__ uint64_t kv_full[S], kv_empty[S], q_full, s_full, s_free, dp_full[2], ds_full[2], dq_done, o_full, drained;
+    __shared__ uint64_t kv_full[S], kv_empty[S], q_full, q_moved, s_full, s_free, dp_full, dp_free, ds_full, dq_done, o_full, drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int stop_flag;
     __shared__ float part[2][128], warp_peak[4];
     volatile int* stop = &stop_flag;
     const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
     char* const smem = raw + (base_at - raw_at);
-    const uint32_t kv_at = base_at + 2 * TILE;
+    const uint32_t kv_at = base_at + TILE, q_at = kv_at + (S - 1) * TILE;    // dy, then the ring; the queries come into its last slot
+    char* const q_tile = smem + S * TILE;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
     const Seq s = dense_seq(a, blockIdx.z);
@@ -126,56 +132,79 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     const int p_hi = min(s.n - 1, f_hi);
     const KeyTiles kt = key_tiles(a, s, f_lo, f_hi, 128);
 
-    if (warp == 8 && lane == 0) {
-        prefetch_map(&maps.k);
-        prefetch_map(&maps.v);
-    }
-    if (tid == 0) {
+    if (warp == kCopier && lane == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
-        mbar_init(&q_full, maps.rows ? 1 : 8);
+        mbar_init(&q_full, maps.rows ? 1 : kWarps);
+        mbar_init(&q_moved, kWarps);
         mbar_init(&s_full, 1);
-        mbar_init(&s_free, 8);
-        for (int i = 0; i < 2; ++i) { mbar_init(&dp_full[i], 1); mbar_init(&ds_full[i], 8); }
+        mbar_init(&s_free, kWarps);
+        mbar_init(&dp_full, 1);
+        mbar_init(&dp_free, kWarps);
+        mbar_init(&ds_full, kWarps);
         mbar_init(&dq_done, 1);
         mbar_init(&o_full, 1);
         mbar_init(&drained, 1);
         stop_flag = 0;
         mbar_fence_init();
+        fence_async_smem();
+        if (maps.rows) {                                       // on their way while the rest is set up
+            mbar_arrive_expect_tx(smem_u32(&q_full), 2 * TILE);
+#pragma unroll
+            for (int p = 0; p < DM / 64; ++p) {
+                tma_load_4d(q_at + p * kPanel, &maps.q_rows, 64 * p, h * a.G, R0 / a.G, s.b, smem_u32(&q_full));
+                tma_load_4d(base_at + p * kPanel, &maps.dy_rows, 64 * p, h * a.G, R0 / a.G, s.b, smem_u32(&q_full));
+            }
+        }
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
     }
-    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (warp == kIssuer) tmem_alloc(smem_u32(&tmem_slot), 512);
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_slot, o_col = tmem + 384;
+    const uint32_t tmem = tmem_slot, q_col = tmem + 320, o_col = tmem + 384;
 
-    if (warp < 8) {
+    if (warp < kWarps) {
         const int u = warp >> 2, r = tid & 127, R = R0 + r, pos = token_of(a, R);
         const bool have = R < rows, live = have && pos < s.n;
         const int64_t stat = ((int64_t)s.b * a.Hkv + h) * rows + R;
+        const float lse = live ? a.lse[stat] : 0.f;
+        const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
         float delta, c = 1.f;
         {
-            typedef TileCopy<DM, 256> C;
+            typedef TileCopy<DM, kWork> C;
             auto row = [&](const ca_seq_view& v) {
                 return [&](int rr) { return seq_row<T>(v, a, s, h, min(R0 + rr, rows - 1)); };
             };
             const int to = (int)min((int64_t)rows, (int64_t)s.n * a.G) - R0;
             uint4 w[C::kCount], y[C::kCount], e[C::kCount];
             if (!maps.rows) {
-                fetch_tile<T, DM, 256>(y, row(a.q), 0, to, a.D, tid);
-                fetch_tile<T, DM, 256>(w, row(a.dy), 0, to, a.D, tid);
-                put_tile<DM, 256>(smem, y, tid);
-                put_tile<DM, 256>(smem + TILE, w, tid);
+                fetch_tile<T, DM, kWork>(y, row(a.q), 0, to, a.D, tid);
+                fetch_tile<T, DM, kWork>(w, row(a.dy), 0, to, a.D, tid);
+                put_tile<DM, kWork>(q_tile, y, tid);
+                put_tile<DM, kWork>(smem, w, tid);
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&q_full));
             }
-            fetch_tile<T, DM, 256>(y, row(a.y), 0, to, a.D, tid);
-            if (a.rest.data) fetch_tile<T, DM, 256>(e, row(a.rest), 0, to, a.D, tid);
+            fetch_tile<T, DM, kWork>(y, row(a.y), 0, to, a.D, tid);
+            if (a.rest.data) fetch_tile<T, DM, kWork>(e, row(a.rest), 0, to, a.D, tid);
+            warp_wait(smem_u32(&q_full), 0, stop);                             // a wait that ran out shows at the next one
+            if (32 * u < DM) {                                                 // features 32 u .. 32 u + 31 of the row
+                uint32_t x[16];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<uint4*>(x + 4 * k) = *reinterpret_cast<const uint4*>(q_tile + C::at(r, 4 * u + k));
+                tmem_st16(q_col + lane_off + 16 * u, x);
+                tmem_wait_st();
+                fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&q_moved));
             if (maps.rows) {
-                warp_wait(smem_u32(&q_full), 0, stop);                         // a wait that ran out shows at the next one
 #pragma unroll
                 for (int i = 0; i < C::kCount; ++i) {
-                    w[i] = *reinterpret_cast<const uint4*>(smem + TILE + C::at(C::row(tid, i), C::piece(tid)));
+                    w[i] = *reinterpret_cast<const uint4*>(smem + C::at(C::row(tid, i), C::piece(tid)));
                     if (C::row(tid, i) >= to) w[i] = make_uint4(0, 0, 0, 0);
                 }
             }
@@ -200,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                     part[1][C::row(tid, i)] = peak;
                 }
             }
-            group_sync<256>(1);
+            group_sync<kWork>(1);
             delta = part[0][r];
             if (u == 0 && have) a.delta[stat] = delta;
             if (!kIsBf16<T>) {
@@ -212,48 +241,47 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 if (u == 0 && lane == 0) warp_peak[warp] = peak;
             }
         }
-        const float lse = live ? a.lse[stat] : 0.f;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta * c, -delta * c), c2 = pack2(c, c);
-        const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
-        const uint32_t S_at = tmem + 64 * u + lane_off;
+        const uint32_t S_at = tmem + kCols * u + lane_off, dp_at = S_at + 128, ds_at = tmem + 256 + kCols / 2 * u + lane_off;
         bool ok = true;
         for (int i = 0; i < kt.count; ++i) {
             const int key0 = kt.key(i, 128), far = key0 + 127;
             if (!warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
             fence_after();
-            uint32_t x[64];
-            read64(S_at, x);
+            uint32_t x[kCols];
+            read_columns(S_at, x);
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_free));
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
+            for (int c = 0; c < kCols; c += 2) {
                 float e0, e1;
                 unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, lse2), e0, e1);
                 x[c] = __float_as_uint(fast_exp2(e0));
                 x[c + 1] = __float_as_uint(fast_exp2(e1));
             }
-            uint32_t mk[2] = {~0u, ~0u};
+            uint32_t mk = ~0u;
             const bool ragged = far >= s.n || f_hi != p_hi;      // the tile holds keys or rows that may be anything
             const bool edge = !(far <= f_lo + a.right && far < s.n && f_hi == p_hi && (key0 >= p_hi - a.left || far < a.sinks));
             if (edge) {
                 const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
-#pragma unroll
-                for (int g = 0; g < 2; ++g) mk[g] = seen_bits(lo - 64 * u - 32 * g, hi - 64 * u - 32 * g, sk - 64 * u - 32 * g);
+                mk = seen_bits(lo - kCols * u, hi - kCols * u, sk - kCols * u);
                 clear_unseen(x, mk);
                 if (far >= s.n && u == 0) {                    // keys behind the length may be anything: zeros
                     const int slot = (2 * i) % S;              // the scores are there, so the keys are
-                    if (key0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
+                    if (key0 + r >= s.n) clear_row<DM>(smem + (1 + slot) * TILE, r);
                     fence_async_smem();
                 }
             }
-            if (!warp_wait(smem_u32(&dp_full[i & 1]), (i >> 1) & 1, stop)) { ok = false; break; }
+            if (!warp_wait(smem_u32(&dp_full), i & 1, stop)) { ok = false; break; }
             fence_after();
-            const uint32_t dp_at = tmem + 128 + (i & 1) * 128 + 64 * u + lane_off;
-            uint32_t y[64], w[32];
-            read64(dp_at, y);
+            uint32_t y[kCols], w[kCols / 2];
+            read_columns(dp_at, y);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&dp_free));
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
+            for (int c = 0; c < kCols; c += 2) {
                 float e0, e1;
                 unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, dl2), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e0, e1);
                 y[c] = __float_as_uint(e0);
@@ -261,23 +289,25 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             }
             if (ragged) clear_unseen(y, mk);                   // dP of such pairs may be anything
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
-            tmem_st32(dp_at, w);
+            for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
+            if (i && !warp_wait(smem_u32(&dq_done), (i - 1) & 1, stop)) { ok = false; break; }
+            fence_after();
+            tmem_st16(ds_at, w);
             tmem_wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&ds_full[i & 1]));
+            if (lane == 0) mbar_arrive(smem_u32(&ds_full));
         }
         if (kt.count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
         fence_after();
         const float f = !ok || *stop ? __int_as_float(0x7fffffff) : a.scale / c;
         if (!kIsBf16<T>) {
-            group_sync<256>(1);
+            group_sync<kWork>(1);
             if (tid == 0)
                 maps.dy_peak[((int64_t)s.b * a.Hkv + h) * gridDim.x + R0 / 128] = fmaxf(fmaxf(warp_peak[0], warp_peak[1]), fmaxf(warp_peak[2], warp_peak[3]));
         }
 #pragma unroll 1
-        for (int col = u * (DM / 2); col < (u + 1) * (DM / 2); col += 32) {
+        for (int col = 32 * u; col < DM; col += 32 * kGroups) {
             uint32_t o[32];
             tmem_ld32(o_col + lane_off + col, o);
             tmem_wait_ld();
@@ -285,30 +315,23 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             float y[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) y[e] = kt.count ? __uint_as_float(o[e]) * f : 0.f * f;
-            put_row32<T>(smem, r, col, y);                         // the queries' place: their last scores are done
+            put_row32<T>(smem, r, col, y);                         // dy's place: its last products are done
         }
         fence_async_smem();
-        group_sync<256>(1);
+        group_sync<kWork>(1);
         if (!maps.rows) {
-            store_tile<T, DM, 256>(smem, [&](int rr) { return seq_row<T>(a.dq, a, s, h, R0 + rr); }, rows - R0, a.D, tid);
+            store_tile<T, DM, kWork>(smem, [&](int rr) { return seq_row<T>(a.dq, a, s, h, R0 + rr); }, rows - R0, a.D, tid);
         } else if (tid == 0) {
 #pragma unroll
             for (int p = 0; p < DM / 64; ++p) tma_store_4d(&maps.dq_rows, base_at + p * kPanel, 64 * p, h * a.G, R0 / a.G, s.b);
             tma_stores_read();
         }
-    } else if (warp == 8 && lane == 0) {
+    } else if (warp == kCopier && lane == 0) {
         bool ok = true;
         int issued = 0;
-        if (maps.rows) {
-            mbar_arrive_expect_tx(smem_u32(&q_full), 2 * TILE);
-#pragma unroll
-            for (int p = 0; p < DM / 64; ++p) {
-                tma_load_4d(base_at + p * kPanel, &maps.q_rows, 64 * p, h * a.G, R0 / a.G, s.b, smem_u32(&q_full));
-                tma_load_4d(base_at + TILE + p * kPanel, &maps.dy_rows, 64 * p, h * a.G, R0 / a.G, s.b, smem_u32(&q_full));
-            }
-        }
         for (; issued < 2 * kt.count; ++issued) {
             const int slot = issued % S;
+            if (issued == S - 1 && !wait_or_stop(smem_u32(&q_moved), 0, stop)) { ok = false; break; }
             if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
             const uint32_t bar = smem_u32(&kv_full[slot]), dst = kv_at + slot * TILE;
             mbar_arrive_expect_tx(bar, TILE);
@@ -316,44 +339,50 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             for (int p = 0; p < DM / 64; ++p)
                 tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.v : &maps.k, 64 * p, kt.key(issued >> 1, 128), h, s.b, bar);
         }
-        if (!ok)                                               // copies in flight land before the memory goes away
+        if (!ok) {                                             // copies in flight land before the memory goes away
+            mbar_wait(smem_u32(&q_full), 0, 1u << 12);
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
-    } else if (warp == 9 && kt.count) {
+        }
+    } else if (warp == kIssuer && kt.count) {
         const uint32_t lead = elect_one();
-        const uint64_t q_desc = desc_features(base_at), dy_desc = desc_features(base_at + TILE), f_desc = desc_features(kv_at), r_desc = desc_rows(kv_at);
+        const uint64_t dy_desc = desc_features(base_at), f_desc = desc_features(kv_at), r_desc = desc_rows(kv_at);
         uint32_t have = 0;                                     // keys and values land in order: each is waited for once
         auto landed = [&](uint32_t items) {
             for (; have < items; ++have)
                 if (!warp_wait(smem_u32(&kv_full[have % S]), (have / S) & 1, stop)) return false;
             return true;
         };
-        auto products = [&](uint32_t i) {                      // scores and dP of tile i
-            const uint32_t ks = (2 * i) % S, vs = (2 * i + 1) % S;
+        auto scores = [&](uint32_t i) {
             fence_after();
-            mma_dot<DM>(lead, tmem, q_desc, f_desc + ks * (TILE >> 4), IDESC_S);
+            mma_dot_ts<DM>(lead, tmem, q_col, f_desc + (2 * i) % S * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&s_full));
-            // dP goes where dS of two tiles before is; with 64 features the product that reads it has another shape than this one,
-            // and products of different shapes need not keep their order
-            if (!landed(2 * i + 2) || (DM == 64 && i > 1 && !warp_wait(smem_u32(&dq_done), i & 1, stop))) return false;
+        };
+        auto dprobs = [&](uint32_t i) {
+            const uint32_t vs = (2 * i + 1) % S;
             fence_after();
-            mma_dot<DM>(lead, tmem + 128 + (i & 1) * 128, dy_desc, f_desc + vs * (TILE >> 4), IDESC_S);
-            mma_commit(lead, smem_u32(&dp_full[i & 1]));
+            mma_dot<DM>(lead, tmem + 128, dy_desc, f_desc + vs * (TILE >> 4), IDESC_S);
+            mma_commit(lead, smem_u32(&dp_full));
             mma_commit(lead, smem_u32(&kv_empty[vs]));
-            return true;
         };
         const uint32_t count = kt.count;
-        bool ok = warp_wait(smem_u32(&q_full), 0, stop) && landed(1) && products(0);
+        bool ok = warp_wait(smem_u32(&q_moved), 0, stop) && landed(1);
+        if (ok) {
+            scores(0);
+            if ((ok = landed(2))) dprobs(0);
+        }
         for (uint32_t i = 0; i < count && ok; ++i) {
             if (i + 1 < count) {
-                if (!(ok = landed(2 * i + 3) && warp_wait(smem_u32(&s_free), i & 1, stop) && products(i + 1))) break;
+                if (!(ok = landed(2 * i + 3) && warp_wait(smem_u32(&s_free), i & 1, stop))) break;
+                scores(i + 1);
+                if (!(ok = landed(2 * i + 4) && warp_wait(smem_u32(&dp_free), i & 1, stop))) break;
+                dprobs(i + 1);
             }
-            ok = warp_wait(smem_u32(&ds_full[i & 1]), (i >> 1) & 1, stop);
-            if (!ok) break;
+            if (!(ok = warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
             fence_after();
             const uint32_t ks = (2 * i) % S;
-            mma_halves(lead, o_col, tmem + 128 + (i & 1) * 128, 64, r_desc + ks * (TILE >> 4), IDESC_O, i != 0);
+            mma_weighted<128>(lead, o_col, tmem + 256, r_desc + ks * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&kv_empty[ks]));
-            if (DM == 64) mma_commit(lead, smem_u32(&dq_done));
+            mma_commit(lead, smem_u32(&dq_done));
         }
         mma_commit(lead, smem_u32(ok ? &o_full : &drained));
         if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
@@ -361,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 9) tmem_free(tmem, 512);
+    if (warp == kIssuer) tmem_free(tmem, 512);
     if (tid == 0 && stop_flag) report_stop(maps.timeouts, a.status);
 }
 
@@ -409,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     const int first = split ? (int)((int64_t)all * seg / maps.segments) : 0;
     const int count = (split ? (int)((int64_t)all * (seg + 1) / maps.segments) : all) - first;
 
-    if (warp == 8 && lane == 0) {
+    if (warp == kCopier && lane == 0) {
         prefetch_map(&maps.k);
         prefetch_map(&maps.v);
         prefetch_map(&maps.q);
@@ -420,24 +449,24 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         mbar_init(&kv_full, 1);
         mbar_init(&s_full, 1);
         mbar_init(&dp_full, 1);
-        mbar_init(&p_full, 8);
-        mbar_init(&ds_full, 8);
-        for (int i = 0; i < 2; ++i) { mbar_init(&st_full[i], 1); mbar_init(&st_empty[i], 8); }
+        mbar_init(&p_full, kWarps);
+        mbar_init(&ds_full, kWarps);
+        for (int i = 0; i < 2; ++i) { mbar_init(&st_full[i], 1); mbar_init(&st_empty[i], kWarps); }
         mbar_init(&dl_full, 1);
-        mbar_init(&dl_empty, 8);
+        mbar_init(&dl_empty, kWarps);
         mbar_init(&o_full, 1);
         mbar_init(&drained, 1);
         stop_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (warp == kIssuer) tmem_alloc(smem_u32(&tmem_slot), 512);
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot, dv_col = tmem + 256, dk_col = tmem + 256 + DM;
     // At 64 features the weights and dS have columns of their own; at 128 they overlay what they are made of, and the products of
     // one shape (all 128 x 128 x 16 there) are carried out in the order of their issue.
-    const uint32_t p_col = DM == 64 ? tmem + 384 : tmem, ds_col = p_col + (DM == 64 ? 64 : 128), apart = DM == 64 ? 32 : 64;
+    const uint32_t p_col = DM == 64 ? tmem + 384 : tmem, ds_col = p_col + (DM == 64 ? 64 : 128), apart = DM == 64 ? kCols / 2 : kCols;
     float c = 1.f;                                                  // factor of dS
     if (!kIsBf16<T> && count) {
         const int tiles = (int)(((int64_t)s.T * a.G + 127) / 128);
@@ -447,10 +476,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         c = ds_factor(warp_max(peak), maps.v_peak[((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128) + tile]);
     }
 
-    if (warp < 8) {
+    if (warp < kWarps) {
         const int u = warp >> 2, r = tid & 127, j = k0 + r;
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
-        const uint32_t S_at = tmem + 64 * u + lane_off, dp_at = S_at + 128, P_at = p_col + apart * u + lane_off, ds_at = ds_col + apart * u + lane_off;
+        const uint32_t S_at = tmem + kCols * u + lane_off, dp_at = S_at + 128, P_at = p_col + apart * u + lane_off, ds_at = ds_col + apart * u + lane_off;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
         const f32x2 c2 = kIsBf16<T> ? pack2(1.f, 1.f) : pack2(c / kPScale, c / kPScale);
         bool ok = true;
@@ -461,18 +490,17 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             const bool edge = !(k0 + 127 <= q0 + a.right && (q0 + 127 <= k0 + a.left || k0 + 127 < a.sinks) && q0 + 127 < s.n && k0 + 127 < s.n);
             if (!warp_wait(smem_u32(&st_full[b]), (i >> 1) & 1, stop) || !warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
             fence_after();
-            uint32_t x[64], w[32];
-            read64(S_at, x);
-            uint32_t mk[2] = {~0u, ~0u};
+            uint32_t x[kCols], w[kCols / 2];
+            read_columns(S_at, x);
+            uint32_t mk = ~0u;
             if (edge) {
                 const int hi = j >= s.n ? -1 : (j < a.sinks ? s.n - 1 : min(j + a.left, s.n - 1)) - q0, lo = j - a.right - q0;
-#pragma unroll
-                for (int g = 0; g < 2; ++g) mk[g] = seen_bits(lo - 64 * u - 32 * g, hi - 64 * u - 32 * g, INT_MIN + 1);
+                mk = seen_bits(lo - kCols * u, hi - kCols * u, INT_MIN + 1);
             }
-            const float4* lse4 = reinterpret_cast<const float4*>(&s_lse[b][64 * u]);
-            const float4* del4 = reinterpret_cast<const float4*>(&s_delta[64 * u]);
+            const float4* lse4 = reinterpret_cast<const float4*>(&s_lse[b][kCols * u]);
+            const float4* del4 = reinterpret_cast<const float4*>(&s_delta[kCols * u]);
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
+            for (int c = 0; c < kCols; c += 4) {
                 const float4 z = lse4[c >> 2];
                 float e[4];
                 unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack2(z.x, z.y)), e[0], e[1]);
@@ -482,10 +510,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             }
             if (edge) clear_unseen(x, mk);
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(x[c]), __uint_as_float(x[c + 1]));
-            tmem_st32(P_at, w);
-            if (ragged && q0 + 127 >= s.n) {                    // queries behind the length may be anything: zeros
-                const int slot = (2 * i + u) % S;               // one warpgroup clears q, the other dy
+            for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(x[c]), __uint_as_float(x[c + 1]));
+            tmem_st16(P_at, w);
+            if (ragged && u < 2 && q0 + 127 >= s.n) {                    // queries behind the length may be anything: zeros
+                const int slot = (2 * i + u) % S;               // one warpgroup clears q, another dy
                 if (!warp_wait(smem_u32(&q_full[slot]), ((2 * i + u) / S) & 1, stop)) { ok = false; break; }
                 if (q0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
                 fence_async_smem();
@@ -499,10 +527,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             }
             if (!warp_wait(smem_u32(&dl_full), i & 1, stop) || !warp_wait(smem_u32(&dp_full), i & 1, stop)) { ok = false; break; }
             fence_after();
-            uint32_t y[64];
-            read64(dp_at, y);
+            uint32_t y[kCols];
+            read_columns(dp_at, y);
 #pragma unroll
-            for (int c = 0; c < 64; c += 4) {
+            for (int c = 0; c < kCols; c += 4) {
                 const float4 z = del4[c >> 2];
                 float e[4];
                 unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, pack2(z.x, z.y)), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e[0], e[1]);
@@ -512,8 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             }
             if (ragged) clear_unseen(y, mk);                    // dP of such pairs may be anything
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
-            tmem_st32(ds_at, w);
+            for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
+            tmem_st16(ds_at, w);
             tmem_wait_st();
             fence_before();
             __syncwarp();
@@ -524,13 +552,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         }
         if (count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
         fence_after();
-        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : u ? a.scale / c : kIsBf16<T> ? 1.f : 1.f / kPScale;       // the first warpgroup stores dv, the second dk
-        float* part = maps.partial + (((((int64_t)s.b * a.Hkv + h) * maps.split_tiles + tile) * maps.segments + seg) * 2 + 1 - u) * (DM * 128) + r;
-        char* const stage = smem + u * TILE;                       // the keys' and values' place
+        const int which = u & 1;                                   // even warpgroups store dv, odd ones dk, each half of the features
+        const float f = !ok || *stop ? __int_as_float(0x7fffffff) : which ? a.scale / c : kIsBf16<T> ? 1.f : 1.f / kPScale;
+        float* part = maps.partial + (((((int64_t)s.b * a.Hkv + h) * maps.split_tiles + tile) * maps.segments + seg) * 2 + 1 - which) * (DM * 128) + r;
+        char* const stage = smem + which * TILE;                       // the keys' and values' place
 #pragma unroll 1
-        for (int col = 0; col < DM; col += 32) {
+        for (int col = (u >> 1) * (DM / 2); col < ((u >> 1) + 1) * (DM / 2); col += 32) {
             uint32_t o[32];
-            tmem_ld32((u ? dk_col : dv_col) + lane_off + col, o);
+            tmem_ld32((which ? dk_col : dv_col) + lane_off + col, o);
             tmem_wait_ld();
             settled32(o);
             float y[32];
@@ -545,14 +574,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         }
         if (!split) {
             fence_async_smem();
-            group_sync<128>(2 + u);
-            if (r == 0) {
+            group_sync<kWork / 2>(2 + which);
+            if (u < 2 && r == 0) {
 #pragma unroll
-                for (int p = 0; p < DM / 64; ++p) tma_store_4d(u ? &maps.dk : &maps.dv, smem_u32(stage) + p * kPanel, 64 * p, k0, h, s.b);
+                for (int p = 0; p < DM / 64; ++p) tma_store_4d(which ? &maps.dk : &maps.dv, smem_u32(stage) + p * kPanel, 64 * p, k0, h, s.b);
                 tma_stores_read();
             }
         }
-    } else if (warp == 8 && lane == 0 && count) {
+    } else if (warp == kCopier && lane == 0 && count) {
         bool ok = true;
         int issued = 0;
         mbar_arrive_expect_tx(smem_u32(&kv_full), 2 * TILE);
@@ -576,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             mbar_wait(smem_u32(&kv_full), 0, 1u << 12);
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&q_full[i % S]), (i / S) & 1, 1u << 12);
         }
-    } else if (warp == 9 && count) {
+    } else if (warp == kIssuer && count) {
         const uint32_t lead = elect_one();
         const uint64_t k_desc = desc_features(base_at), v_desc = desc_features(base_at + TILE), f_desc = desc_features(ring_at), r_desc = desc_rows(ring_at);
         const uint32_t steps = count;
@@ -605,18 +634,18 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             const bool more = i + 1 < steps;
             if (!(ok = (!more || landed(2 * i + 3)) && warp_wait(smem_u32(&p_full), i & 1, stop))) break;
             fence_after();
-            mma_halves(lead, dv_col, p_col, apart, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
+            mma_pieces(lead, dv_col, p_col, apart, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&q_empty[ds]));
             if (more) scores(i + 1);
             if (!(ok = (!more || landed(2 * i + 4)) && warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
             fence_after();
-            mma_halves(lead, dk_col, ds_col, apart, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
+            mma_pieces(lead, dk_col, ds_col, apart, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
             mma_commit(lead, smem_u32(&q_empty[qs]));
             if (more) dprobs(i + 1);
         }
         mma_commit(lead, smem_u32(ok ? &o_full : &drained));
         if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
-    } else if (warp == 10) {
+    } else if (warp == kFetcher) {
         // minus the rows' sums, and minus their delta, with the factors of half precision
         const float shift = kIsBf16<T> ? 0.f : kPLog2, minus = kIsBf16<T> ? -1.f : -c / kPScale;
         const int rows = s.T * a.G;
@@ -647,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 9) tmem_free(tmem, 512);
+    if (warp == kIssuer) tmem_free(tmem, 512);
     if (tid == 0 && stop_flag) report_stop(maps.timeouts, a.status);
 }
 

@@ -58,6 +58,12 @@ __device__ __forceinline__ void mma_dot(uint32_t lead, uint32_t d, uint64_t a, u
     for (int k = 0; k < DM / 16; ++k)         // addresses stand in units of 16 bytes in a descriptor's lowest bits
         mma_ss(lead, d, a + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, b + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, idesc, k != 0);
 }
+// The same with the rows of A in tensor memory, as 16-bit pairs.
+template <int DM>
+__device__ __forceinline__ void mma_dot_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+#pragma unroll
+    for (int k = 0; k < DM / 16; ++k) mma_ts(lead, d, a + k * 8, b + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, idesc, k != 0);
+}
 // D[128, N] (+)= A[128, KEYS] in tensor memory (16-bit pairs) . B[KEYS rows, N]; desc_rows of B.
 template <int KEYS>
 __device__ __forceinline__ void mma_weighted(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -101,6 +107,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
           "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
           "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
           "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
