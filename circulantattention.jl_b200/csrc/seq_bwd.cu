@@ -346,11 +346,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     } else if (warp == kIssuer && kt.count) {
         const uint32_t lead = elect_one();
         const uint64_t dy_desc = desc_features(base_at), f_desc = desc_features(kv_at), r_desc = desc_rows(kv_at);
-        uint32_t have = 0;                                     // keys and values land in order: each is waited for once
-        auto landed = [&](uint32_t items) {
-            for (; have < items; ++have)
-                if (!warp_wait(smem_u32(&kv_full[have % S]), (have / S) & 1, stop)) return false;
-            return true;
+        // Waits for the keys and values of tile i, and for `bar`.  A check costs this warp 130 cycles in which no product starts,
+        // so its lanes check all three at once.
+        auto ready = [&](uint32_t i, uint64_t* bar, uint32_t parity) {
+            const uint32_t item = 2 * i + lane;
+            return warp_wait(lane < 2 ? smem_u32(&kv_full[item % S]) : smem_u32(bar), lane < 2 ? (item / S) & 1 : parity, stop);
         };
         auto scores = [&](uint32_t i) {
             fence_after();
@@ -365,16 +365,16 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             mma_commit(lead, smem_u32(&kv_empty[vs]));
         };
         const uint32_t count = kt.count;
-        bool ok = warp_wait(smem_u32(&q_moved), 0, stop) && landed(1);
+        bool ok = ready(0, &q_moved, 0);
         if (ok) {
             scores(0);
-            if ((ok = landed(2))) dprobs(0);
+            dprobs(0);
         }
         for (uint32_t i = 0; i < count && ok; ++i) {
             if (i + 1 < count) {
-                if (!(ok = landed(2 * i + 3) && warp_wait(smem_u32(&s_free), i & 1, stop))) break;
+                if (!(ok = ready(i + 1, &s_free, i & 1))) break;
                 scores(i + 1);
-                if (!(ok = landed(2 * i + 4) && warp_wait(smem_u32(&dp_free), i & 1, stop))) break;
+                if (!(ok = warp_wait(smem_u32(&dp_free), i & 1, stop))) break;
                 dprobs(i + 1);
             }
             if (!(ok = warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
