@@ -52,23 +52,26 @@ __device__ __forceinline__ float warp_max(float x) {
     return x;
 }
 
-// A operand whose pieces of 32 contracted elements (a warpgroup's columns as 16-bit pairs) lie `apart` columns apart.
-__device__ __forceinline__ void mma_pieces(uint32_t lead, uint32_t d, uint32_t a, uint32_t apart, uint64_t b, uint32_t idesc, bool add) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) mma_ts(lead, d, a + (k >> 1) * apart + (k & 1) * 8, b + k * 128, idesc, add || k != 0);
-}
-
 __device__ __forceinline__ void read_columns(uint32_t at, uint32_t* x) {
     tmem_ld32(at, x);
     tmem_wait_ld();
     settled32(x);
 }
 
+// 16 columns of either half of a tile's 128
+__device__ __forceinline__ void read_halves(uint32_t at, uint32_t* x) {
+    tmem_ld16(at, x);
+    tmem_ld16(at + 64, x + 16);
+    tmem_wait_ld();
+    settled32(x);
+}
+
 // Zeros where the bit is not set.  Always in a block of its own behind one uniform branch: as a condition on each element the
 // selects ran for every tile and took as long as the arithmetic.
+template <int COUNT>
 __device__ __forceinline__ void clear_unseen(uint32_t* x, uint32_t mk) {
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0u;
+    for (int c = 0; c < COUNT; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0u;
 }
 
 template <int DM>
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             if (edge) {
                 const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
                 mk = seen_bits(lo - kCols * u, hi - kCols * u, sk - kCols * u);
-                clear_unseen(x, mk);
+                clear_unseen<kCols>(x, mk);
                 if (far >= s.n && u == 0) {                    // keys behind the length may be anything: zeros
                     const int slot = (2 * i) % S;              // the scores are there, so the keys are
                     if (key0 + r >= s.n) clear_row<DM>(smem + (1 + slot) * TILE, r);
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 y[c] = __float_as_uint(e0);
                 y[c + 1] = __float_as_uint(e1);
             }
-            if (ragged) clear_unseen(y, mk);                   // dP of such pairs may be anything
+            if (ragged) clear_unseen<kCols>(y, mk);                   // dP of such pairs may be anything
 #pragma unroll
             for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
             if (i && !warp_wait(smem_u32(&dq_done), (i - 1) & 1, stop)) { ok = false; break; }
@@ -416,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     constexpr uint32_t TILE = kTileBytes<DM>;
     constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
     extern __shared__ char raw[];
-    __shared__ uint64_t q_full[S], q_empty[S], kv_full, s_full, dp_full, p_full, ds_full, st_full[2], st_empty[2], dl_full, dl_empty, o_full, drained;
+    __shared__ uint64_t q_full[S], q_empty[S], kv_full, s_full, dp_full, p_full[2], ds_full[2], st_full[2], st_empty[2], dl_full, dl_empty, o_full, drained;
     __shared__ uint32_t tmem_slot;
     __shared__ int stop_flag;
     __shared__ __align__(16) float s_lse[2][128], s_delta[128];       // delta once: the tiles take all but 2 KB
@@ -439,25 +442,33 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     const int count = (split ? (int)((int64_t)all * (seg + 1) / maps.segments) : all) - first;
 
     if (warp == kCopier && lane == 0) {
-        prefetch_map(&maps.k);
-        prefetch_map(&maps.v);
-        prefetch_map(&maps.q);
-        prefetch_map(&maps.dy);
-    }
-    if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
         mbar_init(&kv_full, 1);
         mbar_init(&s_full, 1);
         mbar_init(&dp_full, 1);
-        mbar_init(&p_full, kWarps);
-        mbar_init(&ds_full, kWarps);
-        for (int i = 0; i < 2; ++i) { mbar_init(&st_full[i], 1); mbar_init(&st_empty[i], kWarps); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&p_full[i], kWarps);
+            mbar_init(&ds_full[i], kWarps);
+            mbar_init(&st_full[i], 1);
+            mbar_init(&st_empty[i], kWarps);
+        }
         mbar_init(&dl_full, 1);
         mbar_init(&dl_empty, kWarps);
         mbar_init(&o_full, 1);
         mbar_init(&drained, 1);
         stop_flag = 0;
         mbar_fence_init();
+        fence_async_smem();
+        if (count) {                                           // on their way while the rest is set up
+            mbar_arrive_expect_tx(smem_u32(&kv_full), 2 * TILE);
+#pragma unroll
+            for (int p = 0; p < DM / 64; ++p) {
+                tma_load_4d(base_at + p * kPanel, &maps.k, 64 * p, k0, h, s.b, smem_u32(&kv_full));
+                tma_load_4d(base_at + TILE + p * kPanel, &maps.v, 64 * p, k0, h, s.b, smem_u32(&kv_full));
+            }
+        }
+        prefetch_map(&maps.q);
+        prefetch_map(&maps.dy);
     }
     if (warp == kIssuer) tmem_alloc(smem_u32(&tmem_slot), 512);
     fence_before();
@@ -466,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     const uint32_t tmem = tmem_slot, dv_col = tmem + 256, dk_col = tmem + 256 + DM;
     // At 64 features the weights and dS have columns of their own; at 128 they overlay what they are made of, and the products of
     // one shape (all 128 x 128 x 16 there) are carried out in the order of their issue.
-    const uint32_t p_col = DM == 64 ? tmem + 384 : tmem, ds_col = p_col + (DM == 64 ? 64 : 128), apart = DM == 64 ? kCols / 2 : kCols;
+    const uint32_t p_col = DM == 64 ? tmem + 384 : tmem, ds_col = p_col + (DM == 64 ? 64 : 128), apart = DM == 64 ? 8 : 16;
     float c = 1.f;                                                  // factor of dS
     if (!kIsBf16<T> && count) {
         const int tiles = (int)(((int64_t)s.T * a.G + 127) / 128);
@@ -479,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     if (warp < kWarps) {
         const int u = warp >> 2, r = tid & 127, j = k0 + r;
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
-        const uint32_t S_at = tmem + kCols * u + lane_off, dp_at = S_at + 128, P_at = p_col + apart * u + lane_off, ds_at = ds_col + apart * u + lane_off;
+        const uint32_t S_at = tmem + 16 * u + lane_off, dp_at = S_at + 128, P_at = p_col + apart * u + lane_off, ds_at = ds_col + apart * u + lane_off;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
         const f32x2 c2 = kIsBf16<T> ? pack2(1.f, 1.f) : pack2(c / kPScale, c / kPScale);
         bool ok = true;
@@ -490,65 +501,72 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             const bool edge = !(k0 + 127 <= q0 + a.right && (q0 + 127 <= k0 + a.left || k0 + 127 < a.sinks) && q0 + 127 < s.n && k0 + 127 < s.n);
             if (!warp_wait(smem_u32(&st_full[b]), (i >> 1) & 1, stop) || !warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
             fence_after();
-            uint32_t x[kCols], w[kCols / 2];
-            read_columns(S_at, x);
-            uint32_t mk = ~0u;
+            // Columns 16 u .. 16 u + 15 of either half of the tile: the product with the first half starts while the weights
+            // of the second are made.
+            uint32_t x[kCols], mk = ~0u;
+            read_halves(S_at, x);
             if (edge) {
-                const int hi = j >= s.n ? -1 : (j < a.sinks ? s.n - 1 : min(j + a.left, s.n - 1)) - q0, lo = j - a.right - q0;
-                mk = seen_bits(lo - kCols * u, hi - kCols * u, INT_MIN + 1);
+                const int hi = j >= s.n ? -1 : (j < a.sinks ? s.n - 1 : min(j + a.left, s.n - 1)) - q0 - 16 * u, lo = j - a.right - q0 - 16 * u;
+                mk = (seen_bits(lo, hi, INT_MIN + 1) & 0xffffu) | seen_bits(lo - 64, hi - 64, INT_MIN + 1) << 16;
             }
-            const float4* lse4 = reinterpret_cast<const float4*>(&s_lse[b][kCols * u]);
-            const float4* del4 = reinterpret_cast<const float4*>(&s_delta[kCols * u]);
-#pragma unroll
-            for (int c = 0; c < kCols; c += 4) {
-                const float4 z = lse4[c >> 2];
-                float e[4];
-                unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, pack2(z.x, z.y)), e[0], e[1]);
-                unpack2(fma2(pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), sc2, pack2(z.z, z.w)), e[2], e[3]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[c + k] = __float_as_uint(fast_exp2(e[k]));
-            }
-            if (edge) clear_unseen(x, mk);
-#pragma unroll
-            for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(x[c]), __uint_as_float(x[c + 1]));
-            tmem_st16(P_at, w);
-            if (ragged && u < 2 && q0 + 127 >= s.n) {                    // queries behind the length may be anything: zeros
+            if (ragged && u < 2 && q0 + 127 >= s.n) {           // queries behind the length may be anything: zeros
                 const int slot = (2 * i + u) % S;               // one warpgroup clears q, another dy
                 if (!warp_wait(smem_u32(&q_full[slot]), ((2 * i + u) / S) & 1, stop)) { ok = false; break; }
                 if (q0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
                 fence_async_smem();
             }
-            tmem_wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(smem_u32(&p_full));
-                mbar_arrive(smem_u32(&st_empty[b]));
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const float4* lse4 = reinterpret_cast<const float4*>(&s_lse[b][64 * g + 16 * u]);
+                uint32_t* const xg = x + 16 * g;
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) {
+                    const float4 z = lse4[c >> 2];
+                    float e[4];
+                    unpack2(fma2(pack2(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1])), sc2, pack2(z.x, z.y)), e[0], e[1]);
+                    unpack2(fma2(pack2(__uint_as_float(xg[c + 2]), __uint_as_float(xg[c + 3])), sc2, pack2(z.z, z.w)), e[2], e[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) xg[c + k] = __float_as_uint(fast_exp2(e[k]));
+                }
+                if (edge) clear_unseen<16>(xg, mk >> 16 * g);
+                uint32_t w[8];
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1]));
+                tmem_st8(P_at + 4 * apart * g, w);
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&p_full[g]));
             }
+            if (lane == 0) mbar_arrive(smem_u32(&st_empty[b]));
             if (!warp_wait(smem_u32(&dl_full), i & 1, stop) || !warp_wait(smem_u32(&dp_full), i & 1, stop)) { ok = false; break; }
             fence_after();
             uint32_t y[kCols];
-            read_columns(dp_at, y);
+            read_halves(dp_at, y);
 #pragma unroll
-            for (int c = 0; c < kCols; c += 4) {
-                const float4 z = del4[c >> 2];
-                float e[4];
-                unpack2(mul2(fma2(pack2(__uint_as_float(y[c]), __uint_as_float(y[c + 1])), c2, pack2(z.x, z.y)), pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]))), e[0], e[1]);
-                unpack2(mul2(fma2(pack2(__uint_as_float(y[c + 2]), __uint_as_float(y[c + 3])), c2, pack2(z.z, z.w)), pack2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3]))), e[2], e[3]);
+            for (int g = 0; g < 2; ++g) {
+                const float4* del4 = reinterpret_cast<const float4*>(&s_delta[64 * g + 16 * u]);
+                uint32_t *const xg = x + 16 * g, *const yg = y + 16 * g;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) y[c + k] = __float_as_uint(e[k]);
+                for (int c = 0; c < 16; c += 4) {
+                    const float4 z = del4[c >> 2];
+                    float e[4];
+                    unpack2(mul2(fma2(pack2(__uint_as_float(yg[c]), __uint_as_float(yg[c + 1])), c2, pack2(z.x, z.y)), pack2(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1]))), e[0], e[1]);
+                    unpack2(mul2(fma2(pack2(__uint_as_float(yg[c + 2]), __uint_as_float(yg[c + 3])), c2, pack2(z.z, z.w)), pack2(__uint_as_float(xg[c + 2]), __uint_as_float(xg[c + 3]))), e[2], e[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) yg[c + k] = __float_as_uint(e[k]);
+                }
+                if (ragged) clear_unseen<16>(yg, mk >> 16 * g);     // dP of such pairs may be anything
+                uint32_t w[8];
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(yg[c]), __uint_as_float(yg[c + 1]));
+                tmem_st8(ds_at + 4 * apart * g, w);
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ds_full[g]));
             }
-            if (ragged) clear_unseen(y, mk);                    // dP of such pairs may be anything
-#pragma unroll
-            for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(y[c]), __uint_as_float(y[c + 1]));
-            tmem_st16(ds_at, w);
-            tmem_wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(smem_u32(&ds_full));
-                mbar_arrive(smem_u32(&dl_empty));
-            }
+            if (lane == 0) mbar_arrive(smem_u32(&dl_empty));
         }
         if (count && ok) ok = warp_wait(smem_u32(&o_full), 0, stop);
         fence_after();
@@ -584,12 +602,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     } else if (warp == kCopier && lane == 0 && count) {
         bool ok = true;
         int issued = 0;
-        mbar_arrive_expect_tx(smem_u32(&kv_full), 2 * TILE);
-#pragma unroll
-        for (int p = 0; p < DM / 64; ++p) {
-            tma_load_4d(base_at + p * kPanel, &maps.k, 64 * p, k0, h, s.b, smem_u32(&kv_full));
-            tma_load_4d(base_at + TILE + p * kPanel, &maps.v, 64 * p, k0, h, s.b, smem_u32(&kv_full));
-        }
         Steps at(a, t_lo, first);
         for (; issued < 2 * count; ++issued) {
             const int slot = issued % S;
@@ -619,6 +631,17 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             mma_dot<DM>(lead, tmem, k_desc, f_desc + (2 * i) % S * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&s_full));
         };
+        auto weighted = [&](uint32_t to, uint32_t from, uint64_t* full, uint32_t slot, uint32_t i) {
+#pragma unroll
+            for (uint32_t g = 0; g < 2; ++g) {
+                if (!warp_wait(smem_u32(&full[g]), i & 1, stop)) return false;
+                fence_after();
+#pragma unroll
+                for (uint32_t k = 4 * g; k < 4 * g + 4; ++k)
+                    mma_ts(lead, to, from + k * apart, r_desc + slot * (TILE >> 4) + k * 128, IDESC_O, i != 0 || k != 0);
+            }
+            return true;
+        };
         auto dprobs = [&](uint32_t i) {
             mma_dot<DM>(lead, tmem + 128, v_desc, f_desc + (2 * i + 1) % S * (TILE >> 4), IDESC_S);
             mma_commit(lead, smem_u32(&dp_full));
@@ -632,14 +655,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         for (uint32_t i = 0; i < steps && ok; ++i) {
             const uint32_t qs = (2 * i) % S, ds = (2 * i + 1) % S;
             const bool more = i + 1 < steps;
-            if (!(ok = (!more || landed(2 * i + 3)) && warp_wait(smem_u32(&p_full), i & 1, stop))) break;
-            fence_after();
-            mma_pieces(lead, dv_col, p_col, apart, r_desc + ds * (TILE >> 4), IDESC_O, i != 0);
+            if (!(ok = (!more || landed(2 * i + 3)) && weighted(dv_col, p_col, p_full, ds, i))) break;
             mma_commit(lead, smem_u32(&q_empty[ds]));
             if (more) scores(i + 1);
-            if (!(ok = (!more || landed(2 * i + 4)) && warp_wait(smem_u32(&ds_full), i & 1, stop))) break;
-            fence_after();
-            mma_pieces(lead, dk_col, ds_col, apart, r_desc + qs * (TILE >> 4), IDESC_O, i != 0);
+            if (!(ok = (!more || landed(2 * i + 4)) && weighted(dk_col, ds_col, ds_full, qs, i))) break;
             mma_commit(lead, smem_u32(&q_empty[qs]));
             if (more) dprobs(i + 1);
         }
