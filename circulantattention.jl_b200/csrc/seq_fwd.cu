@@ -111,11 +111,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     const Stream st0 = stream_of<PAIR>(a, s, kt, 0, R0, rows), st1 = stream_of<PAIR>(a, s, kt, 1, PAIR ? R0 + 128 : R0, rows);
 
     if (warp == 8 && lane == 0) {
-        if (maps.rows) prefetch_map(&maps.q);
-        prefetch_map(&maps.k);
-        prefetch_map(&maps.v);
-    }
-    if (tid == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
         for (int u = 0; u < 2; ++u) {
             mbar_init(&q_full[u], maps.rows ? 1 : PAIR ? 4 : 8);
@@ -127,6 +122,18 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         mbar_init(&drained, 1);
         stop_flag = 0;
         mbar_fence_init();
+        fence_async_smem();
+        if (maps.rows) {                                                   // on their way while the rest is set up
+            for (int u = 0; u < (PAIR ? 2 : 1); ++u) {
+                if (R0 + 128 * u >= rows) break;
+                mbar_arrive_expect_tx(smem_u32(&q_full[u]), TILE);
+#pragma unroll
+                for (int p = 0; p < DM / 64; ++p)
+                    tma_load_4d(q_at + u * TILE + p * kPanel, &maps.q, 64 * p, h * a.G, s.t0 + (R0 + 128 * u) / a.G, PAGED ? 0 : s.b, smem_u32(&q_full[u]));
+            }
+        }
+        prefetch_map(&maps.k);
+        prefetch_map(&maps.v);
     }
     if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
     fence_before();
@@ -378,16 +385,6 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         // ------------------------------------------------------------ copies
         bool ok = true;
         int issued = 0;
-        if (maps.rows && lane == 0) {
-            for (int u = 0; u < (PAIR ? 2 : 1); ++u) {
-                if (R0 + 128 * u >= rows) break;
-                mbar_arrive_expect_tx(smem_u32(&q_full[u]), TILE);
-#pragma unroll
-                for (int p = 0; p < DM / 64; ++p)
-                    tma_load_4d(q_at + u * TILE + p * kPanel, &maps.q, 64 * p, h * a.G, s.t0 + (R0 + 128 * u) / a.G, PAGED ? 0 : s.b, smem_u32(&q_full[u]));
-            }
-        }
-        __syncwarp();
         if (!PAGED) {
             if (lane == 0) {
                 for (; issued < 2 * kt.count; ++issued) {
