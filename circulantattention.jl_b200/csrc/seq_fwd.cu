@@ -5,13 +5,19 @@
 // row reads them, turns them into weights, and writes those back over the scores as 16-bit pairs, from where the second
 // product takes them as its A operand: the weights never see shared memory.
 //
-// Roles: two groups of four warps do the softmax, one warp copies keys and values by TMA into a ring of tiles, one thread
+// Roles: two groups of four warps do the softmax, one warp copies keys and values by TMA into a ring of tiles, one warp
 // issues the products.  The two groups are two streams that share the tensor cores: while one turns its scores into weights,
-// the products of the other run.  With PAIR the streams are two row tiles that share every key tile; without, they take
-// the even and the odd key tiles of one row tile and are joined at the end (few rows: decoding).
+// the products of the other run.  With PAIR the streams are two row tiles that share every key tile (half the copies); without,
+// they take the even and the odd key tiles of one row tile and are joined at the end (few rows).
 //
 // The accumulator is rescaled only where a row's maximum grew by more than 2^8 since its reference: the weights stay below
-// 2^8, and the products and sums are held in Float32.
+// 2^8, and the products and sums are held in Float32.  Weights are rounded to the tensors' type before their product, once more
+// than the result itself: errors are 1.4 of a plain implementation that keeps them in Float32.
+//
+// Bound: the exponentials and the products, 2048 cycles each for a pair of 128 x 128 tiles at 128 features; a pair takes about
+// 3300 in the steady state, since a row's chain (scores, maximum, exponentials, weights) leaves gaps that two streams do not
+// fill.  Measured: 65536 tokens, window 4096, 16 query and 2 key heads 2.1 ms (0.86 PFLOP/s of visible pairs, 0.63 of what a
+// large matrix product keeps up); 2 x 16384 tokens, window 1024, 16 and 4 heads 415 us.
 #include "seq_umma.cuh"
 
 #include <limits.h>

@@ -80,7 +80,10 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, scale=None):
 
     q `(D, heads, N, B)`, k and v `(D, heads', N, B)` with heads a multiple of heads'; D a multiple of 8 up to 128.
     left=None: no left end.  lengths: Int32 `(B,)`, the tokens that exist in each sequence (what lies behind them has no
-    effect, whatever it holds; y and the gradients are zero there).  scale: 1/sqrt(D) by default."""
+    effect, whatever it holds; y and the gradients are zero there).  scale: 1/sqrt(D) by default.
+
+    Infinities and NaN in keys or values that no token sees have no effect.  Where some token sees them, neighbours that do
+    not may get NaN too: their weight is zero, and zero times infinity is not a number."""
     return host.window_attention(q, k, v, _left(left), int(right), int(sinks), lengths, scale)
 
 

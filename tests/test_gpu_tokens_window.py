@@ -97,6 +97,21 @@ def test_whatever_lies_behind_the_length_has_no_effect(ca, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_is_not_a_number_is_not_hidden(ca, dtype, D):
+    """A key that is not a number shows in every token that sees it, at whatever place of a tile the key is; tokens of tiles
+    further on are not touched."""
+    q, k, v, _ = (t.cuda() for t in problem(D, 2, 1, 600, 1, dtype))
+    for j in (*range(8, 17), 63, 64, 70, 71, 127, 128, 255):
+        bad = k.clone()
+        bad[:, 0, j, 0] = math.nan
+        with torch.no_grad():
+            y = ca.window_attention(q, bad, v, 40)
+        assert y[:, :, j : j + 41, 0].isnan().all()
+        assert not y[:, :, j + 300 :, 0].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=lambda d: str(d)[6:])
 def test_empty_sequences_give_zeros_every_time(ca, dtype):
     """Tiles that see no key at all, next to some that do, many times over: nothing that was on its way lands in the results."""
     q, k, v, dy = (t.cuda() for t in problem(128, 4, 2, 300, 4, dtype))
