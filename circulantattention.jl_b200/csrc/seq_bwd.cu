@@ -12,8 +12,8 @@
 // Bound: the products at 128 features, 1536 cycles a tile (dq) and 2048 (dk, dv); measured 2100 and 2800, the rest is the
 // chain scores - weights - dS - product of one tile, of which neither tensor memory (all 512 columns are taken) nor shared memory
 // holds a second.  Short windows are bound by what stands before the first tile (queries, results and their remainders
-// from memory: 9000 cycles).  2 x 16384 tokens, window 1024, 16 query and 4 key heads: 515 and 545 us; 3 x 5001 tokens, 8 heads of
-// 64 features, window 127, half: 60 and 58 us.
+// from memory: 9000 cycles).  2 x 16384 tokens, window 1024, 16 query and 4 key heads: 497 and 540 us; 3 x 5001 tokens, 8 heads of
+// 64 features, window 127, half: 59 and 58 us.
 #include "seq_umma.cuh"
 
 #include <limits.h>
@@ -32,7 +32,8 @@ template <int DM> constexpr size_t kBwdSmem = (size_t)(2 + kSlots<DM>) * kTileBy
 
 struct BwdMaps {
     CUtensorMap k, v, q, dy;
-    CUtensorMap q_rows, dy_rows, dq_rows, dk, dv;
+    CUtensorMap q_rows, dy_rows, y_rows, rest_rows, dq_rows, dk, dv;
+    int sms;                // dq: the CTA so many further on takes this one's place
     int rows;               // q, dy and dq of the first sweep move by tiles of rows (maps), else by threads
     int* timeouts;
     float *dy_peak, *v_peak;    // half: largest magnitudes of each tile of 128 query rows / keys, [b][key head][tile]
@@ -346,6 +347,22 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
 #pragma unroll
             for (int p = 0; p < DM / 64; ++p)
                 tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.v : &maps.k, 64 * p, kt.key(issued >> 1, 128), h, s.b, bar);
+            if (issued == 1 && maps.rows) {
+                // CTAs start together, and all of them wait for memory then; the rows of the one that follows on this SM come into
+                // L2 while this one computes (512 -> 497 us at 2 x 16384 tokens).
+                const int64_t id = blockIdx.x + gridDim.x * (h + (int64_t)a.Hkv * blockIdx.z) + maps.sms;
+                const int64_t hb = id / gridDim.x;
+                const int hn = (int)(hb % a.Hkv), b = (int)(hb / a.Hkv), Rn = (int)(gridDim.x - 1 - id % gridDim.x) * 128;
+                if (b < a.B && Rn / a.G < dense_seq(a, b).n) {
+#pragma unroll
+                    for (int p = 0; p < DM / 64; ++p) {
+                        tma_prefetch_4d(&maps.q_rows, 64 * p, hn * a.G, Rn / a.G, b);
+                        tma_prefetch_4d(&maps.dy_rows, 64 * p, hn * a.G, Rn / a.G, b);
+                        tma_prefetch_4d(&maps.y_rows, 64 * p, hn * a.G, Rn / a.G, b);
+                        if (a.rest.data) tma_prefetch_4d(&maps.rest_rows, 64 * p, hn * a.G, Rn / a.G, b);
+                    }
+                }
+            }
         }
         if (!ok) {                                             // copies in flight land before the memory goes away
             mbar_wait(smem_u32(&q_full), 0, 1u << 12);
@@ -774,8 +791,10 @@ int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) 
     if ((rc = encode_tokens(&maps.dk, bf16, a.dk, a.D, a.Hkv, a.N, a.B)) || (rc = encode_tokens(&maps.dv, bf16, a.dv, a.D, a.Hkv, a.N, a.B))) return rc;
     maps.rows = rows_fit(a);
     if (maps.rows && ((rc = encode_rows(&maps.q_rows, bf16, a.q, a)) || (rc = encode_rows(&maps.dy_rows, bf16, a.dy, a)) ||
-                      (rc = encode_rows(&maps.dq_rows, bf16, a.dq, a))))
+                      (rc = encode_rows(&maps.dq_rows, bf16, a.dq, a)) || (rc = encode_rows(&maps.y_rows, bf16, a.y, a)) ||
+                      (a.rest.data && (rc = encode_rows(&maps.rest_rows, bf16, a.rest, a)))))
         return rc;
+    maps.sms = sm_count();
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
     maps.dy_peak = parts;
     maps.v_peak = parts + dy_peaks(a);
