@@ -45,8 +45,10 @@ struct BwdMaps {
 // Half precision has too few exponents for the weights of long windows and for dS of scaled losses.  P is at most 1 and goes
 // into its product as 2^8 P.  dS goes in as c dS with c = 2^(7 - floor(log2 max|dy|) - floor(log2 max|v|)): since
 // P_j |v_j - sum P v| <= max|v| / 2, |dS| is at most 128 max|dy| max|v| / 2 for 128 features, and |c dS| < 2^15; and where dP
-// is of the usual size, weights down to 2^-20 still give normal numbers.  Both factors are powers of two and leave with the
-// results.  The peaks cost one pass over v (5 us for 32 MB).  bfloat16 has the exponents of Float32 and needs none of this.
+// is of the usual size, weights down to 2^-20 still give normal numbers.  max|v| is that of every key that the queries see, in
+// dk too: through delta the values of all of them are in dS, whatever the size of the CTA's own.  Both factors are powers of two and
+// leave with the results.  The peaks cost one pass over v (5 us for 32 MB).  bfloat16 has the exponents of Float32 and needs none
+// of this.
 constexpr float kPScale = 256.f, kPLog2 = 8.f;
 __device__ __forceinline__ int exponent(float x) { return x > 0.f && !isinf(x) ? (int)(__float_as_uint(x) >> 23) - 127 : 0; }
 __device__ __forceinline__ float ds_factor(float dy_peak, float v_peak) {
@@ -506,7 +508,13 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         const float* p = maps.dy_peak + ((int64_t)s.b * a.Hkv + h) * tiles;
         float peak = 0.f;
         for (int i = (int)((int64_t)t_lo * a.G / 128) + lane; i <= (int)(((int64_t)t_hi * a.G - 1) / 128); i += 32) peak = fmaxf(peak, p[i]);
-        c = ds_factor(warp_max(peak), maps.v_peak[((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128) + tile]);
+        // keys that the queries t_lo .. t_hi - 1 see: their windows, and first tokens before those
+        const float* pv = maps.v_peak + ((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128);
+        const int from = max(0, t_lo - a.left) / 128, upto = (int)min((int64_t)s.n - 1, (int64_t)t_hi - 1 + a.right) / 128;
+        float v_peak = 0.f;
+        for (int i = lane; i <= upto; i += 32)
+            if (i >= from || i * 128 < a.sinks) v_peak = fmaxf(v_peak, pv[i]);
+        c = ds_factor(warp_max(peak), warp_max(v_peak));
     }
 
     if (warp < kWarps) {
