@@ -121,10 +121,12 @@ __device__ __forceinline__ KeyTiles key_tiles(const SeqArgs& a, const Seq& s, in
     if (p_hi < p_lo) return KeyTiles{0, 0, 0};
     const int limit = key_limit(a, s);
     const int lo = max(0, p_lo - a.left);                                  // left <= 2^30
-    const int hi = (int)min((int64_t)limit, (int64_t)p_hi + a.right + 1);  // > lo where nothing is cut off: it holds p_hi
-    k.lo = min(lo, limit) / keys * keys;
+    const int hi = (int)min((int64_t)limit, (int64_t)p_hi + a.right + 1);  // > lo unless the table ends before the window
+    // A window that begins behind the table has no tile: rounded down to one it would be a tile that no row sees, whose copies nobody
+    // waits for.
+    k.lo = lo < hi ? lo / keys * keys : hi;
     k.first = (min(a.sinks, k.lo) + keys - 1) / keys;
-    k.count = k.first + max(0, hi - k.lo + keys - 1) / keys;
+    k.count = k.first + (lo < hi ? (hi - k.lo + keys - 1) / keys : 0);
     return k;
 }
 

@@ -338,12 +338,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             tma_stores_read();
         }
     } else if (warp == kCopier && lane == 0) {
-        bool ok = true;
         int issued = 0;
         for (; issued < 2 * kt.count; ++issued) {
             const int slot = issued % S;
-            if (issued == S - 1 && !wait_or_stop(smem_u32(&q_moved), 0, stop)) { ok = false; break; }
-            if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
+            if (issued == S - 1 && !wait_or_stop(smem_u32(&q_moved), 0, stop)) break;
+            if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) break;
             const uint32_t bar = smem_u32(&kv_full[slot]), dst = kv_at + slot * TILE;
             mbar_arrive_expect_tx(bar, TILE);
 #pragma unroll
@@ -366,10 +365,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 }
             }
         }
-        if (!ok) {                                             // copies in flight land before the memory goes away
-            mbar_wait(smem_u32(&q_full), 0, 1u << 12);
-            for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
-        }
+        mbar_wait(smem_u32(&q_full), 0, 1u << 12);             // copies in flight land before the memory goes away
+        for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
     } else if (warp == kIssuer && kt.count) {
         const uint32_t lead = elect_one();
         const uint64_t dy_desc = desc_features(base_at), f_desc = desc_features(kv_at), r_desc = desc_rows(kv_at);
@@ -630,12 +627,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             }
         }
     } else if (warp == kCopier && lane == 0 && count) {
-        bool ok = true;
         int issued = 0;
         Steps at(a, t_lo, first);
         for (; issued < 2 * count; ++issued) {
             const int slot = issued % S;
-            if (!wait_or_stop(smem_u32(&q_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
+            if (!wait_or_stop(smem_u32(&q_empty[slot]), ((issued / S) & 1) ^ 1, stop)) break;
             const uint32_t bar = smem_u32(&q_full[slot]), dst = ring_at + slot * TILE;
             mbar_arrive_expect_tx(bar, TILE);
 #pragma unroll
@@ -643,10 +639,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 tma_load_4d(dst + p * kPanel, issued & 1 ? &maps.dy : &maps.q, 64 * p, at.q0, h * a.G + at.g, s.b, bar);
             if (issued & 1) at.next(a);
         }
-        if (!ok) {                                             // copies in flight land before the memory goes away
-            mbar_wait(smem_u32(&kv_full), 0, 1u << 12);
-            for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&q_full[i % S]), (i / S) & 1, 1u << 12);
-        }
+        mbar_wait(smem_u32(&kv_full), 0, 1u << 12);            // copies in flight land before the memory goes away
+        for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&q_full[i % S]), (i / S) & 1, 1u << 12);
     } else if (warp == kIssuer && count) {
         const uint32_t lead = elect_one();
         const uint64_t k_desc = desc_features(base_at), v_desc = desc_features(base_at + TILE), f_desc = desc_features(ring_at), r_desc = desc_rows(ring_at);

@@ -77,11 +77,15 @@ __device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, cons
         return t;
     }
     // the window's tiles begin at kt.lo; those of first tokens lie before it, and beyond it only up to the window
-    const int begin = t.begin_key, end = t.end_key;
-    t.from = kt.first + max(0, begin - kt.lo) / 128;
-    t.upto = end >= kt.lo ? kt.first + (end - kt.lo) / 128 : kt.first - 1;
-    t.first = kt.first;
-    if (a.sinks > kt.lo) t.first = max(t.first, min(min(t.from, t.upto + 1), kt.first + (min(a.sinks, s.n) - kt.lo + 127) / 128));
+    const int known = min(a.sinks, key_limit(a, s)), firsts = kt.first + (known > kt.lo ? (known - kt.lo + 127) / 128 : 0);
+    if (t.end_key < t.begin_key) {          // the table ends before these rows' windows: first tokens only
+        t.first = t.from = firsts;
+        t.upto = firsts - 1;
+        return t;
+    }
+    t.from = kt.first + max(0, t.begin_key - kt.lo) / 128;
+    t.upto = t.end_key >= kt.lo ? kt.first + (t.end_key - kt.lo) / 128 : kt.first - 1;
+    t.first = max(kt.first, min(min(t.from, t.upto + 1), firsts));
     return t;
 }
 
@@ -389,13 +393,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         }
     } else if (warp == 8) {
         // ------------------------------------------------------------ copies
-        bool ok = true;
         int issued = 0;
         if (!PAGED) {
             if (lane == 0) {
                 for (; issued < 2 * kt.count; ++issued) {
                     const int slot = issued % S;
-                    if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) { ok = false; break; }
+                    if (!wait_or_stop(smem_u32(&kv_empty[slot]), ((issued / S) & 1) ^ 1, stop)) break;
                     const uint32_t bar = smem_u32(&kv_full[slot]), dst = kv_at + slot * TILE;
                     mbar_arrive_expect_tx(bar, TILE);
 #pragma unroll
@@ -405,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             }
         } else {
             const int box = maps.box, chunks = 128 / box;
+            bool ok = true;
             for (int i = 0; i < kt.count && ok; ++i) {
                 const int j = kt.key(i, 128) + lane * box;
                 const int page = lane < chunks && j < s.n ? page_of(a, s.b, j) : -1;
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         }
         if (maps.rows && lane == 0)                                        // also where no key tile waits for them
             for (int u = 0; u < (PAIR ? 2 : 1) && R0 + 128 * u < rows; ++u) mbar_wait(smem_u32(&q_full[u]), 0, 1u << 12);
-        if (!ok && lane == 0)                                              // copies in flight land before the memory goes away
+        if (lane == 0)                                                     // copies in flight land before the memory goes away
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
     } else if (warp == 9) {
         // ------------------------------------------------------------ products: the warp in step, one lane issues

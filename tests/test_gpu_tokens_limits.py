@@ -1,12 +1,23 @@
 """Attention on token sequences where sizes and numbers reach the limits of what the kernels' choices assume: values of unequal
-size in half precision."""
+size in half precision, windows behind a cache's table."""
+import random
+
 import pytest
 import torch
 
 from tests import tokens_reference as ref
-from tests.test_gpu_tokens_window import problem, run
+from tests.test_gpu_tokens_paged import ints
+from tests.test_gpu_tokens_window import DTYPES, make, problem, run
 
 pytestmark = pytest.mark.gpu
+
+
+def name_of(dtype):
+    return str(dtype)[6:]
+
+
+def sm_count():
+    return torch.cuda.get_device_properties(0).multi_processor_count
 
 
 @pytest.mark.parametrize("left,sinks", [(None, 0), (150, 4)])
@@ -25,3 +36,34 @@ def test_values_of_unequal_size_in_half_precision(ca, D, ratio, at, left, sinks)
     want = ref.window(q.double(), k.double(), v.double(), left, 0, sinks, None, None, dy.double(), ref.UNIT[torch.float16])
     for name, (x, e) in want.items():
         ref.check(got[name], x, e + 2.0 ** -24, name)       # results below the smallest normal half: multiples of 2^-24
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("left,sinks", [(60, 0), (60, 20), (60, 400), (0, 0), (None, 0)])
+@pytest.mark.parametrize("D,G,S,new", [
+    (64, 2, 4, 1),                  # few rows a key head
+    (64, 4, 4, 150),                # one row tile, two streams over its keys
+    (128, 3, 3, 150),
+    (64, 1, 80, 150),               # two row tiles that share the key tiles
+    (128, 4, 40, 70),
+])
+def test_windows_behind_the_table(ca, D, G, S, new, left, sinks, dtype):
+    """Lengths beyond the places of the table: windows that lie behind it wholly, or those of the last rows only.  Such rows see
+    first tokens or nothing at all, and nothing gives zeros."""
+    page, width, Hkv = 16, 9, 2                                                          # 144 places: not whole tiles of keys
+    lengths = [(1000, 290, 160, 204, 140 + new, 144)[s % 6] for s in range(S)]
+    if S > 4:
+        assert (S * new * G // 256 + S) * Hkv >= sm_count() and new * G > 128
+    order = list(range(S * width))
+    random.Random(1).shuffle(order)
+    table = [order[width * s:width * s + width] for s in range(S)]
+    starts = [new * s for s in range(S + 1)]
+    q = make(9, (D, Hkv * G, S * new), dtype, 1.5)
+    kp, vp = (make(i, (D, page, Hkv, S * width), dtype) for i in (1, 2))
+    args = (q.cuda(), kp.cuda(), vp.cuda(), ints(table).t(), ints(starts), ints(lengths), left)
+    want, bound = ref.paged(q.double(), kp.double(), vp.double(), table, starts, lengths, left, sinks, u=ref.UNIT[dtype])
+    for _ in range(3):
+        y = ca.paged_window_attention(*args, sinks=sinks)
+        ref.check(y, want, bound)
+        assert y[:, :, :new].any() == (sinks > 0 or left is None)                        # the first sequence's length is 1000
+    ca.ops.check_status()
