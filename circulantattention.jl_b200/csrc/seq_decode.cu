@@ -381,10 +381,13 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
     cluster.sync();                                             // nobody leaves while its part is read
 }
 
-// Largest cluster of the kernel that the device schedules (16 where it can, else the portable 8); cached per kernel.
+// Largest cluster of the kernel that the device schedules (16 where it can, else the portable 8).  Cached per kernel and
+// device: a function's attributes are those of the current device.
 template <typename K>
-int largest_cluster(K kernel, size_t smem, std::atomic<int>& cache) {
-    int n = cache.load(std::memory_order_relaxed);
+int largest_cluster(K kernel, size_t smem, std::atomic<int>* cache) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 8;
+    int n = cache[dev].load(std::memory_order_relaxed);
     if (n) return n;
     n = 8;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
@@ -397,13 +400,13 @@ int largest_cluster(K kernel, size_t smem, std::atomic<int>& cache) {
         if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0) n = 16;
     }
     cudaGetLastError();
-    cache.store(n, std::memory_order_relaxed);
+    cache[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
 template <typename T, int DM>
 int launch(const SeqArgs& a, cudaStream_t st) {
-    static std::atomic<int> cluster_cache{0};
+    static std::atomic<int> cluster_cache[64];
     const size_t smem = Decode<T, DM>::kSmem;
     cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");

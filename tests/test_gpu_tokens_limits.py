@@ -1,5 +1,6 @@
 """Attention on token sequences where sizes and numbers reach the limits of what the kernels' choices assume: values of unequal
-size in half precision, windows behind a cache's table."""
+size in half precision, windows behind a cache's table, several devices in
+one process."""
 import random
 
 import pytest
@@ -67,3 +68,18 @@ def test_windows_behind_the_table(ca, D, G, S, new, left, sinks, dtype):
         ref.check(y, want, bound)
         assert y[:, :, :new].any() == (sinks > 0 or left is None)                        # the first sequence's length is 1000
     ca.ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+def test_decoding_on_every_device(ca, dtype):
+    """Few sequences take the largest clusters, which a kernel has to be allowed on each device (two where there are two)."""
+    devices = [f"cuda:{i}" for i in range(min(2, torch.cuda.device_count()))]
+    page, width, S, Hkv = 16, 64, 4, 4
+    table = [list(range(width * s, width * s + width)) for s in range(S)]
+    starts, lengths = list(range(S + 1)), [1024, 900, 17, 333]
+    q = make(9, (128, 16, S), dtype, 1.5)
+    kp, vp = (make(i, (128, page, Hkv, S * width), dtype) for i in (1, 2))
+    want, bound = ref.paged(q.double(), kp.double(), vp.double(), table, starts, lengths, None, 0, u=ref.UNIT[dtype])
+    for device in devices * 2:
+        at = [t.to(device) for t in (q, kp, vp, ints(table).t(), ints(starts), ints(lengths))]
+        ref.check(ca.paged_window_attention(*at), want, bound)
