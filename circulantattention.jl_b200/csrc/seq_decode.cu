@@ -72,8 +72,12 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     int tile = (int)blockIdx.x / ranks;
+    const int2 owned = owned_tokens(a);
     Seq s;
-    if (!paged_seq(a, kRows, tile, &s)) return;                    // alike in the whole cluster
+    if (!paged_seq(a, kRows, tile, &s)) {                          // alike in the whole cluster
+        clear_unowned<T>(a, owned, h, tid, 32 * kWarps);
+        return;
+    }
     const int rows = s.T * a.G, R0 = tile * kRows, nrows = min(kRows, rows - R0);
     const int p_lo = s.base + R0 / a.G, p_hi = s.base + (R0 + nrows - 1) / a.G;
     const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kKeys);
@@ -114,6 +118,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
     auto page = [&](int n) { return __shfl_sync(~0u, n & 32 ? page_next : page_now, n & 31); };      // n is at most 31 behind the first of now
 #pragma unroll
     for (int st = 0; st < L::kStages - 1; ++st) copy_tile(first + warp + kWarps * st, st, page(st));
+    clear_unowned<T>(a, owned, h, tid, 32 * kWarps);
 
     float m[sizeof(T) == 4 ? 8 : 2], l[sizeof(T) == 4 ? 8 : 2];
     constexpr int STATS = sizeof(T) == 4 ? 8 : 2;

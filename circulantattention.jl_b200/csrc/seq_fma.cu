@@ -153,9 +153,14 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
     __shared__ unsigned char gone[2][kTile];
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
     int tile = blockIdx.x;
+    int2 owned;
     Seq s;
     if (a.pages.table) {
-        if (!paged_seq(a, kTile, tile, &s)) return;
+        owned = owned_tokens(a);
+        if (!paged_seq(a, kTile, tile, &s)) {
+            clear_unowned<float>(a, owned, h, tid, kThreads);
+            return;
+        }
     } else {
         s = dense_seq(a, blockIdx.z);
     }
@@ -198,6 +203,7 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
     }
     if (kt.count) prefetch(0);
     copies_commit();
+    if (a.pages.table) clear_unowned<float>(a, owned, h, tid, kThreads);
     for (int it = 0; it < kt.count; ++it) {
         if (it + 1 < kt.count) prefetch(it + 1);
         copies_commit();

@@ -107,9 +107,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
     int tile = (int)(gridDim.x - 1 - blockIdx.x);       // the last rows see the most keys: first
+    int2 owned;
     Seq s;
     if (PAGED) {
-        if (!paged_seq(a, PAIR ? 256 : 128, tile, &s)) return;
+        owned = owned_tokens(a);
+        if (!paged_seq(a, PAIR ? 256 : 128, tile, &s)) {
+            if (tid < 32 * kSoftmaxWarps) clear_unowned<T>(a, owned, h, tid, 32 * kSoftmaxWarps);
+            return;
+        }
     } else {
         s = dense_seq(a, blockIdx.z);
     }
@@ -190,6 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         float m = -INFINITY, l = 0.f;
         int done = 0;
         bool ok = true;
+        if (PAGED) clear_unowned<T>(a, owned, h, tid, 32 * kSoftmaxWarps);
         for (int i = st.begin(); i <= st.upto; i = st.next(i)) {
             const int key0 = kt.key(i, 128), vslot = (2 * i + 1) % S;
             const uint32_t vpar = ((2 * i + 1) / S) & 1;

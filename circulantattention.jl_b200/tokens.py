@@ -61,7 +61,8 @@ def rotary_append_(q, k, v, k_pages, v_pages, table, starts, lengths, positions,
     q, k, v: packed tokens `(D, heads, T)`; tokens `starts[s]` to `starts[s+1] - 1` are the last ones of the `lengths[s]`
     tokens that sequence s has with them.  Token j of the sequence lives at offset `j % page` of page
     `table[j // page, s]` of `k_pages` and `v_pages`, `(D, page, heads, pages)` with pages of a multiple of 16 tokens; where
-    the table has no valid page nothing is stored.  positions: `(axes, T)`.  No gradients."""
+    the table has no valid page nothing is stored.  positions: `(axes, T)`.  Tokens of no sequence, before `starts[0]` and
+    from `starts[S]` on (a call of fixed size that is not full), are turned in q and not stored.  No gradients."""
     return host.rotary_append(q, k, v, k_pages, v_pages, table, starts, lengths, positions, turns, _sections(sections, turns),
                               bool(interleaved))
 

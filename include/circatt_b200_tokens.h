@@ -38,7 +38,9 @@ typedef struct ca_page_view {
 
 /* The sequences of a batch in a paged cache.  Sequence s has the packed tokens starts[s] .. starts[s+1]-1, the last ones
  * of the lengths[s] tokens that its pages hold, and token j lives at offset j % page of page table[j / page + width*s].
- * An entry outside 0 .. pages-1 is a page that is gone: its tokens are not visible and nothing is stored there. */
+ * An entry outside 0 .. pages-1 is a page that is gone: its tokens are not visible and nothing is stored there.  Packed tokens
+ * before starts[0] and from starts[sequences] on belong to no sequence: attention gives zeros for them, and the cache write
+ * leaves them out. */
 typedef struct ca_pages {
     const int32_t* table;     /* (width, sequences) */
     const int32_t* starts;    /* (sequences + 1) */

@@ -1,13 +1,14 @@
 """Attention on token sequences where sizes and numbers reach the limits of what the kernels' choices assume: values of unequal
 size in half precision, windows behind a cache's table, several devices in
-one process."""
+one process, tokens of no sequence."""
+import math
 import random
 
 import pytest
 import torch
 
 from tests import tokens_reference as ref
-from tests.test_gpu_tokens_paged import ints
+from tests.test_gpu_tokens_paged import cache, ints
 from tests.test_gpu_tokens_window import DTYPES, make, problem, run
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +84,21 @@ def test_decoding_on_every_device(ca, dtype):
     for device in devices * 2:
         at = [t.to(device) for t in (q, kp, vp, ints(table).t(), ints(starts), ints(lengths))]
         ref.check(ca.paged_window_attention(*at), want, bound)
+
+
+@pytest.mark.parametrize("new,S", [(1, 2), (150, 2), (150, 80)])
+@pytest.mark.parametrize("D,G", [(64, 1), (64, 3), (128, 4), (24, 2)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+def test_tokens_of_no_sequence(ca, dtype, D, G, new, S):
+    """Packed tokens before the first sequence and behind the last, as in a call of fixed size that is not full: zeros,
+    whatever the result's memory held."""
+    total = max(new, 160)
+    kp, vp, table = cache(D, 2, 16, [(new, total)] * S, dtype, 60, 3)
+    for lead, tail in ((0, 9), (4, 700), (0, 0)):
+        starts, T = [lead + new * s for s in range(S + 1)], lead + new * S + tail
+        q = make(9, (D, 2 * G, T), dtype, 1.5)
+        torch.full((T, 2 * G, D), math.nan, dtype=dtype, device="cuda")        # freed at once: the result's place
+        y = ca.paged_window_attention(q.cuda(), kp.cuda(), vp.cuda(), ints(table).t(), ints(starts), ints([total] * S), 60, sinks=3)
+        want, bound = ref.paged(q.double(), kp.double(), vp.double(), table, starts, [total] * S, 60, 3, u=ref.UNIT[dtype])
+        ref.check(y, want, bound)
+        assert not y[:, :, :lead].any() and not y[:, :, T - tail:].any()
