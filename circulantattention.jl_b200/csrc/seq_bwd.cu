@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             settled32(o);
             float y[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) y[e] = kt.count ? __uint_as_float(o[e]) * f : 0.f * f;
+            for (int e = 0; e < 32; ++e) y[e] = kt.count && live ? __uint_as_float(o[e]) * f : 0.f * f;      // behind the length: zeros, next to infinities too
             put_row32<T>(smem, r, col, y);                         // dy's place: its last products are done
         }
         fence_async_smem();
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             settled32(o);
             float y[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) y[e] = count ? __uint_as_float(o[e]) * f : 0.f * f;
+            for (int e = 0; e < 32; ++e) y[e] = count && j < s.n ? __uint_as_float(o[e]) * f : 0.f * f;
             if (split) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) part[(col + e) * 128] = y[e];

@@ -334,8 +334,10 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
 
     // ------------------------------------------------------------ join: the CTA's warps, then the CTAs; four features a thread
     __syncthreads();
-    auto put = [&](int r, int f, float4 y, float inv) {
+    auto put = [&](int r, int f, float4 y, float sum) {
         if (f >= a.D) return;
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);    // sees nothing: zeros, next to infinities too
         T* dst = seq_row<T>(a.y, a, s, h, R0 + r) + f;
         if constexpr (sizeof(T) == 2)
             *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(y.x * inv, y.y * inv), pack16<T>(y.z * inv, y.w * inv));
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
             add(y, *reinterpret_cast<const float4*>(all + (w * kRows + r) * DM + f), g);
         }
         if (ranks == 1) {
-            put(r, f, y, sum > 0.f ? 1.f / sum : 0.f);
+            put(r, f, y, sum);
         } else {
             *reinterpret_cast<float4*>(all + r * DM + f) = y;
             if (f == 0) { row_m[r] = M; row_l[r] = sum; }
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
             sum = fmaf(*cluster.map_shared_rank(&row_l[r], c), g, sum);
             add(y, *reinterpret_cast<const float4*>(cluster.map_shared_rank(all + r * DM + f, c)), g);
         }
-        put(r, f, y, sum > 0.f ? 1.f / sum : 0.f);
+        put(r, f, y, sum);
     }
     cluster.sync();                                             // nobody leaves while its part is read
 }

@@ -117,6 +117,12 @@ __device__ __forceinline__ float sum16(float x) {
 }
 
 template <int DM>
+__device__ __forceinline__ void clear_row(f32x2 (&o)[DM / 32]) {
+#pragma unroll
+    for (int c = 0; c < DM / 32; ++c) o[c] = 0;
+}
+
+template <int DM>
 __device__ __forceinline__ void store_row(float* dst, const f32x2 (&o)[DM / 32], float f, int D, int tx) {
     const f32x2 f2 = pack2(f, f);
 #pragma unroll
@@ -249,6 +255,7 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
         const int R = R0 + ty + 16 * i;
         const float sum = sum16(l[i]);
         if (R >= rows) continue;
+        if (sum == 0.f) clear_row<DM>(o[i]);                          // sees nothing: zeros, next to infinities too
         store_row<DM>(row_ptr(a.y, a, s, h, R), o[i], sum > 0.f ? 1.f / sum : 0.f, a.D, tx);
         if (a.lse && tx == 0) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = sum > 0.f ? m[i] + log2f(sum) : -INFINITY;
     }
@@ -328,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int R = R0 + ty + 16 * i;
+        if (pos[i] >= s.n) clear_row<DM>(o[i]);
         if (R < rows) store_row<DM>(row_ptr(a.dq, a, s, h, R), o[i], a.scale, a.D, tx);
     }
 }
@@ -415,6 +423,10 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i, j = j0 + r;
+        if (j >= s.n) {
+            clear_row<DM>(dk[i]);
+            clear_row<DM>(dv[i]);
+        }
         if (split) {
             float* p = parts.data + ((((int64_t)s.b * a.Hkv + h) * parts.tiles + tile) * parts.segments + seg) * 2 * kTile * DM + r * DM;
             store_row<DM>(p, dk[i], a.scale, DM, tx);

@@ -348,7 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         if (PAIR || u == 0) {
             float inv = l > 0.f ? 1.f / l : 0.f;
             if (!ok || *stop) inv = __int_as_float(0x7fffffff);            // a wait ran out: NaN, never a wrong number
-            const bool both = !PAIR && kt.count > 1;
+            // Rows that see nothing are zeros by choice, not by their weights: 0 * inf of a value that other rows see is not a number.
+            const bool none = !done || l == 0.f, both = !PAIR && kt.count > 1 && !none;
             if (!PAGED && a.lse && have) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = l > 0.f ? m + log2f(l) : -INFINITY;
             const float w0 = f0 * inv, w1 = f1 * inv;
             // y goes to the queries' place (their last scores are done), what rounding took to a slot of the ring
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 float y[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * w0;
-                if (!done) {
+                if (none) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) y[e] = 0.f * inv;
                 }

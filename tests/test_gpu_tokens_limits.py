@@ -1,6 +1,6 @@
 """Attention on token sequences where sizes and numbers reach the limits of what the kernels' choices assume: values of unequal
 size in half precision, windows behind a cache's table, several devices in
-one process, tokens of no sequence."""
+one process, tokens of no sequence, infinities next to rows that see nothing."""
 import math
 import random
 
@@ -102,3 +102,29 @@ def test_tokens_of_no_sequence(ca, dtype, D, G, new, S):
         want, bound = ref.paged(q.double(), kp.double(), vp.double(), table, starts, [total] * S, 60, 3, u=ref.UNIT[dtype])
         ref.check(y, want, bound)
         assert not y[:, :, :lead].any() and not y[:, :, T - tail:].any()
+
+
+@pytest.mark.parametrize("junk", [math.inf, math.nan])
+@pytest.mark.parametrize("which", range(4), ids=("q", "k", "v", "dy"))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+def test_zeros_behind_the_length_next_to_infinity(ca, dtype, D, which, junk):
+    """The last token of a sequence is not finite, and the places behind it share its tiles: they are zeros all the same, and
+    the other sequence is not touched."""
+    x = list(problem(D, 4, 2, 300, 2, dtype))
+    x[which][:, :, 130, 0] = junk
+    for left, sinks in ((50, 3), (None, 0)):
+        for name, t in run(ca, *x, left, 0, sinks, [131, 300]).items():
+            assert not t[:, :, 131:, 0].any(), name
+            assert torch.isfinite(t[..., 1]).all(), name
+
+
+@pytest.mark.parametrize("new", [5, 150])
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+def test_zeros_of_rows_that_see_nothing_next_to_infinity(ca, dtype, new):
+    """More tokens are new than the cache is said to hold: the first two see nothing, the others see values that are infinite."""
+    kp, vp, table = cache(64, 2, 16, [(new - 2, new - 2)], dtype, None, 0, junk=0.5)
+    vp[..., table[0][0]] = math.inf
+    q = make(9, (64, 4, new), dtype, 1.5)
+    y = ca.paged_window_attention(q.cuda(), kp.cuda(), vp.cuda(), ints(table).t(), ints([0, new]), ints([new - 2]))
+    assert not y[:, :, :2].any() and not torch.isfinite(y[:, :, 2:]).any()
