@@ -229,10 +229,10 @@ int ca_rotary(const ca_rotary_desc* d, const ca_seq_view* x1, const ca_seq_view*
     int rc = fill(d, &a);
     if (rc) return rc;
     if (heads1 < 1 || (x2 && heads2 < 1)) { set_error("heads must be positive"); return CA_ERR_BAD_DESC; }
-    if ((rc = check_view(x1, d->dtype, "x1")) || (rc = check_view(y1, d->dtype, "y1"))) return rc;
+    if ((rc = check_view(x1, d->dtype, "x1", a.tokens > 0)) || (rc = check_view(y1, d->dtype, "y1", a.tokens > 0))) return rc;
     a.t[a.nt++] = tensor(x1, y1, heads1, 1);
     if (x2) {
-        if ((rc = check_view(x2, d->dtype, "x2")) || (rc = check_view(y2, d->dtype, "y2"))) return rc;
+        if ((rc = check_view(x2, d->dtype, "x2", a.tokens > 0)) || (rc = check_view(y2, d->dtype, "y2", a.tokens > 0))) return rc;
         a.t[a.nt++] = tensor(x2, y2, heads2, 1);
     }
     return run(a, d->dtype, d->interleaved, as_stream(stream));
@@ -247,9 +247,9 @@ int ca_rotary_append(const ca_rotary_desc* d, const ca_seq_view* q, const ca_seq
     if (d->batch != 1) { set_error("packed tokens have batch 1 (got %d)", d->batch); return CA_ERR_BAD_DESC; }
     if (heads_q < 1 || heads_kv < 1) { set_error("heads must be positive"); return CA_ERR_BAD_DESC; }
     if ((rc = check_pages(pages, d->tokens))) return rc;
-    if ((rc = check_view(q, d->dtype, "q")) || (rc = check_view(q_out, d->dtype, "q_out")) || (rc = check_view(k, d->dtype, "k")) ||
-        (rc = check_view(v, d->dtype, "v")) || (rc = check_page_view(k_pages, d->dtype, "k_pages")) ||
-        (rc = check_page_view(v_pages, d->dtype, "v_pages")))
+    if ((rc = check_view(q, d->dtype, "q", a.tokens > 0)) || (rc = check_view(q_out, d->dtype, "q_out", a.tokens > 0)) || (rc = check_view(k, d->dtype, "k", a.tokens > 0)) ||
+        (rc = check_view(v, d->dtype, "v", a.tokens > 0)) || (rc = check_page_view(k_pages, d->dtype, "k_pages", a.tokens > 0 && pages->pages)) ||
+        (rc = check_page_view(v_pages, d->dtype, "v_pages", a.tokens > 0 && pages->pages)))
         return rc;
     a.t[0] = tensor(q, q_out, heads_q, 1);
     a.t[1] = tensor(k, nullptr, heads_kv, 1);

@@ -18,8 +18,8 @@ template <> __device__ __forceinline__ __half from_float<__half>(float x) { retu
 
 // ---------------------------------------------------------------- checks (seq_api.cu)
 int check_seq_dtype(int dtype);
-int check_view(const ca_seq_view* v, int dtype, const char* name);
-int check_page_view(const ca_page_view* v, int dtype, const char* name);
+int check_view(const ca_seq_view* v, int dtype, const char* name, bool used);         // used: something is read or written there
+int check_page_view(const ca_page_view* v, int dtype, const char* name, bool used);
 int check_pages(const ca_pages* p, int tokens);
 
 // ---------------------------------------------------------------- attention

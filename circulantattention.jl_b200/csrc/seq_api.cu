@@ -9,8 +9,9 @@ int check_seq_dtype(int dtype) {
     return CA_ERR_BAD_DESC;
 }
 
-static int check_strided(const void* p, const int64_t* strides, int dtype, const char* name) {
+static int check_strided(const void* p, const int64_t* strides, int dtype, const char* name, bool used) {
     const int64_t e = dtype == CA_F32 ? 4 : 2;
+    if (used && !p) { set_error("%s has no data (NULL)", name); return CA_ERR_NULL; }
     if (reinterpret_cast<uintptr_t>(p) % 16) { set_error("%s is not 16-byte aligned", name); return CA_ERR_BAD_DESC; }
     for (int i = 0; i < 3; ++i)
         if (strides[i] < 0 || strides[i] * e % 16 || strides[i] > (1LL << 40) / e - 1) {
@@ -20,16 +21,16 @@ static int check_strided(const void* p, const int64_t* strides, int dtype, const
     return CA_OK;
 }
 
-int check_view(const ca_seq_view* v, int dtype, const char* name) {
+int check_view(const ca_seq_view* v, int dtype, const char* name, bool used) {
     if (!v) { set_error("%s is NULL", name); return CA_ERR_NULL; }
     const int64_t s[3] = {v->head, v->token, v->batch};
-    return check_strided(v->data, s, dtype, name);
+    return check_strided(v->data, s, dtype, name, used);
 }
 
-int check_page_view(const ca_page_view* v, int dtype, const char* name) {
+int check_page_view(const ca_page_view* v, int dtype, const char* name, bool used) {
     if (!v) { set_error("%s is NULL", name); return CA_ERR_NULL; }
     const int64_t s[3] = {v->token, v->head, v->page};
-    return check_strided(v->data, s, dtype, name);
+    return check_strided(v->data, s, dtype, name, used);
 }
 
 int check_pages(const ca_pages* p, int tokens) {
@@ -89,10 +90,11 @@ int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     SeqArgs a{};
     int rc = fill(d, &a);
     if (rc) return rc;
-    if ((rc = check_view(q, d->dtype, "q")) || (rc = check_view(k, d->dtype, "k")) || (rc = check_view(v, d->dtype, "v")) ||
-        (rc = check_view(y, d->dtype, "y")) || (y_rest && (rc = check_view(y_rest, d->dtype, "y_rest"))))
+    const bool some = a.N && a.B;
+    if ((rc = check_view(q, d->dtype, "q", some)) || (rc = check_view(k, d->dtype, "k", some)) || (rc = check_view(v, d->dtype, "v", some)) ||
+        (rc = check_view(y, d->dtype, "y", some)) || (y_rest && (rc = check_view(y_rest, d->dtype, "y_rest", false))))
         return rc;
-    if (!a.N || !a.B) return CA_OK;
+    if (!some) return CA_OK;
     a.q = *q; a.k = *k; a.v = *v; a.y = *y;
     if (y_rest) a.rest = *y_rest;
     a.lengths = lengths;
@@ -112,12 +114,14 @@ int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     SeqArgs a{};
     int rc = fill(d, &a);
     if (rc) return rc;
-    if ((rc = check_view(q, d->dtype, "q")) || (rc = check_view(k, d->dtype, "k")) || (rc = check_view(v, d->dtype, "v")) ||
-        (rc = check_view(y, d->dtype, "y")) || (rc = check_view(dy, d->dtype, "dy")) || (rc = check_view(dq, d->dtype, "dq")) ||
-        (rc = check_view(dk, d->dtype, "dk")) || (rc = check_view(dv, d->dtype, "dv")) || (y_rest && (rc = check_view(y_rest, d->dtype, "y_rest"))))
+    const bool some = a.N && a.B;
+    if ((rc = check_view(q, d->dtype, "q", some)) || (rc = check_view(k, d->dtype, "k", some)) || (rc = check_view(v, d->dtype, "v", some)) ||
+        (rc = check_view(y, d->dtype, "y", some)) || (rc = check_view(dy, d->dtype, "dy", some)) || (rc = check_view(dq, d->dtype, "dq", some)) ||
+        (rc = check_view(dk, d->dtype, "dk", some)) || (rc = check_view(dv, d->dtype, "dv", some)) || (y_rest && (rc = check_view(y_rest, d->dtype, "y_rest", false))))
         return rc;
-    if (!a.N || !a.B) return CA_OK;
+    if (!some) return CA_OK;
     if (!lse || !workspace) { set_error("lse and workspace must not be NULL"); return CA_ERR_NULL; }
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) { set_error("workspace is not 16-byte aligned"); return CA_ERR_BAD_DESC; }
     a.q = *q; a.k = *k; a.v = *v; a.y = *y; a.dy = *dy; a.dq = *dq; a.dk = *dk; a.dv = *dv;
     if (y_rest) a.rest = *y_rest;
     a.lengths = lengths;
@@ -132,12 +136,13 @@ int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_vi
     SeqArgs a{};
     int rc = fill(d, &a);
     if (rc) return rc;
+    const bool some = a.N && a.B;
     if (d->batch != 1) { set_error("packed tokens have batch 1 (got %d)", d->batch); return CA_ERR_BAD_DESC; }
     if (d->right) { set_error("right=%d: a cache holds no later tokens", d->right); return CA_ERR_BAD_DESC; }
-    if ((rc = check_pages(pages, d->tokens)) || (rc = check_view(q, d->dtype, "q")) || (rc = check_view(y, d->dtype, "y")) ||
-        (rc = check_page_view(k_pages, d->dtype, "k_pages")) || (rc = check_page_view(v_pages, d->dtype, "v_pages")))
+    if ((rc = check_pages(pages, d->tokens)) || (rc = check_view(q, d->dtype, "q", some)) || (rc = check_view(y, d->dtype, "y", some)) ||
+        (rc = check_page_view(k_pages, d->dtype, "k_pages", some && pages->pages)) || (rc = check_page_view(v_pages, d->dtype, "v_pages", some && pages->pages)))
         return rc;
-    if (!a.N) return CA_OK;
+    if (!some) return CA_OK;
     a.q = *q; a.y = *y;
     a.kp = *k_pages; a.vp = *v_pages;
     a.pages = *pages;

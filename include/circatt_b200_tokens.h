@@ -93,7 +93,7 @@ typedef struct ca_seq_desc {
 int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
                   const int32_t* lengths, const ca_seq_view* y, const ca_seq_view* y_rest, float* lse, void* stream);
 
-/* Gradients of the above for the cotangent dy.  Deterministic: no atomics. */
+/* Gradients of the above for the cotangent dy.  Deterministic: no atomics.  The workspace is 16-byte aligned. */
 size_t ca_window_bwd_workspace(const ca_seq_desc* d);
 int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
                   const ca_seq_view* y, const ca_seq_view* y_rest, const ca_seq_view* dy, const int32_t* lengths, const float* lse,

@@ -106,3 +106,33 @@ def test_bad_views_and_pages(ca):
     assert rotary(axes=2, sections=(33, -1)) == -1 and "negative" in err()
     assert rotary(positions=None) == -3
     assert rotary(tokens=0) == 0
+
+
+def test_views_without_data(ca):
+    """A view of a call that has something to do holds an address: NULL is refused, not read."""
+    from circatt_b200._lib import ca_page_view, ca_pages, ca_rotary_desc
+    lib, err = ca.lib, lambda: ca.lib.ca_last_error().decode()
+    d, one, good, none = _seq(ca), _seq(ca, batch=1), _views(ca, 9), _views(ca, 1, data=None)[0]
+    for i, name in enumerate(("q", "k", "v", "y")):
+        x = [none if j == i else good[j] for j in range(4)]
+        assert lib.ca_window_fwd(d, *x[:3], None, x[3], None, None, None) == -3 and err().startswith(f"{name} has no data")
+    assert lib.ca_window_fwd(_seq(ca, tokens=0), none, none, none, None, none, None, None, None) == 0
+    for i, name in enumerate(("q", "k", "v", "y", None, "dy", "dq", "dk", "dv")):
+        x = [none if j == i else good[j] for j in range(9)]
+        if name:
+            assert lib.ca_window_bwd(d, *x[:6], None, 256, *x[6:], 256, None) == -3 and err().startswith(f"{name} has no data")
+    assert lib.ca_window_bwd(d, *good[:6], None, 256, *good[6:], 260, None) == -1 and "workspace is not 16-byte" in err()
+    pool, gone = (ca_page_view(data=p, token=64, head=1024, page=2048) for p in (256, None))
+    pages = ca_pages(table=256, starts=256, lengths=256, width=4, page=16, pages=9, sequences=2)
+    for i, name in enumerate(("q", "k_pages", "v_pages", "y")):
+        x = [good[0], pool, pool, good[1]]
+        x[i] = gone if "pages" in name else none
+        assert lib.ca_paged_window(one, *x[:3], pages, x[3], None) == -3 and err().startswith(f"{name} has no data")
+    r = ca_rotary_desc(dtype=2, dim=64, pairs=32, axes=1, tokens=5, batch=1, positions=256, turns=256, sections=(C.c_int32 * 4)(32))
+    for i, name in enumerate(("x1", "y1", "x2", "y2")):
+        x = [none if j == i else good[j] for j in range(4)]
+        assert lib.ca_rotary(r, *x[:2], 4, *x[2:], 2, None) == -3 and err().startswith(f"{name} has no data")
+    for i, name in enumerate(("q", "q_out", "k", "v", "k_pages", "v_pages")):
+        x = [*good[:4], pool, pool]
+        x[i] = gone if "pages" in name else none
+        assert lib.ca_rotary_append(r, *x[:2], 4, *x[2:4], 2, *x[4:], pages, None) == -3 and err().startswith(f"{name} has no data")
