@@ -164,6 +164,24 @@ __device__ __forceinline__ int page_of(const SeqArgs& a, int b, int j) {
     return p < a.pages.pages ? p : -1;
 }
 
+// How the backward deals out the queries of key tiles that hold first tokens: those tiles have every later query, an ordinary one
+// those of its window.
+struct Dealt {
+    int tiles, segments;            // the first key tiles, and the CTAs for each
+};
+static inline Dealt deal_first_tokens(const SeqArgs& a, int tile) {
+    // Pieces of about an ordinary tile's work, as long as they are few: each leaves a Float32 part of dk and dv (128 KB at 128
+    // features).  Seven CTAs for every SM even out the work; many first tokens, heads or sequences fill the chip without.  2 x 8192
+    // tokens, 8 heads of 64 features, window 256, 4096 first tokens, dk and dv: 334 us with 2 pieces, 754 with 22 (640 MB more).
+    constexpr int64_t kMost = 64, kParts = 1024;
+    const int64_t all = ((int64_t)a.N + tile - 1) / tile, window = ((int64_t)a.left + a.right + 2 * tile - 1) / tile;
+    const int64_t tiles = ((int64_t)(a.sinks < a.N ? a.sinks : a.N) + tile - 1) / tile;
+    int64_t segments = (all + window - 1) / window;
+    if (segments > kMost) segments = kMost;
+    if (tiles && segments > kParts / (tiles * a.Hkv * a.B)) segments = kParts / (tiles * a.Hkv * a.B);
+    return tiles && segments > 1 ? Dealt{(int)tiles, (int)segments} : Dealt{0, 1};
+}
+
 // seq_fma.cu: Float32 on the FMA pipe
 int fma_fwd(const SeqArgs& a, cudaStream_t st);               // dense or paged
 size_t fma_bwd_parts(const SeqArgs& a);

@@ -17,7 +17,6 @@
 #include "seq_umma.cuh"
 
 #include <limits.h>
-#include <algorithm>
 
 namespace ca {
 namespace {
@@ -740,14 +739,6 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ SeqAr
     *reinterpret_cast<uint4*>(dst) = make_uint4(pack16<T>(sum[0], sum[1]), pack16<T>(sum[2], sum[3]), pack16<T>(sum[4], sum[5]), pack16<T>(sum[6], sum[7]));
 }
 
-// Key tiles of first tokens have every later query; they are dealt out in pieces of about an ordinary tile's work.
-void split_rule(const SeqArgs& a, int* tiles, int* segments) {
-    const int64_t all = (a.N + 127) / 128, window = ((int64_t)a.left + a.right + 255) / 128;
-    *tiles = (int)((std::min(a.sinks, a.N) + 127) / 128);
-    *segments = (int)std::min<int64_t>(64, (all + window - 1) / window);
-    if (*segments < 2 || *tiles == 0) { *tiles = 0; *segments = 1; }
-}
-
 template <typename T, int DM>
 int launch(const SeqArgs& a, const BwdMaps& maps, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(umma_dq_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
@@ -778,9 +769,8 @@ static size_t peak_floats(const SeqArgs& a) { return (dy_peaks(a) + ((size_t)a.N
 
 // Behind the rows' delta: the peaks of dy, and the Float32 parts of the dealt key tiles.
 size_t umma_bwd_parts(const SeqArgs& a) {
-    int tiles, segments;
-    split_rule(a, &tiles, &segments);
-    return (peak_floats(a) + (size_t)tiles * segments * 2 * (a.D > 64 ? 128 : 64) * 128 * a.Hkv * a.B) * sizeof(float);
+    const Dealt p = deal_first_tokens(a, 128);
+    return (peak_floats(a) + (size_t)p.tiles * p.segments * 2 * (a.D > 64 ? 128 : 64) * 128 * a.Hkv * a.B) * sizeof(float);
 }
 
 int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) {
@@ -801,7 +791,9 @@ int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) 
     maps.dy_peak = parts;
     maps.v_peak = parts + dy_peaks(a);
     maps.partial = parts + peak_floats(a);
-    split_rule(a, &maps.split_tiles, &maps.segments);
+    const Dealt p = deal_first_tokens(a, 128);
+    maps.split_tiles = p.tiles;
+    maps.segments = p.segments;
     const bool wide = a.D > 64;
     if (bf16) return wide ? launch<__nv_bfloat16, 128>(a, maps, st) : launch<__nv_bfloat16, 64>(a, maps, st);
     return wide ? launch<__half, 128>(a, maps, st) : launch<__half, 64>(a, maps, st);

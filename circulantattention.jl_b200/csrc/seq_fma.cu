@@ -13,8 +13,6 @@
 // Bound: shared memory.  A 4 x 4 piece of products takes one 16-byte read for four packed FMA, and reads keep that unit 70 to 75 %
 // busy; larger pieces do not fit the registers next to the accumulators.  2 x 4096 tokens, 8 heads of 64 features,
 // window 256: forward 206 us, dq 275, dk and dv 355.
-#include <algorithm>
-
 #include "seq.cuh"
 #include "umma.cuh"
 
@@ -455,14 +453,6 @@ __global__ void __launch_bounds__(256) fma_join_kernel(const __grid_constant__ S
     }
 }
 
-// Key tiles of first tokens have every later row; they are dealt out in pieces of about an ordinary tile's work.
-Parts split_rule(const SeqArgs& a, float* data) {
-    const int64_t all = (a.N + kTile - 1) / kTile, window = ((int64_t)a.left + a.right + 2 * kTile - 1) / kTile;
-    Parts p{data, (int)((std::min(a.sinks, a.N) + kTile - 1) / kTile), (int)std::min<int64_t>(64, (all + window - 1) / window)};
-    if (p.segments < 2 || p.tiles == 0) { p.tiles = 0; p.segments = 1; }
-    return p;
-}
-
 template <typename K>
 int raise_smem(K kernel, size_t bytes) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
@@ -483,7 +473,8 @@ template <int DM>
 int launch_bwd(const SeqArgs& a, float* data, cudaStream_t st) {
     int rc = raise_smem(fma_dq_kernel<DM>, kDqSmem<DM>);
     if (rc || (rc = raise_smem(fma_dkdv_kernel<DM>, kDkdvSmem<DM>))) return rc;
-    const Parts parts = split_rule(a, data);
+    const Dealt p = deal_first_tokens(a, kTile);
+    const Parts parts{data, p.tiles, p.segments};
     fma_dq_kernel<DM><<<dim3((unsigned)(((int64_t)a.N * a.G + kTile - 1) / kTile), a.Hkv, a.B), kThreads, kDqSmem<DM>, st>>>(a);
     CA_CHECK_LAUNCH("window dq kernel");
     const int tiles = (a.N + kTile - 1) / kTile;
@@ -499,7 +490,7 @@ int launch_bwd(const SeqArgs& a, float* data, cudaStream_t st) {
 }  // namespace
 
 size_t fma_bwd_parts(const SeqArgs& a) {
-    const Parts p = split_rule(a, nullptr);
+    const Dealt p = deal_first_tokens(a, kTile);
     return (size_t)p.tiles * p.segments * 2 * kTile * (a.D > 64 ? 128 : 64) * a.Hkv * a.B * sizeof(float);
 }
 

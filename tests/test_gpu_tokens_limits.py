@@ -1,6 +1,7 @@
 """Attention on token sequences where sizes and numbers reach the limits of what the kernels' choices assume: values of unequal
 size in half precision, windows behind a cache's table, several devices in
-one process, tokens of no sequence, infinities next to rows that see nothing."""
+one process, tokens of no sequence, infinities next to rows that see nothing,
+many first tokens."""
 import math
 import random
 
@@ -9,7 +10,7 @@ import torch
 
 from tests import tokens_reference as ref
 from tests.test_gpu_tokens_paged import cache, ints
-from tests.test_gpu_tokens_window import DTYPES, make, problem, run
+from tests.test_gpu_tokens_window import DTYPES, compare, make, problem, run
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +129,16 @@ def test_zeros_of_rows_that_see_nothing_next_to_infinity(ca, dtype, new):
     q = make(9, (64, 4, new), dtype, 1.5)
     y = ca.paged_window_attention(q.cuda(), kp.cuda(), vp.cuda(), ints(table).t(), ints([0, new]), ints([new - 2]))
     assert not y[:, :, :2].any() and not torch.isfinite(y[:, :, 2:]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("D,Hq,Hkv,N,B,left,sinks,lengths", [
+    (64, 2, 1, 4000, 1, 31, 4, None),                # one tile's queries, dealt to many CTAs
+    (128, 2, 1, 4000, 1, 31, 130, [3001]),
+    (64, 8, 8, 1000, 10, 20, 300, None),             # some tiles, to fewer
+    (64, 16, 16, 600, 9, 20, 590, None),             # all tiles: each has its CTA
+])
+def test_many_first_tokens(ca, D, Hq, Hkv, N, B, left, sinks, lengths, dtype):
+    q, k, v, dy = problem(D, Hq, Hkv, N, B, dtype)
+    got = run(ca, q, k, v, dy, left, 0, sinks, lengths)
+    compare(got, q, k, v, dy, left, 0, sinks, lengths)

@@ -136,3 +136,15 @@ def test_views_without_data(ca):
         x = [*good[:4], pool, pool]
         x[i] = gone if "pages" in name else none
         assert lib.ca_rotary_append(r, *x[:2], 4, *x[2:4], 2, *x[4:], pages, None) == -3 and err().startswith(f"{name} has no data")
+
+
+@pytest.mark.parametrize("dtype", [0, 2, 3])
+@pytest.mark.parametrize("tokens,sinks,left,heads,batch", [(32768, 32768, 127, 8, 2), (32768, 4, 127, 64, 64), (1 << 20, 1 << 19, 255, 1, 1), (1000, 2 ** 31 - 1, 0, 2, 3)])
+def test_scratch_memory_of_first_tokens_is_bounded(ca, dtype, tokens, sinks, left, heads, batch):
+    """The backward's parts of key tiles with first tokens: at most 1024 of them, 128 keys and 128 features of dk and dv in
+    Float32 each; apart from those a few numbers for every row."""
+    d = _seq(ca, dtype=dtype, dim=128, heads_q=heads, heads_kv=heads, tokens=tokens, batch=batch, sinks=sinks, left=left)
+    rows = tokens * heads * batch
+    assert 4 * rows <= ca.lib.ca_window_bwd_workspace(d) <= 4 * rows + rows // 4 + 4096 + 1024 * 2 * 128 * 128 * 4
+    few = _seq(ca, dtype=dtype, dim=128, heads_q=2, heads_kv=2, tokens=16384, batch=1, sinks=4, left=1023)
+    assert ca.lib.ca_window_bwd_workspace(few) > 4 * 2 * 16384 + 2 * 8 * 64 * 128 * 4       # these are dealt out
