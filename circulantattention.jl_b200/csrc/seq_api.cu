@@ -147,7 +147,8 @@ int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_vi
     a.kp = *k_pages; a.vp = *v_pages;
     a.pages = *pages;
     // Few rows a key head, on average: the keys are what counts.  More than one tile of 16 rows reads them again, from L2; beyond
-    // four the tiles of 128 (64) rows win.
+    // four the tiles of 128 (64) rows win.  That is so for sequences alike: a mixed call goes one way as a whole and pays for it (63
+    // single tokens 98 us, a chunk of 900 93 us, both in one call 385; with a chunk of 1000, by the other kernel, 275).
     if ((int64_t)a.N * a.G <= 64LL * a.pages.sequences || !a.pages.pages) return decode_paged(a, d->dtype, as_stream(stream));
     return d->dtype == CA_F32 ? fma_fwd(a, as_stream(stream)) : umma_paged(a, d->dtype, as_stream(stream));
 }

@@ -12,8 +12,8 @@
 // Bound: the products at 128 features, 1536 cycles a tile (dq) and 2048 (dk, dv); measured 2100 and 2800, the rest is the
 // chain scores - weights - dS - product of one tile, of which neither tensor memory (all 512 columns are taken) nor shared memory
 // holds a second.  Short windows are bound by what stands before the first tile (queries, results and their remainders
-// from memory: 9000 cycles).  2 x 16384 tokens, window 1024, 16 query and 4 key heads: 497 and 540 us; 3 x 5001 tokens, 8 heads of
-// 64 features, window 127, half: 59 and 58 us.
+// from memory: 9000 cycles).  2 x 16384 tokens, window 1024, 16 query and 4 key heads: 502 and 543 us; 3 x 5001 tokens, 8 heads of
+// 64 features, window 127, half: 59 and 60 us.
 #include "seq_umma.cuh"
 
 #include <limits.h>

@@ -1,8 +1,7 @@
 // Attention on token sequences in Float32, on the FMA pipe: dense tensors and a paged cache.
 //
-// The tensor cores round Float32 operands; pairs of rounded numbers would bring the products back, but their sums are cut
-// rather than rounded, which shows at the 1e-6 that Float32 users get here.  So every product is an FMA, two at a time
-// (fma.rn.f32x2).
+// The tensor cores round Float32 operands, so every product is an FMA here, two at a time (fma.rn.f32x2).  Pairs of halves with
+// short sums, as the circulant sweeps use them (split.cuh: errors of 2e-7 to 4e-7), are not built for these kernels.
 //
 // Tiles of 64 rows and 64 columns in shared memory, features fastest and rows padded by 4 floats, so that the 16-byte
 // reads of eight lanes (rows 1 apart) fall into different banks.  A thread (ty, tx) of 16 x 16 holds the products of rows
@@ -10,9 +9,9 @@
 // while this one is worked on (forward), or another block works (backward: two blocks on an SM with one stage each beat one
 // with two, 274 us against 311 for dq).
 //
-// Bound: shared memory.  A 4 x 4 piece of products takes one 16-byte read for four packed FMA, and reads keep that unit 70 to 75 %
-// busy; larger pieces do not fit the registers next to the accumulators.  2 x 4096 tokens, 8 heads of 64 features,
-// window 256: forward 206 us, dq 275, dk and dv 355.
+// Bound: shared memory.  A 4 x 4 piece of products takes one 16-byte read for four packed FMA, and reads keep that unit 75 to 83 %
+// busy; larger pieces do not fit 128 registers (two blocks an SM) next to the accumulators.  2 x 4096 tokens, 8 heads of 64
+// features, window 256: forward 206 us, dq 275, dk and dv 354.  12 chunks of up to 900 tokens over a cache (128 features): 3570 us.
 #include "seq.cuh"
 #include "umma.cuh"
 

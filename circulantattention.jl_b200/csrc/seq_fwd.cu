@@ -12,12 +12,12 @@
 //
 // The accumulator is rescaled only where a row's maximum grew by more than 2^8 since its reference: the weights stay below
 // 2^8, and the products and sums are held in Float32.  Weights are rounded to the tensors' type before their product, once more
-// than the result itself: errors are 1.4 of a plain implementation that keeps them in Float32.
+// than the result itself: errors are 1.15 to 1.6 of those of a plain implementation that keeps them in Float32.
 //
 // Bound: the exponentials and the products, 2048 cycles each for a pair of 128 x 128 tiles at 128 features; a pair takes about
 // 3300 in the steady state, since a row's chain (scores, maximum, exponentials, weights) leaves gaps that two streams do not
-// fill.  Measured: 65536 tokens, window 4096, 16 query and 2 key heads 2.1 ms (0.86 PFLOP/s of visible pairs, 0.63 of what a
-// large matrix product keeps up); 2 x 16384 tokens, window 1024, 16 and 4 heads 415 us.
+// fill.  Measured: 65536 tokens, window 4096, 16 query and 2 key heads 2.03 ms (1.05 PFLOP/s of visible pairs; a
+// large matrix product has 1.62 in a burst and keeps up 1.37; 1.99 to 2.14 ms by box, at the power cap); 2 x 16384 tokens, window 1024, 16 and 4 heads 415 us.
 #include "seq_umma.cuh"
 
 #include <limits.h>

@@ -9,10 +9,11 @@ positions (a window alone does not know where a token is), and a cache:
 * `rotary_append_` and `paged_window_attention` are the same two for serving: a chunk of new tokens per sequence (one when
   decoding), whose keys and values live in a paged cache.
 
-Tensors are Julia-shaped like those of the rest of the package, features first: `(D, heads, N, B)`, packed tokens of several
-sequences `(D, heads, T)`, a cache `(D, page, heads, pages)`.  Column-major storage is what `jl` makes; any other strides are
-taken as they are when the features are contiguous and the rest is 16-byte aligned, else the tensor is copied.  Float32,
-BFloat16 and Float16; q may have a multiple of the heads of k and v.  Everything runs on torch's current stream."""
+Tensors are Julia-shaped like those of the rest of the package, but features come first, not the image: `(D, heads, N, B)`,
+packed tokens of several sequences `(D, heads, T)`, a cache `(D, page, heads, pages)`; a tensor of the circulant operators has
+to be transposed.  Column-major storage is what `jl` makes; any other strides are taken as they are when the features are
+contiguous and the rest is 16-byte aligned, else the tensor is copied.  Float32, BFloat16 and Float16; q may have a multiple of
+the heads of k and v.  Everything runs on torch's current stream."""
 from __future__ import annotations
 
 import math
