@@ -18,4 +18,6 @@ from .api import (  # noqa: F401
     circulant_transposed_attention_, dot, entmax15, kernel_length, otimes, scale, softmax, softmax_,
     spatial_dims, spatial_size, splitheads, sum,
 )
-from .tokens import paged_window_attention, rotary, rotary_append_, rotary_turns, window_attention  # noqa: F401
+from .tokens import (  # noqa: F401
+    paged_window_attention, rotary, rotary_append_, rotary_turns, token_spans, window_attention,
+)

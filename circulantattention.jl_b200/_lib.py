@@ -69,6 +69,10 @@ class ca_seq_desc(C.Structure):
                 ("sinks", C.c_int32), ("scale", C.c_float)]
 
 
+class ca_seq_form(C.Structure):
+    _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p), ("spans", C.c_void_p), ("prefix", C.c_void_p)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -83,6 +87,7 @@ _p = C.c_void_p
 _D = C.POINTER(ca_desc)
 _V, _G = C.POINTER(ca_seq_view), C.POINTER(ca_page_view)
 _R, _S, _P = C.POINTER(ca_rotary_desc), C.POINTER(ca_seq_desc), C.POINTER(ca_pages)
+_F = C.POINTER(ca_seq_form)
 _i32, _i64, _f32 = C.c_int32, C.c_int64, C.c_float
 
 PROTOTYPES = {
@@ -125,6 +130,10 @@ PROTOTYPES = {
     "ca_window_bwd_workspace": (C.c_size_t, [_S]),
     "ca_window_bwd": (C.c_int, [_S] + [_V] * 6 + [_p, _p] + [_V] * 3 + [_p, _p]),
     "ca_paged_window": (C.c_int, [_S, _V, _G, _G, _P, _V, _p]),
+    "ca_token_spans": (C.c_int, [_p, _p, _i32, _i32, _p, _p]),
+    "ca_window_form_fwd": (C.c_int, [_S, _F, _V, _V, _V, _p, _V, _V, _p, _p]),
+    "ca_window_form_bwd": (C.c_int, [_S, _F] + [_V] * 6 + [_p, _p] + [_V] * 3 + [_p, _p]),
+    "ca_paged_window_form": (C.c_int, [_S, _F, _V, _G, _G, _P, _V, _p]),
     "ca_probe_launch_count": (C.c_int64, []),
     "ca_probe_tiled_launch_count": (C.c_int64, []),
     "ca_probe_tensor_launch_count": (C.c_int64, []),

@@ -216,9 +216,66 @@ Tensor rotary_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const
     return out;
 }
 
+// ---------------------------------------------------------------- other scores and masks
+struct Form {
+    double cap;                         // 0: none
+    Tensor slopes, spans, prefix;       // undefined: none
+    ca_seq_form view() const {
+        return ca_seq_form{(float)cap, fptr(slopes), static_cast<const int32_t*>(ptr(spans)), static_cast<const int32_t*>(ptr(prefix))};
+    }
+};
+
+// Checks them against q, whose heads and tokens they belong to.
+Form form_of(const Tensor& q, std::optional<double> cap, const std::optional<Tensor>& slopes, const std::optional<Tensor>& spans,
+             const std::optional<Tensor>& prefix) {
+    Form f;
+    if (cap && !(*cap > 0.0)) mismatch("cap (" + std::to_string(*cap) + ") must be positive: None leaves the scores as they are");
+    f.cap = cap ? *cap : 0.0;
+    if (cap && (float)f.cap == 0.f) mismatch("cap is too small for 32 bits");
+    if (slopes) {
+        require_ints(*slopes, q, at::kFloat, "slopes");
+        if (slopes->dim() != 1 || slopes->size(0) != q.size(1) || !slopes->is_contiguous())
+            mismatch("slopes of size " + shape_text(*slopes) + ": one for each of the " + std::to_string(q.size(1)) + " query heads expected");
+        if (tracked({&*slopes})) raise(PyExc_NotImplementedError, "slopes have no gradient: detach them");
+        f.slopes = *slopes;
+    }
+    if (spans) {
+        require_ints(*spans, q, at::kInt, "spans");
+        if (spans->dim() != 3 || spans->size(0) != 4 || spans->size(1) != q.size(2) || spans->size(2) != q.size(3) || !is_colmajor(*spans))
+            mismatch("spans of size " + shape_text(*spans) + ": those of token_spans for " + std::to_string(q.size(2)) + " tokens and a batch of " + std::to_string(q.size(3)) + " expected");
+        f.spans = *spans;
+    }
+    if (prefix) {
+        require_ints(*prefix, q, at::kInt, "prefix");
+        f.prefix = *prefix;
+    }
+    return f;
+}
+
+Tensor token_spans(const Tensor& documents_, const std::optional<Tensor>& groups_) {
+    require_cuda(documents_);
+    require_ints(documents_, documents_, at::kInt, "documents");
+    if (documents_.dim() != 1 && documents_.dim() != 2) mismatch("documents of size " + shape_text(documents_) + ": (N, B) or (N) expected");
+    if (groups_) {
+        require_ints(*groups_, documents_, at::kInt, "groups");
+        if (groups_->sizes() != documents_.sizes()) mismatch("groups of size " + shape_text(*groups_) + ", but documents of size " + shape_text(documents_));
+    }
+    const Tensor documents = colmajor(documents_), groups = groups_ ? colmajor(*groups_) : Tensor();
+    Call call(documents, "circatt.spans");
+    const int64_t N = documents.size(0), B = documents.dim() == 2 ? documents.size(1) : 1;
+    Tensor spans = empty_cm({4, N, B}, documents, at::kInt);
+    check(ca_token_spans(static_cast<const int32_t*>(ptr(documents)), static_cast<const int32_t*>(ptr(groups)), int_of(N, "N"), int_of(B, "B"),
+                         static_cast<int32_t*>(ptr(spans)), call.stream));
+    return spans;
+}
+
 Tensor paged_window(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& starts,
-                    const Tensor& lengths, int64_t left, int64_t sinks, std::optional<double> scale) {
+                    const Tensor& lengths, int64_t left, int64_t sinks, std::optional<double> scale, std::optional<double> cap,
+                    const std::optional<Tensor>& slopes, const std::optional<Tensor>& prefix) {
     check_tokens(q_, "q", true);
+    const Form form = form_of(q_, cap, slopes, std::nullopt, prefix);
+    if (prefix && (prefix->dim() != 1 || prefix->sizes() != lengths.sizes() || !prefix->is_contiguous()))
+        mismatch("prefix of size " + shape_text(*prefix) + ": one for each sequence expected");
     check_cache(k_pages, q_, v_pages, "k_pages");
     check_cache(v_pages, q_, k_pages, "v_pages");
     const Tensor q = ready(q_.detach());
@@ -237,7 +294,8 @@ Tensor paged_window(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pag
     Tensor y = empty_cm(q.sizes(), q, q.scalar_type());
     const ca_seq_view vq = view(q), vy = view(y);
     const ca_page_view kp = page_view(k_pages), vp = page_view(v_pages);
-    check(ca_paged_window(&d, &vq, &kp, &vp, &p, &vy, call.stream));
+    const ca_seq_form vf = form.view();
+    check(ca_paged_window_form(&d, &vf, &vq, &kp, &vp, &p, &vy, call.stream));
     return y;
 }
 
@@ -265,7 +323,7 @@ ca_seq_desc window_desc(const Tensor& q, const Tensor& k, const Window& w) {
 struct WindowOut { Tensor y, rest, lse; };
 
 // `train`: also what the backward needs, the rows' sums and (16-bit types) what rounding took from y.
-WindowOut window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Window& w, bool train) {
+WindowOut window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Window& w, const Form& form, bool train) {
     Call call(q, "circatt.window");
     const ca_seq_desc d = window_desc(q, k, w);
     WindowOut o;
@@ -273,16 +331,20 @@ WindowOut window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     if (train) o.lse = at::empty({q.size(1) * q.size(2) * q.size(3)}, q.options().dtype(at::kFloat));
     if (train && q.element_size() == 2) o.rest = empty_cm(q.sizes(), q, q.scalar_type());
     const ca_seq_view vq = view(q), vk = view(k), vv = view(v), vy = view(o.y), vr = o.rest.defined() ? view(o.rest) : ca_seq_view{};
-    check(ca_window_fwd(&d, &vq, &vk, &vv, static_cast<const int32_t*>(ptr(lengths)), &vy, o.rest.defined() ? &vr : nullptr, fptr(o.lse), call.stream));
+    const ca_seq_form vf = form.view();
+    check(ca_window_form_fwd(&d, &vf, &vq, &vk, &vv, static_cast<const int32_t*>(ptr(lengths)), &vy, o.rest.defined() ? &vr : nullptr, fptr(o.lse), call.stream));
     return o;
 }
 
 struct WindowFn : public Function<WindowFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const std::optional<Tensor>& lengths,
-                          int64_t left, int64_t right, int64_t sinks, double scale) {
+                          int64_t left, int64_t right, int64_t sinks, double scale, double cap, const std::optional<Tensor>& slopes_,
+                          const std::optional<Tensor>& spans_) {
+        const Tensor slopes = slopes_ ? *slopes_ : Tensor(), spans = spans_ ? *spans_ : Tensor();
         const Tensor q = ready(q_), k = ready(k_), v = ready(v_), n = lengths ? *lengths : Tensor();
-        const WindowOut o = window_fwd(q, k, v, n, Window{left, right, sinks, scale}, true);
-        ctx->save_for_backward({q, k, v, o.y, o.lse, n, o.rest});
+        const WindowOut o = window_fwd(q, k, v, n, Window{left, right, sinks, scale}, Form{cap, slopes, spans, Tensor()}, true);
+        ctx->save_for_backward({q, k, v, o.y, o.lse, n, o.rest, slopes, spans});
+        ctx->saved_data["cap"] = cap;
         ctx->saved_data["left"] = left;
         ctx->saved_data["right"] = right;
         ctx->saved_data["sinks"] = sinks;
@@ -299,13 +361,14 @@ struct WindowFn : public Function<WindowFn> {
         const Tensor work = scratch(ca_window_bwd_workspace(&d), q);
         const ca_seq_view vq = view(q), vk = view(k), vv = view(v), vy = view(y), vdy = view(dy), vdq = view(dq), vdk = view(dk), vdv = view(dv),
                           vr = rest.defined() ? view(rest) : ca_seq_view{};
-        check(ca_window_bwd(&d, &vq, &vk, &vv, &vy, rest.defined() ? &vr : nullptr, &vdy, static_cast<const int32_t*>(ptr(n)), fptr(lse), &vdq, &vdk, &vdv, ptr(work), call.stream));
-        return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        const ca_seq_form vf = Form{ctx->saved_data["cap"].toDouble(), s[7], s[8], Tensor()}.view();
+        check(ca_window_form_bwd(&d, &vf, &vq, &vk, &vv, &vy, rest.defined() ? &vr : nullptr, &vdy, static_cast<const int32_t*>(ptr(n)), fptr(lse), &vdq, &vdk, &vdv, ptr(work), call.stream));
+        return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
 Tensor window(const Tensor& q, const Tensor& k, const Tensor& v, int64_t left, int64_t right, int64_t sinks, const std::optional<Tensor>& lengths,
-              std::optional<double> scale_) {
+              std::optional<double> scale_, std::optional<double> cap, const std::optional<Tensor>& slopes, const std::optional<Tensor>& spans) {
     require_cuda(q);
     require_like(k, q, "k");
     require_like(v, q, "v");
@@ -316,9 +379,10 @@ Tensor window(const Tensor& q, const Tensor& k, const Tensor& v, int64_t left, i
         if (lengths->dim() != 1 || lengths->size(0) != q.size(3) || !lengths->is_contiguous()) mismatch("lengths of size " + shape_text(*lengths) + ": one for each of the batch expected");
     }
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)q.size(0));
+    const Form form = form_of(q, cap, slopes, spans, std::nullopt);
     if (!tracked({&q, &k, &v}))
-        return window_fwd(ready(q), ready(k), ready(v), lengths ? *lengths : Tensor(), Window{left, right, sinks, scale}, false).y;
-    return WindowFn::apply(q, k, v, lengths, left, right, sinks, scale);
+        return window_fwd(ready(q), ready(k), ready(v), lengths ? *lengths : Tensor(), Window{left, right, sinks, scale}, form, false).y;
+    return WindowFn::apply(q, k, v, lengths, left, right, sinks, scale, form.cap, slopes, spans);
 }
 
 }  // namespace
@@ -327,6 +391,7 @@ void bind_tokens(py::module_& m) {
     using release = py::call_guard<py::gil_scoped_release>;
     m.def("rotary", &rotary, release());
     m.def("rotary_append", &rotary_append, release());
+    m.def("token_spans", &token_spans, release());
     m.def("window_attention", &window, release());
     m.def("paged_window_attention", &paged_window, release());
 }

@@ -23,6 +23,15 @@ int check_page_view(const ca_page_view* v, int dtype, const char* name, bool use
 int check_pages(const ca_pages* p, int tokens);
 
 // ---------------------------------------------------------------- attention
+// Other scores and masks than the window's.  Kernels that know them are compiled apart (FORM), so that calls without pay nothing.
+struct SeqForm {
+    float cap_in, cap_out;          // z = cap_out tanh(cap_in q.k), with scale / cap and cap log2(e); cap_out = 0: no cap
+    const float* slopes;            // for each query head, nullable: z -= slope log2(e) |i - j|
+    const int4* spans;              // dense: [batch][token], nullable: the token sees x..z, and y..w see it
+    const int* prefix;              // paged, [sequence], nullable: tokens below are visible to all of the sequence
+    int changed;                    // there is a cap or a slope
+};
+
 // A query tile holds consecutive rows R of one key head: row R is query head R % G of the group, token R / G, so that
 // the query heads that share a key head share its tiles.
 struct SeqArgs {
@@ -36,6 +45,8 @@ struct SeqArgs {
     ca_seq_view q, k, v, y, rest, dy, dq, dk, dv;   // rest.data nullable: what rounding took from y
     ca_page_view kp, vp;
     ca_pages pages;                 // table == nullptr: dense
+    SeqForm form;
+    bool formed;                    // a call with other scores or masks
     float* lse;                     // [b][key head][R]: log2 of the sum, -inf for rows that see nothing
     float* delta;                   // the same order: dy . y
     int* status;
@@ -135,14 +146,63 @@ __device__ __forceinline__ int key_limit(const SeqArgs& a, const Seq& s) {
     return a.pages.table ? (int)min((int64_t)min(s.n, 1 << 30), (int64_t)a.pages.width * a.pages.page) : s.n;
 }
 
+// The keys from lo to hi, and of those below `sinks` the ones up to hi.
+struct Reach { int lo, hi; };
+
+// What the token at `pos` sees.  Both ends never fall from one token to the next (documents and groups follow one another), so
+// that a tile's first and last row bound what it sees.
+template <bool FORM>
+__device__ __forceinline__ Reach reach(const SeqArgs& a, const Seq& s, int pos) {
+    Reach r{pos - a.left, (int)min((int64_t)INT32_MAX, (int64_t)pos + a.right)};
+    if constexpr (FORM) {
+        if (a.form.spans) {
+            const int4 w = a.form.spans[(int64_t)s.b * a.N + max(0, min(pos, a.N - 1))];
+            r.lo = max(r.lo, w.x);
+            r.hi = w.z;
+        } else if (a.form.prefix) {
+            r.hi = max(r.hi, a.form.prefix[s.b] - 1);
+        }
+    }
+    return r;
+}
+// The same for the bounds of tiles: always with the token itself, whatever the spans hold, so that the tiles of neighbouring
+// rows leave no gap.
+template <bool FORM>
+__device__ __forceinline__ Reach tile_reach(const SeqArgs& a, const Seq& s, int pos) {
+    Reach r = reach<FORM>(a, s, pos);
+    if (FORM) r.lo = min(r.lo, pos), r.hi = max(r.hi, pos);
+    return r;
+}
+// Queries from lo to hi see key j.
+__device__ __forceinline__ Reach seen_by(const SeqArgs& a, const Seq& s, int j) {
+    const int4 w = a.form.spans[(int64_t)s.b * a.N + max(0, min(j, a.N - 1))];
+    return Reach{w.y, min(w.w, j + a.left)};
+}
+
+// Padding, which sees nothing and which nothing sees: whatever it holds, it counts as zeros.  `mixed`: there may be some among
+// the tokens from..upto, which are not all of one document.
+template <bool FORM>
+__device__ __forceinline__ bool padding(const SeqArgs& a, const Seq& s, int j) {
+    if (!FORM || !a.form.spans) return false;
+    const int4 w = a.form.spans[(int64_t)s.b * a.N + max(0, min(j, a.N - 1))];
+    return w.w < w.y;
+}
+template <bool FORM>
+__device__ __forceinline__ bool mixed(const SeqArgs& a, const Seq& s, int from, int upto) {
+    if (!FORM || !a.form.spans) return false;
+    const int4 w = a.form.spans[(int64_t)s.b * a.N + max(0, min(upto, s.n - 1))];
+    return w.x > from || w.w < w.y;
+}
+
+template <bool FORM = false>
 __device__ __forceinline__ KeyTiles key_tiles(const SeqArgs& a, const Seq& s, int p_lo, int p_hi, int keys) {
     KeyTiles k;
     p_lo = max(p_lo, 0);
     p_hi = min(p_hi, s.n - 1);
     if (p_hi < p_lo) return KeyTiles{0, 0, 0};
     const int limit = key_limit(a, s);
-    const int lo = max(0, p_lo - a.left);                                  // left <= 2^30
-    const int hi = (int)min((int64_t)limit, (int64_t)p_hi + a.right + 1);  // > lo unless the table ends before the window
+    const int lo = max(0, tile_reach<FORM>(a, s, p_lo).lo);                                  // left <= 2^30
+    const int hi = (int)min((int64_t)limit, (int64_t)tile_reach<FORM>(a, s, p_hi).hi + 1);  // > lo unless the table ends before the window
     // A window that begins behind the table has no tile: rounded down to one it would be a tile that no row sees, whose copies nobody
     // waits for.
     k.lo = lo < hi ? lo / keys * keys : hi;
@@ -151,6 +211,10 @@ __device__ __forceinline__ KeyTiles key_tiles(const SeqArgs& a, const Seq& s, in
     return k;
 }
 
+// Whether the query at `pos`, which reaches r, sees key j.
+__device__ __forceinline__ bool sees(const SeqArgs& a, int n, int pos, Reach r, int j) {
+    return pos >= 0 && pos < n && j < n && j <= r.hi && (j >= r.lo || j < a.sinks);
+}
 // Whether the query at `pos` sees key j.
 __device__ __forceinline__ bool sees(const SeqArgs& a, int n, int pos, int j) {
     return pos >= 0 && pos < n && j < n && j - pos <= a.right && (pos - j <= a.left || j < a.sinks);
@@ -162,6 +226,53 @@ __device__ __forceinline__ int page_of(const SeqArgs& a, int b, int j) {
     if (c >= a.pages.width) return -1;
     const int p = a.pages.table[c + (int64_t)a.pages.width * b];
     return p < a.pages.pages ? p : -1;
+}
+
+// ---------------------------------------------------------------- scores with a cap and a slope
+// tanh(x) / x on |x| <= 1 as a polynomial in x^2 that minimises the largest relative error (Lawson's iteration): 6.9e-6 with
+// degree 4, for bfloat16 weights (scores of 40 are off by 3e-4, a seventh of the weights' rounding); 5.9e-7 with 5 for half; 5e-8
+// with 6 for Float32.
+template <int DEGREE> struct TanhPoly;
+template <> struct TanhPoly<4> {
+    static __device__ __forceinline__ float at(int i) {
+        const float c[5] = {0.999993086f, -0.332980663f, 0.130368114f, -0.0448175557f, 0.00903642457f};
+        return c[i];
+    }
+};
+template <> struct TanhPoly<5> {
+    static __device__ __forceinline__ float at(int i) {
+        const float c[6] = {0.999999404f, -0.333290428f, 0.132814333f, -0.0516056754f, 0.0167431161f, -0.00306706037f};
+        return c[i];
+    }
+};
+template <> struct TanhPoly<6> {
+    static __device__ __forceinline__ float at(int i) {
+        const float c[7] = {0.99999994f, -0.333328396f, 0.13325204f, -0.0534570292f, 0.0202899817f, -0.00620337948f, 0.00104102271f};
+        return c[i];
+    }
+};
+// tanh(x) = 1 - 2 / (1 + e^2x): an absolute error of 10^-7 or so, which is a relative one where |x| > 1.
+__device__ __forceinline__ float tanh_far(float x) { return 1.f - __fdividef(2.f, 1.f + fast_exp2(x * (2.f * kLog2e))); }
+__device__ __forceinline__ float tanh_any(float x) {
+    const float u = x * x;
+    float p = TanhPoly<6>::at(6);
+#pragma unroll
+    for (int i = 5; i >= 0; --i) p = fmaf(p, u, TanhPoly<6>::at(i));
+    return fabsf(x) <= 1.f ? p * x : tanh_far(x);          // what is not a number stays so
+}
+// Of query head `head`, in units of log2(e).
+__device__ __forceinline__ float slope_of(const SeqArgs& a, int head) { return a.form.slopes ? a.form.slopes[head] * kLog2e : 0.f; }
+// A score in units of log2(e), from q.k, less `minus`; slope in those units too, `inner`: the derivative of the cap.
+__device__ __forceinline__ float formed_score(const SeqArgs& a, float dot, float slope, int distance, float minus, float& inner) {
+    inner = 1.f;
+    if (!a.form.changed) return fmaf(dot, a.scale_log2, -minus);         // as without a form, to the bit
+    float z = dot * a.scale_log2;
+    if (a.form.cap_out != 0.f) {
+        const float t = tanh_any(dot * a.form.cap_in);
+        z = a.form.cap_out * t;
+        inner = fmaf(-t, t, 1.f);
+    }
+    return fmaf(-slope, fabsf((float)distance), z) - minus;
 }
 
 // How the backward deals out the queries of key tiles that hold first tokens: those tiles have every later query, an ordinary one

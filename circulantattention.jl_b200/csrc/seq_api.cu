@@ -42,6 +42,30 @@ int check_pages(const ca_pages* p, int tokens) {
     return CA_OK;
 }
 
+static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Other scores and masks; form may be NULL.
+static int fill_form(const ca_seq_desc* d, const ca_seq_form* form, bool paged, SeqArgs* a) {
+    if (!form) return CA_OK;
+    if (!(form->cap >= 0.f) || isinf(form->cap)) { set_error("cap must be positive, or 0 for scores as they are"); return CA_ERR_BAD_DESC; }
+    if (form->cap > 0.f && !isfinite(d->scale / form->cap)) { set_error("cap=%g is too small for scale=%g", form->cap, d->scale); return CA_ERR_BAD_DESC; }
+    if (form->cap > 0.f && !isfinite(form->cap * kLog2e)) { set_error("cap=%g is too large", form->cap); return CA_ERR_BAD_DESC; }
+    if (!aligned(form->slopes, 4) || !aligned(form->prefix, 4) || !aligned(form->spans, 16)) { set_error("slopes, prefix or spans (16 bytes) are not aligned"); return CA_ERR_BAD_DESC; }
+    if (form->spans && paged) { set_error("spans are for dense tensors"); return CA_ERR_BAD_DESC; }
+    if (form->prefix && !paged) { set_error("prefix is for calls over a cache: a dense call takes spans"); return CA_ERR_BAD_DESC; }
+    if (form->spans && (d->right || d->sinks)) { set_error("right=%d sinks=%d: spans say what a token sees", d->right, d->sinks); return CA_ERR_BAD_DESC; }
+    if (form->cap > 0.f) {
+        a->form.cap_in = d->scale / form->cap;
+        a->form.cap_out = form->cap * kLog2e;
+    }
+    a->form.slopes = form->slopes;
+    a->form.spans = reinterpret_cast<const int4*>(form->spans);
+    a->form.prefix = form->prefix;
+    a->form.changed = form->cap > 0.f || form->slopes;
+    a->formed = a->form.changed || form->spans || form->prefix;
+    return CA_OK;
+}
+
 static int fill(const ca_seq_desc* d, SeqArgs* a) {
     if (!d) { set_error("descriptor is NULL"); return CA_ERR_NULL; }
     const int rc = check_seq_dtype(d->dtype);
@@ -79,17 +103,11 @@ static int fill(const ca_seq_desc* d, SeqArgs* a) {
 // delta, one float a row, padded so that what follows is aligned
 static size_t delta_bytes(const SeqArgs& a) { return ((size_t)a.N * a.B * a.Hq * sizeof(float) + 255) & ~(size_t)255; }
 
-}  // namespace ca
-
-using namespace ca;
-
-extern "C" {
-
-int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+static int window_fwd(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
                   const int32_t* lengths, const ca_seq_view* y, const ca_seq_view* y_rest, float* lse, void* stream) {
     SeqArgs a{};
     int rc = fill(d, &a);
-    if (rc) return rc;
+    if (rc || (rc = fill_form(d, form, false, &a))) return rc;
     const bool some = a.N && a.B;
     if ((rc = check_view(q, d->dtype, "q", some)) || (rc = check_view(k, d->dtype, "k", some)) || (rc = check_view(v, d->dtype, "v", some)) ||
         (rc = check_view(y, d->dtype, "y", some)) || (y_rest && (rc = check_view(y_rest, d->dtype, "y_rest", false))))
@@ -102,18 +120,12 @@ int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     return d->dtype == CA_F32 ? fma_fwd(a, as_stream(stream)) : umma_window_fwd(a, d->dtype, as_stream(stream));
 }
 
-size_t ca_window_bwd_workspace(const ca_seq_desc* d) {
-    SeqArgs a{};
-    if (fill(d, &a)) return 0;
-    return delta_bytes(a) + (d->dtype == CA_F32 ? fma_bwd_parts(a) : umma_bwd_parts(a));
-}
-
-int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+static int window_bwd(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
                   const ca_seq_view* y, const ca_seq_view* y_rest, const ca_seq_view* dy, const int32_t* lengths, const float* lse,
                   const ca_seq_view* dq, const ca_seq_view* dk, const ca_seq_view* dv, void* workspace, void* stream) {
     SeqArgs a{};
     int rc = fill(d, &a);
-    if (rc) return rc;
+    if (rc || (rc = fill_form(d, form, false, &a))) return rc;
     const bool some = a.N && a.B;
     if ((rc = check_view(q, d->dtype, "q", some)) || (rc = check_view(k, d->dtype, "k", some)) || (rc = check_view(v, d->dtype, "v", some)) ||
         (rc = check_view(y, d->dtype, "y", some)) || (rc = check_view(dy, d->dtype, "dy", some)) || (rc = check_view(dq, d->dtype, "dq", some)) ||
@@ -131,11 +143,11 @@ int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
     return d->dtype == CA_F32 ? fma_bwd(a, parts, as_stream(stream)) : umma_window_bwd(a, d->dtype, parts, as_stream(stream));
 }
 
-int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_view* k_pages, const ca_page_view* v_pages,
-                    const ca_pages* pages, const ca_seq_view* y, void* stream) {
+static int paged_window(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_page_view* k_pages, const ca_page_view* v_pages,
+                        const ca_pages* pages, const ca_seq_view* y, void* stream) {
     SeqArgs a{};
     int rc = fill(d, &a);
-    if (rc) return rc;
+    if (rc || (rc = fill_form(d, form, true, &a))) return rc;
     const bool some = a.N && a.B;
     if (d->batch != 1) { set_error("packed tokens have batch 1 (got %d)", d->batch); return CA_ERR_BAD_DESC; }
     if (d->right) { set_error("right=%d: a cache holds no later tokens", d->right); return CA_ERR_BAD_DESC; }
@@ -151,6 +163,50 @@ int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_vi
     // single tokens 98 us, a chunk of 900 93 us, both in one call 385; with a chunk of 1000, by the other kernel, 275).
     if ((int64_t)a.N * a.G <= 64LL * a.pages.sequences || !a.pages.pages) return decode_paged(a, d->dtype, as_stream(stream));
     return d->dtype == CA_F32 ? fma_fwd(a, as_stream(stream)) : umma_paged(a, d->dtype, as_stream(stream));
+}
+
+}  // namespace ca
+
+using namespace ca;
+
+extern "C" {
+
+int ca_window_fwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+                  const int32_t* lengths, const ca_seq_view* y, const ca_seq_view* y_rest, float* lse, void* stream) {
+    return window_fwd(d, nullptr, q, k, v, lengths, y, y_rest, lse, stream);
+}
+
+int ca_window_form_fwd(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+                       const int32_t* lengths, const ca_seq_view* y, const ca_seq_view* y_rest, float* lse, void* stream) {
+    return window_fwd(d, form, q, k, v, lengths, y, y_rest, lse, stream);
+}
+
+size_t ca_window_bwd_workspace(const ca_seq_desc* d) {
+    SeqArgs a{};
+    if (fill(d, &a)) return 0;
+    return delta_bytes(a) + (d->dtype == CA_F32 ? fma_bwd_parts(a) : umma_bwd_parts(a));
+}
+
+int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+                  const ca_seq_view* y, const ca_seq_view* y_rest, const ca_seq_view* dy, const int32_t* lengths, const float* lse,
+                  const ca_seq_view* dq, const ca_seq_view* dk, const ca_seq_view* dv, void* workspace, void* stream) {
+    return window_bwd(d, nullptr, q, k, v, y, y_rest, dy, lengths, lse, dq, dk, dv, workspace, stream);
+}
+
+int ca_window_form_bwd(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+                       const ca_seq_view* y, const ca_seq_view* y_rest, const ca_seq_view* dy, const int32_t* lengths, const float* lse,
+                       const ca_seq_view* dq, const ca_seq_view* dk, const ca_seq_view* dv, void* workspace, void* stream) {
+    return window_bwd(d, form, q, k, v, y, y_rest, dy, lengths, lse, dq, dk, dv, workspace, stream);
+}
+
+int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_view* k_pages, const ca_page_view* v_pages,
+                    const ca_pages* pages, const ca_seq_view* y, void* stream) {
+    return paged_window(d, nullptr, q, k_pages, v_pages, pages, y, stream);
+}
+
+int ca_paged_window_form(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_page_view* k_pages,
+                         const ca_page_view* v_pages, const ca_pages* pages, const ca_seq_view* y, void* stream) {
+    return paged_window(d, form, q, k_pages, v_pages, pages, y, stream);
 }
 
 }  // extern "C"

@@ -89,6 +89,7 @@ __device__ __forceinline__ void clear_row(char* tile, int r) {
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + p * kPanel + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
 }
 
+template <bool FORM>
 __global__ void __launch_bounds__(256) peak_kernel(const __grid_constant__ SeqArgs a, float* __restrict__ peaks) {
     __shared__ float part[8];
     const Seq s = dense_seq(a, blockIdx.z);
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(256) peak_kernel(const __grid_constant__ SeqAr
     for (int i = threadIdx.x; i < 128 * pieces; i += 256) {
         const int j = key0 + i / pieces;
         if (j >= s.n) break;
+        if (padding<FORM>(a, s, j)) continue;
         const uint4 w = *reinterpret_cast<const uint4*>(v + (int64_t)j * a.v.token + i % pieces * 8);
         const uint32_t* p = &w.x;
 #pragma unroll
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(256) peak_kernel(const __grid_constant__ SeqAr
 // The queries move into tensor memory, and their place becomes one more slot of the ring: a tile of keys stays until its product
 // with dS, two steps behind its scores, so that with five slots the values of every tile came late (2450 cycles a tile; 1536
 // are products).
-template <typename T, int DM>
+template <typename T, int DM, bool FORM>
 __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ BwdMaps maps) {
     constexpr int S = kSlots<DM> + 1;
     constexpr uint32_t TILE = kTileBytes<DM>;
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
     const int rows = s.T * a.G, R0 = (int)(gridDim.x - 1 - blockIdx.x) * 128;
     const int f_lo = R0 / a.G, f_hi = (min(R0 + 128, rows) - 1) / a.G;      // tokens of the tile
     const int p_hi = min(s.n - 1, f_hi);
-    const KeyTiles kt = key_tiles(a, s, f_lo, f_hi, 128);
+    const KeyTiles kt = key_tiles<FORM>(a, s, f_lo, f_hi, 128);
 
     if (warp == kCopier && lane == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
 
     if (warp < kWarps) {
         const int u = warp >> 2, r = tid & 127, R = R0 + r, pos = token_of(a, R);
-        const bool have = R < rows, live = have && pos < s.n;
+        const bool have = R < rows, live = have && pos < s.n && !padding<FORM>(a, s, pos);
         const int64_t stat = ((int64_t)s.b * a.Hkv + h) * rows + R;
         const float lse = live ? a.lse[stat] : 0.f;
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
@@ -240,10 +242,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 }
             }
             group_sync<kWork>(1);
-            delta = part[0][r];
+            delta = !FORM || live ? part[0][r] : 0.f;
             if (u == 0 && have) a.delta[stat] = delta;
             if (!kIsBf16<T>) {
-                float peak = part[1][r], v_peak = 0.f;
+                float peak = !FORM || live ? part[1][r] : 0.f, v_peak = 0.f;
                 const float* p = maps.v_peak + ((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128);
                 for (int i = lane; i < kt.count; i += 32) v_peak = fmaxf(v_peak, p[kt.key(i, 128) / 128]);
                 c = ds_factor(peak, warp_max(v_peak));
@@ -252,6 +254,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             }
         }
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta * c, -delta * c), c2 = pack2(c, c);
+        const bool changed = FORM && a.form.changed;
+        const float slope = FORM && changed ? slope_of(a, h * a.G + R - pos * a.G) : 0.f;
+        const Reach mine = reach<FORM>(a, s, pos);
+        const bool row_pads = mixed<FORM>(a, s, f_lo, f_hi);
+        const int in_hi = reach<FORM>(a, s, f_lo).hi, in_lo = reach<FORM>(a, s, p_hi).lo;      // tiles from in_lo to in_hi need no mask
         const uint32_t S_at = tmem + kCols * u + lane_off, dp_at = S_at + 128, ds_at = tmem + 256 + kCols / 2 * u + lane_off;
         bool ok = true;
         for (int i = 0; i < kt.count; ++i) {
@@ -263,23 +270,33 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_free));
-#pragma unroll
-            for (int c = 0; c < kCols; c += 2) {
-                float e0, e1;
-                unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, lse2), e0, e1);
-                x[c] = __float_as_uint(fast_exp2(e0));
-                x[c + 1] = __float_as_uint(fast_exp2(e1));
-            }
             uint32_t mk = ~0u;
-            const bool ragged = far >= s.n || f_hi != p_hi;      // the tile holds keys or rows that may be anything
-            const bool edge = !(far <= f_lo + a.right && far < s.n && f_hi == p_hi && (key0 >= p_hi - a.left || far < a.sinks));
+            const bool pads = mixed<FORM>(a, s, key0, far);
+            const bool ragged = far >= s.n || f_hi != p_hi || pads || row_pads;      // the tile holds keys or rows that may be anything
+            const bool edge = !(far <= in_hi && far < s.n && f_hi == p_hi && (key0 >= in_lo || far < a.sinks));
             if (edge) {
-                const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
+                const int hi = live ? min(mine.hi, s.n - 1) - key0 : -1, lo = mine.lo - key0, sk = a.sinks - key0;
                 mk = seen_bits(lo - kCols * u, hi - kCols * u, sk - kCols * u);
+            }
+            if (FORM && changed) {
+                float inner[kCols];                            // P (1 - tanh^2) is all that dS needs
+                form_scores<T, kCols, true>(x, inner, a, a.scale_log2, a.form.cap_in, slope, (float)(pos - key0 - kCols * u), edge, mk);
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) x[c] = __float_as_uint(fast_exp2(__uint_as_float(x[c]) - lse) * inner[c]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < kCols; c += 2) {
+                    float e0, e1;
+                    unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), sc2, lse2), e0, e1);
+                    x[c] = __float_as_uint(fast_exp2(e0));
+                    x[c + 1] = __float_as_uint(fast_exp2(e1));
+                }
+            }
+            if (edge) {
                 clear_unseen<kCols>(x, mk);
-                if (far >= s.n && u == 0) {                    // keys behind the length may be anything: zeros
+                if ((far >= s.n || pads) && u == 0) {          // keys behind the length, and padding, may be anything: zeros
                     const int slot = (2 * i) % S;              // the scores are there, so the keys are
-                    if (key0 + r >= s.n) clear_row<DM>(smem + (1 + slot) * TILE, r);
+                    if (key0 + r >= s.n || (pads && padding<FORM>(a, s, key0 + r))) clear_row<DM>(smem + (1 + slot) * TILE, r);
                     fence_async_smem();
                 }
             }
@@ -433,7 +450,7 @@ struct Steps {
 //
 // Keys that stay visible to every later token would give their CTA all queries of the sequence; the queries of such tiles are
 // dealt to `segments` CTAs, which store Float32 parts for join_kernel to add up in order.
-template <typename T, int DM>
+template <typename T, int DM, bool FORM>
 __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ BwdMaps maps) {
     constexpr int S = kSlots<DM>;
     constexpr uint32_t TILE = kTileBytes<DM>;
@@ -455,8 +472,17 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     const int tile = split ? (int)blockIdx.x / maps.segments : maps.split_tiles + (int)blockIdx.x - dealt;
     const int seg = split ? (int)blockIdx.x % maps.segments : 0;
     const int k0 = tile * 128;
-    const int t_lo = max(0, k0 - a.right);
-    const int t_hi = k0 >= s.n ? t_lo : k0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)k0 + 128 + a.left);
+    int t_lo = max(0, k0 - a.right);                               // queries that see any of the keys
+    int t_hi = k0 >= s.n ? t_lo : k0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)k0 + 128 + a.left);
+    int whole_lo = k0 + 127 - a.right, whole_hi = k0 + 127 < a.sinks ? INT_MAX : k0 + a.left;      // that see all of them
+    const bool spans = FORM && a.form.spans && k0 < s.n;
+    if (FORM && spans) {                                           // neither end of what sees a key falls from one key to the next
+        const Reach by0 = seen_by(a, s, k0), by1 = seen_by(a, s, min(k0 + 127, s.n - 1));
+        t_lo = max(0, min(by0.lo, k0));
+        t_hi = max(k0, min(by1.hi, s.n - 1)) + 1;
+        whole_lo = by1.lo;
+        whole_hi = by0.hi;
+    }
     const int all = max(0, t_hi - t_lo + 127) / 128 * a.G;          // steps: token tiles outside, query heads inside
     const int first = split ? (int)((int64_t)all * seg / maps.segments) : 0;
     const int count = (split ? (int)((int64_t)all * (seg + 1) / maps.segments) : all) - first;
@@ -506,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         for (int i = (int)((int64_t)t_lo * a.G / 128) + lane; i <= (int)(((int64_t)t_hi * a.G - 1) / 128); i += 32) peak = fmaxf(peak, p[i]);
         // keys that the queries t_lo .. t_hi - 1 see: their windows, and first tokens before those
         const float* pv = maps.v_peak + ((int64_t)s.b * a.Hkv + h) * ((a.N + 127) / 128);
-        const int from = max(0, t_lo - a.left) / 128, upto = (int)min((int64_t)s.n - 1, (int64_t)t_hi - 1 + a.right) / 128;
+        const int from = max(0, reach<FORM>(a, s, t_lo).lo) / 128, upto = min(s.n - 1, reach<FORM>(a, s, t_hi - 1).hi) / 128;
         float v_peak = 0.f;
         for (int i = lane; i <= upto; i += 32)
             if (i >= from || i * 128 < a.sinks) v_peak = fmaxf(v_peak, pv[i]);
@@ -519,12 +545,21 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         const uint32_t S_at = tmem + 16 * u + lane_off, dp_at = S_at + 128, P_at = p_col + apart * u + lane_off, ds_at = ds_col + apart * u + lane_off;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
         const f32x2 c2 = kIsBf16<T> ? pack2(1.f, 1.f) : pack2(c / kPScale, c / kPScale);
+        const bool changed = FORM && a.form.changed, key_pads = k0 < s.n && mixed<FORM>(a, s, k0, k0 + 127);
+        int by_lo = j - a.right, by_hi = j < a.sinks ? s.n - 1 : min(j + a.left, s.n - 1);      // queries that see the key
+        if (FORM && spans) {
+            const Reach by = seen_by(a, s, j);
+            by_lo = by.lo;
+            by_hi = min(by.hi, s.n - 1);
+        }
         bool ok = true;
         Steps at(a, t_lo, first);
         for (int i = 0; i < count; ++i, at.next(a)) {
             const int q0 = at.q0, b = i & 1;
-            const bool ragged = q0 + 127 >= s.n || k0 + 127 >= s.n;
-            const bool edge = !(k0 + 127 <= q0 + a.right && (q0 + 127 <= k0 + a.left || k0 + 127 < a.sinks) && q0 + 127 < s.n && k0 + 127 < s.n);
+            const bool pads = mixed<FORM>(a, s, q0, q0 + 127);
+            const bool ragged = q0 + 127 >= s.n || k0 + 127 >= s.n || pads || key_pads;
+            const bool edge = !(whole_lo <= q0 && q0 + 127 <= whole_hi && q0 + 127 < s.n && k0 + 127 < s.n);
+            const float slope = FORM && changed ? slope_of(a, h * a.G + at.g) : 0.f;
             if (!warp_wait(smem_u32(&st_full[b]), (i >> 1) & 1, stop) || !warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
             fence_after();
             // Columns 16 u .. 16 u + 15 of either half of the tile: the product with the first half starts while the weights
@@ -532,25 +567,28 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             uint32_t x[kCols], mk = ~0u;
             read_halves(S_at, x);
             if (edge) {
-                const int hi = j >= s.n ? -1 : (j < a.sinks ? s.n - 1 : min(j + a.left, s.n - 1)) - q0 - 16 * u, lo = j - a.right - q0 - 16 * u;
+                const int hi = j >= s.n ? -1 : by_hi - q0 - 16 * u, lo = by_lo - q0 - 16 * u;
                 mk = (seen_bits(lo, hi, INT_MIN + 1) & 0xffffu) | seen_bits(lo - 64, hi - 64, INT_MIN + 1) << 16;
             }
-            if (ragged && u < 2 && q0 + 127 >= s.n) {           // queries behind the length may be anything: zeros
+            if (ragged && u < 2 && (q0 + 127 >= s.n || pads)) { // queries behind the length, and padding, may be anything: zeros
                 const int slot = (2 * i + u) % S;               // one warpgroup clears q, another dy
                 if (!warp_wait(smem_u32(&q_full[slot]), ((2 * i + u) / S) & 1, stop)) { ok = false; break; }
-                if (q0 + r >= s.n) clear_row<DM>(smem + (2 + slot) * TILE, r);
+                if (q0 + r >= s.n || (pads && padding<FORM>(a, s, q0 + r))) clear_row<DM>(smem + (2 + slot) * TILE, r);
                 fence_async_smem();
             }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const float4* lse4 = reinterpret_cast<const float4*>(&s_lse[b][64 * g + 16 * u]);
                 uint32_t* const xg = x + 16 * g;
+                float inner[16];
+                if (FORM && changed) form_scores<T, 16, true>(xg, inner, a, a.scale_log2, a.form.cap_in, slope, (float)(j - q0 - 64 * g - 16 * u), edge, mk >> 16 * g);
+                const f32x2 f2 = FORM && changed ? pack2(1.f, 1.f) : sc2;
 #pragma unroll
                 for (int c = 0; c < 16; c += 4) {
                     const float4 z = lse4[c >> 2];
                     float e[4];
-                    unpack2(fma2(pack2(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1])), sc2, pack2(z.x, z.y)), e[0], e[1]);
-                    unpack2(fma2(pack2(__uint_as_float(xg[c + 2]), __uint_as_float(xg[c + 3])), sc2, pack2(z.z, z.w)), e[2], e[3]);
+                    unpack2(fma2(pack2(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1])), f2, pack2(z.x, z.y)), e[0], e[1]);
+                    unpack2(fma2(pack2(__uint_as_float(xg[c + 2]), __uint_as_float(xg[c + 3])), f2, pack2(z.z, z.w)), e[2], e[3]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) xg[c + k] = __float_as_uint(fast_exp2(e[k]));
                 }
@@ -558,6 +596,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 uint32_t w[8];
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1]));
+                if (FORM && changed) {                             // dS has the cap's derivative
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) xg[c] = __float_as_uint(__uint_as_float(xg[c]) * inner[c]);
+                }
                 tmem_st8(P_at + 4 * apart * g, w);
                 tmem_wait_st();
                 fence_before();
@@ -739,20 +781,20 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ SeqAr
     *reinterpret_cast<uint4*>(dst) = make_uint4(pack16<T>(sum[0], sum[1]), pack16<T>(sum[2], sum[3]), pack16<T>(sum[4], sum[5]), pack16<T>(sum[6], sum[7]));
 }
 
-template <typename T, int DM>
+template <typename T, int DM, bool FORM>
 int launch(const SeqArgs& a, const BwdMaps& maps, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(umma_dq_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(umma_dkdv_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
+    cudaError_t e = cudaFuncSetAttribute(umma_dq_kernel<T, DM, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(umma_dkdv_kernel<T, DM, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
     if (!kIsBf16<T>) {
-        peak_kernel<<<dim3((a.N + 127) / 128, a.Hkv, a.B), 256, 0, st>>>(a, maps.v_peak);
+        peak_kernel<FORM><<<dim3((a.N + 127) / 128, a.Hkv, a.B), 256, 0, st>>>(a, maps.v_peak);
         CA_CHECK_LAUNCH("window peak kernel");
     }
-    umma_dq_kernel<T, DM><<<dim3((unsigned)(((int64_t)a.N * a.G + 127) / 128), a.Hkv, a.B), kThreads, kBwdSmem<DM>, st>>>(a, maps);
+    umma_dq_kernel<T, DM, FORM><<<dim3((unsigned)(((int64_t)a.N * a.G + 127) / 128), a.Hkv, a.B), kThreads, kBwdSmem<DM>, st>>>(a, maps);
     count_tensor_launch();
     CA_CHECK_LAUNCH("window dq kernel (tensor cores)");
     const int tiles = (a.N + 127) / 128;
-    umma_dkdv_kernel<T, DM><<<dim3(tiles - maps.split_tiles + maps.split_tiles * maps.segments, a.Hkv, a.B), kThreads, kBwdSmem<DM>, st>>>(a, maps);
+    umma_dkdv_kernel<T, DM, FORM><<<dim3(tiles - maps.split_tiles + maps.split_tiles * maps.segments, a.Hkv, a.B), kThreads, kBwdSmem<DM>, st>>>(a, maps);
     count_tensor_launch();
     CA_CHECK_LAUNCH("window dk/dv kernel (tensor cores)");
     if (maps.split_tiles) {
@@ -795,8 +837,14 @@ int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) 
     maps.split_tiles = p.tiles;
     maps.segments = p.segments;
     const bool wide = a.D > 64;
-    if (bf16) return wide ? launch<__nv_bfloat16, 128>(a, maps, st) : launch<__nv_bfloat16, 64>(a, maps, st);
-    return wide ? launch<__half, 128>(a, maps, st) : launch<__half, 64>(a, maps, st);
+#define CA_BWD(T, FORM) return wide ? launch<T, 128, FORM>(a, maps, st) : launch<T, 64, FORM>(a, maps, st)
+    if (a.formed) {
+        if (bf16) CA_BWD(__nv_bfloat16, true);
+        CA_BWD(__half, true);
+    }
+    if (bf16) CA_BWD(__nv_bfloat16, false);
+    CA_BWD(__half, false);
+#undef CA_BWD
 }
 
 }  // namespace ca

@@ -64,7 +64,7 @@ __device__ __forceinline__ bool grows(float& m, float top, float& f) {
     return true;
 }
 
-template <typename T, int DM>
+template <typename T, int DM, bool FORM>
 __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_constant__ SeqArgs a) {
     typedef Decode<T, DM> L;
     extern __shared__ __align__(128) char smem[];
@@ -81,9 +81,10 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
     }
     const int rows = s.T * a.G, R0 = tile * kRows, nrows = min(kRows, rows - R0);
     const int p_lo = s.base + R0 / a.G, p_hi = s.base + (R0 + nrows - 1) / a.G;
-    const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kKeys);
+    const KeyTiles kt = key_tiles<FORM>(a, s, p_lo, p_hi, kKeys);
     const int first = (int)((int64_t)kt.count * rank / ranks), last = (int)((int64_t)kt.count * (rank + 1) / ranks);
-    const int c_lo = max(p_lo, 0) - a.left, c_hi = min(p_hi, s.n - 1);        // keys that any row sees (or < sinks)
+    const Reach lowest = tile_reach<FORM>(a, s, max(p_lo, 0)), highest = tile_reach<FORM>(a, s, min(p_hi, s.n - 1));
+    const int c_lo = lowest.lo, c_hi = min(highest.hi, s.n - 1);              // keys that any row sees (or < sinks)
 
     // ------------------------------------------------------------ copies: tile i of this warp into stage `st`
     const uint32_t ring = smem_u32(smem) + warp * L::kStages * L::kStageBytes;
@@ -151,6 +152,13 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
 
     if constexpr (sizeof(T) == 2) {
         const int ra = lane >> 2, pa = s.base + token_of(a, min(R0 + ra, rows - 1)), pb = s.base + token_of(a, min(R0 + ra + 8, rows - 1));
+        const Reach ra_reach = reach<FORM>(a, s, pa), rb_reach = reach<FORM>(a, s, pb);
+        float slope_a = 0.f, slope_b = 0.f;
+        if (FORM && a.form.slopes) {
+            const int Ra = min(R0 + ra, rows - 1), Rb = min(R0 + ra + 8, rows - 1);
+            slope_a = slope_of(a, h * a.G + Ra - token_of(a, Ra) * a.G);
+            slope_b = slope_of(a, h * a.G + Rb - token_of(a, Rb) * a.G);
+        }
         uint32_t q[DM / 16][4];
         {
             const T* qa = ra < nrows ? seq_row<T>(a.q, a, s, h, R0 + ra) : nullptr;
@@ -178,14 +186,17 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
                 mma16<T>(c[1], q[k], b[2], b[3]);
             }
             const int j = key0 + (lane & 3) * 2;
-            const bool edge = !(p_lo >= 0 && key0 + kKeys - 1 <= p_lo && (key0 >= p_hi - a.left || key0 + kKeys <= a.sinks));
+            const bool edge = !(p_lo >= 0 && key0 + kKeys - 1 <= min(lowest.hi, s.n - 1) && (key0 >= p_hi - a.left || key0 + kKeys <= a.sinks));
             float ta = -INFINITY, tb = -INFINITY;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    c[n][e] *= a.scale_log2;
-                    if (edge && !sees(a, s.n, e < 2 ? pa : pb, j + 8 * n + (e & 1))) c[n][e] = -INFINITY;
+                    const int jj = j + 8 * n + (e & 1);
+                    float inner;
+                    if (FORM && a.form.changed) c[n][e] = formed_score(a, c[n][e], e < 2 ? slope_a : slope_b, (e < 2 ? pa : pb) - jj, 0.f, inner);
+                    else c[n][e] *= a.scale_log2;
+                    if (edge && !sees(a, s.n, e < 2 ? pa : pb, e < 2 ? ra_reach : rb_reach, jj)) c[n][e] = -INFINITY;
                     if (e < 2) ta = fmaxf(ta, c[n][e]); else tb = fmaxf(tb, c[n][e]);
                 }
             ta = fmaxf(ta, __shfl_xor_sync(~0u, ta, 1));
@@ -205,9 +216,14 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[n][e] = fast_exp2(c[n][e] - (e < 2 ? ma : mb));
-            l[0] += (c[0][0] + c[0][1]) + (c[1][0] + c[1][1]);
-            l[1] += (c[0][2] + c[0][3]) + (c[1][2] + c[1][3]);
             const uint32_t p[4] = {pack16<T>(c[0][0], c[0][1]), pack16<T>(c[0][2], c[0][3]), pack16<T>(c[1][0], c[1][1]), pack16<T>(c[1][2], c[1][3])};
+            if constexpr (FORM) {                               // the weights as they were rounded (see seq_fwd.cu)
+                l[0] += (low16<T>(p[0]) + high16<T>(p[0])) + (low16<T>(p[2]) + high16<T>(p[2]));
+                l[1] += (low16<T>(p[1]) + high16<T>(p[1])) + (low16<T>(p[3]) + high16<T>(p[3]));
+            } else {
+                l[0] += (c[0][0] + c[0][1]) + (c[1][0] + c[1][1]);
+                l[1] += (c[0][2] + c[0][3]) + (c[1][2] + c[1][3]);
+            }
 #pragma unroll
             for (int i = 0; i < DM / 16; ++i) {
                 uint32_t b[4];                                  // keys 0-7 and 8-15 of features 16i .. +7, then of the next 8
@@ -243,8 +259,13 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
         __syncthreads();
         const int half = lane >> 4, key = lane & 15;
         int pos[8];
+        float slopes[FORM ? 8 : 1];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pos[i] = 2 * i + half < nrows ? s.base + token_of(a, R0 + 2 * i + half) : -1;
+        for (int i = 0; i < 8; ++i) {
+            const int t = token_of(a, R0 + 2 * i + half);
+            pos[i] = 2 * i + half < nrows ? s.base + t : -1;
+            if (FORM) slopes[i] = pos[i] >= 0 ? slope_of(a, h * a.G + R0 + 2 * i + half - t * a.G) : 0.f;
+        }
         float o[kRows][C];
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
@@ -278,7 +299,13 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
             for (int i = 0; i < 8; ++i) {
                 f[i] = 1.f;
                 if (2 * i >= nrows) continue;
-                sc[i] = sees(a, s.n, pos[i], key0 + key) ? sc[i] * a.scale_log2 : -INFINITY;
+                if constexpr (FORM) {
+                    float inner;
+                    const float z = a.form.changed ? formed_score(a, sc[i], slopes[i], pos[i] - key0 - key, 0.f, inner) : sc[i] * a.scale_log2;
+                    sc[i] = sees(a, s.n, pos[i], reach<FORM>(a, s, pos[i]), key0 + key) ? z : -INFINITY;
+                } else {
+                    sc[i] = sees(a, s.n, pos[i], key0 + key) ? sc[i] * a.scale_log2 : -INFINITY;
+                }
                 float top = sc[i];
 #pragma unroll
                 for (int x = 8; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
@@ -412,17 +439,17 @@ int largest_cluster(K kernel, size_t smem, std::atomic<int>* cache) {
     return n;
 }
 
-template <typename T, int DM>
+template <typename T, int DM, bool FORM>
 int launch(const SeqArgs& a, cudaStream_t st) {
     static std::atomic<int> cluster_cache[64];
     const size_t smem = Decode<T, DM>::kSmem;
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<T, DM, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
     const int64_t tiles = paged_tiles(a.N, a.G, a.pages.sequences, kRows);
     // Split the keys while that fills idle SMs (two CTAs each) and leaves every warp a few tiles.  What is known here is the
     // most keys that a row can see: the table's width, or the window with the first tokens.
     const int64_t keys = std::min<int64_t>((int64_t)a.pages.width * a.pages.page, (int64_t)a.left + a.sinks + a.N);
-    const int most = largest_cluster(decode_kernel<T, DM>, smem, cluster_cache);
+    const int most = largest_cluster(decode_kernel<T, DM, FORM>, smem, cluster_cache);
     int split = 1;
     while (split < most && tiles * a.Hkv * split * 2 <= 2LL * sm_count() && keys >= (int64_t)split * 2 * kWarps * kKeys * 2) split *= 2;
     cudaLaunchConfig_t cfg{};
@@ -431,7 +458,7 @@ int launch(const SeqArgs& a, cudaStream_t st) {
     at[0].val.clusterDim.x = split; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(tiles * split), a.Hkv, 1); cfg.blockDim = dim3(32 * kWarps); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cfg.attrs = at; cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, decode_kernel<T, DM>, a);
+    e = cudaLaunchKernelEx(&cfg, decode_kernel<T, DM, FORM>, a);
     if (e != cudaSuccess) return cuda_fail(e, "paged decode kernel");
     CA_CHECK_LAUNCH("paged decode kernel");
     return CA_OK;
@@ -441,9 +468,13 @@ int launch(const SeqArgs& a, cudaStream_t st) {
 
 int decode_paged(const SeqArgs& a, int dtype, cudaStream_t st) {
     const bool wide = a.D > 64;
-    if (dtype == CA_F32) return wide ? launch<float, 128>(a, st) : launch<float, 64>(a, st);
-    if (dtype == CA_BF16) return wide ? launch<__nv_bfloat16, 128>(a, st) : launch<__nv_bfloat16, 64>(a, st);
-    return wide ? launch<__half, 128>(a, st) : launch<__half, 64>(a, st);
+#define CA_DECODE(T)                                                                                                   \
+    return a.formed ? (wide ? launch<T, 128, true>(a, st) : launch<T, 64, true>(a, st))                                \
+                    : (wide ? launch<T, 128, false>(a, st) : launch<T, 64, false>(a, st))
+    if (dtype == CA_F32) CA_DECODE(float);
+    if (dtype == CA_BF16) CA_DECODE(__nv_bfloat16);
+    CA_DECODE(__half);
+#undef CA_DECODE
 }
 
 }  // namespace ca

@@ -137,9 +137,10 @@ __device__ __forceinline__ float* row_ptr(const ca_seq_view& v, const SeqArgs& a
     const int t = token_of(a, R), g = R - t * a.G;
     return (float*)v.data + (h * a.G + g) * v.head + (int64_t)(s.t0 + t) * v.token + (a.pages.table ? 0 : s.b * v.batch);
 }
-// Key row j; clears `on` where it does not exist.
+// Key row j; clears `on` where it does not exist or is padding.
+template <bool FORM>
 __device__ __forceinline__ const float* key_ptr(const ca_seq_view& v, const ca_page_view& pv, const SeqArgs& a, const Seq& s, int h, int j, bool& on) {
-    on = on && j < s.n;
+    on = on && j < s.n && !padding<FORM>(a, s, j);
     if (!a.pages.table) return (const float*)v.data + h * v.head + (int64_t)j * v.token + s.b * v.batch;
     const int p = on ? page_of(a, s.b, j) : -1;
     on = on && p >= 0;
@@ -149,7 +150,7 @@ __device__ __forceinline__ const float* key_ptr(const ca_seq_view& v, const ca_p
 // ---------------------------------------------------------------- forward
 template <int DM> constexpr size_t kFwdSmem = (5 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
 
-template <int DM>
+template <int DM, bool FORM>
 __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
     float *Q = (float*)smem4, *KV = Q + kTileFloats<DM>, *Pm = KV + 4 * kTileFloats<DM>;      // K, V, K, V
@@ -172,33 +173,40 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
     const float* any = (const float*)a.q.data;
     fetch<DM>(Q, [&](int r, bool& on) {
         const int R = min(R0 + r, rows - 1), pos = s.base + token_of(a, R);
-        on = on && R0 + r < rows && pos >= 0 && pos < s.n;
+        on = on && R0 + r < rows && pos >= 0 && pos < s.n && !padding<FORM>(a, s, pos);
         return row_ptr(a.q, a, s, h, R);
     }, any, a.D, tid);
-    const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kTile);
+    const KeyTiles kt = key_tiles<FORM>(a, s, p_lo, p_hi, kTile);
+    const Reach lowest = tile_reach<FORM>(a, s, p_lo), highest = tile_reach<FORM>(a, s, p_hi);
     auto prefetch = [&](int it) {
         const int j0 = kt.key(it, kTile), b = it & 1;
         float* K = KV + 2 * b * kTileFloats<DM>;
         fetch<DM>(K, [&](int r, bool& on) {
             const bool whole = on;
-            const float* p = key_ptr(a.k, a.kp, a, s, h, j0 + r, on);
+            const float* p = key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on);
             if (tid % (DM / 4) == 0 && whole) gone[b][r] = !on;
             return p;
         }, any, a.D, tid);
         // rows of v that no query of this tile sees may hold anything: they count as zeros
         fetch<DM>(K + kTileFloats<DM>, [&](int r, bool& on) {
             const int j = j0 + r;
-            on = on && (j >= p_lo - a.left || j < a.sinks) && j <= (int64_t)p_hi + a.right;
-            return key_ptr(a.v, a.vp, a, s, h, j, on);
+            on = on && (j >= lowest.lo || j < a.sinks) && j <= highest.hi;
+            return key_ptr<FORM>(a.v, a.vp, a, s, h, j, on);
         }, any, a.D, tid);
     };
     int pos[4];
+    Reach mine[FORM ? 4 : 1];
+    float slope[FORM ? 4 : 1];
     float m[4], l[4];
     f32x2 o[4][DM / 32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int R = R0 + ty + 16 * i;
         pos[i] = R < rows ? s.base + token_of(a, R) : -1;
+        if constexpr (FORM) {
+            mine[i] = reach<FORM>(a, s, pos[i]);
+            slope[i] = R < rows ? slope_of(a, h * a.G + R - token_of(a, R) * a.G) : 0.f;
+        }
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
@@ -216,15 +224,22 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
         const float* K = KV + 2 * b * kTileFloats<DM>;
         float sc[4][4];
         dot_tile<DM>(Q, K, ty, tx, sc);
-        const bool edge = !(p_lo >= 0 && p_hi < s.n && j0 + kTile - 1 <= (int64_t)p_lo + a.right && j0 + kTile <= s.n &&
+        const bool edge = FORM || !(p_lo >= 0 && p_hi < s.n && j0 + kTile - 1 <= (int64_t)p_lo + a.right && j0 + kTile <= s.n &&
                             (j0 >= p_hi - a.left || j0 + kTile <= a.sinks)) || a.pages.table;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float top = m[i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                sc[i][j] *= a.scale_log2;
-                if (edge && (!sees(a, s.n, pos[i], j0 + tx + 16 * j) || gone[b][tx + 16 * j])) sc[i][j] = -INFINITY;
+                const int key = j0 + tx + 16 * j;
+                if constexpr (FORM) {
+                    float inner;
+                    sc[i][j] = formed_score(a, sc[i][j], slope[i], pos[i] - key, 0.f, inner);
+                    if (!sees(a, s.n, pos[i], mine[i], key) || gone[b][tx + 16 * j]) sc[i][j] = -INFINITY;
+                } else {
+                    sc[i][j] *= a.scale_log2;
+                    if (edge && (!sees(a, s.n, pos[i], key) || gone[b][tx + 16 * j])) sc[i][j] = -INFINITY;
+                }
                 top = fmaxf(top, sc[i][j]);
             }
             top = max16(top);
@@ -262,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
 // P = 2^(scale q.k log2 e - lse), dP = dy.v, dS = P (dP - delta), delta = dy.y; dq = scale dS k.
 template <int DM> constexpr size_t kDqSmem = (4 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
 
-template <int DM>
+template <int DM, bool FORM>
 __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
     float *Q = (float*)smem4, *O = Q + kTileFloats<DM>, *K = O + kTileFloats<DM>, *V = K + kTileFloats<DM>, *Pm = V + kTileFloats<DM>;
@@ -275,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
     auto from = [&](const ca_seq_view& v) {
         return [&](int r, bool& on) {
             const int R = min(R0 + r, rows - 1);
-            on = on && R0 + r < rows && token_of(a, R) < s.n;
+            on = on && R0 + r < rows && token_of(a, R) < s.n && !padding<FORM>(a, s, token_of(a, R));
             return (const float*)row_ptr(v, a, s, h, R);
         };
     };
@@ -284,15 +299,17 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
     float* yrow = V;                                              // y passes through the values' place
     fetch<DM>(yrow, from(a.y), any, a.D, tid);
     copies_commit();
-    const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, kTile);
+    const KeyTiles kt = key_tiles<FORM>(a, s, p_lo, p_hi, kTile);
     auto prefetch = [&](int it) {
         const int j0 = kt.key(it, kTile);
-        fetch<DM>(K, [&](int r, bool& on) { return key_ptr(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
-        fetch<DM>(V, [&](int r, bool& on) { return key_ptr(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
+        fetch<DM>(K, [&](int r, bool& on) { return key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
+        fetch<DM>(V, [&](int r, bool& on) { return key_ptr<FORM>(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
     };
     copies_wait<0>();
     __syncthreads();
     int pos[4];
+    Reach mine[FORM ? 4 : 1];
+    float slope[FORM ? 4 : 1];
     float lse[4], delta[4];
     f32x2 o[4][DM / 32];
 #pragma unroll
@@ -302,6 +319,10 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
         for (int f = tx; f < DM; f += 16) d = fmaf(O[r * kPitch<DM> + f], yrow[r * kPitch<DM> + f], d);
         delta[i] = sum16(d);
         pos[i] = R < rows ? token_of(a, R) : -1;
+        if constexpr (FORM) {
+            mine[i] = reach<FORM>(a, s, pos[i]);
+            slope[i] = R < rows ? slope_of(a, h * a.G + R - pos[i] * a.G) : 0.f;
+        }
         lse[i] = R < rows ? a.lse[stat0 + R] : 0.f;
         if (R < rows && tx == 0) a.delta[stat0 + R] = delta[i];
 #pragma unroll
@@ -322,8 +343,17 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bool see = !edge || sees(a, s.n, pos[i], j0 + tx + 16 * j);
-                Pm[(ty + 16 * i) * kPPitch + tx + 16 * j] = see ? fast_exp2(sc[i][j] * a.scale_log2 - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
+                const int key = j0 + tx + 16 * j;
+                float ds;
+                if constexpr (FORM) {
+                    float inner;
+                    const float z = formed_score(a, sc[i][j], slope[i], pos[i] - key, lse[i], inner);
+                    ds = sees(a, s.n, pos[i], mine[i], key) ? fast_exp2(z) * inner * (dp[i][j] - delta[i]) : 0.f;
+                } else {
+                    const bool see = !edge || sees(a, s.n, pos[i], key);
+                    ds = see ? fast_exp2(sc[i][j] * a.scale_log2 - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
+                }
+                Pm[(ty + 16 * i) * kPPitch + tx + 16 * j] = ds;
             }
         __syncwarp();
         acc_tile<DM>(Pm, K, ty, tx, o);
@@ -346,7 +376,7 @@ struct Parts {
     int tiles, segments;
 };
 
-template <int DM>
+template <int DM, bool FORM>
 __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(const __grid_constant__ SeqArgs a, const Parts parts) {
     extern __shared__ float4 smem4[];
     float *K = (float*)smem4, *V = K + kTileFloats<DM>, *Q = V + kTileFloats<DM>, *O = Q + kTileFloats<DM>, *Pm = O + kTileFloats<DM>, *Sm = Pm + kTile * kPPitch;
@@ -360,15 +390,28 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
     const int rows = s.T * a.G;
     const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
     const float* any = (const float*)a.q.data;
-    fetch<DM>(K, [&](int r, bool& on) { return key_ptr(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
-    fetch<DM>(V, [&](int r, bool& on) { return key_ptr(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
+    fetch<DM>(K, [&](int r, bool& on) { return key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
+    fetch<DM>(V, [&](int r, bool& on) { return key_ptr<FORM>(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
     f32x2 dk[4][DM / 32], dv[4][DM / 32];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < DM / 32; ++c) dk[i][c] = dv[i][c] = 0;
-    const int t_lo = max(0, j0 - a.right);
-    const int t_hi = j0 >= s.n ? t_lo : j0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)j0 + kTile + a.left);
+    int t_lo = max(0, j0 - a.right);
+    int t_hi = j0 >= s.n ? t_lo : j0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)j0 + kTile + a.left);
+    Reach by[FORM ? 4 : 1];                                       // queries that see the thread's keys
+    if constexpr (FORM) {
+        if (a.form.spans && j0 < s.n) {
+            t_lo = max(0, min(seen_by(a, s, j0).lo, j0));
+            t_hi = max(j0, min(seen_by(a, s, min(j0 + kTile, s.n) - 1).hi, s.n - 1)) + 1;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = j0 + ty + 16 * i;
+            by[i] = a.form.spans ? seen_by(a, s, j) : Reach{j - a.right, j < a.sinks ? s.n - 1 : j + a.left};
+            if (j >= s.n) by[i] = Reach{0, -1};
+        }
+    }
     const int lo = t_lo * a.G, hi = max(t_lo, t_hi) * a.G, all = (hi - lo + kTile - 1) / kTile;
     const int first = split ? (int)((int64_t)all * seg / parts.segments) : 0;
     const int count = (split ? (int)((int64_t)all * (seg + 1) / parts.segments) : all) - first;
@@ -376,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
         const int R0 = lo + (first + it) * kTile;
         auto from = [&](const ca_seq_view& v) {
             return [&](int r, bool& on) {
-                on = on && R0 + r < hi;
+                on = on && R0 + r < hi && !padding<FORM>(a, s, token_of(a, min(R0 + r, hi - 1)));
                 return (const float*)row_ptr(v, a, s, h, min(R0 + r, hi - 1));
             };
         };
@@ -403,11 +446,20 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int R = R0 + tx + 16 * c;
-                const bool see = !edge || (R < hi && sees(a, s.n, token_of(a, R), j0 + ty + 16 * i));
-                const float p = see ? fast_exp2(sc[i][c] * a.scale_log2 - s_lse[tx + 16 * c]) : 0.f;
+                const int R = R0 + tx + 16 * c, key = j0 + ty + 16 * i;
+                float z, inner = 1.f;
+                bool see;
+                if constexpr (FORM) {
+                    const int token = token_of(a, R);
+                    see = R < hi && token < s.n && token >= by[i].lo && token <= by[i].hi;
+                    z = formed_score(a, sc[i][c], R < hi ? slope_of(a, h * a.G + R - token * a.G) : 0.f, token - key, s_lse[tx + 16 * c], inner);
+                } else {
+                    see = !edge || (R < hi && sees(a, s.n, token_of(a, R), key));
+                    z = sc[i][c] * a.scale_log2 - s_lse[tx + 16 * c];
+                }
+                const float p = see ? fast_exp2(z) : 0.f;
                 Pm[(ty + 16 * i) * kPPitch + tx + 16 * c] = p;
-                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? p * (dp[i][c] - s_delta[tx + 16 * c]) : 0.f;
+                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? p * inner * (dp[i][c] - s_delta[tx + 16 * c]) : 0.f;
             }
         __syncwarp();
         acc_tile<DM>(Pm, O, ty, tx, dv);
@@ -458,26 +510,26 @@ int raise_smem(K kernel, size_t bytes) {
     return e == cudaSuccess ? CA_OK : cuda_fail(e, "cudaFuncSetAttribute");
 }
 
-template <int DM>
+template <int DM, bool FORM>
 int launch_fwd(const SeqArgs& a, cudaStream_t st) {
-    const int rc = raise_smem(fma_fwd_kernel<DM>, kFwdSmem<DM>);
+    const int rc = raise_smem(fma_fwd_kernel<DM, FORM>, kFwdSmem<DM>);
     if (rc) return rc;
     const int64_t tiles = a.pages.table ? paged_tiles(a.N, a.G, a.pages.sequences, kTile) : ((int64_t)a.N * a.G + kTile - 1) / kTile;
-    fma_fwd_kernel<DM><<<dim3((unsigned)tiles, a.Hkv, a.B), kThreads, kFwdSmem<DM>, st>>>(a);
+    fma_fwd_kernel<DM, FORM><<<dim3((unsigned)tiles, a.Hkv, a.B), kThreads, kFwdSmem<DM>, st>>>(a);
     CA_CHECK_LAUNCH("window forward kernel");
     return CA_OK;
 }
 
-template <int DM>
+template <int DM, bool FORM>
 int launch_bwd(const SeqArgs& a, float* data, cudaStream_t st) {
-    int rc = raise_smem(fma_dq_kernel<DM>, kDqSmem<DM>);
-    if (rc || (rc = raise_smem(fma_dkdv_kernel<DM>, kDkdvSmem<DM>))) return rc;
+    int rc = raise_smem(fma_dq_kernel<DM, FORM>, kDqSmem<DM>);
+    if (rc || (rc = raise_smem(fma_dkdv_kernel<DM, FORM>, kDkdvSmem<DM>))) return rc;
     const Dealt p = deal_first_tokens(a, kTile);
     const Parts parts{data, p.tiles, p.segments};
-    fma_dq_kernel<DM><<<dim3((unsigned)(((int64_t)a.N * a.G + kTile - 1) / kTile), a.Hkv, a.B), kThreads, kDqSmem<DM>, st>>>(a);
+    fma_dq_kernel<DM, FORM><<<dim3((unsigned)(((int64_t)a.N * a.G + kTile - 1) / kTile), a.Hkv, a.B), kThreads, kDqSmem<DM>, st>>>(a);
     CA_CHECK_LAUNCH("window dq kernel");
     const int tiles = (a.N + kTile - 1) / kTile;
-    fma_dkdv_kernel<DM><<<dim3(tiles - parts.tiles + parts.tiles * parts.segments, a.Hkv, a.B), kThreads, kDkdvSmem<DM>, st>>>(a, parts);
+    fma_dkdv_kernel<DM, FORM><<<dim3(tiles - parts.tiles + parts.tiles * parts.segments, a.Hkv, a.B), kThreads, kDkdvSmem<DM>, st>>>(a, parts);
     CA_CHECK_LAUNCH("window dk/dv kernel");
     if (parts.tiles) {
         fma_join_kernel<DM><<<dim3(8 * parts.tiles, a.Hkv, a.B), 256, 0, st>>>(a, parts);
@@ -493,7 +545,13 @@ size_t fma_bwd_parts(const SeqArgs& a) {
     return (size_t)p.tiles * p.segments * 2 * kTile * (a.D > 64 ? 128 : 64) * a.Hkv * a.B * sizeof(float);
 }
 
-int fma_fwd(const SeqArgs& a, cudaStream_t st) { return a.D > 64 ? launch_fwd<128>(a, st) : launch_fwd<64>(a, st); }
-int fma_bwd(const SeqArgs& a, float* parts, cudaStream_t st) { return a.D > 64 ? launch_bwd<128>(a, parts, st) : launch_bwd<64>(a, parts, st); }
+int fma_fwd(const SeqArgs& a, cudaStream_t st) {
+    if (a.formed) return a.D > 64 ? launch_fwd<128, true>(a, st) : launch_fwd<64, true>(a, st);
+    return a.D > 64 ? launch_fwd<128, false>(a, st) : launch_fwd<64, false>(a, st);
+}
+int fma_bwd(const SeqArgs& a, float* parts, cudaStream_t st) {
+    if (a.formed) return a.D > 64 ? launch_bwd<128, true>(a, parts, st) : launch_bwd<64, true>(a, parts, st);
+    return a.D > 64 ? launch_bwd<128, false>(a, parts, st) : launch_bwd<64, false>(a, parts, st);
+}
 
 }  // namespace ca

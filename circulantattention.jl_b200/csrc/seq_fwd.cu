@@ -55,13 +55,13 @@ struct Stream {
     }
 };
 
-template <bool PAIR>
+template <bool PAIR, bool FORM>
 __device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, const KeyTiles& kt, int u, int r, int rows) {
     Stream t;
     t.lo = max(0, s.base + r / a.G);
     t.hi = r < rows ? min(s.n - 1, s.base + (min(r + 128, rows) - 1) / a.G) : -1;
-    t.begin_key = max(0, t.lo - a.left);
-    t.end_key = (int)min((int64_t)key_limit(a, s) - 1, (int64_t)t.hi + a.right);
+    t.begin_key = max(0, tile_reach<FORM>(a, s, t.lo).lo);
+    t.end_key = min(key_limit(a, s) - 1, t.hi < 0 ? -1 : tile_reach<FORM>(a, s, t.hi).hi);
     if (!PAIR) {
         t.first = 0;
         t.from = u;
@@ -85,11 +85,12 @@ __device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, cons
     }
     t.from = kt.first + max(0, t.begin_key - kt.lo) / 128;
     t.upto = t.end_key >= kt.lo ? kt.first + (t.end_key - kt.lo) / 128 : kt.first - 1;
+    if (FORM) t.upto = min(t.upto, kt.count - 1);
     t.first = max(kt.first, min(min(t.from, t.upto + 1), firsts));
     return t;
 }
 
-template <typename T, int DM, bool PAIR, bool PAGED>
+template <typename T, int DM, bool PAIR, bool PAGED, bool FORM>
 __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ FwdMaps maps) {
     constexpr int S = kSlots<DM>;
     constexpr uint32_t TILE = kTileBytes<DM>;
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     __shared__ uint64_t kv_full[S], kv_empty[S], q_full[2], s_full[2], p_full[2][2], o_full[2], drained;
     __shared__ uint32_t tmem_slot, valid[S];
     __shared__ int stop_flag;
-    __shared__ float merge_m[128], merge_l[128];
+    __shared__ float merge_m[128], merge_l[128], merge_r[FORM ? 128 : 1];
     volatile int* stop = &stop_flag;
 
     const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
@@ -120,10 +121,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     }
     const int rows = s.T * a.G, R0 = tile * (PAIR ? 256 : 128);
     const int p_lo = max(0, s.base + R0 / a.G), p_hi = min(s.n - 1, s.base + (min(R0 + (PAIR ? 256 : 128), rows) - 1) / a.G);
-    const KeyTiles kt = key_tiles(a, s, p_lo, p_hi, 128);
+    const KeyTiles kt = key_tiles<FORM>(a, s, p_lo, p_hi, 128);
 
     // Which key tiles a stream takes: with PAIR both see nearly the same, but each leaves out what all of its rows are blind to.
-    const Stream st0 = stream_of<PAIR>(a, s, kt, 0, R0, rows), st1 = stream_of<PAIR>(a, s, kt, 1, PAIR ? R0 + 128 : R0, rows);
+    const Stream st0 = stream_of<PAIR, FORM>(a, s, kt, 0, R0, rows), st1 = stream_of<PAIR, FORM>(a, s, kt, 1, PAIR ? R0 + 128 : R0, rows);
 
     if (warp == 8 && lane == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
@@ -187,17 +188,21 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         }
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;              // lane 32 * (warp % 4) in bits 16..
         const uint32_t S_at = s_col + u * 128 + lane_off, P_at = p_col + u * p_step + lane_off, O_at = o_col + u * DM + lane_off;
-        const float sl2 = a.mag_log2;
-        const int c_lo = p_lo - a.left, c_hi = min(p_hi + a.right, s.n - 1);   // keys that any row of the CTA sees (or < sinks)
+        const bool changed = FORM && a.form.changed;                           // scores return to tensor memory in units of log2(e)
+        const float sl2 = changed ? 1.f : a.mag_log2;
+        const float slope = FORM && changed ? slope_of(a, h * a.G + R - token_of(a, R) * a.G) : 0.f, cap_in = fabsf(a.form.cap_in);
+        const Reach mine = reach<FORM>(a, s, pos);
+        const int c_lo = tile_reach<FORM>(a, s, p_lo).lo, c_hi = min(tile_reach<FORM>(a, s, p_hi).hi, s.n - 1);   // keys that any row of the CTA sees (or < sinks)
         // tiles from in_lo (or below in_sink) to in_hi need no mask
         const bool whole = st.lo == s.base + (R - r) / a.G && st.hi == s.base + (min(R - r + 128, rows) - 1) / a.G;
-        const int in_hi = whole ? min(st.lo + a.right, s.n - 1) - 127 : INT_MIN, in_lo = st.hi - a.left, in_sink = a.sinks - 127;
-        float m = -INFINITY, l = 0.f;
+        const int in_hi = whole ? min(reach<FORM>(a, s, st.lo).hi, s.n - 1) - 127 : INT_MIN, in_lo = reach<FORM>(a, s, st.hi).lo, in_sink = a.sinks - 127;
+        float m = -INFINITY, l = 0.f, lr = 0.f;            // FORM: lr is the sum of the rounded weights
         int done = 0;
         bool ok = true;
         if (PAGED) clear_unowned<T>(a, owned, h, tid, 32 * kSoftmaxWarps);
         for (int i = st.begin(); i <= st.upto; i = st.next(i)) {
             const int key0 = kt.key(i, 128), vslot = (2 * i + 1) % S;
+            const bool pads = mixed<FORM>(a, s, key0, key0 + 127);
             const uint32_t vpar = ((2 * i + 1) / S) & 1;
             if (!warp_wait(smem_u32(&s_full[u]), done & 1, stop)) { ok = false; break; }
             fence_after();
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             }
             const int far = key0 + 127;
             const bool edge = !(key0 <= in_hi && (key0 >= in_lo || key0 < in_sink) && there == 0xff);
-            const int hi = live ? min(pos + a.right, s.n - 1) - key0 : -1, lo = pos - a.left - key0, sk = a.sinks - key0;
+            const int hi = live ? min(mine.hi, s.n - 1) - key0 : -1, lo = mine.lo - key0, sk = a.sinks - key0;
             auto scores = [&](int g, uint32_t* x) {                        // the columns 64 g .. 64 g + 63
                 tmem_ld32(S_at + 64 * g, x);
                 tmem_ld32(S_at + 64 * g + 32, x + 32);
@@ -219,23 +224,26 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             // The same for the maximum: -inf where the row does not see the key, written back for the exponentials
             auto masked_scores = [&](int g, uint32_t* x) {
                 scores(g, x);
-                if (edge) {
+                if (edge || (FORM && changed)) {
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const int at = 64 * g + 32 * q;
                         uint32_t mk = seen_bits(lo - at, hi - at, sk - at);
                         if (PAGED) mk &= ((there >> (at / 16)) & 1 ? 0xffffu : 0u) | ((there >> (at / 16 + 1)) & 1 ? 0xffff0000u : 0u);
+                        if (FORM && changed) form_scores<T, 32, false>(x + 32 * q, nullptr, a, a.mag_log2, cap_in, slope, (float)(pos - key0 - at), edge, mk);
+                        if (!FORM || edge) {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) x[32 * q + c] = (mk >> c) & 1 ? x[32 * q + c] : 0xff800000u;
+                            for (int c = 0; c < 32; ++c) x[32 * q + c] = (mk >> c) & 1 ? x[32 * q + c] : 0xff800000u;
+                        }
                         tmem_st32(S_at + at, x + 32 * q);
                     }
                 }
             };
             // values that no row sees may be anything (a page that was freed, tokens behind the length): zeros
-            if (!((key0 >= c_lo || far < a.sinks) && far <= c_hi && there == 0xff)) {
+            if (!((key0 >= c_lo || far < a.sinks) && far <= c_hi && there == 0xff) || pads) {
                 if (!PAGED && !warp_wait(smem_u32(&kv_full[vslot]), vpar, stop)) { ok = false; break; }
                 const int j = key0 + r;
-                if (!(j <= c_hi && (j >= c_lo || j < a.sinks) && (there >> (r >> 4) & 1))) {
+                if (!(j <= c_hi && (j >= c_lo || j < a.sinks) && (there >> (r >> 4) & 1)) || (pads && padding<FORM>(a, s, j))) {
 #pragma unroll 1
                     for (int p = 0; p < DM / 64; ++p)
 #pragma unroll
@@ -280,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             }
             const float ref = m == -INFINITY ? 0.f : m;                    // a row that has seen nothing yet
             const f32x2 sc2 = pack2(sl2, sl2), ref2 = pack2(-ref, -ref);
-            f32x2 sum2 = pack2(l * f, 0.f);
+            f32x2 sum2 = pack2(l * f, 0.f), round2 = pack2(lr * f, 0.f);
 #pragma unroll 1
             for (int g = 0; g < 2; ++g) {
                 if (!st.sees_half(a, key0 + 64 * g)) continue;
@@ -300,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     }
                     sum2 = add2(sum2, pack2(e0, e1));
                     w[c] = pack16<T>(e0, e1);
+                    if (FORM) round2 = add2(round2, pack2(low16<T>(w[c]), high16<T>(w[c])));
                 }
                 tmem_st32(P_at + 32 * g, w);                               // at 128 features over scores that this warp has read twice
                 tmem_wait_st();
@@ -310,6 +319,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             float a0, a1;
             unpack2(sum2, a0, a1);
             l = a0 + a1;
+            if (FORM) {
+                unpack2(round2, a0, a1);
+                lr = a0 + a1;
+            }
             ++done;
         }
         if (done && ok) ok = warp_wait(smem_u32(&o_full[u]), 0, stop);
@@ -326,6 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             if (u == 1) {
                 merge_m[r] = m;
                 merge_l[r] = l;
+                if (FORM) merge_r[r] = lr;
                 if (done && ok) {
 #pragma unroll 1
                     for (int c = 0; c < DM; c += 32) {
@@ -343,10 +357,15 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             f0 = fast_exp2(m - ref);
             f1 = fast_exp2(m1 - ref);
             l = l * f0 + l1 * f1;
+            if (FORM) lr = lr * f0 + merge_r[r] * f1;
             m = M;
         }
         if (PAIR || u == 0) {
-            float inv = l > 0.f ? 1.f / l : 0.f;
+            // The weighted sum is divided by the sum of the weights as they were rounded: where a few keys have most of the weight,
+            // their rounding nearly cancels, and so it does in delta = dy.y, which the backward subtracts from each dy.v (capped
+            // scores of standard deviation 8: gradients off by 2.5e-3 of the norm in bfloat16, 3.5e-3 by the other sum).
+            const float total = FORM ? lr : l;
+            float inv = total > 0.f ? 1.f / total : 0.f;
             if (!ok || *stop) inv = __int_as_float(0x7fffffff);            // a wait ran out: NaN, never a wrong number
             // Rows that see nothing are zeros by choice, not by their weights: 0 * inf of a value that other rows see is not a number.
             const bool none = !done || l == 0.f, both = !PAIR && kt.count > 1 && !none;
@@ -500,8 +519,15 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             scores(u, i);
             return true;
         };
-        ok = begin(0) && begin(1);
+        // The second stream's rows may be of a document that begins many tiles behind the first stream's: its first keys are
+        // waited for one tile ahead, when the ring has come to them.
+        bool late = FORM && PAIR && st1.begin() > 1;
+        ok = begin(0) && (late || begin(1));
         for (int i = 0; i < kt.count && ok; ++i) {
+            if (late && st1.begin() <= i + 1) {
+                late = false;
+                if (!(ok = begin(1))) break;
+            }
             if (st0.takes(i)) ok = weighted(0, i, n0);
             if (ok && st1.takes(i)) ok = weighted(1, i, n1);
         }
@@ -517,22 +543,22 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     if (tid == 0 && stop_flag) report_stop(maps.timeouts, a.status);
 }
 
-template <typename T, int DM, bool PAIR, bool PAGED>
+template <typename T, int DM, bool PAIR, bool PAGED, bool FORM>
 int launch(const SeqArgs& a, const FwdMaps& maps, dim3 grid, cudaStream_t st) {
-    const cudaError_t e = cudaFuncSetAttribute(umma_fwd_kernel<T, DM, PAIR, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFwdSmem<DM>);
+    const cudaError_t e = cudaFuncSetAttribute(umma_fwd_kernel<T, DM, PAIR, PAGED, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFwdSmem<DM>);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-    umma_fwd_kernel<T, DM, PAIR, PAGED><<<grid, kThreads, kFwdSmem<DM>, st>>>(a, maps);
+    umma_fwd_kernel<T, DM, PAIR, PAGED, FORM><<<grid, kThreads, kFwdSmem<DM>, st>>>(a, maps);
     count_tensor_launch();
     CA_CHECK_LAUNCH("window forward kernel (tensor cores)");
     return CA_OK;
 }
 
-template <bool PAGED>
+template <bool PAGED, bool FORM>
 int launch_any(const SeqArgs& a, const FwdMaps& maps, int dtype, bool pair, dim3 grid, cudaStream_t st) {
     const bool wide = a.D > 64;
 #define CA_FWD(T)                                                                                                             \
-    return wide ? (pair ? launch<T, 128, true, PAGED>(a, maps, grid, st) : launch<T, 128, false, PAGED>(a, maps, grid, st))   \
-                : (pair ? launch<T, 64, true, PAGED>(a, maps, grid, st) : launch<T, 64, false, PAGED>(a, maps, grid, st))
+    return wide ? (pair ? launch<T, 128, true, PAGED, FORM>(a, maps, grid, st) : launch<T, 128, false, PAGED, FORM>(a, maps, grid, st))   \
+                : (pair ? launch<T, 64, true, PAGED, FORM>(a, maps, grid, st) : launch<T, 64, false, PAGED, FORM>(a, maps, grid, st))
     if (dtype == CA_BF16) CA_FWD(__nv_bfloat16);
     CA_FWD(__half);
 #undef CA_FWD
@@ -602,7 +628,8 @@ int umma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st) {
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
     const int64_t rows = (int64_t)a.N * a.G;
     const bool pair = (rows + 255) / 256 * a.Hkv * a.B >= sm_count();
-    return launch_any<false>(a, maps, dtype, pair, dim3((unsigned)((rows + (pair ? 255 : 127)) / (pair ? 256 : 128)), a.Hkv, a.B), st);
+    const dim3 grid((unsigned)((rows + (pair ? 255 : 127)) / (pair ? 256 : 128)), a.Hkv, a.B);
+    return a.formed ? launch_any<false, true>(a, maps, dtype, pair, grid, st) : launch_any<false, false>(a, maps, dtype, pair, grid, st);
 }
 
 int umma_paged(const SeqArgs& a, int dtype, cudaStream_t st) {
@@ -625,7 +652,8 @@ int umma_paged(const SeqArgs& a, int dtype, cudaStream_t st) {
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
     const bool pair = paged_tiles(a.N, a.G, a.pages.sequences, 256) * a.Hkv >= sm_count() && (int64_t)a.N * a.G > 128LL * a.pages.sequences;
     const int64_t tiles = paged_tiles(a.N, a.G, a.pages.sequences, pair ? 256 : 128);
-    return launch_any<true>(a, maps, dtype, pair, dim3((unsigned)tiles, a.Hkv, 1), st);
+    const dim3 grid((unsigned)tiles, a.Hkv, 1);
+    return a.formed ? launch_any<true, true>(a, maps, dtype, pair, grid, st) : launch_any<true, false>(a, maps, dtype, pair, grid, st);
 }
 
 }  // namespace ca

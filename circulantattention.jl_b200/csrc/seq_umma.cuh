@@ -63,6 +63,58 @@ __device__ __forceinline__ void settled32(uint32_t* r) {
         asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
+// COUNT neighbouring columns of a row: from q.k to scores in units of log2(e), capped, less slope times the distance |d0 - c| of
+// column c.  INNER: also the cap's derivative 1 - tanh^2.  The polynomial serves |score| <= cap; a warp that holds a larger one
+// takes two passes of the exponential unit an element, 1.5e-7 of the cap off.  Columns that the row does not see (`edge`: those
+// whose bit in mk is not set) have no say in this.  The warp calls it together.
+template <typename T, int COUNT, bool INNER>
+__device__ __forceinline__ void form_scores(uint32_t* x, float* inner, const SeqArgs& a, float scale_log2, float cap_in, float slope, float d0, bool edge, uint32_t mk) {
+    constexpr int DEGREE = kIsBf16<T> ? 4 : 5;
+    typedef TanhPoly<DEGREE> P;
+    if (a.form.cap_out != 0.f) {
+        float big = 0.f;
+        if (edge) {
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) big = fmaxf(big, (mk >> c) & 1 ? fabsf(__uint_as_float(x[c])) : 0.f);
+        } else {
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) big = fmaxf(big, fabsf(__uint_as_float(x[c])));
+        }
+        const f32x2 in2 = pack2(cap_in, cap_in), out2 = pack2(a.form.cap_out, a.form.cap_out), one2 = pack2(1.f, 1.f);
+        if (__any_sync(~0u, big * fabsf(cap_in) > 1.f)) {
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) {
+                const float t = tanh_far(__uint_as_float(x[c]) * cap_in);
+                x[c] = __float_as_uint(t * a.form.cap_out);
+                if (INNER) inner[c] = fmaf(-t, t, 1.f);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < COUNT; c += 2) {
+                const f32x2 X = mul2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), in2), u = mul2(X, X);
+                f32x2 p = pack2(P::at(DEGREE), P::at(DEGREE));
+#pragma unroll
+                for (int i = DEGREE - 1; i >= 0; --i) p = fma2(p, u, pack2(P::at(i), P::at(i)));
+                const f32x2 t = mul2(p, X);
+                float z0, z1;
+                unpack2(mul2(t, out2), z0, z1);
+                x[c] = __float_as_uint(z0);
+                x[c + 1] = __float_as_uint(z1);
+                if (INNER) unpack2(fma2(mul2(t, pack2(-1.f, -1.f)), t, one2), inner[c], inner[c + 1]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) {
+            x[c] = __float_as_uint(__uint_as_float(x[c]) * scale_log2);
+            if (INNER) inner[c] = 1.f;
+        }
+    }
+    if (a.form.slopes) {
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(fmaf(-slope, fabsf(d0 - (float)c), __uint_as_float(x[c])));
+    }
+}
 // Tiles between global and shared memory: consecutive threads take consecutive 16-byte pieces of a row, so that a warp covers
 // two to four whole rows at a time (a thread for each row would touch 32 lines an instruction: 4096 cycles a tile of 128 rows,
 // and three such tiles made the prologue of dq 10 us).  `row(r)`: address of row r.  Rows

@@ -76,23 +76,43 @@ def _left(left):
     return int(left)
 
 
-def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, scale=None):
-    """y_i = sum_j softmax_j(scale * q_i . k_j) v_j over the tokens j that token i sees: those from i - left to i + right,
-    and the first `sinks` ones as long as they are not later than i + right.  Differentiable in q, k, v; deterministic.
+def token_spans(documents, groups=None):
+    """Document and prefix masks for `window_attention`: which tokens each token sees, from numbers that say what it belongs to.
+
+    documents: Int32 `(N, B)` or `(N,)`.  A document is a run of equal numbers; tokens see their own document only.  Negative
+    numbers are padding, which sees nothing and is seen by nothing.  groups: the same size; a group is a run of equal positive
+    numbers within a document, whose tokens see each other both ways (the prefix of a prompt, a picture between text, a whole
+    document); all others see up to themselves.  The result, Int32 `(4, N, B)`, serves the calls of all layers on this batch."""
+    return host.token_spans(documents, groups)
+
+
+def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, scale=None, cap=None, slopes=None, spans=None):
+    """y_i = sum_j softmax_j(score_ij) v_j over the tokens j that token i sees: those from i - left to i + right, and the first
+    `sinks` ones as long as they are not later than i + right.  Differentiable in q, k, v; deterministic.
 
     q `(D, heads, N, B)`, k and v `(D, heads', N, B)` with heads a multiple of heads'; D a multiple of 8 up to 128.
     left=None: no left end.  lengths: Int32 `(B,)`, the tokens that exist in each sequence (what lies behind them has no
-    effect, whatever it holds; y and the gradients are zero there).  scale: 1/sqrt(D) by default.
+    effect, whatever it holds; y and the gradients are zero there).
+
+    The score is scale * q_i . k_j, scale 1/sqrt(D) by default.  cap: it becomes cap * tanh(score / cap).  slopes: Float32
+    `(heads,)`, slopes[head] * |i - j| is taken from it after the cap; no gradient.  spans: what `token_spans` says of the
+    tokens' documents and groups takes the place of `right` and `sinks`, which are 0 then: token i sees those of its document
+    from i - left to i or, if that is further, to the end of its group.
 
     Infinities and NaN in keys or values that no token sees have no effect.  Where some token sees them, neighbours that do
     not may get NaN too: their weight is zero, and zero times infinity is not a number."""
-    return host.window_attention(q, k, v, _left(left), int(right), int(sinks), lengths, scale)
+    return host.window_attention(q, k, v, _left(left), int(right), int(sinks), lengths, scale, cap, slopes, spans)
 
 
-def paged_window_attention(q, k_pages, v_pages, table, starts, lengths, left=None, sinks=0, scale=None):
+def paged_window_attention(q, k_pages, v_pages, table, starts, lengths, left=None, sinks=0, scale=None, cap=None, slopes=None,
+                           prefix=None):
     """`window_attention` (right = 0) of a chunk of new tokens for each sequence over a paged cache that holds their keys
     and values already (see `rotary_append_` for the layout).  Returns y `(D, heads, T)`.
 
+    cap, slopes: as there.  prefix: Int32 `(S,)`, the first prefix[s] tokens of sequence s are visible to all of its tokens,
+    later ones among them, as far as the window's left end leaves them and the cache holds them.
+
     Tokens that no new token sees are not read, so the pages behind the window may be freed: any page number, -1 among
     them, may stand in their place in the table.  A missing page (-1) inside the window is skipped.  No gradients."""
-    return host.paged_window_attention(q, k_pages, v_pages, table, starts, lengths, _left(left), int(sinks), scale)
+    return host.paged_window_attention(q, k_pages, v_pages, table, starts, lengths, _left(left), int(sinks), scale, cap, slopes,
+                                       prefix)

@@ -103,6 +103,37 @@ int ca_window_bwd(const ca_seq_desc* d, const ca_seq_view* q, const ca_seq_view*
 int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_view* k_pages, const ca_page_view* v_pages,
                     const ca_pages* pages, const ca_seq_view* y, void* stream);
 
+/* ---------------------------------------------------------------- the same with other scores and masks
+ * Scores are cap * tanh(scale * q.k / cap) where there is a cap, less slopes[query head] * |i - j| where there are slopes.
+ *
+ * spans (dense calls): what each token sees, made once a batch by ca_token_spans for the calls of all layers.  With spans the
+ * key j is visible to the query i when both are below the sequence's length, they are of one document, j >= i - left (or
+ * left < 0), and j <= i or both are of one group; right and sinks are 0.
+ *
+ * prefix (calls over a cache): prefix[s] tokens of sequence s are visible to all of its tokens, whether they come later or
+ * not, as far as the window's left end leaves them. */
+typedef struct ca_seq_form {
+    float cap;                /* 0: scores as they are */
+    const float* slopes;      /* heads_q, nullable */
+    const int32_t* spans;     /* (4, N, B), 16-byte aligned, nullable */
+    const int32_t* prefix;    /* (sequences), nullable */
+} ca_seq_form;
+
+/* From the number of each token's document and group to spans.  A document is a run of equal numbers that are not negative,
+ * negative numbers are padding, which sees nothing and is seen by nothing; a group is a run of equal positive numbers within a
+ * document.  documents, groups (nullable): (N, B); spans: (4, N, B), for each token the first one that it sees, the first one
+ * that sees it, the last one that it sees, the last one that sees it. */
+int ca_token_spans(const int32_t* documents, const int32_t* groups, int32_t tokens, int32_t batch, int32_t* spans, void* stream);
+
+int ca_window_form_fwd(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+                       const int32_t* lengths, const ca_seq_view* y, const ca_seq_view* y_rest, float* lse, void* stream);
+/* Takes a workspace of ca_window_bwd_workspace(d) bytes.  There is no gradient of the slopes. */
+int ca_window_form_bwd(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_seq_view* k, const ca_seq_view* v,
+                       const ca_seq_view* y, const ca_seq_view* y_rest, const ca_seq_view* dy, const int32_t* lengths, const float* lse,
+                       const ca_seq_view* dq, const ca_seq_view* dk, const ca_seq_view* dv, void* workspace, void* stream);
+int ca_paged_window_form(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_page_view* k_pages,
+                         const ca_page_view* v_pages, const ca_pages* pages, const ca_seq_view* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
