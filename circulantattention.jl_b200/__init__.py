@@ -19,5 +19,6 @@ from .api import (  # noqa: F401
     spatial_dims, spatial_size, splitheads, sum,
 )
 from .tokens import (  # noqa: F401
-    paged_window_attention, rotary, rotary_append_, rotary_turns, token_spans, window_attention,
+    advance_pages, compact_pages, fork_pages, paged_window_attention, rotary, rotary_append_, rotary_turns, token_spans,
+    window_attention,
 )

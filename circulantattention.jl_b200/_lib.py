@@ -73,6 +73,16 @@ class ca_seq_form(C.Structure):
     _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p), ("spans", C.c_void_p), ("prefix", C.c_void_p)]
 
 
+class ca_table(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("refs", C.c_void_p), ("lengths", C.c_void_p), ("width", C.c_int32),
+                ("sequences", C.c_int32), ("page", C.c_int32), ("pages", C.c_int32)]
+
+
+class ca_pool(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token", C.c_int64), ("head", C.c_int64), ("page", C.c_int64), ("row", C.c_int32),
+                ("tokens", C.c_int32), ("heads", C.c_int32)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -87,7 +97,7 @@ _p = C.c_void_p
 _D = C.POINTER(ca_desc)
 _V, _G = C.POINTER(ca_seq_view), C.POINTER(ca_page_view)
 _R, _S, _P = C.POINTER(ca_rotary_desc), C.POINTER(ca_seq_desc), C.POINTER(ca_pages)
-_F = C.POINTER(ca_seq_form)
+_F, _T, _L = C.POINTER(ca_seq_form), C.POINTER(ca_table), C.POINTER(ca_pool)
 _i32, _i64, _f32 = C.c_int32, C.c_int64, C.c_float
 
 PROTOTYPES = {
@@ -134,6 +144,10 @@ PROTOTYPES = {
     "ca_window_form_fwd": (C.c_int, [_S, _F, _V, _V, _V, _p, _V, _V, _p, _p]),
     "ca_window_form_bwd": (C.c_int, [_S, _F] + [_V] * 6 + [_p, _p] + [_V] * 3 + [_p, _p]),
     "ca_paged_window_form": (C.c_int, [_S, _F, _V, _G, _G, _P, _V, _p]),
+    "ca_pages_workspace": (C.c_size_t, [_T]),
+    "ca_advance_pages": (C.c_int, [_T, _p, _i32, _i32, _p, _p, _p, _p, _p]),
+    "ca_fork_pages": (C.c_int, [_T, _p, _L, _i32, _p, _p, _p, _p, _p, _p]),
+    "ca_compact_pages": (C.c_int, [_T, _L, _i32, _p, _p, _p, _p, _p]),
     "ca_probe_launch_count": (C.c_int64, []),
     "ca_probe_tiled_launch_count": (C.c_int64, []),
     "ca_probe_tensor_launch_count": (C.c_int64, []),

@@ -299,6 +299,76 @@ Tensor paged_window(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pag
     return y;
 }
 
+// ---------------------------------------------------------------- the pages of a cache
+ca_table table_of(const Tensor& table, const Tensor& refs, const Tensor& lengths, int64_t page) {
+    require_cuda(table);
+    require_ints(table, table, at::kInt, "table");
+    require_ints(refs, table, at::kInt, "refs");
+    if (table.dim() != 2 || refs.dim() != 1) mismatch("table of size " + shape_text(table) + ", refs of size " + shape_text(refs) + ": (width, S) and (pages) expected");
+    if ((table.numel() && !is_colmajor(table)) || !refs.is_contiguous()) mismatch("table and refs must be dense (table column-major)");
+    if (lengths.defined()) {
+        require_ints(lengths, table, at::kInt, "lengths");
+        if (lengths.dim() != 1 || lengths.size(0) != table.size(1) || !lengths.is_contiguous()) mismatch("lengths of size " + shape_text(lengths) + ": one for each sequence expected");
+    }
+    return ca_table{static_cast<const int32_t*>(ptr(table)), static_cast<const int32_t*>(ptr(refs)), static_cast<const int32_t*>(ptr(lengths)),
+                    int_of(table.size(0), "width"), int_of(table.size(1), "S"), int_of(page, "page"), int_of(refs.size(0), "pages")};
+}
+
+// Their strides in bytes; pools are written in place, so that they have to lie as they are needed.
+std::vector<ca_pool> pools_of(const std::vector<Tensor>& pools, const Tensor& table, const Tensor& refs) {
+    if (pools.empty()) mismatch("no pools: at least one tensor (D, page, heads, pages) expected");
+    std::vector<ca_pool> out;
+    for (const Tensor& p : pools) {
+        require_cuda(p);
+        if (p.device() != table.device()) raise(PyExc_RuntimeError, "a pool is on " + p.device().str() + ", not on " + table.device().str());
+        if (p.dim() != 4 || p.size(3) != refs.size(0)) mismatch("a pool of size " + shape_text(p) + ": (D, page, heads, pages) with " + std::to_string(refs.size(0)) + " pages expected");
+        if (p.size(1) != pools[0].size(1)) mismatch("pools with pages of " + std::to_string(pools[0].size(1)) + " and " + std::to_string(p.size(1)) + " tokens");
+        const int64_t e = p.element_size();
+        if (!as_it_is(p) || p.size(0) * e % 16) mismatch("a pool's features must be contiguous, and its address, strides and the features of a head multiples of 16 bytes");
+        auto st = [&](int64_t i) { return p.size(i) > 1 ? p.stride(i) * e : 16; };
+        out.push_back(ca_pool{p.data_ptr(), st(1), st(2), st(3), int_of(p.size(0) * e, "D"), int_of(p.size(1), "page"), int_of(p.size(2), "heads")});
+    }
+    return out;
+}
+
+Tensor like_ints(const Tensor& t) { return empty_cm(t.sizes(), t, at::kInt); }
+
+std::tuple<Tensor, Tensor, Tensor> advance_pages(const Tensor& table, const Tensor& refs, const Tensor& starts, const Tensor& lengths, int64_t page,
+                                                 int64_t left, int64_t sinks) {
+    const ca_table t = table_of(table, refs, lengths, page);
+    require_ints(starts, table, at::kInt, "starts");
+    if (starts.dim() != 1 || starts.size(0) != table.size(1) + 1 || !starts.is_contiguous()) mismatch("starts of size " + shape_text(starts) + ": (S + 1) expected");
+    Call call(table, "circatt.pages.advance");
+    const Tensor out = like_ints(table), counts = like_ints(refs), missing = at::empty({1}, table.options()), work = scratch(ca_pages_workspace(&t), table);
+    check(ca_advance_pages(&t, starts.data_ptr<int32_t>(), int_of(left, "left"), int_of(sinks, "sinks"), static_cast<int32_t*>(ptr(out)), static_cast<int32_t*>(ptr(counts)),
+                           missing.data_ptr<int32_t>(), ptr(work), call.stream));
+    return {out, counts, missing};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> fork_pages(const std::vector<Tensor>& pools_, const Tensor& table, const Tensor& refs, const Tensor& lengths,
+                                                      const Tensor& parents) {
+    const std::vector<ca_pool> pools = pools_of(pools_, table, refs);
+    const ca_table t = table_of(table, refs, lengths, pools[0].tokens);
+    require_ints(parents, table, at::kInt, "parents");
+    if (parents.dim() != 1 || parents.size(0) != table.size(1) || !parents.is_contiguous()) mismatch("parents of size " + shape_text(parents) + ": one for each sequence expected");
+    Call call(table, "circatt.pages.fork");
+    const Tensor out = like_ints(table), counts = like_ints(refs), n = like_ints(lengths), missing = at::empty({1}, table.options()),
+                 work = scratch(ca_pages_workspace(&t), table);
+    check(ca_fork_pages(&t, static_cast<const int32_t*>(ptr(parents)), pools.data(), (int32_t)pools.size(), static_cast<int32_t*>(ptr(out)), static_cast<int32_t*>(ptr(counts)),
+                        static_cast<int32_t*>(ptr(n)), missing.data_ptr<int32_t>(), ptr(work), call.stream));
+    return {out, counts, n, missing};
+}
+
+std::tuple<Tensor, Tensor, Tensor> compact_pages(const std::vector<Tensor>& pools_, const Tensor& table, const Tensor& refs) {
+    const std::vector<ca_pool> pools = pools_of(pools_, table, refs);
+    const ca_table t = table_of(table, refs, Tensor(), pools[0].tokens);
+    Call call(table, "circatt.pages.compact");
+    const Tensor out = like_ints(table), counts = like_ints(refs), live = at::empty({1}, table.options()), work = scratch(ca_pages_workspace(&t), table);
+    check(ca_compact_pages(&t, pools.data(), (int32_t)pools.size(), static_cast<int32_t*>(ptr(out)), static_cast<int32_t*>(ptr(counts)), live.data_ptr<int32_t>(), ptr(work),
+                           call.stream));
+    return {out, counts, live};
+}
+
 // ---------------------------------------------------------------- window attention
 struct Window {
     int64_t left, right, sinks;
@@ -392,6 +462,9 @@ void bind_tokens(py::module_& m) {
     m.def("rotary", &rotary, release());
     m.def("rotary_append", &rotary_append, release());
     m.def("token_spans", &token_spans, release());
+    m.def("advance_pages", &advance_pages, release());
+    m.def("fork_pages", &fork_pages, release());
+    m.def("compact_pages", &compact_pages, release());
     m.def("window_attention", &window, release());
     m.def("paged_window_attention", &paged_window, release());
 }

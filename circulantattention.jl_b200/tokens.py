@@ -7,7 +7,9 @@ positions (a window alone does not know where a token is), and a cache:
 * `rotary` turns q and k by their positions, on one axis or several (time, height, width); differentiable;
 * `window_attention` is attention with such a window, forward and backward;
 * `rotary_append_` and `paged_window_attention` are the same two for serving: a chunk of new tokens per sequence (one when
-  decoding), whose keys and values live in a paged cache.
+  decoding), whose keys and values live in a paged cache;
+* `token_spans` makes the document and prefix masks of a batch for `window_attention`;
+* `advance_pages`, `fork_pages` and `compact_pages` keep the pages of such a cache.
 
 Tensors are Julia-shaped like those of the rest of the package, but features come first, not the image: `(D, heads, N, B)`,
 packed tokens of several sequences `(D, heads, T)`, a cache `(D, page, heads, pages)`; a tensor of the circulant operators has
@@ -116,3 +118,36 @@ def paged_window_attention(q, k_pages, v_pages, table, starts, lengths, left=Non
     them, may stand in their place in the table.  A missing page (-1) inside the window is skipped.  No gradients."""
     return host.paged_window_attention(q, k_pages, v_pages, table, starts, lengths, _left(left), int(sinks), scale, cap, slopes,
                                        prefix)
+
+
+def advance_pages(table, refs, starts, lengths, page, left=None, sinks=0):
+    """The pages of a serving step, before `rotary_append_` stores its new tokens.  Returns the next (table, refs, missing).
+
+    table, starts, lengths: as for `paged_window_attention`, with the new tokens counted.  refs: Int32 `(pages,)`, how many
+    table entries hold each page; a page is free where that is not above 0.  Pages that neither the new nor later tokens see
+    through a window of `left` and `sinks`, and those behind a sequence's length, go back: all of them where the length is 0 (a
+    sequence that has ended).  Places of new tokens without a page get the lowest free ones, sequence by sequence, pages of
+    this call among them.  missing: Int32 `(1,)`, places that got none; tokens there are not stored.
+
+    Like the other operators on pages it gives a new state and leaves the old one as it is, and nothing waits for the host; a
+    captured step copies the new table and refs over the old ones at its end."""
+    return host.advance_pages(table, refs, starts, lengths, int(page), _left(left), int(sinks))
+
+
+def fork_pages(pools, table, refs, lengths, parents):
+    """Sequences that continue as copies of others: answers to one prompt, beams.  Returns the next (table, refs, lengths,
+    missing) and copies pages in `pools`, in place.
+
+    parents: Int32 `(S,)`; sequence s continues sequence parents[s] as it was before the call.  Its own number: it stays as it
+    is.  A number that is no sequence, -1: it becomes empty, and its pages go back.  pools: the `(D, page, heads, pages)`
+    tensors of all layers, keys and values, of any types.  Full pages are shared; the partly filled last one stays with the
+    parent if it goes on, else with the first that continues it, and the others get copies in the lowest free pages.  missing:
+    Int32 `(1,)`, copies that found none; the place is then -1 and its tokens are not visible."""
+    return host.fork_pages(list(pools), table, refs, lengths, parents)
+
+
+def compact_pages(pools, table, refs):
+    """Moves the pages in use to the lowest numbers, in order, so that the rest of the cache can be given up or cut off.  Returns
+    the next (table, refs, live), live Int32 `(1,)` the pages in use; `pools` are changed in place.  Pages that lie low enough
+    already stay.  A table entry whose page has no count becomes -1."""
+    return host.compact_pages(list(pools), table, refs)

@@ -134,6 +134,43 @@ int ca_window_form_bwd(const ca_seq_desc* d, const ca_seq_form* form, const ca_s
 int ca_paged_window_form(const ca_seq_desc* d, const ca_seq_form* form, const ca_seq_view* q, const ca_page_view* k_pages,
                          const ca_page_view* v_pages, const ca_pages* pages, const ca_seq_view* y, void* stream);
 
+/* ---------------------------------------------------------------- the pages of a cache
+ * A state: the table, for each page the number of table entries that hold it (refs; a page is free if that is not above 0), and
+ * the tokens of each sequence.  The operators read one and write the next into other memory; all of it is on the device and
+ * nothing waits for the host.  Pages are taken from the lowest number on, for sequences and places in their order. */
+typedef struct ca_table {
+    const int32_t* table;     /* (width, sequences) */
+    const int32_t* refs;      /* (pages) */
+    const int32_t* lengths;   /* (sequences); ca_compact_pages does not read it */
+    int32_t width, sequences, page, pages;
+} ca_table;
+
+/* The keys or the values of one layer, of any type; strides in bytes.  One row is a token's features of one head. */
+typedef struct ca_pool {
+    void* data;
+    int64_t token, head, page;
+    int32_t row, tokens, heads;
+} ca_pool;
+
+size_t ca_pages_workspace(const ca_table* t);
+
+/* Before a call's new tokens are stored: lengths[s] counts the starts[s+1] - starts[s] new tokens of sequence s with it.  Pages
+ * that neither they nor later tokens see (a window of `left`, negative: no left end; the first `sinks` tokens), and those
+ * behind the length, are given back, all of them where the length is 0; places of new tokens without a page get one.  *missing:
+ * places that got none. */
+int ca_advance_pages(const ca_table* t, const int32_t* starts, int32_t left, int32_t sinks, int32_t* table, int32_t* refs, int32_t* missing,
+                     void* workspace, void* stream);
+
+/* Sequence s continues as a copy of sequence parents[s] as it was before the call; itself: it stays as it is; no sequence: it
+ * becomes empty.  Pages are shared, but for the partly filled last one: the parent keeps it if it goes on, else the first that
+ * continues it, and the others get copies in all pools.  *missing: copies that found no free page; their place has no page. */
+int ca_fork_pages(const ca_table* t, const int32_t* parents, const ca_pool* pools, int32_t npools, int32_t* table, int32_t* refs,
+                  int32_t* lengths, int32_t* missing, void* workspace, void* stream);
+
+/* Moves the pages in use to the lowest numbers; *live: how many there are.  Entries of pages that are not in use become -1. */
+int ca_compact_pages(const ca_table* t, const ca_pool* pools, int32_t npools, int32_t* table, int32_t* refs, int32_t* live,
+                     void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
