@@ -12,7 +12,7 @@ INCLUDE = os.path.join(PKG_DIR, "..", "include")
 OUT = os.path.join(PKG_DIR, "libcircatt_b200.so")
 SOURCES = ["fwd_exact.cu", "fwd_any.cu", "fwd_values_exact.cu", "fwd_values_any.cu", "bwd_exact.cu", "bwd_any.cu", "emit_exact.cu", "emit_any.cu",
            "apply_exact.cu", "apply_any.cu", "operators.cu", "tiled.cu", "pack.cu", "split_pack.cu", "split_fwd.cu", "split_bwd.cu", "line.cu", "api.cu", "static_scratch.cu", "comm.cu",
-           "rotary.cu", "spans.cu", "pages.cu", "seq_api.cu", "seq_fma.cu", "seq_fwd.cu", "seq_bwd.cu", "seq_decode.cu"]
+           "rotary.cu", "spans.cu", "pages.cu", "seq_api.cu", "seq_fma.cu", "seq_fwd.cu", "seq_fwd_slopes.cu", "seq_fwd_cap.cu", "seq_fwd_cap_slopes.cu", "seq_bwd.cu", "seq_decode.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--use_fast_math", "-Xcompiler", "-fPIC"]
 

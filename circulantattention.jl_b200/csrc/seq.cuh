@@ -26,11 +26,16 @@ int check_pages(const ca_pages* p, int tokens);
 // Other scores and masks than the window's.  Kernels that know them are compiled apart (FORM), so that calls without pay nothing.
 struct SeqForm {
     float cap_in, cap_out;          // z = cap_out tanh(cap_in q.k), with scale / cap and cap log2(e); cap_out = 0: no cap
+    float poly[6];                  // tanh(|cap_in| x) = x poly(x^2) where that is at most 1: TanhPoly's numbers times powers of |cap_in|
     const float* slopes;            // for each query head, nullable: z -= slope log2(e) |i - j|
     const int4* spans;              // dense: [batch][token], nullable: the token sees x..z, and y..w see it
     const int* prefix;              // paged, [sequence], nullable: tokens below are visible to all of the sequence
-    int changed;                    // there is a cap or a slope
 };
+// What of it a call has.  A kernel is compiled for each kind that needs other arithmetic; kMasks has spans or a prefix only, and all
+// of them may have those.
+enum FormKind { kNoForm, kMasks, kSlopes, kCap, kCapSlopes };
+__host__ __device__ constexpr bool has_cap(int form) { return form >= kCap; }
+__host__ __device__ constexpr bool has_slopes(int form) { return form == kSlopes || form == kCapSlopes; }
 
 // A query tile holds consecutive rows R of one key head: row R is query head R % G of the group, token R / G, so that
 // the query heads that share a key head share its tiles.
@@ -46,7 +51,7 @@ struct SeqArgs {
     ca_page_view kp, vp;
     ca_pages pages;                 // table == nullptr: dense
     SeqForm form;
-    bool formed;                    // a call with other scores or masks
+    int kind;                       // of FormKind
     float* lse;                     // [b][key head][R]: log2 of the sum, -inf for rows that see nothing
     float* delta;                   // the same order: dy . y
     int* status;
@@ -151,7 +156,7 @@ struct Reach { int lo, hi; };
 
 // What the token at `pos` sees.  Both ends never fall from one token to the next (documents and groups follow one another), so
 // that a tile's first and last row bound what it sees.
-template <bool FORM>
+template <int FORM>
 __device__ __forceinline__ Reach reach(const SeqArgs& a, const Seq& s, int pos) {
     Reach r{pos - a.left, (int)min((int64_t)INT32_MAX, (int64_t)pos + a.right)};
     if constexpr (FORM) {
@@ -167,7 +172,7 @@ __device__ __forceinline__ Reach reach(const SeqArgs& a, const Seq& s, int pos) 
 }
 // The same for the bounds of tiles: always with the token itself, whatever the spans hold, so that the tiles of neighbouring
 // rows leave no gap.
-template <bool FORM>
+template <int FORM>
 __device__ __forceinline__ Reach tile_reach(const SeqArgs& a, const Seq& s, int pos) {
     Reach r = reach<FORM>(a, s, pos);
     if (FORM) r.lo = min(r.lo, pos), r.hi = max(r.hi, pos);
@@ -181,20 +186,20 @@ __device__ __forceinline__ Reach seen_by(const SeqArgs& a, const Seq& s, int j) 
 
 // Padding, which sees nothing and which nothing sees: whatever it holds, it counts as zeros.  `mixed`: there may be some among
 // the tokens from..upto, which are not all of one document.
-template <bool FORM>
+template <int FORM>
 __device__ __forceinline__ bool padding(const SeqArgs& a, const Seq& s, int j) {
     if (!FORM || !a.form.spans) return false;
     const int4 w = a.form.spans[(int64_t)s.b * a.N + max(0, min(j, a.N - 1))];
     return w.w < w.y;
 }
-template <bool FORM>
+template <int FORM>
 __device__ __forceinline__ bool mixed(const SeqArgs& a, const Seq& s, int from, int upto) {
     if (!FORM || !a.form.spans) return false;
     const int4 w = a.form.spans[(int64_t)s.b * a.N + max(0, min(upto, s.n - 1))];
     return w.x > from || w.w < w.y;
 }
 
-template <bool FORM = false>
+template <int FORM = kNoForm>
 __device__ __forceinline__ KeyTiles key_tiles(const SeqArgs& a, const Seq& s, int p_lo, int p_hi, int keys) {
     KeyTiles k;
     p_lo = max(p_lo, 0);
@@ -234,20 +239,20 @@ __device__ __forceinline__ int page_of(const SeqArgs& a, int b, int j) {
 // with 6 for Float32.
 template <int DEGREE> struct TanhPoly;
 template <> struct TanhPoly<4> {
-    static __device__ __forceinline__ float at(int i) {
-        const float c[5] = {0.999993086f, -0.332980663f, 0.130368114f, -0.0448175557f, 0.00903642457f};
+    static __host__ __device__ constexpr float at(int i) {
+        constexpr float c[5] = {0.999993086f, -0.332980663f, 0.130368114f, -0.0448175557f, 0.00903642457f};
         return c[i];
     }
 };
 template <> struct TanhPoly<5> {
-    static __device__ __forceinline__ float at(int i) {
-        const float c[6] = {0.999999404f, -0.333290428f, 0.132814333f, -0.0516056754f, 0.0167431161f, -0.00306706037f};
+    static __host__ __device__ constexpr float at(int i) {
+        constexpr float c[6] = {0.999999404f, -0.333290428f, 0.132814333f, -0.0516056754f, 0.0167431161f, -0.00306706037f};
         return c[i];
     }
 };
 template <> struct TanhPoly<6> {
-    static __device__ __forceinline__ float at(int i) {
-        const float c[7] = {0.99999994f, -0.333328396f, 0.13325204f, -0.0534570292f, 0.0202899817f, -0.00620337948f, 0.00104102271f};
+    static __host__ __device__ constexpr float at(int i) {
+        constexpr float c[7] = {0.99999994f, -0.333328396f, 0.13325204f, -0.0534570292f, 0.0202899817f, -0.00620337948f, 0.00104102271f};
         return c[i];
     }
 };
@@ -263,16 +268,17 @@ __device__ __forceinline__ float tanh_any(float x) {
 // Of query head `head`, in units of log2(e).
 __device__ __forceinline__ float slope_of(const SeqArgs& a, int head) { return a.form.slopes ? a.form.slopes[head] * kLog2e : 0.f; }
 // A score in units of log2(e), from q.k, less `minus`; slope in those units too, `inner`: the derivative of the cap.
+template <int FORM>
 __device__ __forceinline__ float formed_score(const SeqArgs& a, float dot, float slope, int distance, float minus, float& inner) {
     inner = 1.f;
-    if (!a.form.changed) return fmaf(dot, a.scale_log2, -minus);         // as without a form, to the bit
+    if (!has_cap(FORM) && !has_slopes(FORM)) return fmaf(dot, a.scale_log2, -minus);         // as without a form, to the bit
     float z = dot * a.scale_log2;
-    if (a.form.cap_out != 0.f) {
+    if (has_cap(FORM)) {
         const float t = tanh_any(dot * a.form.cap_in);
         z = a.form.cap_out * t;
         inner = fmaf(-t, t, 1.f);
     }
-    return fmaf(-slope, fabsf((float)distance), z) - minus;
+    return has_slopes(FORM) ? fmaf(-slope, fabsf((float)distance), z) - minus : z - minus;
 }
 
 // How the backward deals out the queries of key tiles that hold first tokens: those tiles have every later query, an ordinary one

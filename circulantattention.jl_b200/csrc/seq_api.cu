@@ -61,8 +61,15 @@ static int fill_form(const ca_seq_desc* d, const ca_seq_form* form, bool paged, 
     a->form.slopes = form->slopes;
     a->form.spans = reinterpret_cast<const int4*>(form->spans);
     a->form.prefix = form->prefix;
-    a->form.changed = form->cap > 0.f || form->slopes;
-    a->formed = a->form.changed || form->spans || form->prefix;
+    // The polynomial with the powers of |cap_in| in its coefficients saves a product a score; where they leave Float32's range the
+    // kernels of kCapSlopes do the work, without slopes.
+    bool fits = form->cap > 0.f;
+    for (int i = 0; i < 6 && fits; ++i) {
+        const double c = (d->dtype == CA_BF16 ? (i < 5 ? TanhPoly<4>::at(i) : 0.0) : TanhPoly<5>::at(i)) * pow(fabs((double)a->form.cap_in), 2 * i + 1);
+        a->form.poly[i] = (float)c;
+        fits = c == 0.0 ? d->dtype == CA_BF16 && i == 5 : fabs(c) > 1e-30 && fabs(c) < 1e30;
+    }
+    a->kind = form->cap > 0.f ? (form->slopes || !fits ? kCapSlopes : kCap) : form->slopes ? kSlopes : form->spans || form->prefix ? kMasks : kNoForm;
     return CA_OK;
 }
 

@@ -89,7 +89,7 @@ __device__ __forceinline__ void clear_row(char* tile, int r) {
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + p * kPanel + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
 }
 
-template <bool FORM>
+template <int FORM>
 __global__ void __launch_bounds__(256) peak_kernel(const __grid_constant__ SeqArgs a, float* __restrict__ peaks) {
     __shared__ float part[8];
     const Seq s = dense_seq(a, blockIdx.z);
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256) peak_kernel(const __grid_constant__ SeqAr
 // The queries move into tensor memory, and their place becomes one more slot of the ring: a tile of keys stays until its product
 // with dS, two steps behind its scores, so that with five slots the values of every tile came late (2450 cycles a tile; 1536
 // are products).
-template <typename T, int DM, bool FORM>
+template <typename T, int DM, int FORM>
 __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ BwdMaps maps) {
     constexpr int S = kSlots<DM> + 1;
     constexpr uint32_t TILE = kTileBytes<DM>;
@@ -253,9 +253,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 if (u == 0 && lane == 0) warp_peak[warp] = peak;
             }
         }
-        const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta * c, -delta * c), c2 = pack2(c, c);
-        const bool changed = FORM && a.form.changed;
-        const float slope = FORM && changed ? slope_of(a, h * a.G + R - pos * a.G) : 0.f;
+        const float factor = has_cap(FORM) ? a.form.cap_out : a.scale_log2;
+        const float sign = has_cap(FORM) ? -1.f : 1.f;             // with a cap x is P (tanh^2 - 1)
+        const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2), lse2 = pack2(-lse, -lse), dl2 = pack2(-delta * c * sign, -delta * c * sign), c2 = pack2(c * sign, c * sign);
+        const float slope = has_slopes(FORM) ? slope_of(a, h * a.G + R - pos * a.G) : 0.f;
+        const CapPoly<T> poly(a, a.form.cap_in, 1.f);
         const Reach mine = reach<FORM>(a, s, pos);
         const bool row_pads = mixed<FORM>(a, s, f_lo, f_hi);
         const int in_hi = reach<FORM>(a, s, f_lo).hi, in_lo = reach<FORM>(a, s, p_hi).lo;      // tiles from in_lo to in_hi need no mask
@@ -278,11 +280,23 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
                 const int hi = live ? min(mine.hi, s.n - 1) - key0 : -1, lo = mine.lo - key0, sk = a.sinks - key0;
                 mk = seen_bits(lo - kCols * u, hi - kCols * u, sk - kCols * u);
             }
-            if (FORM && changed) {
-                float inner[kCols];                            // P (1 - tanh^2) is all that dS needs
-                form_scores<T, kCols, true>(x, inner, a, a.scale_log2, a.form.cap_in, slope, (float)(pos - key0 - kCols * u), edge, mk);
+            if (has_cap(FORM) || has_slopes(FORM)) {
+                f32x2 inner[has_cap(FORM) ? kCols / 2 : 1];    // P (1 - tanh^2) is all that dS needs
+                if (FORM == kCap) poly.template scores<kCols>(x, edge, mk);
+                else if (has_cap(FORM)) cap_scores<T, kCols>(x, a.form.cap_in, 1.f, edge, mk);
+                if (has_cap(FORM)) cap_inner<kCols>(inner, x);
+                if (has_slopes(FORM)) slope_scores<kCols>(x, factor, slope, (float)(pos - key0 - kCols * u), far <= f_lo ? 1 : key0 >= f_hi ? -1 : 0);
+                const f32x2 f2 = has_slopes(FORM) ? pack2(1.f, 1.f) : pack2(factor, factor);
 #pragma unroll
-                for (int c = 0; c < kCols; ++c) x[c] = __float_as_uint(fast_exp2(__uint_as_float(x[c]) - lse) * inner[c]);
+                for (int c = 0; c < kCols; c += 2) {
+                    float e0, e1;
+                    unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2, lse2), e0, e1);
+                    e0 = fast_exp2(e0);
+                    e1 = fast_exp2(e1);
+                    if (has_cap(FORM)) unpack2(mul2(pack2(e0, e1), inner[c / 2]), e0, e1);
+                    x[c] = __float_as_uint(e0);
+                    x[c + 1] = __float_as_uint(e1);
+                }
             } else {
 #pragma unroll
                 for (int c = 0; c < kCols; c += 2) {
@@ -450,7 +464,7 @@ struct Steps {
 //
 // Keys that stay visible to every later token would give their CTA all queries of the sequence; the queries of such tiles are
 // dealt to `segments` CTAs, which store Float32 parts for join_kernel to add up in order.
-template <typename T, int DM, bool FORM>
+template <typename T, int DM, int FORM>
 __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ BwdMaps maps) {
     constexpr int S = kSlots<DM>;
     constexpr uint32_t TILE = kTileBytes<DM>;
@@ -544,8 +558,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;
         const uint32_t S_at = tmem + 16 * u + lane_off, dp_at = S_at + 128, P_at = p_col + apart * u + lane_off, ds_at = ds_col + apart * u + lane_off;
         const f32x2 sc2 = pack2(a.scale_log2, a.scale_log2);
-        const f32x2 c2 = kIsBf16<T> ? pack2(1.f, 1.f) : pack2(c / kPScale, c / kPScale);
-        const bool changed = FORM && a.form.changed, key_pads = k0 < s.n && mixed<FORM>(a, s, k0, k0 + 127);
+        const float dp_factor = (has_cap(FORM) ? -1.f : 1.f) * (kIsBf16<T> ? 1.f : c / kPScale);
+        const f32x2 c2 = pack2(dp_factor, dp_factor);
+        const CapPoly<T> poly(a, a.form.cap_in, 1.f);
+        const float factor = has_cap(FORM) ? a.form.cap_out : a.scale_log2;
+        const bool key_pads = k0 < s.n && mixed<FORM>(a, s, k0, k0 + 127);
         int by_lo = j - a.right, by_hi = j < a.sinks ? s.n - 1 : min(j + a.left, s.n - 1);      // queries that see the key
         if (FORM && spans) {
             const Reach by = seen_by(a, s, j);
@@ -559,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             const bool pads = mixed<FORM>(a, s, q0, q0 + 127);
             const bool ragged = q0 + 127 >= s.n || k0 + 127 >= s.n || pads || key_pads;
             const bool edge = !(whole_lo <= q0 && q0 + 127 <= whole_hi && q0 + 127 < s.n && k0 + 127 < s.n);
-            const float slope = FORM && changed ? slope_of(a, h * a.G + at.g) : 0.f;
+            const float slope = has_slopes(FORM) ? slope_of(a, h * a.G + at.g) : 0.f;
             if (!warp_wait(smem_u32(&st_full[b]), (i >> 1) & 1, stop) || !warp_wait(smem_u32(&s_full), i & 1, stop)) { ok = false; break; }
             fence_after();
             // Columns 16 u .. 16 u + 15 of either half of the tile: the product with the first half starts while the weights
@@ -580,9 +597,15 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
             for (int g = 0; g < 2; ++g) {
                 const float4* lse4 = reinterpret_cast<const float4*>(&s_lse[b][64 * g + 16 * u]);
                 uint32_t* const xg = x + 16 * g;
-                float inner[16];
-                if (FORM && changed) form_scores<T, 16, true>(xg, inner, a, a.scale_log2, a.form.cap_in, slope, (float)(j - q0 - 64 * g - 16 * u), edge, mk >> 16 * g);
-                const f32x2 f2 = FORM && changed ? pack2(1.f, 1.f) : sc2;
+                f32x2 inner[has_cap(FORM) ? 8 : 1];
+                if (has_cap(FORM)) {
+                    if (FORM == kCap) poly.template scores<16>(xg, edge, mk >> 16 * g);
+                    else cap_scores<T, 16>(xg, a.form.cap_in, 1.f, edge, mk >> 16 * g);
+                    cap_inner<16>(inner, xg);
+                }
+                if (has_slopes(FORM))
+                    slope_scores<16>(xg, factor, slope, (float)(j - q0 - 64 * g - 16 * u), k0 + 127 <= q0 ? -1 : q0 + 127 <= k0 ? 1 : 0);
+                const f32x2 f2 = has_slopes(FORM) ? pack2(1.f, 1.f) : has_cap(FORM) ? pack2(factor, factor) : sc2;
 #pragma unroll
                 for (int c = 0; c < 16; c += 4) {
                     const float4 z = lse4[c >> 2];
@@ -596,9 +619,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 uint32_t w[8];
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) w[c >> 1] = pack16<T>(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1]));
-                if (FORM && changed) {                             // dS has the cap's derivative
+                if (has_cap(FORM)) {                               // dS has the cap's derivative
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) xg[c] = __float_as_uint(__uint_as_float(xg[c]) * inner[c]);
+                    for (int c = 0; c < 16; c += 2) {
+                        float e0, e1;
+                        unpack2(mul2(pack2(__uint_as_float(xg[c]), __uint_as_float(xg[c + 1])), inner[c / 2]), e0, e1);
+                        xg[c] = __float_as_uint(e0);
+                        xg[c + 1] = __float_as_uint(e1);
+                    }
                 }
                 tmem_st8(P_at + 4 * apart * g, w);
                 tmem_wait_st();
@@ -731,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         if (!ok) mbar_wait(smem_u32(&drained), 0, 1u << 14);   // products in flight end before tensor memory is freed
     } else if (warp == kFetcher) {
         // minus the rows' sums, and minus their delta, with the factors of half precision
-        const float shift = kIsBf16<T> ? 0.f : kPLog2, minus = kIsBf16<T> ? -1.f : -c / kPScale;
+        const float shift = kIsBf16<T> ? 0.f : kPLog2, minus = (has_cap(FORM) ? 1.f : -1.f) * (kIsBf16<T> ? 1.f : c / kPScale);
         const int rows = s.T * a.G;
         const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
         Steps at(a, t_lo, first);
@@ -781,7 +809,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ SeqAr
     *reinterpret_cast<uint4*>(dst) = make_uint4(pack16<T>(sum[0], sum[1]), pack16<T>(sum[2], sum[3]), pack16<T>(sum[4], sum[5]), pack16<T>(sum[6], sum[7]));
 }
 
-template <typename T, int DM, bool FORM>
+template <typename T, int DM, int FORM>
 int launch(const SeqArgs& a, const BwdMaps& maps, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(umma_dq_kernel<T, DM, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(umma_dkdv_kernel<T, DM, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem<DM>);
@@ -837,13 +865,16 @@ int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) 
     maps.split_tiles = p.tiles;
     maps.segments = p.segments;
     const bool wide = a.D > 64;
-#define CA_BWD(T, FORM) return wide ? launch<T, 128, FORM>(a, maps, st) : launch<T, 64, FORM>(a, maps, st)
-    if (a.formed) {
-        if (bf16) CA_BWD(__nv_bfloat16, true);
-        CA_BWD(__half, true);
+#define CA_BWD(FORM)                                                                                                      \
+    return bf16 ? (wide ? launch<__nv_bfloat16, 128, FORM>(a, maps, st) : launch<__nv_bfloat16, 64, FORM>(a, maps, st))   \
+                : (wide ? launch<__half, 128, FORM>(a, maps, st) : launch<__half, 64, FORM>(a, maps, st))
+    switch (a.kind) {
+        case kMasks: CA_BWD(kMasks);
+        case kSlopes: CA_BWD(kSlopes);
+        case kCap: CA_BWD(kCap);
+        case kCapSlopes: CA_BWD(kCapSlopes);
+        default: CA_BWD(kNoForm);
     }
-    if (bf16) CA_BWD(__nv_bfloat16, false);
-    CA_BWD(__half, false);
 #undef CA_BWD
 }
 

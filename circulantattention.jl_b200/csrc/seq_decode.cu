@@ -64,7 +64,7 @@ __device__ __forceinline__ bool grows(float& m, float top, float& f) {
     return true;
 }
 
-template <typename T, int DM, bool FORM>
+template <typename T, int DM, int FORM>
 __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_constant__ SeqArgs a) {
     typedef Decode<T, DM> L;
     extern __shared__ __align__(128) char smem[];
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
         const int ra = lane >> 2, pa = s.base + token_of(a, min(R0 + ra, rows - 1)), pb = s.base + token_of(a, min(R0 + ra + 8, rows - 1));
         const Reach ra_reach = reach<FORM>(a, s, pa), rb_reach = reach<FORM>(a, s, pb);
         float slope_a = 0.f, slope_b = 0.f;
-        if (FORM && a.form.slopes) {
+        if (has_slopes(FORM)) {
             const int Ra = min(R0 + ra, rows - 1), Rb = min(R0 + ra + 8, rows - 1);
             slope_a = slope_of(a, h * a.G + Ra - token_of(a, Ra) * a.G);
             slope_b = slope_of(a, h * a.G + Rb - token_of(a, Rb) * a.G);
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
                 for (int e = 0; e < 4; ++e) {
                     const int jj = j + 8 * n + (e & 1);
                     float inner;
-                    if (FORM && a.form.changed) c[n][e] = formed_score(a, c[n][e], e < 2 ? slope_a : slope_b, (e < 2 ? pa : pb) - jj, 0.f, inner);
+                    if (has_cap(FORM) || has_slopes(FORM)) c[n][e] = formed_score<FORM>(a, c[n][e], e < 2 ? slope_a : slope_b, (e < 2 ? pa : pb) - jj, 0.f, inner);
                     else c[n][e] *= a.scale_log2;
                     if (edge && !sees(a, s.n, e < 2 ? pa : pb, e < 2 ? ra_reach : rb_reach, jj)) c[n][e] = -INFINITY;
                     if (e < 2) ta = fmaxf(ta, c[n][e]); else tb = fmaxf(tb, c[n][e]);
@@ -259,12 +259,12 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
         __syncthreads();
         const int half = lane >> 4, key = lane & 15;
         int pos[8];
-        float slopes[FORM ? 8 : 1];
+        float slopes[has_slopes(FORM) ? 8 : 1];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int t = token_of(a, R0 + 2 * i + half);
             pos[i] = 2 * i + half < nrows ? s.base + t : -1;
-            if (FORM) slopes[i] = pos[i] >= 0 ? slope_of(a, h * a.G + R0 + 2 * i + half - t * a.G) : 0.f;
+            if (has_slopes(FORM)) slopes[i] = pos[i] >= 0 ? slope_of(a, h * a.G + R0 + 2 * i + half - t * a.G) : 0.f;
         }
         float o[kRows][C];
 #pragma unroll
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
                 if (2 * i >= nrows) continue;
                 if constexpr (FORM) {
                     float inner;
-                    const float z = a.form.changed ? formed_score(a, sc[i], slopes[i], pos[i] - key0 - key, 0.f, inner) : sc[i] * a.scale_log2;
+                    const float z = formed_score<FORM>(a, sc[i], slopes[has_slopes(FORM) ? i : 0], pos[i] - key0 - key, 0.f, inner);
                     sc[i] = sees(a, s.n, pos[i], reach<FORM>(a, s, pos[i]), key0 + key) ? z : -INFINITY;
                 } else {
                     sc[i] = sees(a, s.n, pos[i], key0 + key) ? sc[i] * a.scale_log2 : -INFINITY;
@@ -439,7 +439,7 @@ int largest_cluster(K kernel, size_t smem, std::atomic<int>* cache) {
     return n;
 }
 
-template <typename T, int DM, bool FORM>
+template <typename T, int DM, int FORM>
 int launch(const SeqArgs& a, cudaStream_t st) {
     static std::atomic<int> cluster_cache[64];
     const size_t smem = Decode<T, DM>::kSmem;
@@ -468,12 +468,19 @@ int launch(const SeqArgs& a, cudaStream_t st) {
 
 int decode_paged(const SeqArgs& a, int dtype, cudaStream_t st) {
     const bool wide = a.D > 64;
-#define CA_DECODE(T)                                                                                                   \
-    return a.formed ? (wide ? launch<T, 128, true>(a, st) : launch<T, 64, true>(a, st))                                \
-                    : (wide ? launch<T, 128, false>(a, st) : launch<T, 64, false>(a, st))
-    if (dtype == CA_F32) CA_DECODE(float);
-    if (dtype == CA_BF16) CA_DECODE(__nv_bfloat16);
-    CA_DECODE(__half);
+#define CA_DECODE_KIND(T, FORM) return wide ? launch<T, 128, FORM>(a, st) : launch<T, 64, FORM>(a, st)
+#define CA_DECODE(T)                                         \
+    switch (a.kind) {                                        \
+        case kMasks: CA_DECODE_KIND(T, kMasks);              \
+        case kSlopes: CA_DECODE_KIND(T, kSlopes);            \
+        case kCap: CA_DECODE_KIND(T, kCap);                  \
+        case kCapSlopes: CA_DECODE_KIND(T, kCapSlopes);      \
+        default: CA_DECODE_KIND(T, kNoForm);                 \
+    }
+    if (dtype == CA_F32) CA_DECODE(float)
+    if (dtype == CA_BF16) CA_DECODE(__nv_bfloat16)
+    CA_DECODE(__half)
+#undef CA_DECODE_KIND
 #undef CA_DECODE
 }
 

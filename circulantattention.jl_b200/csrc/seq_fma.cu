@@ -138,7 +138,7 @@ __device__ __forceinline__ float* row_ptr(const ca_seq_view& v, const SeqArgs& a
     return (float*)v.data + (h * a.G + g) * v.head + (int64_t)(s.t0 + t) * v.token + (a.pages.table ? 0 : s.b * v.batch);
 }
 // Key row j; clears `on` where it does not exist or is padding.
-template <bool FORM>
+template <int FORM>
 __device__ __forceinline__ const float* key_ptr(const ca_seq_view& v, const ca_page_view& pv, const SeqArgs& a, const Seq& s, int h, int j, bool& on) {
     on = on && j < s.n && !padding<FORM>(a, s, j);
     if (!a.pages.table) return (const float*)v.data + h * v.head + (int64_t)j * v.token + s.b * v.batch;
@@ -150,7 +150,7 @@ __device__ __forceinline__ const float* key_ptr(const ca_seq_view& v, const ca_p
 // ---------------------------------------------------------------- forward
 template <int DM> constexpr size_t kFwdSmem = (5 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
 
-template <int DM, bool FORM>
+template <int DM, int FORM>
 __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
     float *Q = (float*)smem4, *KV = Q + kTileFloats<DM>, *Pm = KV + 4 * kTileFloats<DM>;      // K, V, K, V
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
                 const int key = j0 + tx + 16 * j;
                 if constexpr (FORM) {
                     float inner;
-                    sc[i][j] = formed_score(a, sc[i][j], slope[i], pos[i] - key, 0.f, inner);
+                    sc[i][j] = formed_score<FORM>(a, sc[i][j], slope[i], pos[i] - key, 0.f, inner);
                     if (!sees(a, s.n, pos[i], mine[i], key) || gone[b][tx + 16 * j]) sc[i][j] = -INFINITY;
                 } else {
                     sc[i][j] *= a.scale_log2;
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
 // P = 2^(scale q.k log2 e - lse), dP = dy.v, dS = P (dP - delta), delta = dy.y; dq = scale dS k.
 template <int DM> constexpr size_t kDqSmem = (4 * kTileFloats<DM> + kTile * kPPitch) * sizeof(float);
 
-template <int DM, bool FORM>
+template <int DM, int FORM>
 __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
     float *Q = (float*)smem4, *O = Q + kTileFloats<DM>, *K = O + kTileFloats<DM>, *V = K + kTileFloats<DM>, *Pm = V + kTileFloats<DM>;
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
                 float ds;
                 if constexpr (FORM) {
                     float inner;
-                    const float z = formed_score(a, sc[i][j], slope[i], pos[i] - key, lse[i], inner);
+                    const float z = formed_score<FORM>(a, sc[i][j], slope[i], pos[i] - key, lse[i], inner);
                     ds = sees(a, s.n, pos[i], mine[i], key) ? fast_exp2(z) * inner * (dp[i][j] - delta[i]) : 0.f;
                 } else {
                     const bool see = !edge || sees(a, s.n, pos[i], key);
@@ -376,7 +376,7 @@ struct Parts {
     int tiles, segments;
 };
 
-template <int DM, bool FORM>
+template <int DM, int FORM>
 __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(const __grid_constant__ SeqArgs a, const Parts parts) {
     extern __shared__ float4 smem4[];
     float *K = (float*)smem4, *V = K + kTileFloats<DM>, *Q = V + kTileFloats<DM>, *O = Q + kTileFloats<DM>, *Pm = O + kTileFloats<DM>, *Sm = Pm + kTile * kPPitch;
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
                 if constexpr (FORM) {
                     const int token = token_of(a, R);
                     see = R < hi && token < s.n && token >= by[i].lo && token <= by[i].hi;
-                    z = formed_score(a, sc[i][c], R < hi ? slope_of(a, h * a.G + R - token * a.G) : 0.f, token - key, s_lse[tx + 16 * c], inner);
+                    z = formed_score<FORM>(a, sc[i][c], has_slopes(FORM) && R < hi ? slope_of(a, h * a.G + R - token * a.G) : 0.f, token - key, s_lse[tx + 16 * c], inner);
                 } else {
                     see = !edge || (R < hi && sees(a, s.n, token_of(a, R), key));
                     z = sc[i][c] * a.scale_log2 - s_lse[tx + 16 * c];
@@ -510,7 +510,7 @@ int raise_smem(K kernel, size_t bytes) {
     return e == cudaSuccess ? CA_OK : cuda_fail(e, "cudaFuncSetAttribute");
 }
 
-template <int DM, bool FORM>
+template <int DM, int FORM>
 int launch_fwd(const SeqArgs& a, cudaStream_t st) {
     const int rc = raise_smem(fma_fwd_kernel<DM, FORM>, kFwdSmem<DM>);
     if (rc) return rc;
@@ -520,7 +520,7 @@ int launch_fwd(const SeqArgs& a, cudaStream_t st) {
     return CA_OK;
 }
 
-template <int DM, bool FORM>
+template <int DM, int FORM>
 int launch_bwd(const SeqArgs& a, float* data, cudaStream_t st) {
     int rc = raise_smem(fma_dq_kernel<DM, FORM>, kDqSmem<DM>);
     if (rc || (rc = raise_smem(fma_dkdv_kernel<DM, FORM>, kDkdvSmem<DM>))) return rc;
@@ -545,13 +545,16 @@ size_t fma_bwd_parts(const SeqArgs& a) {
     return (size_t)p.tiles * p.segments * 2 * kTile * (a.D > 64 ? 128 : 64) * a.Hkv * a.B * sizeof(float);
 }
 
-int fma_fwd(const SeqArgs& a, cudaStream_t st) {
-    if (a.formed) return a.D > 64 ? launch_fwd<128, true>(a, st) : launch_fwd<64, true>(a, st);
-    return a.D > 64 ? launch_fwd<128, false>(a, st) : launch_fwd<64, false>(a, st);
-}
-int fma_bwd(const SeqArgs& a, float* parts, cudaStream_t st) {
-    if (a.formed) return a.D > 64 ? launch_bwd<128, true>(a, parts, st) : launch_bwd<64, true>(a, parts, st);
-    return a.D > 64 ? launch_bwd<128, false>(a, parts, st) : launch_bwd<64, false>(a, parts, st);
-}
+#define CA_KINDS(F, ...)                                                                                             \
+    switch (a.kind) {                                                                                                \
+        case kMasks: return a.D > 64 ? F<128, kMasks>(__VA_ARGS__) : F<64, kMasks>(__VA_ARGS__);                     \
+        case kSlopes: return a.D > 64 ? F<128, kSlopes>(__VA_ARGS__) : F<64, kSlopes>(__VA_ARGS__);                  \
+        case kCap: return a.D > 64 ? F<128, kCap>(__VA_ARGS__) : F<64, kCap>(__VA_ARGS__);                           \
+        case kCapSlopes: return a.D > 64 ? F<128, kCapSlopes>(__VA_ARGS__) : F<64, kCapSlopes>(__VA_ARGS__);         \
+        default: return a.D > 64 ? F<128, kNoForm>(__VA_ARGS__) : F<64, kNoForm>(__VA_ARGS__);                       \
+    }
+int fma_fwd(const SeqArgs& a, cudaStream_t st) { CA_KINDS(launch_fwd, a, st) }
+int fma_bwd(const SeqArgs& a, float* parts, cudaStream_t st) { CA_KINDS(launch_bwd, a, parts, st) }
+#undef CA_KINDS
 
 }  // namespace ca

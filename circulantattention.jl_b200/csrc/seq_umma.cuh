@@ -63,58 +63,108 @@ __device__ __forceinline__ void settled32(uint32_t* r) {
         asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-// COUNT neighbouring columns of a row: from q.k to scores in units of log2(e), capped, less slope times the distance |d0 - c| of
-// column c.  INNER: also the cap's derivative 1 - tanh^2.  The polynomial serves |score| <= cap; a warp that holds a larger one
-// takes two passes of the exponential unit an element, 1.5e-7 of the cap off.  Columns that the row does not see (`edge`: those
-// whose bit in mk is not set) have no say in this.  The warp calls it together.
-template <typename T, int COUNT, bool INNER>
-__device__ __forceinline__ void form_scores(uint32_t* x, float* inner, const SeqArgs& a, float scale_log2, float cap_in, float slope, float d0, bool edge, uint32_t mk) {
+// ---------------------------------------------------------------- scores with a cap and a slope, COUNT neighbouring columns of a row
+// Largest magnitude; `edge`: of the columns whose bit in mk is set.
+template <int COUNT>
+__device__ __forceinline__ float largest(const uint32_t* x, bool edge, uint32_t mk) {
+    float big = 0.f;
+    if (edge) {
+#pragma unroll
+        for (int c = 0; c < COUNT; ++c) big = fmaxf(big, (mk >> c) & 1 ? fabsf(__uint_as_float(x[c])) : 0.f);
+    } else {
+#pragma unroll
+        for (int c = 0; c < COUNT; c += 2) big = fmaxf(fmaxf(big, fabsf(__uint_as_float(x[c]))), fabsf(__uint_as_float(x[c + 1])));
+    }
+    return big;
+}
+
+// x = tanh(cap_in x), or `out` times that.  The polynomial serves |score| <= cap; a warp that holds a larger one takes two passes of
+// the exponential unit an element, 1.5e-7 off.  Columns that the row does not see have no say in this.  The warp calls it
+// together.
+template <typename T, int COUNT>
+__device__ __forceinline__ void cap_scores(uint32_t* x, float cap_in, float out, bool edge, uint32_t mk) {
     constexpr int DEGREE = kIsBf16<T> ? 4 : 5;
     typedef TanhPoly<DEGREE> P;
-    if (a.form.cap_out != 0.f) {
-        float big = 0.f;
-        if (edge) {
+    if (__any_sync(~0u, largest<COUNT>(x, edge, mk) * fabsf(cap_in) > 1.f)) {
 #pragma unroll
-            for (int c = 0; c < COUNT; ++c) big = fmaxf(big, (mk >> c) & 1 ? fabsf(__uint_as_float(x[c])) : 0.f);
-        } else {
+        for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(tanh_far(__uint_as_float(x[c]) * cap_in) * out);
+        return;
+    }
+    const f32x2 in2 = pack2(cap_in, cap_in);
 #pragma unroll
-            for (int c = 0; c < COUNT; ++c) big = fmaxf(big, fabsf(__uint_as_float(x[c])));
+    for (int c = 0; c < COUNT; c += 2) {
+        const f32x2 X = mul2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), in2), u = mul2(X, X);
+        f32x2 p = pack2(P::at(DEGREE) * out, P::at(DEGREE) * out);
+#pragma unroll
+        for (int i = DEGREE - 1; i >= 0; --i) p = fma2(p, u, pack2(P::at(i) * out, P::at(i) * out));
+        float z0, z1;
+        unpack2(mul2(p, X), z0, z1);
+        x[c] = __float_as_uint(z0);
+        x[c + 1] = __float_as_uint(z1);
+    }
+}
+// The same with the factors in the coefficients (kCap).
+template <typename T> struct CapPoly {
+    static constexpr int DEGREE = kIsBf16<T> ? 4 : 5;
+    float k[DEGREE + 1], cap_in, out;
+    __device__ __forceinline__ CapPoly(const SeqArgs& a, float cap_in, float out) : cap_in(cap_in), out(out) {
+        const float f = cap_in < 0.f ? -out : out;
+#pragma unroll
+        for (int i = 0; i <= DEGREE; ++i) k[i] = a.form.poly[i] * f;
+    }
+    template <int COUNT>
+    __device__ __forceinline__ void scores(uint32_t* x, bool edge, uint32_t mk) const {
+        if (__any_sync(~0u, largest<COUNT>(x, edge, mk) * fabsf(cap_in) > 1.f)) {
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(tanh_far(__uint_as_float(x[c]) * cap_in) * out);
+            return;
         }
-        const f32x2 in2 = pack2(cap_in, cap_in), out2 = pack2(a.form.cap_out, a.form.cap_out), one2 = pack2(1.f, 1.f);
-        if (__any_sync(~0u, big * fabsf(cap_in) > 1.f)) {
 #pragma unroll
-            for (int c = 0; c < COUNT; ++c) {
-                const float t = tanh_far(__uint_as_float(x[c]) * cap_in);
-                x[c] = __float_as_uint(t * a.form.cap_out);
-                if (INNER) inner[c] = fmaf(-t, t, 1.f);
-            }
-        } else {
+        for (int c = 0; c < COUNT; c += 2) {
+            const f32x2 s = pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), u = mul2(s, s);
+            f32x2 p = pack2(k[DEGREE], k[DEGREE]);
 #pragma unroll
-            for (int c = 0; c < COUNT; c += 2) {
-                const f32x2 X = mul2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), in2), u = mul2(X, X);
-                f32x2 p = pack2(P::at(DEGREE), P::at(DEGREE));
+            for (int i = DEGREE - 1; i >= 0; --i) p = fma2(p, u, pack2(k[i], k[i]));
+            float z0, z1;
+            unpack2(mul2(p, s), z0, z1);
+            x[c] = __float_as_uint(z0);
+            x[c + 1] = __float_as_uint(z1);
+        }
+    }
+};
+// Minus the cap's derivative, tanh^2 - 1, of values that are tanh.
+template <int COUNT>
+__device__ __forceinline__ void cap_inner(f32x2* inner, const uint32_t* x) {
+    const f32x2 minus = pack2(-1.f, -1.f);
 #pragma unroll
-                for (int i = DEGREE - 1; i >= 0; --i) p = fma2(p, u, pack2(P::at(i), P::at(i)));
-                const f32x2 t = mul2(p, X);
-                float z0, z1;
-                unpack2(mul2(t, out2), z0, z1);
-                x[c] = __float_as_uint(z0);
-                x[c + 1] = __float_as_uint(z1);
-                if (INNER) unpack2(fma2(mul2(t, pack2(-1.f, -1.f)), t, one2), inner[c], inner[c + 1]);
-            }
+    for (int c = 0; c < COUNT; c += 2) {
+        const f32x2 t = pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1]));
+        inner[c / 2] = fma2(t, t, minus);
+    }
+}
+
+// x = x factor - slope |d0 - c| for column c.  `side`: 1 where d0 - c is nowhere negative, -1 where it is nowhere positive, 0 where it
+// may be either.
+template <int COUNT>
+__device__ __forceinline__ void slope_scores(uint32_t* x, float factor, float slope, float d0, int side) {
+    if (side) {
+        const float s = side > 0 ? slope : -slope;
+        const f32x2 f2 = pack2(factor, factor), step = pack2(2.f * s, 2.f * s);
+        f32x2 bias = pack2(-s * d0, fmaf(-s, d0, s));
+#pragma unroll
+        for (int c = 0; c < COUNT; c += 2) {
+            float z0, z1;
+            unpack2(fma2(pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), f2, bias), z0, z1);
+            x[c] = __float_as_uint(z0);
+            x[c + 1] = __float_as_uint(z1);
+            bias = add2(bias, step);
         }
     } else {
 #pragma unroll
-        for (int c = 0; c < COUNT; ++c) {
-            x[c] = __float_as_uint(__uint_as_float(x[c]) * scale_log2);
-            if (INNER) inner[c] = 1.f;
-        }
-    }
-    if (a.form.slopes) {
-#pragma unroll
-        for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(fmaf(-slope, fabsf(d0 - (float)c), __uint_as_float(x[c])));
+        for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(fmaf(-slope, fabsf(d0 - (float)c), __uint_as_float(x[c]) * factor));
     }
 }
+
 // Tiles between global and shared memory: consecutive threads take consecutive 16-byte pieces of a row, so that a warp covers
 // two to four whole rows at a time (a thread for each row would touch 32 lines an instruction: 4096 cycles a tile of 128 rows,
 // and three such tiles made the prologue of dq 10 us).  `row(r)`: address of row r.  Rows
