@@ -199,6 +199,50 @@ __device__ __forceinline__ bool mixed(const SeqArgs& a, const Seq& s, int from, 
     return w.x > from || w.w < w.y;
 }
 
+// Tiles from..upto that lie between the begin of the last row's document and that row are known to be of one document without
+// a look at the spans.
+template <int FORM>
+__device__ __forceinline__ int document_of(const SeqArgs& a, const Seq& s, int last) {
+    return FORM && a.form.spans && last >= 0 ? a.form.spans[(int64_t)s.b * a.N + min(last, a.N - 1)].x : 0;
+}
+
+// Keys that the rows from..to - 1 together see: the work of their tile.
+template <int FORM>
+__device__ __forceinline__ int row_work(const SeqArgs& a, const Seq& s, int from, int to) {
+    const int lo = from / a.G, hi = min(s.n - 1, (min(to, s.T * a.G) - 1) / a.G);
+    return hi < lo ? 0 : tile_reach<FORM>(a, s, hi).hi - max(0, tile_reach<FORM>(a, s, lo).lo);
+}
+
+// Documents make tiles of unequal work, and those are best begun with the largest (packed training: dk and dv 342 -> 249 us, forward
+// 259 -> 234).  Each block finds the tile of its rank by itself: runs of neighbouring tiles, at most 128 so that this stays short
+// (512 of them took 5 us a block), are ordered by `work(first, last)`, for equal work by number; a last run that is shorter comes
+// last.  It costs a block 1.7 us, which dq with its many and even tiles does not get back (263 -> 289 us).
+// The block's threads call it together; `counts` has room for 128 numbers, and is free again behind it.
+template <typename Work>
+__device__ __forceinline__ int ranked_tile(int tiles, int rank, int* counts, int* result, Work work) {
+    const int length = (tiles + 127) / 128, runs = (tiles + length - 1) / length, t = threadIdx.x;
+    if (t < 128) counts[t] = t >= runs ? -2 : (t + 1) * length > tiles ? -1 : work(t * length, (t + 1) * length - 1);
+    __syncthreads();
+    if (t < runs) {
+        const int own = counts[t];
+        int before = 0;
+        for (int i = 0; i < 128; i += 4) {
+            const int4 c = *reinterpret_cast<const int4*>(counts + i);
+            before += (c.x > own || (c.x == own && i < t)) + (c.y > own || (c.y == own && i + 1 < t)) + (c.z > own || (c.z == own && i + 2 < t)) +
+                      (c.w > own || (c.w == own && i + 3 < t));
+        }
+        if (before == rank / length) *result = t * length + rank % length;
+    }
+    __syncthreads();
+    return *result;
+}
+// The block's rank, head and sequence, with the heads and sequences innermost, so that the largest tiles of all come first.
+struct Place { int x, h, b; };
+__device__ __forceinline__ Place place_by_rank() {
+    const uint32_t id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), all = gridDim.y * gridDim.z;
+    return Place{(int)(id / all), (int)(id % all % gridDim.y), (int)(id % all / gridDim.y)};
+}
+
 template <int FORM = kNoForm>
 __device__ __forceinline__ KeyTiles key_tiles(const SeqArgs& a, const Seq& s, int p_lo, int p_hi, int keys) {
     KeyTiles k;

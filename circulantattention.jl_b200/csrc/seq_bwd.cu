@@ -33,6 +33,7 @@ struct BwdMaps {
     CUtensorMap k, v, q, dy;
     CUtensorMap q_rows, dy_rows, y_rows, rest_rows, dq_rows, dk, dv;
     int sms;                // dq: the CTA so many further on takes this one's place
+    int ranked;             // dk, dv: the largest tiles first
     int rows;               // q, dy and dq of the first sweep move by tiles of rows (maps), else by threads
     int* timeouts;
     float *dy_peak, *v_peak;    // half: largest magnitudes of each tile of 128 query rows / keys, [b][key head][tile]
@@ -260,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
         const CapPoly<T> poly(a, a.form.cap_in, 1.f);
         const Reach mine = reach<FORM>(a, s, pos);
         const bool row_pads = mixed<FORM>(a, s, f_lo, f_hi);
+        const int doc_lo = document_of<FORM>(a, s, p_hi);
         const int in_hi = reach<FORM>(a, s, f_lo).hi, in_lo = reach<FORM>(a, s, p_hi).lo;      // tiles from in_lo to in_hi need no mask
         const uint32_t S_at = tmem + kCols * u + lane_off, dp_at = S_at + 128, ds_at = tmem + 256 + kCols / 2 * u + lane_off;
         bool ok = true;
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&s_free));
             uint32_t mk = ~0u;
-            const bool pads = mixed<FORM>(a, s, key0, far);
+            const bool pads = FORM && (key0 < doc_lo || far > p_hi) && mixed<FORM>(a, s, key0, far);
             const bool ragged = far >= s.n || f_hi != p_hi || pads || row_pads;      // the tile holds keys or rows that may be anything
             const bool edge = !(far <= in_hi && far < s.n && f_hi == p_hi && (key0 >= in_lo || far < a.sinks));
             if (edge) {
@@ -479,12 +481,20 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
     char* const smem = raw + (base_at - raw_at);
     const uint32_t ring_at = base_at + 2 * TILE;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
-    const Seq s = dense_seq(a, blockIdx.z);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ int ranked;
+    const bool rank = FORM && maps.ranked;                         // spans: no first tokens, nothing is dealt out
+    const Place place = rank ? place_by_rank() : Place{(int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z};
+    const int h = place.h, x = place.x;
+    const Seq s = dense_seq(a, place.b);
     const int dealt = maps.split_tiles * maps.segments;
-    const bool split = (int)blockIdx.x < dealt;
-    const int tile = split ? (int)blockIdx.x / maps.segments : maps.split_tiles + (int)blockIdx.x - dealt;
-    const int seg = split ? (int)blockIdx.x % maps.segments : 0;
+    const bool split = x < dealt;
+    int tile = split ? x / maps.segments : maps.split_tiles + x - dealt;
+    if (rank)
+        tile = ranked_tile(gridDim.x, x, reinterpret_cast<int*>(smem + 2 * TILE), &ranked, [&](int first, int last) {
+            return first * 128 >= s.n ? 0 : seen_by(a, s, min(last * 128 + 127, s.n - 1)).hi - max(0, seen_by(a, s, first * 128).lo);
+        });
+    const int seg = split ? x % maps.segments : 0;
     const int k0 = tile * 128;
     int t_lo = max(0, k0 - a.right);                               // queries that see any of the keys
     int t_hi = k0 >= s.n ? t_lo : k0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)k0 + 128 + a.left);
@@ -573,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
         Steps at(a, t_lo, first);
         for (int i = 0; i < count; ++i, at.next(a)) {
             const int q0 = at.q0, b = i & 1;
-            const bool pads = mixed<FORM>(a, s, q0, q0 + 127);
+            const bool pads = FORM && !(q0 >= whole_lo && q0 + 127 <= whole_hi) && mixed<FORM>(a, s, q0, q0 + 127);
             const bool ragged = q0 + 127 >= s.n || k0 + 127 >= s.n || pads || key_pads;
             const bool edge = !(whole_lo <= q0 && q0 + 127 <= whole_hi && q0 + 127 < s.n && k0 + 127 < s.n);
             const float slope = has_slopes(FORM) ? slope_of(a, h * a.G + at.g) : 0.f;
@@ -857,6 +867,7 @@ int umma_window_bwd(const SeqArgs& a, int dtype, float* parts, cudaStream_t st) 
                       (a.rest.data && (rc = encode_rows(&maps.rest_rows, bf16, a.rest, a)))))
         return rc;
     maps.sms = sm_count();
+    maps.ranked = a.form.spans && (int64_t)((a.N + 127) / 128) * a.Hkv * a.B > maps.sms;      // else all blocks start at once
     if (!(maps.timeouts = stage_timeout_counter())) return cuda_fail(cudaGetLastError(), "cudaGetSymbolAddress(stage timeouts)");
     maps.dy_peak = parts;
     maps.v_peak = parts + dy_peaks(a);

@@ -84,6 +84,7 @@ int umma_window_fwd(const SeqArgs& a, int dtype, cudaStream_t st) {
     const int64_t rows = (int64_t)a.N * a.G;
     const bool pair = (rows + 255) / 256 * a.Hkv * a.B >= sm_count();
     const dim3 grid((unsigned)((rows + (pair ? 255 : 127)) / (pair ? 256 : 128)), a.Hkv, a.B);
+    maps.ranked = a.form.spans && (int64_t)grid.x * grid.y * grid.z > sm_count();             // else all blocks start at once
     return run(a, maps, dtype, pair, grid, st);
 }
 

@@ -29,13 +29,19 @@ struct FwdMaps {
     CUtensorMap k, v, q, y, rest;
     int rows;           // q, y and rest move by tiles of rows (maps), else by threads
     int box;            // paged: keys of a box
+    int ranked;         // dense: the largest tiles first
     int* timeouts;
 };
 
 namespace {
 
-// Two warpgroups of softmax, a warp that copies and one that issues the products.
-constexpr int kThreads = 320, kSoftmaxWarps = 8;
+// Warpgroups of softmax, a warp that copies and one that issues the products.  A stream has one warpgroup, a thread for each row; with
+// other scores two, a thread for each row and half of the keys: their arithmetic is twice that of plain scores, and two warps on a
+// scheduler leave half of its slots empty (16384 tokens, window 1024, bfloat16, cap: 262 us with two, 295 with one; slopes 287 and
+// 295; but other masks only 241 and 217).
+template <int FORM> constexpr int kGroups = has_cap(FORM) || has_slopes(FORM) ? 2 : 1;
+template <int FORM> constexpr int kSoftmaxWarps = 8 * kGroups<FORM>;
+template <int FORM> constexpr int kThreads = 32 * (kSoftmaxWarps<FORM> + 2);
 
 template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
 template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
@@ -93,7 +99,7 @@ __device__ __forceinline__ Stream stream_of(const SeqArgs& a, const Seq& s, cons
 }
 
 template <typename T, int DM, bool PAIR, bool PAGED, int FORM>
-__global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ FwdMaps maps) {
+__global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __grid_constant__ SeqArgs a, const __grid_constant__ FwdMaps maps) {
     // Dense calls with other scores or masks keep what rounding takes from the weights as a second 16-bit number, for one more
     // product with the values: where a few keys have most of the weight, their rounding would come out multiplied in delta = dy.y,
     // which the backward subtracts from each dy.v.  Calls over a cache have no gradients; there (ROUNDED) the weighted sum is divided
@@ -101,32 +107,43 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     // deviation 8, bfloat16: gradients off by 2.4e-3 of the norm with the second product, 2.6e-3 with the other sum, 3.5e-3 with
     // neither.
     constexpr bool SPLIT = FORM && !PAGED, ROUNDED = FORM && PAGED;
+    constexpr int GROUPS = kGroups<FORM>, WARPS = kSoftmaxWarps<FORM>, STREAM = 128 * GROUPS;      // STREAM: threads of a stream's softmax
     constexpr int S = kSlots<DM>;
     constexpr uint32_t TILE = kTileBytes<DM>;
     constexpr uint32_t IDESC_S = instr_desc(kIsBf16<T>, 128, false), IDESC_O = instr_desc(kIsBf16<T>, DM, true);
     extern __shared__ char raw[];
-    __shared__ uint64_t kv_full[S], kv_empty[S], q_full[2], s_full[2], p_full[2][2], o_full[2], drained;
+    __shared__ uint64_t kv_full[S], kv_empty[S], q_full[2], s_full[2], p_full[2][2], o_full[2], max_full[2], drained;
     __shared__ uint32_t tmem_slot, valid[S];
     __shared__ int stop_flag;
-    __shared__ float merge_m[128], merge_l[128], merge_r[ROUNDED ? 128 : 1];
+    __shared__ float merge_m[GROUPS == 1 ? 128 : 1], merge_l[GROUPS == 1 ? 128 : 1], merge_r[GROUPS == 1 && ROUNDED ? 128 : 1];
+    __shared__ __nv_bfloat16 part_max[GROUPS == 2 && FORM != kCap ? 2 : 1][2][128];
     volatile int* stop = &stop_flag;
 
     const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
     char* const smem = raw + (base_at - raw_at);
     const uint32_t q_at = base_at, kv_at = base_at + 2 * TILE;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
-    int tile = (int)(gridDim.x - 1 - blockIdx.x);       // the last rows see the most keys: first
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int tile = (int)(gridDim.x - 1 - blockIdx.x), h = blockIdx.y;       // the last rows see the most keys: first
     int2 owned;
     Seq s;
     if (PAGED) {
         owned = owned_tokens(a);
         if (!paged_seq(a, PAIR ? 256 : 128, tile, &s)) {
-            if (tid < 32 * kSoftmaxWarps) clear_unowned<T>(a, owned, h, tid, 32 * kSoftmaxWarps);
+            if (tid < 32 * WARPS) clear_unowned<T>(a, owned, h, tid, 32 * WARPS);
             return;
         }
     } else {
-        s = dense_seq(a, blockIdx.z);
+        __shared__ int ranked;
+        const bool rank = FORM && maps.ranked;
+        const Place place = rank ? place_by_rank() : Place{tile, (int)blockIdx.y, (int)blockIdx.z};
+        tile = place.x;
+        h = place.h;
+        s = dense_seq(a, place.b);
+        if (rank)
+            tile = ranked_tile(gridDim.x, tile, reinterpret_cast<int*>(smem + 2 * TILE), &ranked, [&](int first, int last) {
+                return row_work<FORM>(a, s, first * (PAIR ? 256 : 128), (last + 1) * (PAIR ? 256 : 128));
+            });
     }
     const int rows = s.T * a.G, R0 = tile * (PAIR ? 256 : 128);
     const int p_lo = max(0, s.base + R0 / a.G), p_hi = min(s.n - 1, s.base + (min(R0 + (PAIR ? 256 : 128), rows) - 1) / a.G);
@@ -135,14 +152,15 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     // Which key tiles a stream takes: with PAIR both see nearly the same, but each leaves out what all of its rows are blind to.
     const Stream st0 = stream_of<PAIR, FORM>(a, s, kt, 0, R0, rows), st1 = stream_of<PAIR, FORM>(a, s, kt, 1, PAIR ? R0 + 128 : R0, rows);
 
-    if (warp == 8 && lane == 0) {
+    if (warp == WARPS && lane == 0) {
         for (int i = 0; i < S; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
         for (int u = 0; u < 2; ++u) {
-            mbar_init(&q_full[u], maps.rows ? 1 : PAIR ? 4 : 8);
+            mbar_init(&q_full[u], maps.rows ? 1 : PAIR ? STREAM / 32 : WARPS);
             mbar_init(&s_full[u], 1);
-            mbar_init(&p_full[u][0], 4);
-            mbar_init(&p_full[u][1], 4);
+            mbar_init(&p_full[u][0], GROUPS == 2 && FORM != kCap ? 8 : 4);        // the other half's threads rescale their columns of the sum
+            mbar_init(&p_full[u][1], GROUPS == 2 && FORM != kCap ? 8 : 4);
             mbar_init(&o_full[u], 1);
+            mbar_init(&max_full[u], STREAM / 32);
         }
         mbar_init(&drained, 1);
         stop_flag = 0;
@@ -160,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         prefetch_map(&maps.k);
         prefetch_map(&maps.v);
     }
-    if (warp == 9) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (warp == WARPS + 1) tmem_alloc(smem_u32(&tmem_slot), 512);
     fence_before();
     __syncthreads();
     fence_after();
@@ -168,13 +186,14 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     // Scores of both streams, then their accumulators.  At 64 features there is room for weights beside the scores; at 128 they
     // overlay them, which needs the next scores to be written after the product with the weights has read them: products of
     // one shape (both 128 x 128 x 16 there) are carried out in the order of their issue.
-    // The weights of half a tile lie in its half of the columns, with the remainders behind them, or side by side.
-    const uint32_t s_col = tmem, o_col = tmem + 256, p_col = DM == 64 ? tmem + 384 : s_col, p_step = DM == 64 ? 64 : 128, p_half = SPLIT ? 64 : 32;
+    // Weights that are written by two warpgroups lie in the columns of their own scores: those of half a tile in its half.  With
+    // remainders those of 32 keys lie in 16 columns and their remainders in the next 16.
+    const uint32_t s_col = tmem, o_col = tmem + 256, p_col = DM == 64 ? tmem + 384 : s_col, p_step = DM == 64 ? 64 : 128, p_half = DM == 128 && (GROUPS == 2 || SPLIT) ? 64 : 32;
     static_assert(!SPLIT || DM == 128, "tensor memory has room for the remainders where weights lie over the scores");
 
-    if (warp < kSoftmaxWarps) {
+    if (warp < WARPS) {
         // ------------------------------------------------------------ softmax: thread = row
-        const int u = warp >> 2, r = tid & 127;
+        const int u = warp / (4 * GROUPS), g = GROUPS == 2 ? warp >> 2 & 1 : 0, r = tid & 127;      // stream, half of the keys, row
         const Stream st = u ? st1 : st0;
         const int R = R0 + (PAIR ? 128 * u : 0) + r;
         const int pos = s.base + token_of(a, R);
@@ -186,8 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             const int from = (int)min((int64_t)128, max((int64_t)0, -(int64_t)s.base * a.G - tile0));
             const int to = (int)min((int64_t)rows, ((int64_t)s.n - s.base) * a.G) - tile0;
             auto row = [&](int rr) { return seq_row<T>(a.q, a, s, h, min(tile0 + rr, rows - 1)); };
-            constexpr int THREADS = PAIR ? 128 : 256;
-            const int t = PAIR ? r : tid;
+            constexpr int THREADS = PAIR ? STREAM : 2 * STREAM;
+            const int t = tid % THREADS;
             uint4 w[TileCopy<DM, THREADS>::kCount];
             fetch_tile<T, DM, THREADS>(w, row, from, to, a.D, t);
 #pragma unroll
@@ -203,10 +222,12 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         // is enough.  Scores with a slope need the maximum of the changed ones: with a cap they return to tensor memory in units
         // of log2(e), without they are computed twice.
         constexpr bool BOUNDED = FORM == kCap, KEPT = FORM == kCapSlopes;
+        (void)KEPT;
         const float sl2 = has_cap(FORM) || has_slopes(FORM) ? 1.f : a.mag_log2, cap_in = fabsf(a.form.cap_in);
         const float slope = has_slopes(FORM) ? slope_of(a, h * a.G + R - token_of(a, R) * a.G) : 0.f;
         const CapPoly<T> poly(a, cap_in, a.form.cap_out);
         const Reach mine = reach<FORM>(a, s, pos);
+        const int doc_lo = document_of<FORM>(a, s, st.hi);
         const int c_lo = tile_reach<FORM>(a, s, p_lo).lo, c_hi = min(tile_reach<FORM>(a, s, p_hi).hi, s.n - 1);   // keys that any row of the CTA sees (or < sinks)
         // tiles from in_lo (or below in_sink) to in_hi need no mask
         const bool whole = st.lo == s.base + (R - r) / a.G && st.hi == s.base + (min(R - r + 128, rows) - 1) / a.G;
@@ -214,10 +235,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         float m = -INFINITY, l = 0.f, lr = 0.f;            // ROUNDED: lr is the sum of the rounded weights
         int done = 0;
         bool ok = true;
-        if (PAGED) clear_unowned<T>(a, owned, h, tid, 32 * kSoftmaxWarps);
+        if (PAGED) clear_unowned<T>(a, owned, h, tid, 32 * WARPS);
         for (int i = st.begin(); i <= st.upto; i = st.next(i)) {
             const int key0 = kt.key(i, 128), vslot = (2 * i + 1) % S;
-            const bool pads = mixed<FORM>(a, s, key0, key0 + 127);
+            const bool pads = FORM && (key0 < doc_lo || key0 + 127 > st.hi) && mixed<FORM>(a, s, key0, key0 + 127);
             const uint32_t vpar = ((2 * i + 1) / S) & 1;
             if (!warp_wait(smem_u32(&s_full[u]), done & 1, stop)) { ok = false; break; }
             fence_after();
@@ -229,51 +250,18 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             const int far = key0 + 127;
             const bool edge = !(key0 <= in_hi && (key0 >= in_lo || key0 < in_sink) && there == 0xff);
             const int hi = live ? min(mine.hi, s.n - 1) - key0 : -1, lo = mine.lo - key0, sk = a.sinks - key0;
-            auto scores = [&](int g, uint32_t* x) {                        // the columns 64 g .. 64 g + 63
-                tmem_ld32(S_at + 64 * g, x);
-                tmem_ld32(S_at + 64 * g + 32, x + 32);
-                tmem_wait_ld();
-                settled32(x);
-                settled32(x + 32);
-            };
             // Bits of the columns at .. at + 31 that the row sees
             auto seen = [&](int at) {
                 uint32_t mk = seen_bits(lo - at, hi - at, sk - at);
                 if (PAGED) mk &= ((there >> (at / 16)) & 1 ? 0xffffu : 0u) | ((there >> (at / 16 + 1)) & 1 ? 0xffff0000u : 0u);
                 return mk;
             };
-            const int side = far <= st.lo ? 1 : key0 >= st.hi ? -1 : 0;    // of the keys, for all rows
-            // 32 columns of changed scores
-            auto changed = [&](int at, uint32_t* x) {
-                if (BOUNDED) poly.template scores<32>(x, edge, edge ? seen(at) : ~0u);
-                else if (has_cap(FORM)) cap_scores<T, 32>(x, cap_in, a.form.cap_out, edge, edge ? seen(at) : ~0u);
-                if (has_slopes(FORM)) slope_scores<32>(x, has_cap(FORM) ? 1.f : a.mag_log2, slope, (float)(pos - key0 - at), side);
-            };
-            auto hide = [&](int at, uint32_t* x) {
-                const uint32_t mk = seen(at);
-#pragma unroll
-                for (int c = 0; c < 32; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0xff800000u;
-            };
-            // The same for the maximum: -inf where the row does not see the key, written back for the exponentials
-            auto masked_scores = [&](int g, uint32_t* x) {
-                scores(g, x);
-                if (has_cap(FORM) || has_slopes(FORM)) {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) changed(64 * g + 32 * q, x + 32 * q);
-                }
-                if (edge || KEPT) {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        if (!KEPT || edge) hide(64 * g + 32 * q, x + 32 * q);
-                        if (FORM != kSlopes) tmem_st32(S_at + 64 * g + 32 * q, x + 32 * q);
-                    }
-                }
-            };
-            // values that no row sees may be anything (a page that was freed, tokens behind the length): zeros
+            // values that no row sees may be anything (a page that was freed, tokens behind the length, padding): zeros; of two
+            // warpgroups each clears those of its half of the keys, which are all that the product with its weights reads
             if (!((key0 >= c_lo || far < a.sinks) && far <= c_hi && there == 0xff) || pads) {
                 if (!PAGED && !warp_wait(smem_u32(&kv_full[vslot]), vpar, stop)) { ok = false; break; }
                 const int j = key0 + r;
-                if (!(j <= c_hi && (j >= c_lo || j < a.sinks) && (there >> (r >> 4) & 1)) || (pads && padding<FORM>(a, s, j))) {
+                if ((GROUPS == 1 || r >> 6 == g) && (!(j <= c_hi && (j >= c_lo || j < a.sinks) && (there >> (r >> 4) & 1)) || (pads && padding<FORM>(a, s, j)))) {
 #pragma unroll 1
                     for (int p = 0; p < DM / 64; ++p)
 #pragma unroll
@@ -282,31 +270,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 }
                 fence_async_smem();
             }
-            float mx = BOUNDED ? 0.f : -INFINITY;
+            // Columns from..to - 1 of the weighted sum, by the factor of a new reference.  The scores came after the previous weighted
+            // sum, which is therefore complete.
+            auto rescale = [&](int from, int to, float f) {
 #pragma unroll 1
-            for (int g = 0; g < (BOUNDED ? 0 : 2); ++g) {
-                if (!st.sees_half(a, key0 + 64 * g)) continue;
-                uint32_t x[64];
-                masked_scores(g, x);
-                float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 64; c += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]));
-                mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            }
-            tmem_wait_st();
-            mx *= sl2;
-            float f = 1.f;
-            const bool grew = mx > m + 8.f;                                // also from -inf
-            if (grew) {
-                f = fast_exp2(m - mx);
-                m = mx;
-            }
-            if (done && __any_sync(~0u, grew)) {
-                // the scores came after the previous weighted sum, which is therefore complete
-#pragma unroll 1
-                for (int c = 0; c < DM; c += 32) {
+                for (int c = from; c < to; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(O_at + c, o);
                     tmem_wait_ld();
@@ -315,55 +283,199 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                     tmem_st32(O_at + c, o);
                 }
-            }
-            const float ref = m == -INFINITY ? 0.f : m;                    // a row that has seen nothing yet
-            const f32x2 sc2 = pack2(sl2, sl2), ref2 = pack2(-ref, -ref);
-            f32x2 sum2 = pack2(l * f, 0.f), round2 = pack2(lr * f, 0.f);
+            };
+            auto given = [&](float mx) {                                   // a reference for scores up to mx; the factor for what is there
+                float f = 1.f;
+                if (mx > m + 8.f) {                                        // also from -inf
+                    f = fast_exp2(m - mx);
+                    m = mx;
+                }
+                return f;
+            };
+            // What rounding took from a pair of weights, or the sum of the rounded ones
+            auto remainder = [&](uint32_t w, float e0, float e1, f32x2& round2, uint32_t& rest) {
+                float w0, w1;
+                unpack16<T>(w, w0, w1);
+                if (ROUNDED) round2 = add2(round2, pack2(w0, w1));
+                if (SPLIT) {
+                    unpack2(fma2(pack2(w0, w1), pack2(-1.f, -1.f), pack2(e0, e1)), w0, w1);
+                    rest = pack16<T>(w0, w1);
+                }
+            };
+            if constexpr (GROUPS == 1) {
+                auto scores = [&](int g, uint32_t* x) {                    // the columns 64 g .. 64 g + 63
+                    tmem_ld32(S_at + 64 * g, x);
+                    tmem_ld32(S_at + 64 * g + 32, x + 32);
+                    tmem_wait_ld();
+                    settled32(x);
+                    settled32(x + 32);
+                };
+                // The same for the maximum: -inf where the row does not see the key, written back for the exponentials
+                auto masked_scores = [&](int g, uint32_t* x) {
+                    scores(g, x);
+                    if (edge) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const int at = 64 * g + 32 * q;
+                            const uint32_t mk = seen(at);
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) x[32 * q + c] = (mk >> c) & 1 ? x[32 * q + c] : 0xff800000u;
+                            tmem_st32(S_at + at, x + 32 * q);
+                        }
+                    }
+                };
+                float mx = -INFINITY;
 #pragma unroll 1
-            for (int g = 0; g < 2; ++g) {
-                if (!st.sees_half(a, key0 + 64 * g)) continue;
-                uint32_t x[64], w[32], rest[SPLIT ? 32 : 1];
-                scores(g, x);
-                if (BOUNDED || FORM == kSlopes) {
+                for (int g = 0; g < 2; ++g) {
+                    if (!st.sees_half(a, key0 + 64 * g)) continue;
+                    uint32_t x[64];
+                    masked_scores(g, x);
+                    float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        changed(64 * g + 32 * q, x + 32 * q);
-                        if (edge) hide(64 * g + 32 * q, x + 32 * q);
-                    }
-                }
+                    for (int c = 0; c < 64; c += 8)
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    float e0, e1;
-                    if (BOUNDED) e0 = __uint_as_float(x[2 * c]), e1 = __uint_as_float(x[2 * c + 1]);
-                    else if (FORM == kSlopes || KEPT) unpack2(add2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), ref2), e0, e1);
-                    else unpack2(fma2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), sc2, ref2), e0, e1);
-                    // The exponential unit and the tensor pipe take the same 2048 cycles a pair of tiles; a quarter of the
-                    // exponentials as polynomials: 443 -> 418 us for a sequence of 16384 (an eighth: 431, a half: 430).
-                    // Polynomials for the cap fill the FMA pipe: no quarter then.
-                    if (c % 4 == 3 && !has_cap(FORM)) {
-                        unpack2(exp2_fma<T>(e0, e1), e0, e1);
-                    } else {
-                        e0 = fast_exp2(e0);
-                        e1 = fast_exp2(e1);
-                    }
-                    sum2 = add2(sum2, pack2(e0, e1));
-                    w[c] = pack16<T>(e0, e1);
-                    if (ROUNDED) round2 = add2(round2, pack2(low16<T>(w[c]), high16<T>(w[c])));
-                    if (SPLIT) rest[c] = pack16<T>(e0 - low16<T>(w[c]), e1 - high16<T>(w[c]));
+                        for (int e = 0; e < 4; ++e) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]));
+                    mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 }
-                if (SPLIT) tmem_st32(P_at + p_half * g + 32, rest);
-                tmem_st32(P_at + p_half * g, w);                               // at 128 features over scores that this warp has read twice
                 tmem_wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&p_full[u][g]));       // the product with the first half may start
-            }
-            float a0, a1;
-            unpack2(sum2, a0, a1);
-            l = a0 + a1;
-            if (ROUNDED) {
+                const float before = m, f = given(mx * sl2);
+                if (done && __any_sync(~0u, m != before)) rescale(0, DM, f);
+                const float ref = m == -INFINITY ? 0.f : m;                // a row that has seen nothing yet
+                const f32x2 sc2 = pack2(sl2, sl2), ref2 = pack2(-ref, -ref);
+                f32x2 sum2 = pack2(l * f, 0.f), round2 = pack2(lr * f, 0.f);
+#pragma unroll 1
+                for (int g = 0; g < 2; ++g) {
+                    if (!st.sees_half(a, key0 + 64 * g)) continue;
+                    uint32_t x[64], w[32], rest[SPLIT ? 32 : 1];
+                    scores(g, x);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        float e0, e1;
+                        unpack2(fma2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), sc2, ref2), e0, e1);
+                        // The exponential unit and the tensor pipe take the same 2048 cycles a pair of tiles; a quarter of the
+                        // exponentials as polynomials: 443 -> 418 us for a sequence of 16384 (an eighth: 431, a half: 430).
+                        if (c % 4 == 3) {
+                            unpack2(exp2_fma<T>(e0, e1), e0, e1);
+                        } else {
+                            e0 = fast_exp2(e0);
+                            e1 = fast_exp2(e1);
+                        }
+                        sum2 = add2(sum2, pack2(e0, e1));
+                        w[c] = pack16<T>(e0, e1);
+                        if (ROUNDED || SPLIT) remainder(w[c], e0, e1, round2, rest[SPLIT ? c : 0]);
+                    }
+                    if (SPLIT) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            tmem_st16(P_at + p_half * g + 32 * q, w + 16 * q);
+                            tmem_st16(P_at + p_half * g + 32 * q + 16, rest + (SPLIT ? 16 * q : 0));
+                        }
+                    } else
+                    tmem_st32(P_at + p_half * g, w);                       // at 128 features over scores that this warp has read twice
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&p_full[u][g]));   // the product with the first half may start
+                }
+                float a0, a1;
+                unpack2(sum2, a0, a1);
+                l = a0 + a1;
                 unpack2(round2, a0, a1);
                 lr = a0 + a1;
+            } else {
+                const bool own = st.sees_half(a, key0 + 64 * g), others = st.sees_half(a, key0 + 64 - 64 * g);
+                const int side = far <= st.lo ? 1 : key0 >= st.hi ? -1 : 0;        // of the keys, for all rows
+                // 32 columns from 64 g + 32 q as they go into the exponential, but for the reference; hidden ones are -inf
+                auto scores = [&](int q, uint32_t* x, bool kept) {
+                    const int at = 64 * g + 32 * q;
+                    tmem_ld32(S_at + at, x);
+                    tmem_wait_ld();
+                    settled32(x);
+                    if (kept) return;
+                    const uint32_t mk = edge ? seen(at) : ~0u;
+                    if (BOUNDED)
+                        poly.template scores<32>(x, edge, mk, [&] {
+                            tmem_ld32(S_at + at, x);
+                            tmem_wait_ld();
+                            settled32(x);
+                        });
+                    else if (has_cap(FORM)) cap_scores<T, 32>(x, cap_in, a.form.cap_out, edge, mk);
+                    if (has_slopes(FORM)) slope_scores<32>(x, has_cap(FORM) ? 1.f : a.mag_log2, slope, (float)(pos - key0 - at), side);
+                    if (edge) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0xff800000u;
+                    }
+                };
+                float f = 1.f;
+                if (BOUNDED) {
+                    m = 0.f;
+                } else {
+                    float mx = -INFINITY;
+                    if (own) {
+#pragma unroll 1
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t x[32];
+                            scores(q, x, false);
+                            if (KEPT) tmem_st32(S_at + 64 * g + 32 * q, x);
+                            float top[2] = {mx, -INFINITY};
+#pragma unroll
+                            for (int c = 0; c < 32; c += 4)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 2 + e]));
+                            mx = fmaxf(top[0], top[1]);
+                        }
+                    }
+                    tmem_wait_st();
+                    // Both halves' maxima, rounded (which the reference stands) so that they fit: the tiles take all but 2 KB
+                    part_max[u][g][r] = __float2bfloat16_rn(mx * sl2);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&max_full[u]));
+                    if (!warp_wait(smem_u32(&max_full[u]), done & 1, stop)) { ok = false; break; }
+                    const float before = m;
+                    f = given(fmaxf(__bfloat162float(part_max[u][0][r]), __bfloat162float(part_max[u][1][r])));
+                    if (done && __any_sync(~0u, m != before)) rescale(DM / 2 * g, DM / 2 * (g + 1), f);
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0 && others) mbar_arrive(smem_u32(&p_full[u][1 - g]));
+                }
+                if (own) {
+                    const float ref = m == -INFINITY ? 0.f : m;            // a row that has seen nothing yet
+                    const f32x2 sc2 = pack2(sl2, sl2), ref2 = pack2(-ref, -ref);
+                    f32x2 sum2 = pack2(l * f, 0.f), round2 = pack2(lr * f, 0.f);
+#pragma unroll 1
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t x[32], w[16], rest[SPLIT ? 16 : 1];
+                        scores(q, x, KEPT);
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) {
+                            float e0, e1;
+                            if (BOUNDED) e0 = __uint_as_float(x[2 * c]), e1 = __uint_as_float(x[2 * c + 1]);
+                            else if (FORM != kMasks) unpack2(add2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), ref2), e0, e1);
+                            else unpack2(fma2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), sc2, ref2), e0, e1);
+                            e0 = fast_exp2(e0);
+                            e1 = fast_exp2(e1);
+                            sum2 = add2(sum2, pack2(e0, e1));
+                            w[c] = pack16<T>(e0, e1);
+                            remainder(w[c], e0, e1, round2, rest[SPLIT ? c : 0]);
+                        }
+                        const uint32_t to = P_at + p_half * g + (SPLIT ? 32 : 16) * q;
+                        tmem_st16(to, w);
+                        if (SPLIT) tmem_st16(to + 16, rest);
+                    }
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&p_full[u][g]));
+                    float a0, a1;
+                    unpack2(sum2, a0, a1);
+                    l = a0 + a1;
+                    unpack2(round2, a0, a1);
+                    lr = a0 + a1;
+                } else {
+                    l *= f;
+                    lr *= f;
+                }
             }
             ++done;
         }
@@ -376,15 +488,28 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
         float f0 = 1.f, f1 = 0.f;
         float* const other = reinterpret_cast<float*>(smem + 2 * TILE);    // [column][row] of the odd stream, in the ring's place
         const bool keep_rest = !PAGED && a.rest.data;
-        if (!PAIR || keep_rest) group_sync<256>(1);                        // both streams are through with the ring
+        if (!PAIR || keep_rest || GROUPS == 2) group_sync<2 * STREAM>(1);  // both streams are through with the ring
+        // two warpgroups: what their halves of the keys summed up, in the ring's last slot; the reference is the same
+        float* const sums = reinterpret_cast<float*>(smem + (1 + S) * TILE);                // [stream][half][row]
+        if (GROUPS == 2) {
+            sums[(2 * u + g) * 128 + r] = l;
+            sums[512 + (2 * u + g) * 128 + r] = lr;
+            sums[1024 + u * 128 + r] = m;
+            group_sync<2 * STREAM>(1);
+            l = sums[2 * u * 128 + r] + sums[(2 * u + 1) * 128 + r];
+            lr = sums[512 + 2 * u * 128 + r] + sums[512 + (2 * u + 1) * 128 + r];
+        }
+        const int col_from = DM / GROUPS * g, col_to = DM / GROUPS * (g + 1);               // the thread's columns of the results
         if (!PAIR) {
             if (u == 1) {
-                merge_m[r] = m;
-                merge_l[r] = l;
-                if (ROUNDED) merge_r[r] = lr;
+                if (GROUPS == 1) {
+                    merge_m[r] = m;
+                    merge_l[r] = l;
+                    if (ROUNDED) merge_r[r] = lr;
+                }
                 if (done && ok) {
 #pragma unroll 1
-                    for (int c = 0; c < DM; c += 32) {
+                    for (int c = col_from; c < col_to; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(O_at + c, o);
                         tmem_wait_ld();
@@ -394,12 +519,13 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                     }
                 }
             }
-            group_sync<256>(1);
-            const float m1 = merge_m[r], l1 = merge_l[r], M = fmaxf(m, m1), ref = M == -INFINITY ? 0.f : M;
+            group_sync<2 * STREAM>(1);
+            const float m1 = GROUPS == 2 ? sums[1024 + 128 + r] : merge_m[r], l1 = GROUPS == 2 ? sums[256 + r] + sums[384 + r] : merge_l[r];
+            const float M = fmaxf(m, m1), ref = M == -INFINITY ? 0.f : M;
             f0 = fast_exp2(m - ref);
             f1 = fast_exp2(m1 - ref);
             l = l * f0 + l1 * f1;
-            if (ROUNDED) lr = lr * f0 + merge_r[r] * f1;
+            if (ROUNDED) lr = lr * f0 + (GROUPS == 2 ? sums[512 + 256 + r] + sums[512 + 384 + r] : merge_r[r]) * f1;
             m = M;
         }
         if (PAIR || u == 0) {
@@ -408,13 +534,13 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             if (!ok || *stop) inv = __int_as_float(0x7fffffff);            // a wait ran out: NaN, never a wrong number
             // Rows that see nothing are zeros by choice, not by their weights: 0 * inf of a value that other rows see is not a number.
             const bool none = !done || l == 0.f, both = !PAIR && kt.count > 1 && !none;
-            if (!PAGED && a.lse && have) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = l > 0.f ? m + log2f(l) : -INFINITY;
+            if (!PAGED && a.lse && have && g == 0) a.lse[((int64_t)s.b * a.Hkv + h) * rows + R] = l > 0.f ? m + log2f(l) : -INFINITY;
             const float w0 = f0 * inv, w1 = f1 * inv;
             // y goes to the queries' place (their last scores are done), what rounding took to a slot of the ring
             const int tile0 = R - r;
             char *const out = smem + (PAIR ? u : 0) * TILE, *const out_rest = smem + (2 + (PAIR ? u : 2)) * TILE;
 #pragma unroll 1
-            for (int c = 0; c < DM; c += 32) {
+            for (int c = col_from; c < col_to; c += 32) {
                 uint32_t o[32];
                 tmem_ld32(O_at + c, o);
                 tmem_wait_ld();
@@ -438,10 +564,10 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 }
             }
             fence_async_smem();
-            group_sync<128>(2 + u);
+            group_sync<STREAM>(2 + u);
             // by maps, which leave out tokens behind the tensor's; a cache's packed rows go on with the next sequence
             if (maps.rows && (!PAGED || tile0 + 128 <= rows)) {
-                if (r == 0 && tile0 < rows) {
+                if (r == 0 && g == 0 && tile0 < rows) {
                     const int token = s.t0 + tile0 / a.G, b = PAGED ? 0 : s.b;
 #pragma unroll
                     for (int p = 0; p < DM / 64; ++p) {
@@ -453,11 +579,11 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
                 }
             } else {
                 auto row = [&](const ca_seq_view& v) { return [&](int rr) { return seq_row<T>(v, a, s, h, max(tile0 + rr, 0)); }; };
-                store_tile<T, DM, 128>(out, row(a.y), rows - tile0, a.D, r);
-                if (keep_rest) store_tile<T, DM, 128>(out_rest, row(a.rest), rows - tile0, a.D, r);
+                store_tile<T, DM, STREAM>(out, row(a.y), rows - tile0, a.D, tid % STREAM);
+                if (keep_rest) store_tile<T, DM, STREAM>(out_rest, row(a.rest), rows - tile0, a.D, tid % STREAM);
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == WARPS) {
         // ------------------------------------------------------------ copies
         int issued = 0;
         if (!PAGED) {
@@ -504,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             for (int u = 0; u < (PAIR ? 2 : 1) && R0 + 128 * u < rows; ++u) mbar_wait(smem_u32(&q_full[u]), 0, 1u << 12);
         if (lane == 0)                                                     // copies in flight land before the memory goes away
             for (int i = max(0, issued - S); i < issued; ++i) mbar_wait(smem_u32(&kv_full[i % S]), (i / S) & 1, 1u << 12);
-    } else if (warp == 9) {
+    } else if (warp == WARPS + 1) {
         // ------------------------------------------------------------ products: the warp in step, one lane issues
         const uint32_t lead = elect_one();
         const uint64_t q_desc = desc_features(q_at), k_desc = desc_features(kv_at), v_desc = desc_rows(kv_at);
@@ -534,18 +660,30 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
             // the weights are what is late: everything else is waited for first.  The next keys' slot was freed by products
             // that came before (a stream is at most two tiles ahead, and the ring holds five).
             if (!landed(nx <= st.upto ? 2 * nx : 2 * i + 1)) return false;
+            // the product with half a tile's weights; with remainders 32 keys at a time
+            auto add_half = [&](uint32_t half) {
+                const uint32_t to = o_col + u * DM, from = p_col + u * p_step + p_half * half;
+                const uint64_t values = v_desc + slot * (TILE >> 4) + half * (4 * 128);
+                if (SPLIT) {
+#pragma unroll
+                    for (uint32_t q = 0; q < 2; ++q) {
+                        mma_weighted<32>(lead, to, from + 32 * q, values + q * (2 * 128), IDESC_O, n.low + n.high != 0 || q);
+                        mma_weighted<32>(lead, to, from + 32 * q + 16, values + q * (2 * 128), IDESC_O, true);
+                    }
+                } else {
+                    mma_weighted<64>(lead, to, from, values, IDESC_O, n.low + n.high != 0);
+                }
+            };
             if (st.sees_half(a, key0)) {
                 if (!warp_wait(smem_u32(&p_full[u][0]), n.low & 1, stop)) return false;
                 fence_after();
-                mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step, v_desc + slot * (TILE >> 4), IDESC_O, n.low + n.high != 0);
-                if (SPLIT) mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step + 32, v_desc + slot * (TILE >> 4), IDESC_O, true);
+                add_half(0);
                 ++n.low;
             }
             if (st.sees_half(a, key0 + 64)) {
                 if (!warp_wait(smem_u32(&p_full[u][1]), n.high & 1, stop)) return false;
                 fence_after();
-                mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step + p_half, v_desc + slot * (TILE >> 4) + 4 * 128, IDESC_O, n.low + n.high != 0);
-                if (SPLIT) mma_weighted<64>(lead, o_col + u * DM, p_col + u * p_step + p_half + 32, v_desc + slot * (TILE >> 4) + 4 * 128, IDESC_O, true);
+                add_half(1);
                 ++n.high;
             }
             if (!PAIR || u == 1 || !st1.takes(i)) mma_commit(lead, smem_u32(&kv_empty[slot]));
@@ -581,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1) umma_fwd_kernel(const __grid_cons
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 9) tmem_free(tmem, 512);
+    if (warp == WARPS + 1) tmem_free(tmem, 512);
     if (tid == 0 && stop_flag) report_stop(maps.timeouts, a.status);
 }
 
@@ -589,7 +727,7 @@ template <typename T, int DM, bool PAIR, bool PAGED, int FORM>
 int launch(const SeqArgs& a, const FwdMaps& maps, dim3 grid, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(umma_fwd_kernel<T, DM, PAIR, PAGED, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFwdSmem<DM>);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-    umma_fwd_kernel<T, DM, PAIR, PAGED, FORM><<<grid, kThreads, kFwdSmem<DM>, st>>>(a, maps);
+    umma_fwd_kernel<T, DM, PAIR, PAGED, FORM><<<grid, kThreads<FORM>, kFwdSmem<DM>, st>>>(a, maps);
     count_tensor_launch();
     CA_CHECK_LAUNCH("window forward kernel (tensor cores)");
     return CA_OK;

@@ -23,6 +23,18 @@ template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float h
 template <typename T> __device__ __forceinline__ float low16(uint32_t w) { return to_float(reinterpret_cast<const T*>(&w)[0]); }
 template <typename T> __device__ __forceinline__ float high16(uint32_t w) { return to_float(reinterpret_cast<const T*>(&w)[1]); }
 
+// Both at once, by their bits where that is enough.
+template <typename T> __device__ __forceinline__ void unpack16(uint32_t w, float& lo, float& hi) {
+    if (kIsBf16<T>) {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xffff0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        lo = f.x;
+        hi = f.y;
+    }
+}
+
 // The larger of two numbers; not a number if one of them is not
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -111,6 +123,33 @@ template <typename T> struct CapPoly {
         const float f = cap_in < 0.f ? -out : out;
 #pragma unroll
         for (int i = 0; i <= DEGREE; ++i) k[i] = a.form.poly[i] * f;
+    }
+    // `again` reads x once more, for a warp that holds a score beyond the cap: the squares, which the polynomial needs anyway, tell.
+    template <int COUNT, typename Again>
+    __device__ __forceinline__ void scores(uint32_t* x, bool edge, uint32_t mk, Again again) const {
+        if (edge) {
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0u;
+        }
+        float big = 0.f;
+#pragma unroll
+        for (int c = 0; c < COUNT; c += 2) {
+            const f32x2 s = pack2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), u = mul2(s, s);
+            float u0, u1, z0, z1;
+            unpack2(u, u0, u1);
+            big = fmaxf(fmaxf(big, u0), u1);
+            f32x2 p = pack2(k[DEGREE], k[DEGREE]);
+#pragma unroll
+            for (int i = DEGREE - 1; i >= 0; --i) p = fma2(p, u, pack2(k[i], k[i]));
+            unpack2(mul2(p, s), z0, z1);
+            x[c] = __float_as_uint(z0);
+            x[c + 1] = __float_as_uint(z1);
+        }
+        if (__any_sync(~0u, big * cap_in * cap_in > 1.f)) {
+            again();
+#pragma unroll
+            for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(tanh_far(__uint_as_float(x[c]) * cap_in) * out);
+        }
     }
     template <int COUNT>
     __device__ __forceinline__ void scores(uint32_t* x, bool edge, uint32_t mk) const {
