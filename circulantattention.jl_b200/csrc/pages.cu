@@ -17,15 +17,19 @@ namespace cg = cooperative_groups;
 namespace ca {
 namespace {
 
-constexpr int kThreads = 1024, kBlocks = 8, kMovePools = 32;
+constexpr int kThreads = 1024, kBlocks = 16, kMovePools = 32;
 
 struct PageArgs {
     ca_table t;
     const int *starts, *parents;
     int left, sinks;
     int *table, *refs, *lengths, *result;       // the next state; result: pages that were wanting, or pages in use
-    int *list, *source, *target, *keeper, *offset, *moves;
+    int *list, *source, *target, *keeper, *need, *offset, *moves;      // offset: for each block
 };
+
+// The copies' kernel may begin: it waits where it needs what this one lists.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 struct Team {
     cg::cluster_group cluster;
@@ -34,14 +38,11 @@ struct Team {
         thread = rank * kThreads + threadIdx.x;
         threads = ranks * kThreads;
     }
-    // Everything that the cluster's threads wrote before is seen behind this
-    __device__ __forceinline__ void sync() const {
-        __threadfence();
-        cluster.sync();
-    }
-    // Sum of v over the threads before this one, and over all of them
-    __device__ int2 scan(int v) const {
-        __shared__ int warps[kThreads / 32], block;
+    // Everything that the cluster's threads wrote before is seen behind this (by loads that pass by the L1 cache)
+    __device__ __forceinline__ void sync() const { cluster.sync(); }
+    // Sum of v over the block's threads before this one, and over all of them
+    __device__ int2 block_scan(int v) const {
+        __shared__ int warps[kThreads / 32];
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         int upto = v;
 #pragma unroll
@@ -49,23 +50,34 @@ struct Team {
             const int x = __shfl_up_sync(~0u, upto, o);
             if (lane >= o) upto += x;
         }
+        __syncthreads();                                        // the sums of a scan before have been read
         if (lane == 31) warps[warp] = upto;
         __syncthreads();
-        int before = 0, all = 0;
-        for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) before += warps[w];
-            all += warps[w];
+        int sum = warps[lane];                               // every warp scans the warps' sums
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += x;
         }
-        if (threadIdx.x == 0) block = all;
+        const int before = __shfl_sync(~0u, sum, max(warp - 1, 0));
+        return make_int2((warp ? before : 0) + upto - v, __shfl_sync(~0u, sum, 31));
+    }
+    // The same over the cluster.  SLOT: one for each scan of a kernel, so that no barrier has to guard the totals; a kernel's last
+    // scan is followed by a barrier.
+    template <int SLOT>
+    __device__ int2 scan(int v) const {
+        __shared__ int total[2];
+        const int2 own = block_scan(v);
+        if (ranks == 1) return own;
+        if (threadIdx.x == 0) total[SLOT] = own.y;
         cluster.sync();
-        int total = 0;
+        int before = own.x, all = 0;
         for (int r = 0; r < ranks; ++r) {
-            const int x = *cluster.map_shared_rank(&block, r);
+            const int x = *cluster.map_shared_rank(&total[SLOT], r);
             if (r < rank) before += x;
-            total += x;
+            all += x;
         }
-        cluster.sync();                                         // the totals have been read
-        return make_int2(before + upto - v, total);
+        return make_int2(before, all);
     }
 };
 
@@ -78,16 +90,77 @@ __device__ __forceinline__ int2 share(const Team& team, int n) {
 
 __device__ __forceinline__ bool is_page(const ca_table& t, int e) { return e >= 0 && e < t.pages; }
 
+// The places of the table, a warp for 128 places of one sequence: body(sequence, whatever of(sequence) is, place, index in the table).
+constexpr int kPlaces = 128;
+template <typename Of, typename Body>
+__device__ __forceinline__ void for_places(const PageArgs& a, const Team& team, Of of, Body body) {
+    const int W = a.t.width, pieces = (W + kPlaces - 1) / kPlaces, lane = threadIdx.x & 31;
+    const int64_t units = (int64_t)pieces * a.t.sequences;
+    for (int64_t unit = team.thread >> 5; unit < units; unit += team.threads >> 5) {
+        const int s = units <= INT32_MAX ? (int)((uint32_t)unit / (uint32_t)pieces) : (int)(unit / pieces), c0 = (int)(unit - (int64_t)s * pieces) * kPlaces + lane;
+        const auto x = of(s);
+        int e[kPlaces / 32];
+#pragma unroll
+        for (int k = 0; k < kPlaces / 32; ++k) e[k] = c0 + 32 * k < W ? a.t.table[(int64_t)s * W + c0 + 32 * k] : -1;
+#pragma unroll
+        for (int k = 0; k < kPlaces / 32; ++k)
+            if (c0 + 32 * k < W) body(s, x, c0 + 32 * k, (int64_t)s * W + c0 + 32 * k, e[k]);
+    }
+}
+
+// The warp's share of the pages: whole groups of 32, so that its loads are of neighbours.
+__device__ __forceinline__ int2 warp_pages(const PageArgs& a, const Team& team) {
+    const int warps = team.threads >> 5, groups = (a.t.pages + 31) / 32, piece = (groups + warps - 1) / warps * 32;
+    const int64_t at = (int64_t)piece * (team.thread >> 5);
+    return make_int2((int)min((int64_t)a.t.pages, at), (int)min((int64_t)a.t.pages, at + piece));
+}
+// How many of the warp's pages are `picked`; known to its first lane, which stands for the warp in a scan.
+template <typename Picked>
+__device__ __forceinline__ int count_pages(int2 mine, Picked picked) {
+    const int lane = threadIdx.x & 31;
+    int count = 0;
+#pragma unroll 4
+    for (int i = mine.x + lane; i < mine.y; i += 32) count += picked(i);
+    count = __reduce_add_sync(~0u, count);
+    return lane == 0 ? count : 0;
+}
+// body(page, picked or not, pages picked before it) for the warp's pages, of which `before` come earlier; the warp in step.
+template <typename Picked, typename Body>
+__device__ __forceinline__ void number_pages(int2 mine, int before, Picked picked, Body body) {
+    const int lane = threadIdx.x & 31;
+    before = __shfl_sync(~0u, before, 0);
+    for (int i0 = mine.x; i0 < mine.y; i0 += 32) {
+        const int i = i0 + lane;
+        const bool on = i < mine.y && picked(i);
+        const unsigned all = __ballot_sync(~0u, on);
+        if (i < mine.y) body(i, on, before + __popc(all & ((1u << lane) - 1)));
+        before += __popc(all);
+    }
+}
+
 // Lists the lowest `wanted` pages without users; returns how many of them there are.
 __device__ int list_free(const PageArgs& a, const Team& team, int wanted) {
-    const int2 mine = share(team, a.t.pages);
-    int count = 0;
-    for (int i = mine.x; i < mine.y; ++i) count += __ldcg(a.refs + i) <= 0;
-    const int2 rank = team.scan(count);
-    int at = rank.x;
-    for (int i = mine.x; i < mine.y && at < wanted; ++i)
-        if (__ldcg(a.refs + i) <= 0) a.list[at++] = i;
+    const int2 mine = warp_pages(a, team);
+    auto free = [&](int i) { return __ldcg(a.refs + i) <= 0; };
+    const int2 rank = team.scan<0>(count_pages(mine, free));
+    number_pages(mine, rank.x, free, [&](int i, bool on, int at) {
+        if (on && at < wanted) a.list[at] = i;
+    });
     return min(rank.y, wanted);
+}
+
+// Sums over the sequences before each, in place; every block does it for itself and returns the sum of all.
+__device__ int offsets(const PageArgs& a, const Team& team, int* offset) {
+    const int S = a.t.sequences, piece = (S + kThreads - 1) / kThreads;
+    const int from = min(S, piece * (int)threadIdx.x), to = min(S, from + piece);
+    int count = 0;
+    for (int s = from; s < to; ++s) count += __ldcg(a.need + s);
+    int2 rank = team.block_scan(count);
+    for (int s = from; s < to; ++s) {
+        offset[s] = rank.x;                                     // alike in all blocks
+        rank.x += __ldcg(a.need + s);
+    }
+    return rank.y;
 }
 
 // ---------------------------------------------------------------- a serving step
@@ -95,13 +168,13 @@ __device__ int list_free(const PageArgs& a, const Team& team, int wanted) {
 struct Stay {
     int first, upto, sinks, fresh;
     __device__ __forceinline__ Stay(const PageArgs& a, int s) {
-        const int page = a.t.page;
-        const int64_t n = max(0, a.t.lengths[s]), count = (int64_t)a.starts[s + 1] - a.starts[s];
-        const int64_t begin = max((int64_t)0, n - max((int64_t)0, count));
-        upto = (int)min((int64_t)a.t.width, (n + page - 1) / page);
-        first = a.left < 0 ? 0 : (int)(max((int64_t)0, begin - a.left) / page);
-        sinks = (int)((min((int64_t)a.sinks, n) + page - 1) / page);
-        fresh = count > 0 ? (int)min((int64_t)upto, begin / page) : upto;
+        const uint32_t page = a.t.page, n = max(0, a.t.lengths[s]);
+        const int64_t count = (int64_t)a.starts[s + 1] - a.starts[s];
+        const uint32_t begin = (uint32_t)max((int64_t)0, n - max((int64_t)0, count));
+        upto = (int)min((uint32_t)a.t.width, (n + page - 1) / page);
+        first = a.left < 0 ? 0 : (int)(begin > (uint32_t)a.left ? (begin - a.left) / page : 0);
+        sinks = (int)((min((uint32_t)a.sinks, n) + page - 1) / page);
+        fresh = count > 0 ? min(upto, (int)(begin / page)) : upto;
     }
     __device__ __forceinline__ bool has(int c) const { return c < upto && (c >= first || c < sinks); }
 };
@@ -110,53 +183,42 @@ __global__ void __launch_bounds__(kThreads) advance_kernel(const __grid_constant
     const Team team;
     const int S = a.t.sequences, W = a.t.width, lane = threadIdx.x & 31;
     for (int i = team.thread; i < a.t.pages; i += team.threads) a.refs[i] = a.t.refs[i];
-    team.sync();
-    for (int64_t i = team.thread; i < (int64_t)S * W; i += team.threads) {
-        const int s = (int)(i / W), c = (int)(i - (int64_t)s * W), e = a.t.table[i];
-        const bool there = is_page(a.t, e), stays = Stay(a, s).has(c);
-        a.table[i] = there && stays ? e : -1;
-        if (there && !stays) atomicSub(a.refs + e, 1);
-    }
     // a warp for each sequence: its new places without a page
-    int wanted = 0;
     for (int s = team.thread >> 5; s < S; s += team.threads >> 5) {
         const Stay stay(a, s);
         int need = 0;
         for (int c = stay.fresh + lane; c < stay.upto; c += 32) need += !is_page(a.t, a.t.table[(int64_t)s * W + c]);
         need = __reduce_add_sync(~0u, need);
-        if (lane == 0) a.offset[s] = need;
-        wanted += lane == 0 ? need : 0;
+        if (lane == 0) a.need[s] = need;
     }
     team.sync();
-    // the sequences in order
-    const int2 mine = share(team, S);
-    int count = 0;
-    for (int s = mine.x; s < mine.y; ++s) count += __ldcg(a.offset + s);
-    int2 rank = team.scan(count);
-    for (int s = mine.x; s < mine.y; ++s) {
-        const int need = __ldcg(a.offset + s);
-        a.offset[s] = rank.x;
-        rank.x += need;
-    }
-    const int got = list_free(a, team, rank.y);
+    for_places(a, team, [&](int s) { return Stay(a, s); }, [&](int, const Stay& stay, int c, int64_t i, int e) {
+        const bool there = is_page(a.t, e), stays = stay.has(c);
+        if (there || c < stay.fresh || c >= stay.upto) a.table[i] = there && stays ? e : -1;       // other places get theirs below
+        if (there && !stays) atomicSub(a.refs + e, 1);
+    });
+    int* const offset = a.offset + (size_t)team.rank * S;
+    const int wanted = offsets(a, team, offset);
+    team.sync();
+    const int got = list_free(a, team, wanted);
     team.sync();
     for (int s = team.thread >> 5; s < S; s += team.threads >> 5) {
         const Stay stay(a, s);
-        int at = __ldcg(a.offset + s);
+        int at = offset[s];
         for (int c0 = stay.fresh; c0 < stay.upto; c0 += 32) {
             const int c = c0 + lane;
             const bool need = c < stay.upto && !is_page(a.t, a.t.table[(int64_t)s * W + c]);
             const unsigned all = __ballot_sync(~0u, need);
             const int k = at + __popc(all & ((1u << lane) - 1));
-            if (need && k < got) {
-                const int p = __ldcg(a.list + k);
+            if (need) {
+                const int p = k < got ? __ldcg(a.list + k) : -1;
                 a.table[(int64_t)s * W + c] = p;
-                a.refs[p] = 1;
+                if (p >= 0) a.refs[p] = 1;
             }
             at += __popc(all);
         }
     }
-    if (team.thread == 0) *a.result = rank.y - got;
+    if (team.thread == 0) *a.result = wanted - got;
 }
 
 // ---------------------------------------------------------------- forking
@@ -164,61 +226,68 @@ __device__ __forceinline__ int parent_of(const PageArgs& a, int s) {
     const int p = a.parents[s];
     return p >= 0 && p < a.t.sequences ? p : -1;
 }
-__device__ __forceinline__ int length_of(const PageArgs& a, int p) {
-    return p < 0 ? 0 : (int)min((int64_t)max(0, a.t.lengths[p]), (int64_t)a.t.width * a.t.page);
-}
-// Whether sequence s needs a copy of its parent's last page: it is partly filled, and another sequence keeps it.
-__device__ __forceinline__ bool wants_copy(const PageArgs& a, int s, int p, int n) {
-    return p >= 0 && p != s && n % a.t.page && __ldcg(a.keeper + p) != s && is_page(a.t, a.t.table[(int64_t)p * a.t.width + n / a.t.page]);
-}
+// What sequence s becomes.
+struct Child {
+    int parent, full;           // places below `full` are the parent's
+    bool part, keeps;           // the next one is partly filled; s keeps its page
+    __device__ __forceinline__ Child(const PageArgs& a, int s) : parent(parent_of(a, s)) {
+        const uint32_t n = parent < 0 ? 0u : (uint32_t)min((int64_t)max(0, a.t.lengths[parent]), (int64_t)a.t.width * a.t.page);
+        full = n / (uint32_t)a.t.page;
+        part = n % (uint32_t)a.t.page != 0;
+        keeps = parent >= 0 && __ldcg(a.keeper + parent) == s;
+    }
+    // Whether it needs a copy of that page.
+    __device__ __forceinline__ bool copies(const PageArgs& a, int s) const {
+        return part && !keeps && parent != s && is_page(a.t, a.t.table[(int64_t)parent * a.t.width + full]);
+    }
+};
 
 __global__ void __launch_bounds__(kThreads) fork_kernel(const __grid_constant__ PageArgs a) {
     const Team team;
-    const int S = a.t.sequences, W = a.t.width, page = a.t.page;
+    let_next_begin();
+    const int S = a.t.sequences, W = a.t.width;
     for (int i = team.thread; i < a.t.pages; i += team.threads) a.refs[i] = a.t.refs[i];
-    for (int s = team.thread; s < S; s += team.threads) a.keeper[s] = S;
-    team.sync();
     // the partly filled page stays with the parent if it goes on, else with the first sequence that continues it
     for (int s = team.thread; s < S; s += team.threads) {
         const int p = parent_of(a, s);
-        if (p >= 0) atomicMin(a.keeper + p, p == s ? -1 : s);
         a.lengths[s] = p < 0 ? 0 : a.t.lengths[p];
+        a.keeper[s] = parent_of(a, s) == s ? -1 : S;
     }
     team.sync();
-    for (int64_t i = team.thread; i < (int64_t)S * W; i += team.threads) {
-        const int s = (int)(i / W), c = (int)(i - (int64_t)s * W), p = parent_of(a, s), old = a.t.table[i];
+    for (int s = team.thread; s < S; s += team.threads) {
+        const int p = parent_of(a, s);
+        if (p >= 0 && p != s) atomicMin(a.keeper + p, s);
+    }
+    team.sync();
+    for_places(a, team, [&](int s) { return Child(a, s); }, [&](int s, const Child& x, int c, int64_t i, int old) {
         int e = old;
-        if (p != s) {
+        if (x.parent != s) {
             if (is_page(a.t, old)) atomicSub(a.refs + old, 1);
-            const int n = length_of(a, p), full = n / page;
             e = -1;
-            if (c < full || (c == full && n % page && __ldcg(a.keeper + p) == s)) {
-                e = a.t.table[(int64_t)p * W + c];
+            if (x.parent >= 0 && (c < x.full || (c == x.full && x.part && x.keeps))) {
+                e = a.t.table[(int64_t)x.parent * W + c];
                 if (is_page(a.t, e)) atomicAdd(a.refs + e, 1);
                 else e = -1;
             }
         }
-        a.table[i] = e;
-    }
+        if (c != x.full || !x.copies(a, s)) a.table[i] = e;     // copies get their page below
+    });
     const int2 mine = share(team, S);
     int count = 0;
-    for (int s = mine.x; s < mine.y; ++s) {
-        const int p = parent_of(a, s);
-        count += wants_copy(a, s, p, length_of(a, p));
-    }
-    team.sync();
-    const int2 rank = team.scan(count);
+    for (int s = mine.x; s < mine.y; ++s) count += Child(a, s).copies(a, s);
+    const int2 rank = team.scan<1>(count);                      // its barrier is behind the changes of the counts, unless there is one block
+    if (team.ranks == 1) __syncthreads();
     const int got = list_free(a, team, rank.y);
     team.sync();
     int at = rank.x;
     for (int s = mine.x; s < mine.y; ++s) {
-        const int p = parent_of(a, s), n = length_of(a, p);
-        if (!wants_copy(a, s, p, n)) continue;
-        if (at < got) {
-            const int to = __ldcg(a.list + at);
-            a.source[at] = a.t.table[(int64_t)p * W + n / page];
+        const Child x(a, s);
+        if (!x.copies(a, s)) continue;
+        const int to = at < got ? __ldcg(a.list + at) : -1;
+        a.table[(int64_t)s * W + x.full] = to;
+        if (to >= 0) {
+            a.source[at] = a.t.table[(int64_t)x.parent * W + x.full];
             a.target[at] = to;
-            a.table[(int64_t)s * W + n / page] = to;
             a.refs[to] = 1;
         }
         ++at;
@@ -233,42 +302,28 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const __grid_constant__ 
 // With L pages in use, those from L on move to the places below L that are free, in order.
 __global__ void __launch_bounds__(kThreads) compact_kernel(const __grid_constant__ PageArgs a) {
     const Team team;
-    const int S = a.t.sequences, W = a.t.width;
-    const int2 mine = share(team, a.t.pages);
-    int count = 0;
-    for (int i = mine.x; i < mine.y; ++i) count += a.t.refs[i] > 0;
-    const int2 rank = team.scan(count);
+    let_next_begin();
+    const int2 mine = warp_pages(a, team);
+    auto live = [&](int i) { return a.t.refs[i] > 0; };
+    const int2 rank = team.scan<0>(count_pages(mine, live));
     const int L = rank.y;
-    int holes = 0;
-    for (int i = mine.x; i < mine.y; ++i) holes += i < L && a.t.refs[i] <= 0;
-    const int2 hole = team.scan(holes);
-    // pages in use below L: L less the holes
-    int used = rank.x, free = hole.x;
-    for (int i = mine.x; i < mine.y; ++i) {
-        const bool live = a.t.refs[i] > 0;
-        if (live && i >= L) a.source[used - (L - hole.y)] = i;
-        if (!live && i < L) a.target[free++] = i;
-        used += live;
-    }
-    team.sync();
-    used = rank.x;
-    free = hole.x;
-    for (int i = mine.x; i < mine.y; ++i) {
-        const int r = a.t.refs[i];
-        const bool live = r > 0;
-        a.list[i] = !live ? -1 : i < L ? i : __ldcg(a.target + used - (L - hole.y));     // where it goes
-        a.refs[i] = i >= L ? 0 : live ? r : a.t.refs[__ldcg(a.source + free++)];
-        used += live;
-    }
-    team.sync();
-    for (int64_t i = team.thread; i < (int64_t)S * W; i += team.threads) {
-        const int e = a.t.table[i];
-        a.table[i] = is_page(a.t, e) ? __ldcg(a.list + e) : -1;
-    }
+    const int2 hole = team.scan<1>(count_pages(mine, [&](int i) { return i < L && !live(i); }));
+    const int low = L - hole.y;                                 // pages in use below L
+    number_pages(mine, rank.x, live, [&](int i, bool on, int at) {
+        if (on && i >= L) a.source[at - low] = i;
+        if (!on && i < L) a.target[i - at] = i;                 // holes before it: places less pages in use
+    });
     if (team.thread == 0) {
         *a.moves = hole.y;
         *a.result = L;
     }
+    team.sync();
+    number_pages(mine, rank.x, live, [&](int i, bool on, int at) {
+        a.list[i] = !on ? -1 : i < L ? i : __ldcg(a.target + at - low);                      // where it goes
+        a.refs[i] = i >= L ? 0 : a.t.refs[on ? i : __ldcg(a.source + i - at)];
+    });
+    team.sync();
+    for_places(a, team, [](int) { return 0; }, [&](int, int, int, int64_t i, int e) { a.table[i] = is_page(a.t, e) ? __ldcg(a.list + e) : -1; });
 }
 
 // ---------------------------------------------------------------- copies
@@ -280,6 +335,7 @@ struct MoveArgs {
 constexpr int kMoveThreads = 256, kMoveUnroll = 8, kChunk = kMoveThreads * kMoveUnroll;     // pieces of 16 bytes
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ MoveArgs a) {
+    wait_for_previous();
     const int64_t units = (int64_t)*a.moves * a.npools * a.chunks;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const int chunk = (int)(u % a.chunks), pool = (int)(u / a.chunks % a.npools);
@@ -345,21 +401,48 @@ void split_workspace(PageArgs* a, void* workspace) {
     a->source = a->list + a->t.pages;
     a->target = a->source + a->t.pages;
     a->keeper = a->target + a->t.pages;
+    a->need = a->keeper;
     a->offset = a->keeper + a->t.sequences;
 }
 
+// Blocks of a cluster: 16 where the device schedules that, else the portable 8.  Cached per kernel and device.
 template <typename K>
-int launch_team(K kernel, const PageArgs& a, cudaStream_t st, const char* name) {
-    // One block where that has a thread for every place and page
+int most_blocks(K kernel, std::atomic<int>* cache) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 8;
+    int n = cache[dev].load(std::memory_order_relaxed);
+    if (n) return n;
+    n = 8;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = kBlocks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3(kBlocks); cfg.blockDim = dim3(kThreads); cfg.attrs = at; cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0) n = kBlocks;
+    }
+    cudaGetLastError();
+    cache[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+template <void (*KERNEL)(const PageArgs)>
+int launch_team(const PageArgs& a, cudaStream_t st, const char* name) {
+    static std::atomic<int> cache[64];
+    // Blocks that leave a thread four places or pages: a barrier of a larger cluster costs more (fork of 4352 places with 16 blocks
+    // 15.3 us, with 8 12.9), fewer threads take longer (step over 85000 pages with 8 blocks 24.8 us, with 16 19.9).
     const int64_t things = std::max<int64_t>((int64_t)a.t.width * a.t.sequences, a.t.pages);
-    const int blocks = things <= 2 * kThreads ? 1 : kBlocks;
+    int blocks = 1;
+    while (blocks < kBlocks && things > 4LL * kThreads * blocks) blocks *= 2;
+    blocks = std::min(blocks, blocks > 8 ? most_blocks(KERNEL, cache) : 8);
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = blocks; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(kThreads); cfg.stream = st;
     cfg.attrs = at; cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, KERNEL, a);
     if (e != cudaSuccess) return cuda_fail(e, name);
     CA_CHECK_LAUNCH(name);
     return CA_OK;
@@ -377,7 +460,14 @@ int launch_moves(const PageArgs& a, const ca_pool* pools, int npools, int64_t mo
         m.target = a.target;
         m.moves = a.moves;
         const int64_t units = most * m.npools * m.chunks;
-        move_kernel<<<(unsigned)std::min<int64_t>(units, 8LL * sm_count()), kMoveThreads, 0, st>>>(m);
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = first == 0;
+        cfg.gridDim = dim3((unsigned)std::min<int64_t>(units, 8LL * sm_count())); cfg.blockDim = dim3(kMoveThreads); cfg.stream = st;
+        cfg.attrs = at; cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, move_kernel, m);
+        if (e != cudaSuccess) return cuda_fail(e, "page copy kernel");
         CA_CHECK_LAUNCH("page copy kernel");
     }
     return CA_OK;
@@ -392,7 +482,7 @@ extern "C" {
 
 size_t ca_pages_workspace(const ca_table* t) {
     if (check_table(t, false)) return 0;
-    return ((size_t)4 + 3 * (size_t)t->pages + 2 * (size_t)t->sequences) * sizeof(int32_t);
+    return ((size_t)4 + 3 * (size_t)t->pages + (1 + kBlocks) * (size_t)t->sequences) * sizeof(int32_t);
 }
 
 int ca_advance_pages(const ca_table* t, const int32_t* starts, int32_t left, int32_t sinks, int32_t* table, int32_t* refs, int32_t* missing,
@@ -408,7 +498,7 @@ int ca_advance_pages(const ca_table* t, const int32_t* starts, int32_t left, int
     a.sinks = sinks;
     a.table = table; a.refs = refs; a.result = missing;
     split_workspace(&a, workspace);
-    return launch_team(advance_kernel, a, as_stream(stream), "page step kernel");
+    return launch_team<advance_kernel>(a, as_stream(stream), "page step kernel");
 }
 
 int ca_fork_pages(const ca_table* t, const int32_t* parents, const ca_pool* pools, int32_t npools, int32_t* table, int32_t* refs,
@@ -422,7 +512,7 @@ int ca_fork_pages(const ca_table* t, const int32_t* parents, const ca_pool* pool
     a.parents = parents;
     a.table = table; a.refs = refs; a.lengths = lengths; a.result = missing;
     split_workspace(&a, workspace);
-    rc = launch_team(fork_kernel, a, as_stream(stream), "page fork kernel");
+    rc = launch_team<fork_kernel>(a, as_stream(stream), "page fork kernel");
     return rc ? rc : launch_moves(a, pools, npools, std::min(t->sequences, t->pages), as_stream(stream));
 }
 
@@ -434,7 +524,7 @@ int ca_compact_pages(const ca_table* t, const ca_pool* pools, int32_t npools, in
     a.t = *t;
     a.table = table; a.refs = refs; a.result = live;
     split_workspace(&a, workspace);
-    rc = launch_team(compact_kernel, a, as_stream(stream), "page compaction kernel");
+    rc = launch_team<compact_kernel>(a, as_stream(stream), "page compaction kernel");
     return rc ? rc : launch_moves(a, pools, npools, t->pages / 2, as_stream(stream));
 }
 
