@@ -52,6 +52,7 @@ struct SeqArgs {
     ca_pages pages;                 // table == nullptr: dense
     SeqForm form;
     int kind;                       // of FormKind
+    int ranked;                     // Float32: tiles of unequal work, the largest first
     float* lse;                     // [b][key head][R]: log2 of the sum, -inf for rows that see nothing
     float* delta;                   // the same order: dy . y
     int* status;

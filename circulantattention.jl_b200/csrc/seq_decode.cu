@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
     if constexpr (sizeof(T) == 2) {
         const int ra = lane >> 2, pa = s.base + token_of(a, min(R0 + ra, rows - 1)), pb = s.base + token_of(a, min(R0 + ra + 8, rows - 1));
         const Reach ra_reach = reach<FORM>(a, s, pa), rb_reach = reach<FORM>(a, s, pb);
+        const CapPoly<T> poly(a, a.form.cap_in, a.form.cap_out);
         float slope_a = 0.f, slope_b = 0.f;
         if (has_slopes(FORM)) {
             const int Ra = min(R0 + ra, rows - 1), Rb = min(R0 + ra + 8, rows - 1);
@@ -187,15 +188,23 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
             }
             const int j = key0 + (lane & 3) * 2;
             const bool edge = !(p_lo >= 0 && key0 + kKeys - 1 <= min(lowest.hi, s.n - 1) && (key0 >= p_hi - a.left || key0 + kKeys <= a.sinks));
+            if constexpr (has_cap(FORM)) {                      // what no row sees is zeros here
+                uint32_t x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(c[e >> 2][e & 3]);
+                if (FORM == kCap) poly.template scores<8>(x, false, ~0u);
+                else cap_scores<T, 8>(x, a.form.cap_in, a.form.cap_out, false, ~0u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) c[e >> 2][e & 3] = __uint_as_float(x[e]);
+            }
             float ta = -INFINITY, tb = -INFINITY;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int jj = j + 8 * n + (e & 1);
-                    float inner;
-                    if (has_cap(FORM) || has_slopes(FORM)) c[n][e] = formed_score<FORM>(a, c[n][e], e < 2 ? slope_a : slope_b, (e < 2 ? pa : pb) - jj, 0.f, inner);
-                    else c[n][e] *= a.scale_log2;
+                    if (!has_cap(FORM)) c[n][e] *= a.scale_log2;
+                    if (has_slopes(FORM)) c[n][e] = fmaf(-(e < 2 ? slope_a : slope_b), fabsf((float)((e < 2 ? pa : pb) - jj)), c[n][e]);
                     if (edge && !sees(a, s.n, e < 2 ? pa : pb, e < 2 ? ra_reach : rb_reach, jj)) c[n][e] = -INFINITY;
                     if (e < 2) ta = fmaxf(ta, c[n][e]); else tb = fmaxf(tb, c[n][e]);
                 }

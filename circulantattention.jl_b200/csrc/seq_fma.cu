@@ -139,12 +139,69 @@ __device__ __forceinline__ float* row_ptr(const ca_seq_view& v, const SeqArgs& a
 }
 // Key row j; clears `on` where it does not exist or is padding.
 template <int FORM>
-__device__ __forceinline__ const float* key_ptr(const ca_seq_view& v, const ca_page_view& pv, const SeqArgs& a, const Seq& s, int h, int j, bool& on) {
-    on = on && j < s.n && !padding<FORM>(a, s, j);
+__device__ __forceinline__ const float* key_ptr(const ca_seq_view& v, const ca_page_view& pv, const SeqArgs& a, const Seq& s, int h, int j, bool& on, bool pads) {
+    on = on && j < s.n && !(pads && padding<FORM>(a, s, j));
     if (!a.pages.table) return (const float*)v.data + h * v.head + (int64_t)j * v.token + s.b * v.batch;
     const int p = on ? page_of(a, s.b, j) : -1;
     on = on && p >= 0;
     return (const float*)pv.data + h * pv.head + (int64_t)(j % a.pages.page) * pv.token + p * pv.page;
+}
+
+// The block's place, by rank where the tiles are of unequal work, and the tile of rows at it.
+template <int FORM>
+__device__ __forceinline__ Place place_of(const SeqArgs& a) {
+    return FORM && a.ranked ? place_by_rank() : Place{(int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z};
+}
+template <int FORM>
+__device__ __forceinline__ int row_tile(const SeqArgs& a, const Seq& s, int x, int* counts) {
+    __shared__ int ranked;
+    if (!FORM || !a.ranked) return x;
+    return ranked_tile(gridDim.x, x, counts, &ranked, [&](int first, int last) { return row_work<FORM>(a, s, first * kTile, (last + 1) * kTile); });
+}
+
+// From the products of a thread's 4 x 4 piece to scores in units of log2(e), less the slope's part, and the cap's derivative.  Two at
+// a time by the polynomial; a warp that holds a score beyond the cap takes them one by one, with the same bits for the others.
+template <int FORM>
+__device__ __forceinline__ void cap_piece(const SeqArgs& a, float (&x)[4][4], float (&inner)[4][4]) {
+    typedef TanhPoly<6> P;
+    const float in = a.form.cap_in, out = a.form.cap_out;
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(x[i][j]));
+    if (__any_sync(~0u, big * fabsf(in) > 1.f)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = tanh_any(x[i][j] * in);
+    } else {
+        const f32x2 in2 = pack2(in, in);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                const f32x2 X = mul2(pack2(x[i][j], x[i][j + 1]), in2), u = mul2(X, X);
+                f32x2 p = pack2(P::at(6), P::at(6));
+#pragma unroll
+                for (int k = 5; k >= 0; --k) p = fma2(p, u, pack2(P::at(k), P::at(k)));
+                unpack2(mul2(p, X), x[i][j], x[i][j + 1]);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            inner[i][j] = fmaf(-x[i][j], x[i][j], 1.f);
+            x[i][j] *= out;
+        }
+}
+// The score of one product, less `minus`, after cap_piece; `distance` in whole tokens.
+template <int FORM>
+__device__ __forceinline__ float piece_score(const SeqArgs& a, float x, float slope, float distance, float minus) {
+    if (!has_cap(FORM) && !has_slopes(FORM)) return fmaf(x, a.scale_log2, -minus);        // as without a form, to the bit
+    const float z = has_cap(FORM) ? x : x * a.scale_log2;
+    return has_slopes(FORM) ? fmaf(-slope, fabsf(distance), z) - minus : z - minus;
 }
 
 // ---------------------------------------------------------------- forward
@@ -155,8 +212,10 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
     extern __shared__ float4 smem4[];
     float *Q = (float*)smem4, *KV = Q + kTileFloats<DM>, *Pm = KV + 4 * kTileFloats<DM>;      // K, V, K, V
     __shared__ unsigned char gone[2][kTile];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
-    int tile = blockIdx.x;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const Place place = place_of<FORM>(a);
+    const int h = place.h;
+    int tile = place.x;
     int2 owned;
     Seq s;
     if (a.pages.table) {
@@ -166,7 +225,8 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
             return;
         }
     } else {
-        s = dense_seq(a, blockIdx.z);
+        s = dense_seq(a, place.b);
+        tile = row_tile<FORM>(a, s, tile, reinterpret_cast<int*>(Q));
     }
     const int rows = s.T * a.G, R0 = tile * kTile;
     const int p_lo = s.base + R0 / a.G, p_hi = s.base + (min(R0 + kTile, rows) - 1) / a.G;
@@ -177,13 +237,15 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
         return row_ptr(a.q, a, s, h, R);
     }, any, a.D, tid);
     const KeyTiles kt = key_tiles<FORM>(a, s, p_lo, p_hi, kTile);
+    const int doc_lo = document_of<FORM>(a, s, min(p_hi, s.n - 1));
     const Reach lowest = tile_reach<FORM>(a, s, p_lo), highest = tile_reach<FORM>(a, s, p_hi);
     auto prefetch = [&](int it) {
         const int j0 = kt.key(it, kTile), b = it & 1;
+        const bool pads = FORM && (j0 < doc_lo || j0 + kTile - 1 > p_hi) && mixed<FORM>(a, s, j0, j0 + kTile - 1);
         float* K = KV + 2 * b * kTileFloats<DM>;
         fetch<DM>(K, [&](int r, bool& on) {
             const bool whole = on;
-            const float* p = key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on);
+            const float* p = key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on, pads);
             if (tid % (DM / 4) == 0 && whole) gone[b][r] = !on;
             return p;
         }, any, a.D, tid);
@@ -191,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
         fetch<DM>(K + kTileFloats<DM>, [&](int r, bool& on) {
             const int j = j0 + r;
             on = on && (j >= lowest.lo || j < a.sinks) && j <= highest.hi;
-            return key_ptr<FORM>(a.v, a.vp, a, s, h, j, on);
+            return key_ptr<FORM>(a.v, a.vp, a, s, h, j, on, pads);
         }, any, a.D, tid);
     };
     int pos[4];
@@ -212,6 +274,7 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
 #pragma unroll
         for (int c = 0; c < DM / 32; ++c) o[i][c] = 0;
     }
+    const int all_hi = reach<FORM>(a, s, p_lo).hi, all_lo = reach<FORM>(a, s, p_hi).lo;      // what all of the tile's rows see
     if (kt.count) prefetch(0);
     copies_commit();
     if (a.pages.table) clear_unowned<float>(a, owned, h, tid, kThreads);
@@ -224,8 +287,10 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
         const float* K = KV + 2 * b * kTileFloats<DM>;
         float sc[4][4];
         dot_tile<DM>(Q, K, ty, tx, sc);
-        const bool edge = FORM || !(p_lo >= 0 && p_hi < s.n && j0 + kTile - 1 <= (int64_t)p_lo + a.right && j0 + kTile <= s.n &&
-                            (j0 >= p_hi - a.left || j0 + kTile <= a.sinks)) || a.pages.table;
+        const bool edge = !(p_lo >= 0 && p_hi < s.n && j0 + kTile - 1 <= (FORM ? all_hi : (int64_t)p_lo + a.right) && j0 + kTile <= s.n &&
+                            (j0 >= (FORM ? all_lo : p_hi - a.left) || j0 + kTile <= a.sinks)) || a.pages.table;
+        float inner[FORM ? 4 : 1][4];
+        if constexpr (has_cap(FORM)) cap_piece<FORM>(a, sc, inner);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float top = m[i];
@@ -233,9 +298,8 @@ __global__ void __launch_bounds__(kThreads) fma_fwd_kernel(const __grid_constant
             for (int j = 0; j < 4; ++j) {
                 const int key = j0 + tx + 16 * j;
                 if constexpr (FORM) {
-                    float inner;
-                    sc[i][j] = formed_score<FORM>(a, sc[i][j], slope[i], pos[i] - key, 0.f, inner);
-                    if (!sees(a, s.n, pos[i], mine[i], key) || gone[b][tx + 16 * j]) sc[i][j] = -INFINITY;
+                    sc[i][j] = piece_score<FORM>(a, sc[i][j], slope[i], (float)(pos[i] - j0 - tx) - 16.f * j, 0.f);
+                    if (edge && (!sees(a, s.n, pos[i], mine[i], key) || gone[b][tx + 16 * j])) sc[i][j] = -INFINITY;
                 } else {
                     sc[i][j] *= a.scale_log2;
                     if (edge && (!sees(a, s.n, pos[i], key) || gone[b][tx + 16 * j])) sc[i][j] = -INFINITY;
@@ -281,9 +345,11 @@ template <int DM, int FORM>
 __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(const __grid_constant__ SeqArgs a) {
     extern __shared__ float4 smem4[];
     float *Q = (float*)smem4, *O = Q + kTileFloats<DM>, *K = O + kTileFloats<DM>, *V = K + kTileFloats<DM>, *Pm = V + kTileFloats<DM>;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
-    const Seq s = dense_seq(a, blockIdx.z);
-    const int rows = s.T * a.G, R0 = blockIdx.x * kTile;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const Place place = place_of<FORM>(a);
+    const int h = place.h;
+    const Seq s = dense_seq(a, place.b);
+    const int rows = s.T * a.G, R0 = row_tile<FORM>(a, s, place.x, reinterpret_cast<int*>(Q)) * kTile;
     const int p_lo = R0 / a.G, p_hi = (min(R0 + kTile, rows) - 1) / a.G;
     const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
     const float* any = (const float*)a.q.data;
@@ -300,10 +366,12 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
     fetch<DM>(yrow, from(a.y), any, a.D, tid);
     copies_commit();
     const KeyTiles kt = key_tiles<FORM>(a, s, p_lo, p_hi, kTile);
+    const int doc_lo = document_of<FORM>(a, s, min(p_hi, s.n - 1));
     auto prefetch = [&](int it) {
         const int j0 = kt.key(it, kTile);
-        fetch<DM>(K, [&](int r, bool& on) { return key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
-        fetch<DM>(V, [&](int r, bool& on) { return key_ptr<FORM>(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
+        const bool pads = FORM && (j0 < doc_lo || j0 + kTile - 1 > p_hi) && mixed<FORM>(a, s, j0, j0 + kTile - 1);
+        fetch<DM>(K, [&](int r, bool& on) { return key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on, pads); }, any, a.D, tid);
+        fetch<DM>(V, [&](int r, bool& on) { return key_ptr<FORM>(a.v, a.vp, a, s, h, j0 + r, on, pads); }, any, a.D, tid);
     };
     copies_wait<0>();
     __syncthreads();
@@ -328,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
 #pragma unroll
         for (int c = 0; c < DM / 32; ++c) o[i][c] = 0;
     }
+    const int all_hi = reach<FORM>(a, s, p_lo).hi, all_lo = reach<FORM>(a, s, p_hi).lo;      // what all of the tile's rows see
     __syncthreads();
     for (int it = 0; it < kt.count; ++it) {
         prefetch(it);
@@ -335,10 +404,12 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
         copies_wait<0>();
         __syncthreads();
         const int j0 = kt.key(it, kTile);
-        const bool edge = !(p_hi < s.n && j0 + kTile - 1 <= (int64_t)p_lo + a.right && j0 + kTile <= s.n && (j0 >= p_hi - a.left || j0 + kTile <= a.sinks));
-        float sc[4][4], dp[4][4];
+        const bool edge = !(p_hi < s.n && j0 + kTile - 1 <= (FORM ? all_hi : (int64_t)p_lo + a.right) && j0 + kTile <= s.n &&
+                            (j0 >= (FORM ? all_lo : p_hi - a.left) || j0 + kTile <= a.sinks));
+        float sc[4][4], dp[4][4], inner[FORM ? 4 : 1][4];
         dot_tile<DM>(Q, K, ty, tx, sc);
         dot_tile<DM>(O, V, ty, tx, dp);
+        if constexpr (has_cap(FORM)) cap_piece<FORM>(a, sc, inner);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -346,9 +417,8 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dq_kernel(cons
                 const int key = j0 + tx + 16 * j;
                 float ds;
                 if constexpr (FORM) {
-                    float inner;
-                    const float z = formed_score<FORM>(a, sc[i][j], slope[i], pos[i] - key, lse[i], inner);
-                    ds = sees(a, s.n, pos[i], mine[i], key) ? fast_exp2(z) * inner * (dp[i][j] - delta[i]) : 0.f;
+                    const float z = piece_score<FORM>(a, sc[i][j], slope[i], (float)(pos[i] - j0 - tx) - 16.f * j, lse[i]);
+                    ds = !edge || sees(a, s.n, pos[i], mine[i], key) ? fast_exp2(z) * (has_cap(FORM) ? inner[i][j] : 1.f) * (dp[i][j] - delta[i]) : 0.f;
                 } else {
                     const bool see = !edge || sees(a, s.n, pos[i], key);
                     ds = see ? fast_exp2(sc[i][j] * a.scale_log2 - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
@@ -381,17 +451,26 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
     extern __shared__ float4 smem4[];
     float *K = (float*)smem4, *V = K + kTileFloats<DM>, *Q = V + kTileFloats<DM>, *O = Q + kTileFloats<DM>, *Pm = O + kTileFloats<DM>, *Sm = Pm + kTile * kPPitch;
     __shared__ float s_lse[kTile], s_delta[kTile];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, h = blockIdx.y;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const Place place = place_of<FORM>(a);
+    const int h = place.h;
+    const Seq s = dense_seq(a, place.b);
     const int dealt = parts.tiles * parts.segments;
-    const bool split = (int)blockIdx.x < dealt;
-    const int tile = split ? (int)blockIdx.x / parts.segments : parts.tiles + (int)blockIdx.x - dealt, seg = split ? (int)blockIdx.x % parts.segments : 0;
+    const bool split = place.x < dealt;
+    int tile = split ? place.x / parts.segments : parts.tiles + place.x - dealt;
+    const int seg = split ? place.x % parts.segments : 0;
+    __shared__ int ranked;
+    if (FORM && a.ranked)                                                 // spans: no first tokens, nothing is dealt out
+        tile = ranked_tile(gridDim.x, place.x, reinterpret_cast<int*>(K), &ranked, [&](int first, int last) {
+            return first * kTile >= s.n ? 0 : seen_by(a, s, min((last + 1) * kTile, s.n) - 1).hi - max(0, seen_by(a, s, first * kTile).lo);
+        });
     const int j0 = tile * kTile;
-    const Seq s = dense_seq(a, blockIdx.z);
     const int rows = s.T * a.G;
     const int64_t stat0 = ((int64_t)s.b * a.Hkv + h) * rows;
     const float* any = (const float*)a.q.data;
-    fetch<DM>(K, [&](int r, bool& on) { return key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on); }, any, a.D, tid);
-    fetch<DM>(V, [&](int r, bool& on) { return key_ptr<FORM>(a.v, a.vp, a, s, h, j0 + r, on); }, any, a.D, tid);
+    const bool key_pads = mixed<FORM>(a, s, j0, j0 + kTile - 1);
+    fetch<DM>(K, [&](int r, bool& on) { return key_ptr<FORM>(a.k, a.kp, a, s, h, j0 + r, on, key_pads); }, any, a.D, tid);
+    fetch<DM>(V, [&](int r, bool& on) { return key_ptr<FORM>(a.v, a.vp, a, s, h, j0 + r, on, key_pads); }, any, a.D, tid);
     f32x2 dk[4][DM / 32], dv[4][DM / 32];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -399,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
         for (int c = 0; c < DM / 32; ++c) dk[i][c] = dv[i][c] = 0;
     int t_lo = max(0, j0 - a.right);
     int t_hi = j0 >= s.n ? t_lo : j0 < a.sinks ? s.n : (int)min((int64_t)s.n, (int64_t)j0 + kTile + a.left);
-    Reach by[FORM ? 4 : 1];                                       // queries that see the thread's keys
+    Reach by[FORM ? 4 : 1], whole{0, 0};                          // queries that see the thread's keys, and that see all of the tile's
     if constexpr (FORM) {
         if (a.form.spans && j0 < s.n) {
             t_lo = max(0, min(seen_by(a, s, j0).lo, j0));
@@ -411,15 +490,18 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
             by[i] = a.form.spans ? seen_by(a, s, j) : Reach{j - a.right, j < a.sinks ? s.n - 1 : j + a.left};
             if (j >= s.n) by[i] = Reach{0, -1};
         }
+        const int j1 = min(j0 + kTile, s.n) - 1;
+        whole = a.form.spans ? Reach{seen_by(a, s, j1).lo, seen_by(a, s, j0).hi} : Reach{j0 + kTile - 1 - a.right, j0 + kTile <= a.sinks ? s.n - 1 : j0 + a.left};
     }
     const int lo = t_lo * a.G, hi = max(t_lo, t_hi) * a.G, all = (hi - lo + kTile - 1) / kTile;
     const int first = split ? (int)((int64_t)all * seg / parts.segments) : 0;
     const int count = (split ? (int)((int64_t)all * (seg + 1) / parts.segments) : all) - first;
     auto prefetch = [&](int it) {
         const int R0 = lo + (first + it) * kTile;
+        const bool pads = FORM && mixed<FORM>(a, s, R0 / a.G, (min(R0 + kTile, hi) - 1) / a.G);
         auto from = [&](const ca_seq_view& v) {
             return [&](int r, bool& on) {
-                on = on && R0 + r < hi && !padding<FORM>(a, s, token_of(a, min(R0 + r, hi - 1)));
+                on = on && R0 + r < hi && !(pads && padding<FORM>(a, s, token_of(a, min(R0 + r, hi - 1))));
                 return (const float*)row_ptr(v, a, s, h, min(R0 + r, hi - 1));
             };
         };
@@ -441,25 +523,36 @@ __global__ void __launch_bounds__(kThreads, DM == 64 ? 2 : 1) fma_dkdv_kernel(co
         dot_tile<DM>(K, Q, ty, tx, sc);
         dot_tile<DM>(V, O, ty, tx, dp);
         const int t0 = R0 / a.G, t1 = min(R0 + kTile, hi) - 1 < R0 ? t0 : (min(R0 + kTile, hi) - 1) / a.G;
-        const bool edge = !(R0 + kTile <= hi && t1 < s.n && j0 + kTile <= s.n && j0 + kTile - 1 <= (int64_t)t0 + a.right && (j0 >= t1 - a.left || j0 + kTile <= a.sinks));
+        const bool edge = !(R0 + kTile <= hi && t1 < s.n && j0 + kTile <= s.n &&
+                            (FORM ? t0 >= whole.lo && t1 <= whole.hi : j0 + kTile - 1 <= (int64_t)t0 + a.right && (j0 >= t1 - a.left || j0 + kTile <= a.sinks)));
+        int token[FORM ? 4 : 1];
+        float slope[has_slopes(FORM) ? 4 : 1], inner[FORM ? 4 : 1][4];
+        if constexpr (FORM) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int R = R0 + tx + 16 * c;
+                token[c] = token_of(a, R);
+                if constexpr (has_slopes(FORM)) slope[c] = R < hi ? slope_of(a, h * a.G + R - token[c] * a.G) : 0.f;
+            }
+            if constexpr (has_cap(FORM)) cap_piece<FORM>(a, sc, inner);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int R = R0 + tx + 16 * c, key = j0 + ty + 16 * i;
-                float z, inner = 1.f;
+                float z;
                 bool see;
                 if constexpr (FORM) {
-                    const int token = token_of(a, R);
-                    see = R < hi && token < s.n && token >= by[i].lo && token <= by[i].hi;
-                    z = formed_score<FORM>(a, sc[i][c], has_slopes(FORM) && R < hi ? slope_of(a, h * a.G + R - token * a.G) : 0.f, token - key, s_lse[tx + 16 * c], inner);
+                    see = !edge || (R < hi && token[c] < s.n && token[c] >= by[i].lo && token[c] <= by[i].hi);
+                    z = piece_score<FORM>(a, sc[i][c], slope[has_slopes(FORM) ? c : 0], (float)(token[c] - key), s_lse[tx + 16 * c]);
                 } else {
                     see = !edge || (R < hi && sees(a, s.n, token_of(a, R), key));
                     z = sc[i][c] * a.scale_log2 - s_lse[tx + 16 * c];
                 }
                 const float p = see ? fast_exp2(z) : 0.f;
                 Pm[(ty + 16 * i) * kPPitch + tx + 16 * c] = p;
-                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? p * inner * (dp[i][c] - s_delta[tx + 16 * c]) : 0.f;
+                Sm[(ty + 16 * i) * kPPitch + tx + 16 * c] = see ? (has_cap(FORM) ? p * inner[i][c] : p) * (dp[i][c] - s_delta[tx + 16 * c]) : 0.f;
             }
         __syncwarp();
         acc_tile<DM>(Pm, O, ty, tx, dv);
@@ -553,8 +646,19 @@ size_t fma_bwd_parts(const SeqArgs& a) {
         case kCapSlopes: return a.D > 64 ? F<128, kCapSlopes>(__VA_ARGS__) : F<64, kCapSlopes>(__VA_ARGS__);         \
         default: return a.D > 64 ? F<128, kNoForm>(__VA_ARGS__) : F<64, kNoForm>(__VA_ARGS__);                       \
     }
-int fma_fwd(const SeqArgs& a, cudaStream_t st) { CA_KINDS(launch_fwd, a, st) }
-int fma_bwd(const SeqArgs& a, float* parts, cudaStream_t st) { CA_KINDS(launch_bwd, a, parts, st) }
+// More tiles than start at once: the largest first.
+static SeqArgs ranked(SeqArgs a) {
+    a.ranked = a.form.spans && ((int64_t)a.N * a.G + kTile - 1) / kTile * a.Hkv * a.B > sm_count();
+    return a;
+}
+int fma_fwd(const SeqArgs& args, cudaStream_t st) {
+    const SeqArgs a = ranked(args);
+    CA_KINDS(launch_fwd, a, st)
+}
+int fma_bwd(const SeqArgs& args, float* parts, cudaStream_t st) {
+    const SeqArgs a = ranked(args);
+    CA_KINDS(launch_bwd, a, parts, st)
+}
 #undef CA_KINDS
 
 }  // namespace ca
