@@ -36,10 +36,11 @@ struct FwdMaps {
 namespace {
 
 // Warpgroups of softmax, a warp that copies and one that issues the products.  A stream has one warpgroup, a thread for each row; with
-// other scores two, a thread for each row and half of the keys: their arithmetic is twice that of plain scores, and two warps on a
-// scheduler leave half of its slots empty (16384 tokens, window 1024, bfloat16, cap: 262 us with two, 295 with one; slopes 287 and
-// 295; but other masks only 241 and 217).
-template <int FORM> constexpr int kGroups = has_cap(FORM) || has_slopes(FORM) ? 2 : 1;
+// a cap two, a thread for each row and half of the keys: that arithmetic is twice as much, and two warps on a scheduler leave
+// half of its slots empty (16384 tokens, window 1024, bfloat16: cap 259 us with two, 284 with one, 297 and 359 where some scores
+// lie beyond the cap; cap and slopes 341 and 354; but slopes alone 267 and 247, other masks 241 and 224: a tile costs a warp its
+// waits whatever it does in it).
+template <int FORM> constexpr int kGroups = has_cap(FORM) ? 2 : 1;
 template <int FORM> constexpr int kSoftmaxWarps = 8 * kGroups<FORM>;
 template <int FORM> constexpr int kThreads = 32 * (kSoftmaxWarps<FORM> + 2);
 
@@ -219,10 +220,9 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;              // lane 32 * (warp % 4) in bits 16..
         const uint32_t S_at = s_col + u * 128 + lane_off, P_at = p_col + u * p_step + lane_off, O_at = o_col + u * DM + lane_off;
         // A capped score is at most cap log2(e), which the exponents of bfloat16 stand without a reference: one pass over the scores
-        // is enough.  Scores with a slope need the maximum of the changed ones: with a cap they return to tensor memory in units
-        // of log2(e), without they are computed twice.
-        constexpr bool BOUNDED = FORM == kCap, KEPT = FORM == kCapSlopes;
-        (void)KEPT;
+        // is enough.  Scores with a slope need the maximum of the changed ones, and return to tensor memory in units of log2(e) for
+        // the exponentials (247 us; computed twice 288).
+        constexpr bool BOUNDED = FORM == kCap, KEPT = has_slopes(FORM);
         const float sl2 = has_cap(FORM) || has_slopes(FORM) ? 1.f : a.mag_log2, cap_in = fabsf(a.form.cap_in);
         const float slope = has_slopes(FORM) ? slope_of(a, h * a.G + R - token_of(a, R) * a.G) : 0.f;
         const CapPoly<T> poly(a, cap_in, a.form.cap_out);
@@ -302,6 +302,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                     rest = pack16<T>(w0, w1);
                 }
             };
+            const int side = far <= st.lo ? 1 : key0 >= st.hi ? -1 : 0;    // of the keys, for all rows
             if constexpr (GROUPS == 1) {
                 auto scores = [&](int g, uint32_t* x) {                    // the columns 64 g .. 64 g + 63
                     tmem_ld32(S_at + 64 * g, x);
@@ -313,13 +314,20 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                 // The same for the maximum: -inf where the row does not see the key, written back for the exponentials
                 auto masked_scores = [&](int g, uint32_t* x) {
                     scores(g, x);
-                    if (edge) {
+                    if (has_slopes(FORM)) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            slope_scores<32>(x + 32 * q, a.mag_log2, slope, (float)(pos - key0 - 64 * g - 32 * q), side);
+                    }
+                    if (edge || KEPT) {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             const int at = 64 * g + 32 * q;
-                            const uint32_t mk = seen(at);
+                            if (!KEPT || edge) {
+                                const uint32_t mk = seen(at);
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) x[32 * q + c] = (mk >> c) & 1 ? x[32 * q + c] : 0xff800000u;
+                                for (int c = 0; c < 32; ++c) x[32 * q + c] = (mk >> c) & 1 ? x[32 * q + c] : 0xff800000u;
+                            }
                             tmem_st32(S_at + at, x + 32 * q);
                         }
                     }
@@ -370,8 +378,9 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                             tmem_st16(P_at + p_half * g + 32 * q, w + 16 * q);
                             tmem_st16(P_at + p_half * g + 32 * q + 16, rest + (SPLIT ? 16 * q : 0));
                         }
-                    } else
-                    tmem_st32(P_at + p_half * g, w);                       // at 128 features over scores that this warp has read twice
+                    } else {
+                        tmem_st32(P_at + p_half * g, w);
+                    }                                                      // at 128 features over scores that this warp has read twice
                     tmem_wait_st();
                     fence_before();
                     __syncwarp();
@@ -384,7 +393,6 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                 lr = a0 + a1;
             } else {
                 const bool own = st.sees_half(a, key0 + 64 * g), others = st.sees_half(a, key0 + 64 - 64 * g);
-                const int side = far <= st.lo ? 1 : key0 >= st.hi ? -1 : 0;        // of the keys, for all rows
                 // 32 columns from 64 g + 32 q as they go into the exponential, but for the reference; hidden ones are -inf
                 auto scores = [&](int q, uint32_t* x, bool kept) {
                     const int at = 64 * g + 32 * q;
@@ -393,14 +401,14 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                     settled32(x);
                     if (kept) return;
                     const uint32_t mk = edge ? seen(at) : ~0u;
-                    if (BOUNDED)
+                    if constexpr (BOUNDED)
                         poly.template scores<32>(x, edge, mk, [&] {
                             tmem_ld32(S_at + at, x);
                             tmem_wait_ld();
                             settled32(x);
                         });
-                    else if (has_cap(FORM)) cap_scores<T, 32>(x, cap_in, a.form.cap_out, edge, mk);
-                    if (has_slopes(FORM)) slope_scores<32>(x, has_cap(FORM) ? 1.f : a.mag_log2, slope, (float)(pos - key0 - at), side);
+                    else cap_scores<T, 32>(x, cap_in, a.form.cap_out, edge, mk);
+                    if (has_slopes(FORM)) slope_scores<32>(x, 1.f, slope, (float)(pos - key0 - at), side);
                     if (edge) {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0xff800000u;
@@ -416,7 +424,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                         for (int q = 0; q < 2; ++q) {
                             uint32_t x[32];
                             scores(q, x, false);
-                            if (KEPT) tmem_st32(S_at + 64 * g + 32 * q, x);
+                            tmem_st32(S_at + 64 * g + 32 * q, x);
                             float top[2] = {mx, -INFINITY};
 #pragma unroll
                             for (int c = 0; c < 32; c += 4)
@@ -427,7 +435,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                     }
                     tmem_wait_st();
                     // Both halves' maxima, rounded (which the reference stands) so that they fit: the tiles take all but 2 KB
-                    part_max[u][g][r] = __float2bfloat16_rn(mx * sl2);
+                    part_max[u][g][r] = __float2bfloat16_rn(mx);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&max_full[u]));
                     if (!warp_wait(smem_u32(&max_full[u]), done & 1, stop)) { ok = false; break; }
@@ -441,7 +449,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                 }
                 if (own) {
                     const float ref = m == -INFINITY ? 0.f : m;            // a row that has seen nothing yet
-                    const f32x2 sc2 = pack2(sl2, sl2), ref2 = pack2(-ref, -ref);
+                    const f32x2 ref2 = pack2(-ref, -ref);
                     f32x2 sum2 = pack2(l * f, 0.f), round2 = pack2(lr * f, 0.f);
 #pragma unroll 1
                     for (int q = 0; q < 2; ++q) {
@@ -451,9 +459,8 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                         for (int c = 0; c < 16; ++c) {
                             float e0, e1;
                             if (BOUNDED) e0 = __uint_as_float(x[2 * c]), e1 = __uint_as_float(x[2 * c + 1]);
-                            else if (FORM != kMasks) unpack2(add2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), ref2), e0, e1);
-                            else unpack2(fma2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), sc2, ref2), e0, e1);
-                            e0 = fast_exp2(e0);
+                            else unpack2(add2(pack2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), ref2), e0, e1);
+                            e0 = fast_exp2(e0);             // the cap's polynomial fills the FMA pipe: none of these on it
                             e1 = fast_exp2(e1);
                             sum2 = add2(sum2, pack2(e0, e1));
                             w[c] = pack16<T>(e0, e1);

@@ -69,23 +69,29 @@ __global__ void __launch_bounds__(kSpanThreads) span_kernel(const __grid_constan
     if (lane == 0) before = Places{-1, -1};
     if (lane == 31) behind = Places{a.N, a.N};
     __syncthreads();
-    Places all_last{-1, -1}, all_first{a.N, a.N};
-    for (int w = 0; w < kSpanWarps; ++w) {
-        all_last = later(all_last, warp_last[w]);
-        all_first = sooner(all_first, warp_first[w]);
-        if (w < warp) before = later(before, warp_last[w]);
-        if (w > warp) behind = sooner(behind, warp_first[w]);
-    }
+    // every warp joins the warps' places, a lane for each, and then the blocks'
+    auto join = [&](Places last, Places first, int own) {
+        before = later(before, Places{__reduce_max_sync(~0u, lane < own ? last.document : -1), __reduce_max_sync(~0u, lane < own ? last.group : -1)});
+        behind = sooner(behind, Places{__reduce_min_sync(~0u, lane > own ? first.document : a.N), __reduce_min_sync(~0u, lane > own ? first.group : a.N)});
+    };
+    const Places lasts = warp_last[lane], firsts = warp_first[lane];
+    join(lasts, firsts, warp);
     if (ranks > 1) {
-        if (tid == 0) {
-            block_last = all_last;
-            block_first = all_first;
+        if (warp == 0) {
+            const Places all_last{__reduce_max_sync(~0u, lasts.document), __reduce_max_sync(~0u, lasts.group)};
+            const Places all_first{__reduce_min_sync(~0u, firsts.document), __reduce_min_sync(~0u, firsts.group)};
+            if (lane == 0) {
+                block_last = all_last;
+                block_first = all_first;
+            }
         }
         cluster.sync();
-        for (int r = 0; r < ranks; ++r) {
-            if (r < rank) before = later(before, *cluster.map_shared_rank(&block_last, r));
-            if (r > rank) behind = sooner(behind, *cluster.map_shared_rank(&block_first, r));
+        Places last{-1, -1}, first{a.N, a.N};
+        if (lane < ranks) {
+            last = *cluster.map_shared_rank(&block_last, lane);
+            first = *cluster.map_shared_rank(&block_first, lane);
         }
+        join(last, first, rank);
         cluster.sync();                                         // nobody leaves while its places are read
     }
     if (from >= to) return;
