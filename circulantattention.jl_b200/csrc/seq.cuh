@@ -222,7 +222,7 @@ __device__ __forceinline__ int row_work(const SeqArgs& a, const Seq& s, int from
 template <typename Work>
 __device__ __forceinline__ int ranked_tile(int tiles, int rank, int* counts, int* result, Work work) {
     const int length = (tiles + 127) / 128, runs = (tiles + length - 1) / length, t = threadIdx.x;
-    if (t < 128) counts[t] = t >= runs ? -2 : (t + 1) * length > tiles ? -1 : work(t * length, (t + 1) * length - 1);
+    if (t < 128) counts[t] = t >= runs ? -2 : (t + 1) * length > tiles ? -1 : max(0, work(t * length, (t + 1) * length - 1));
     __syncthreads();
     if (t < runs) {
         const int own = counts[t];

@@ -74,14 +74,6 @@ __device__ __forceinline__ void read_halves(uint32_t at, uint32_t* x) {
     settled32(x);
 }
 
-// Zeros where the bit is not set.  Always in a block of its own behind one uniform branch: as a condition on each element the
-// selects ran for every tile and took as long as the arithmetic.
-template <int COUNT>
-__device__ __forceinline__ void clear_unseen(uint32_t* x, uint32_t mk) {
-#pragma unroll
-    for (int c = 0; c < COUNT; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0u;
-}
-
 template <int DM>
 __device__ __forceinline__ void clear_row(char* tile, int r) {
 #pragma unroll
@@ -284,8 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dq_kernel(const __grid_const
             }
             if (has_cap(FORM) || has_slopes(FORM)) {
                 f32x2 inner[has_cap(FORM) ? kCols / 2 : 1];    // P (1 - tanh^2) is all that dS needs
-                if (FORM == kCap) poly.template scores<kCols>(x, edge, mk);
-                else if (has_cap(FORM)) cap_scores<T, kCols>(x, a.form.cap_in, 1.f, edge, mk);
+                if (has_cap(FORM) && edge) clear_unseen<kCols>(x, mk);
+                if (FORM == kCap) poly.template scores<kCols>(x);
+                else if (has_cap(FORM)) cap_scores<T, kCols>(x, a.form.cap_in, 1.f);
                 if (has_cap(FORM)) cap_inner<kCols>(inner, x);
                 if (has_slopes(FORM)) slope_scores<kCols>(x, factor, slope, (float)(pos - key0 - kCols * u), far <= f_lo ? 1 : key0 >= f_hi ? -1 : 0);
                 const f32x2 f2 = has_slopes(FORM) ? pack2(1.f, 1.f) : pack2(factor, factor);
@@ -609,8 +602,9 @@ __global__ void __launch_bounds__(kThreads, 1) umma_dkdv_kernel(const __grid_con
                 uint32_t* const xg = x + 16 * g;
                 f32x2 inner[has_cap(FORM) ? 8 : 1];
                 if (has_cap(FORM)) {
-                    if (FORM == kCap) poly.template scores<16>(xg, edge, mk >> 16 * g);
-                    else cap_scores<T, 16>(xg, a.form.cap_in, 1.f, edge, mk >> 16 * g);
+                    if (edge) clear_unseen<16>(xg, mk >> 16 * g);
+                    if (FORM == kCap) poly.template scores<16>(xg);
+                    else cap_scores<T, 16>(xg, a.form.cap_in, 1.f);
                     cap_inner<16>(inner, xg);
                 }
                 if (has_slopes(FORM))

@@ -193,11 +193,11 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(c[e >> 2][e & 3]);
                 if (FORM == kCap)
-                    poly.template scores<8>(x, false, ~0u, [&] {
+                    poly.template scores<8>(x, [&] {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(c[e >> 2][e & 3]);
                     });
-                else cap_scores<T, 8>(x, a.form.cap_in, a.form.cap_out, false, ~0u);
+                else cap_scores<T, 8>(x, a.form.cap_in, a.form.cap_out);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) c[e >> 2][e & 3] = __uint_as_float(x[e]);
             }

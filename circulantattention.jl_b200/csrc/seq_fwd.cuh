@@ -401,13 +401,14 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                     settled32(x);
                     if (kept) return;
                     const uint32_t mk = edge ? seen(at) : ~0u;
+                    if (edge) clear_unseen<32>(x, mk);
                     if constexpr (BOUNDED)
-                        poly.template scores<32>(x, edge, mk, [&] {
+                        poly.template scores<32>(x, [&] {
                             tmem_ld32(S_at + at, x);
                             tmem_wait_ld();
                             settled32(x);
                         });
-                    else cap_scores<T, 32>(x, cap_in, a.form.cap_out, edge, mk);
+                    else cap_scores<T, 32>(x, cap_in, a.form.cap_out);
                     if (has_slopes(FORM)) slope_scores<32>(x, 1.f, slope, (float)(pos - key0 - at), side);
                     if (edge) {
 #pragma unroll

@@ -76,28 +76,30 @@ __device__ __forceinline__ void settled32(uint32_t* r) {
 }
 
 // ---------------------------------------------------------------- scores with a cap and a slope, COUNT neighbouring columns of a row
-// Largest magnitude; `edge`: of the columns whose bit in mk is set.
+// Zeros where the bit is not set.  Always in a block of its own behind one uniform branch: as a condition on each element the
+// selects ran for every tile and took as long as the arithmetic.
 template <int COUNT>
-__device__ __forceinline__ float largest(const uint32_t* x, bool edge, uint32_t mk) {
-    float big = 0.f;
-    if (edge) {
+__device__ __forceinline__ void clear_unseen(uint32_t* x, uint32_t mk) {
 #pragma unroll
-        for (int c = 0; c < COUNT; ++c) big = fmaxf(big, (mk >> c) & 1 ? fabsf(__uint_as_float(x[c])) : 0.f);
-    } else {
-#pragma unroll
-        for (int c = 0; c < COUNT; c += 2) big = fmaxf(fmaxf(big, fabsf(__uint_as_float(x[c]))), fabsf(__uint_as_float(x[c + 1])));
-    }
-    return big;
+    for (int c = 0; c < COUNT; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0u;
 }
 
+// Columns that the row does not see are cleared before: whatever they hold has no say in which way a warp takes, and no factor of a
+// masked weight is infinite.
 // x = tanh(cap_in x), or `out` times that.  The polynomial serves |score| <= cap; a warp that holds a larger one takes two passes of
-// the exponential unit an element, 1.5e-7 off.  Columns that the row does not see have no say in this.  The warp calls it
-// together.
+// the exponential unit an element, 1.5e-7 off.  The warp calls it together.
+template <int COUNT>
+__device__ __forceinline__ float largest(const uint32_t* x) {
+    float big = 0.f;
+#pragma unroll
+    for (int c = 0; c < COUNT; c += 2) big = fmaxf(fmaxf(big, fabsf(__uint_as_float(x[c]))), fabsf(__uint_as_float(x[c + 1])));
+    return big;
+}
 template <typename T, int COUNT>
-__device__ __forceinline__ void cap_scores(uint32_t* x, float cap_in, float out, bool edge, uint32_t mk) {
+__device__ __forceinline__ void cap_scores(uint32_t* x, float cap_in, float out) {
     constexpr int DEGREE = kIsBf16<T> ? 4 : 5;
     typedef TanhPoly<DEGREE> P;
-    if (__any_sync(~0u, largest<COUNT>(x, edge, mk) * fabsf(cap_in) > 1.f)) {
+    if (__any_sync(~0u, largest<COUNT>(x) * fabsf(cap_in) > 1.f)) {
 #pragma unroll
         for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(tanh_far(__uint_as_float(x[c]) * cap_in) * out);
         return;
@@ -126,11 +128,7 @@ template <typename T> struct CapPoly {
     }
     // `again` reads x once more, for a warp that holds a score beyond the cap: the squares, which the polynomial needs anyway, tell.
     template <int COUNT, typename Again>
-    __device__ __forceinline__ void scores(uint32_t* x, bool edge, uint32_t mk, Again again) const {
-        if (edge) {
-#pragma unroll
-            for (int c = 0; c < COUNT; ++c) x[c] = (mk >> c) & 1 ? x[c] : 0u;
-        }
+    __device__ __forceinline__ void scores(uint32_t* x, Again again) const {
         float big = 0.f;
 #pragma unroll
         for (int c = 0; c < COUNT; c += 2) {
@@ -154,8 +152,8 @@ template <typename T> struct CapPoly {
     // The same where x cannot be read again (the backward, which lets its scores be overwritten early: waiting for this made dq
     // 324 -> 384 us).
     template <int COUNT>
-    __device__ __forceinline__ void scores(uint32_t* x, bool edge, uint32_t mk) const {
-        if (__any_sync(~0u, largest<COUNT>(x, edge, mk) * fabsf(cap_in) > 1.f)) {
+    __device__ __forceinline__ void scores(uint32_t* x) const {
+        if (__any_sync(~0u, largest<COUNT>(x) * fabsf(cap_in) > 1.f)) {
 #pragma unroll
             for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(tanh_far(__uint_as_float(x[c]) * cap_in) * out);
             return;

@@ -49,7 +49,9 @@ def attend(q, k, v, i, mask, scale, cap, slope, dtype, dy=None):
     slack = SLACK + size + (p * size).sum(1, keepdim=True)
     y = p @ v
     tiny = 2.0 ** -24 * mask.shape[1] if dtype is torch.float16 else 0.0
-    out = {"y": (y, u * y.abs() + ((u + slack) * p) @ v.abs() + tiny * v.abs().amax())}
+    # a result of half precision is off by up to half of its smallest step, 2^-24, however small it is
+    least = 2.0 ** -25 if dtype is torch.float16 else 0.0
+    out = {"y": (y, u * y.abs() + ((u + slack) * p) @ v.abs() + tiny * v.abs().amax() + least)}
     if dy is None:
         return out
     inner = 1 - t * t
@@ -59,9 +61,9 @@ def attend(q, k, v, i, mask, scale, cap, slope, dtype, dy=None):
     off = p * (u * (dy * y).abs().sum(1, keepdim=True))                            # delta comes from the rounded y
     e = u * ds.abs() + (slack * parts + off) * inner + (2.5 * rel + 1e-6) * parts * bool(cap) + tiny * (u > 0)
     dq, dk, dv = ds @ k * scale, ds.T @ q * scale, p.T @ dy
-    out["dq"] = (dq, u * dq.abs() + (e @ k.abs()) * abs(scale))
-    out["dk"] = (dk, u * dk.abs() + (e.T @ q.abs()) * abs(scale))
-    out["dv"] = (dv, u * dv.abs() + ((u + slack) * p).T @ dy.abs() + tiny * dy.abs().sum(0))
+    out["dq"] = (dq, u * dq.abs() + (e @ k.abs()) * abs(scale) + least)
+    out["dk"] = (dk, u * dk.abs() + (e.T @ q.abs()) * abs(scale) + least)
+    out["dv"] = (dv, u * dv.abs() + ((u + slack) * p).T @ dy.abs() + tiny * dy.abs().sum(0) + least)
     return out
 
 
