@@ -86,6 +86,11 @@ inline int sm_count() {
     return n;
 }
 
+// ---------------------------------------------------------------- launches that overlap
+// The next kernel in the stream may begin, if it is launched so, and waits where it needs what this one does.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- device math
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;

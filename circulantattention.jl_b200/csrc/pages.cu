@@ -27,10 +27,6 @@ struct PageArgs {
     int *list, *source, *target, *keeper, *need, *offset, *moves;      // offset: for each block
 };
 
-// The copies' kernel may begin: it waits where it needs what this one lists.
-__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 struct Team {
     cg::cluster_group cluster;
     int thread, threads, rank, ranks;
@@ -71,13 +67,8 @@ struct Team {
         if (ranks == 1) return own;
         if (threadIdx.x == 0) total[SLOT] = own.y;
         cluster.sync();
-        int before = own.x, all = 0;
-        for (int r = 0; r < ranks; ++r) {
-            const int x = *cluster.map_shared_rank(&total[SLOT], r);
-            if (r < rank) before += x;
-            all += x;
-        }
-        return make_int2(before, all);
+        const int lane = threadIdx.x & 31, x = lane < ranks ? *cluster.map_shared_rank(&total[SLOT], lane) : 0;      // a lane for each block
+        return make_int2(own.x + __reduce_add_sync(~0u, lane < rank ? x : 0), __reduce_add_sync(~0u, x));
     }
 };
 

@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
     char* const smem = raw + (base_at - raw_at);
     const uint32_t q_at = base_at, kv_at = base_at + 2 * TILE;
 
+    if (FORM && !PAGED) wait_for_previous();            // spans are made by the kernel before, which lets this one begin
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int tile = (int)(gridDim.x - 1 - blockIdx.x), h = blockIdx.y;       // the last rows see the most keys: first
     int2 owned;
@@ -735,7 +736,18 @@ template <typename T, int DM, bool PAIR, bool PAGED, int FORM>
 int launch(const SeqArgs& a, const FwdMaps& maps, dim3 grid, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(umma_fwd_kernel<T, DM, PAIR, PAGED, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFwdSmem<DM>);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-    umma_fwd_kernel<T, DM, PAIR, PAGED, FORM><<<grid, kThreads<FORM>, kFwdSmem<DM>, st>>>(a, maps);
+    if (FORM && !PAGED) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = grid; cfg.blockDim = dim3(kThreads<FORM>); cfg.dynamicSmemBytes = kFwdSmem<DM>; cfg.stream = st;
+        cfg.attrs = at; cfg.numAttrs = 1;
+        const cudaError_t l = cudaLaunchKernelEx(&cfg, umma_fwd_kernel<T, DM, PAIR, PAGED, FORM>, a, maps);
+        if (l != cudaSuccess) return cuda_fail(l, "window forward kernel (tensor cores)");
+    } else {
+        umma_fwd_kernel<T, DM, PAIR, PAGED, FORM><<<grid, kThreads<FORM>, kFwdSmem<DM>, st>>>(a, maps);
+    }
     count_tensor_launch();
     CA_CHECK_LAUNCH("window forward kernel (tensor cores)");
     return CA_OK;

@@ -30,6 +30,7 @@ __device__ __forceinline__ Places sooner(Places a, Places b) { return Places{min
 
 __global__ void __launch_bounds__(kSpanThreads) span_kernel(const __grid_constant__ SpanArgs a) {
     __shared__ Places warp_last[kSpanWarps], warp_first[kSpanWarps], block_last, block_first;
+    let_next_begin();
     const cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.y;

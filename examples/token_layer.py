@@ -48,33 +48,25 @@ class Layer(torch.nn.Module):
         positions = cache.grow(x.shape[1])
         where = (cache.table, cache.starts, cache.lengths)
         q = ca.rotary_append_(q, k, v, cache.k, cache.v, *where, positions, self.turns)
-        y = self.merge(ca.paged_window_attention(q, cache.k, cache.v, *where, WINDOW, sinks=SINKS))
-        cache.free_behind_window()
-        return y
+        return self.merge(ca.paged_window_attention(q, cache.k, cache.v, *where, WINDOW, sinks=SINKS))
 
 
 class Cache:
-    """Pages for one sequence; those behind the window go back to the free list."""
+    """Pages for one sequence.  Each step gives back those that the window has left and takes some for the new tokens; where a
+    step's pages are is known on the device only."""
 
     def __init__(self, pages, width, dtype, device="cuda"):
         self.k, self.v = (ca.jl.empty((D, PAGE, KEY_HEADS, pages), dtype, device) for _ in range(2))
-        self.free, self.rows, self.total, self.device = list(range(pages)), [-1] * width, 0, device
+        self.table = torch.full((1, width), -1, dtype=torch.int32, device=device).t()
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self.total, self.device = 0, device
 
     def grow(self, n):
-        for p in range(-(-self.total // PAGE), -(-(self.total + n) // PAGE)):
-            self.rows[p] = self.free.pop()
         at, self.total = self.total, self.total + n
-        self.table = torch.tensor([self.rows], dtype=torch.int32, device=self.device).t()
         self.starts = torch.tensor([0, n], dtype=torch.int32, device=self.device)
         self.lengths = torch.tensor([self.total], dtype=torch.int32, device=self.device)
+        self.table, self.refs, _ = ca.advance_pages(self.table, self.refs, self.starts, self.lengths, PAGE, WINDOW, sinks=SINKS)
         return torch.arange(at, self.total, dtype=torch.int32, device=self.device)[None]
-
-    def free_behind_window(self):
-        """The next token sees the last WINDOW tokens and the first SINKS."""
-        for p in range(-(-SINKS // PAGE), max(0, self.total - WINDOW) // PAGE):
-            if self.rows[p] >= 0:
-                self.free.append(self.rows[p])
-                self.rows[p] = -1
 
 
 def train(layer, steps=60, N=500, B=4, device="cuda"):
