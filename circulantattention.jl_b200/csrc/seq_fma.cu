@@ -11,7 +11,8 @@
 //
 // Bound: shared memory.  A 4 x 4 piece of products takes one 16-byte read for four packed FMA, and reads keep that unit 75 to 83 %
 // busy; larger pieces do not fit 128 registers (two blocks an SM) next to the accumulators.  2 x 4096 tokens, 8 heads of 64
-// features, window 256: forward 206 us, dq 275, dk and dv 354.  12 chunks of up to 900 tokens over a cache (128 features): 3570 us.
+// features, window 256: forward 206 us, dq 275, dk and dv 354; the same with documents, groups, cap and slopes (8 % more tiles) 219, 277
+// and 315 us, the largest tiles first (294, 376 and 442 in their order: one of 17 tiles is as long as the whole call).  12 chunks of up to 900 tokens over a cache (128 features): 3570 us.
 #include "seq.cuh"
 #include "umma.cuh"
 

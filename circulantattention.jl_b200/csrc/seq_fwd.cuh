@@ -5,7 +5,7 @@
 // row reads them, turns them into weights, and writes those back over the scores as 16-bit pairs, from where the second
 // product takes them as its A operand: the weights never see shared memory.
 //
-// Roles: two groups of four warps do the softmax, one warp copies keys and values by TMA into a ring of tiles, one warp
+// Roles: two groups of four (with a cap: eight) warps do the softmax, one warp copies keys and values by TMA into a ring of tiles, one warp
 // issues the products.  The two groups are two streams that share the tensor cores: while one turns its scores into weights,
 // the products of the other run.  With PAIR the streams are two row tiles that share every key tile (half the copies); without,
 // they take the even and the odd key tiles of one row tile and are joined at the end (few rows).
@@ -18,6 +18,11 @@
 // 3300 in the steady state, since a row's chain (scores, maximum, exponentials, weights) leaves gaps that two streams do not
 // fill.  Measured: 65536 tokens, window 4096, 16 query and 2 key heads 2.03 ms (1.05 PFLOP/s of visible pairs; a
 // large matrix product has 1.62 in a burst and keeps up 1.37; 1.99 to 2.14 ms by box, at the power cap); 2 x 16384 tokens, window 1024, 16 and 4 heads 415 us.
+//
+// Other scores and masks (FORM) are compiled apart.  What they cost: 16384 tokens, window 1024, 16 and 4 heads, bfloat16: plain 180 us,
+// one document 224 (the remainders' product), slopes 247, cap 259 (297 with scores beyond the cap), both 341.  Bound: issue slots and
+// the chain of a tile; a capped score takes 13 instructions, a plain one 7.  Packed training (16384 tokens in 13 documents, capped)
+// 298 us.
 #pragma once
 #include "seq_umma.cuh"
 

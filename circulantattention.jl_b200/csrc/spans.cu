@@ -5,7 +5,8 @@
 // thread a piece of consecutive tokens: it finds the first and the last place in its piece, places are joined over warps,
 // the block and the cluster, and then it walks its piece again, forwards for the begins and backwards for the ends.
 //
-// Bound: latency.
+// Bound: latency.  300 tokens 2.6 us, 16384 in a cluster of eight blocks 7.6 us (9.8 with the warps' and blocks' places read one by
+// one).
 #include <cooperative_groups.h>
 #include <limits.h>
 #include "seq.cuh"
