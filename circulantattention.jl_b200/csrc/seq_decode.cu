@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(c[e >> 2][e & 3]);
                 if (FORM == kCap)
-                    poly.template scores<8>(x, [&] {
+                    poly.template scores<8>(x, 0.f, [&] {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(c[e >> 2][e & 3]);
                     });

@@ -49,9 +49,18 @@ template <int FORM> constexpr int kGroups = has_cap(FORM) ? 2 : 1;
 template <int FORM> constexpr int kSoftmaxWarps = 8 * kGroups<FORM>;
 template <int FORM> constexpr int kThreads = 32 * (kSoftmaxWarps<FORM> + 2);
 
+__device__ __forceinline__ float cap_reference(const SeqArgs& a) { return a.form.cap_out - 20.f; }
+
 template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
 template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
 template <int DM> constexpr size_t kFwdSmem = (size_t)(2 + kSlots<DM>) * kTileBytes<DM> + 1024;
+
+// Whole numbers in the order of the Float32 ones, and back.
+__device__ __forceinline__ int order_of(float x) {
+    const int b = __float_as_int(x);
+    return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float number_of(int o) { return __int_as_float(o ^ ((o >> 31) & 0x7fffffff)); }
 
 // A stream's tiles: those of first tokens below `first`, then from..upto, in steps of one (PAIR) or two.
 struct Stream {
@@ -122,7 +131,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
     __shared__ uint32_t tmem_slot, valid[S];
     __shared__ int stop_flag;
     __shared__ float merge_m[GROUPS == 1 ? 128 : 1], merge_l[GROUPS == 1 ? 128 : 1], merge_r[GROUPS == 1 && ROUNDED ? 128 : 1];
-    __shared__ __nv_bfloat16 part_max[GROUPS == 2 && FORM != kCap ? 2 : 1][2][128];
+    __shared__ int row_max[GROUPS == 2 && FORM != kCap ? 2 : 1][128];      // ordered as the numbers (order_of)
     volatile int* stop = &stop_flag;
 
     const uint32_t raw_at = smem_u32(raw), base_at = (raw_at + 1023) & ~1023u;
@@ -185,6 +194,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
         prefetch_map(&maps.k);
         prefetch_map(&maps.v);
     }
+    if (GROUPS == 2 && FORM != kCap && tid < 256) row_max[tid >> 7][tid & 127] = order_of(-INFINITY);
     if (warp == WARPS + 1) tmem_alloc(smem_u32(&tmem_slot), 512);
     fence_before();
     __syncthreads();
@@ -225,8 +235,8 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
         }
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;              // lane 32 * (warp % 4) in bits 16..
         const uint32_t S_at = s_col + u * 128 + lane_off, P_at = p_col + u * p_step + lane_off, O_at = o_col + u * DM + lane_off;
-        // A capped score is at most cap log2(e), which the exponents of bfloat16 stand without a reference: one pass over the scores
-        // is enough.  Scores with a slope need the maximum of the changed ones, and return to tensor memory in units of log2(e) for
+        // A capped score is at most cap log2(e): with a reference of 2^20 less than that, weights of caps up to 50 fit into bfloat16
+        // (from 2^-125 on), and one pass over the scores is enough.  Scores with a slope need the maximum of the changed ones, and return to tensor memory in units of log2(e) for
         // the exponentials (247 us; computed twice 288).
         constexpr bool BOUNDED = FORM == kCap, KEPT = has_slopes(FORM);
         const float sl2 = has_cap(FORM) || has_slopes(FORM) ? 1.f : a.mag_log2, cap_in = fabsf(a.form.cap_in);
@@ -409,7 +419,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                     const uint32_t mk = edge ? seen(at) : ~0u;
                     if (edge) clear_unseen<32>(x, mk);
                     if constexpr (BOUNDED)
-                        poly.template scores<32>(x, [&] {
+                        poly.template scores<32>(x, -cap_reference(a), [&] {
                             tmem_ld32(S_at + at, x);
                             tmem_wait_ld();
                             settled32(x);
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                 };
                 float f = 1.f;
                 if (BOUNDED) {
-                    m = 0.f;
+                    m = cap_reference(a);
                 } else {
                     float mx = -INFINITY;
                     if (own) {
@@ -441,13 +451,13 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
                         }
                     }
                     tmem_wait_st();
-                    // Both halves' maxima, rounded (which the reference stands) so that they fit: the tiles take all but 2 KB
-                    part_max[u][g][r] = __float2bfloat16_rn(mx);
+                    // The largest of all tiles so far, of both halves: a number for each row is all that fits beside the tiles
+                    atomicMax(&row_max[u][r], order_of(mx));
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&max_full[u]));
                     if (!warp_wait(smem_u32(&max_full[u]), done & 1, stop)) { ok = false; break; }
                     const float before = m;
-                    f = given(fmaxf(__bfloat162float(part_max[u][0][r]), __bfloat162float(part_max[u][1][r])));
+                    f = given(number_of(*(volatile int*)&row_max[u][r]));
                     if (done && __any_sync(~0u, m != before)) rescale(DM / 2 * g, DM / 2 * (g + 1), f);
                     tmem_wait_st();
                     fence_before();

@@ -126,9 +126,9 @@ template <typename T> struct CapPoly {
 #pragma unroll
         for (int i = 0; i <= DEGREE; ++i) k[i] = a.form.poly[i] * f;
     }
-    // `again` reads x once more, for a warp that holds a score beyond the cap: the squares, which the polynomial needs anyway, tell.
+    // Plus `shift`.  `again` reads x once more, for a warp that holds a score beyond the cap: the squares, which the polynomial needs anyway, tell.
     template <int COUNT, typename Again>
-    __device__ __forceinline__ void scores(uint32_t* x, Again again) const {
+    __device__ __forceinline__ void scores(uint32_t* x, float shift, Again again) const {
         float big = 0.f;
 #pragma unroll
         for (int c = 0; c < COUNT; c += 2) {
@@ -139,14 +139,14 @@ template <typename T> struct CapPoly {
             f32x2 p = pack2(k[DEGREE], k[DEGREE]);
 #pragma unroll
             for (int i = DEGREE - 1; i >= 0; --i) p = fma2(p, u, pack2(k[i], k[i]));
-            unpack2(mul2(p, s), z0, z1);
+            unpack2(fma2(p, s, pack2(shift, shift)), z0, z1);
             x[c] = __float_as_uint(z0);
             x[c + 1] = __float_as_uint(z1);
         }
         if (__any_sync(~0u, big * cap_in * cap_in > 1.f)) {
             again();
 #pragma unroll
-            for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(tanh_far(__uint_as_float(x[c]) * cap_in) * out);
+            for (int c = 0; c < COUNT; ++c) x[c] = __float_as_uint(fmaf(tanh_far(__uint_as_float(x[c]) * cap_in), out, shift));
         }
     }
     // The same where x cannot be read again (the backward, which lets its scores be overwritten early: waiting for this made dq

@@ -36,6 +36,37 @@ def test_caps_and_scales(ca, dtype, cap, scale, size):
         ref.check(got[name], value, bound, name)
 
 
+@pytest.mark.parametrize("dtype,cap,large", [(torch.bfloat16, 50.0, 1e25), (torch.bfloat16, 30.0, 1e25), (torch.bfloat16, 60.0, 1e25), (torch.float16, 50.0, 500.0),
+                                             (torch.float32, 50.0, 1e25)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_large_values_and_scores_at_the_cap(ca, dtype, cap, large, sign):
+    """All of a row's scores near +cap, or near -cap, and values near the type's limits: weights without a reference hold both."""
+    case = (64, 2, 1, 260, 1, None, 0, 0, None, cap, False, 0, 0)
+    q, k, v, dy, *form = problem(case, dtype)
+    q, k = (t.abs() * f for t, f in ((q, 20.0), (k, 5.0 * sign)))           # scores of about 8 * 64 * 80 / 8
+    v = (v.float() * large).to(dtype)
+    got = gradients(ca, case, (q, k, v), dy, *form)
+    for name, (value, bound) in ref.window(q, k, v, None, 0, 0, None, cap, None, None, None, dy).items():
+        if name in ("y", "dv"):                                             # the cap's derivative is 0, so dq and dk are what is left of it
+            ref.check(got[name], value, bound, name)
+        assert torch.isfinite(got[name]).all(), name
+
+
+@types
+def test_only_far_keys(ca, dtype):
+    """The near pages are gone: every key is thousands of tokens away, the bias alone is some 17000 in the exponent."""
+    D, Hq, Hkv, page, new, n = 64, 2, 1, 16, 150, 6000
+    kp, vp = (make(s, (D, page, Hkv, 10), dtype) for s in (2, 3))
+    q = make(1, (D, Hq, new), dtype, 2.0)
+    table = [[4, 5, 6] + [-1] * 373]
+    slopes = torch.tensor([2.0, 0.5])
+    for cap in (10.0, None):
+        got = ca.paged_window_attention(q.cuda(), kp.cuda(), vp.cuda(), ints(table).t(), ints([0, new]), ints([n]), cap=cap, slopes=slopes.cuda())
+        ref.check(got, *ref.paged(q, kp, vp, table, [0, new], [n], None, 0, cap, slopes, None))
+        one = ca.paged_window_attention(q[:, :, -1:].cuda(), kp.cuda(), vp.cuda(), ints(table).t(), ints([0, 1]), ints([n]), cap=cap, slopes=slopes.cuda())
+        ref.check(one, *ref.paged(q[:, :, -1:], kp, vp, table, [0, 1], [n], None, 0, cap, slopes, None))
+
+
 @types
 @pytest.mark.parametrize("D,Hq,Hkv,N,B,longest,group", [(64, 8, 1, 5001, 2, 900, 20), (128, 1, 1, 17000, 1, 17000, 0)])
 def test_many_tiles(ca, D, Hq, Hkv, N, B, longest, group, dtype):
