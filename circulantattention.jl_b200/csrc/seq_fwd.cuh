@@ -20,9 +20,9 @@
 // large matrix product has 1.62 in a burst and keeps up 1.37; 1.99 to 2.14 ms by box, at the power cap); 2 x 16384 tokens, window 1024, 16 and 4 heads 415 us.
 //
 // Other scores and masks (FORM) are compiled apart.  What they cost: 16384 tokens, window 1024, 16 and 4 heads, bfloat16: plain 180 us,
-// one document 224 (the remainders' product), slopes 247, cap 259 (297 with scores beyond the cap), both 341.  Bound: issue slots and
+// one document 224 (the remainders' product), slopes 246, cap 259 (282 with scores beyond the cap), both 336.  Bound: issue slots and
 // the chain of a tile; a capped score takes 13 instructions, a plain one 7.  Packed training (16384 tokens in 13 documents, capped)
-// 298 us.
+// 290 us.
 #pragma once
 #include "seq_umma.cuh"
 
@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;              // lane 32 * (warp % 4) in bits 16..
         const uint32_t S_at = s_col + u * 128 + lane_off, P_at = p_col + u * p_step + lane_off, O_at = o_col + u * DM + lane_off;
         // A capped score is at most cap log2(e): with a reference of 2^20 less than that, weights of caps up to 50 fit into bfloat16
-        // (from 2^-125 on), and one pass over the scores is enough.  Scores with a slope need the maximum of the changed ones, and return to tensor memory in units of log2(e) for
-        // the exponentials (247 us; computed twice 288).
+        // (from 2^-125 on), and one pass over the scores is enough.  Scores with a slope need the maximum of the changed ones, and
+        // return to tensor memory in units of log2(e) for the exponentials (247 us; computed twice 288).
         constexpr bool BOUNDED = FORM == kCap, KEPT = has_slopes(FORM);
         const float sl2 = has_cap(FORM) || has_slopes(FORM) ? 1.f : a.mag_log2, cap_in = fabsf(a.form.cap_in);
         const float slope = has_slopes(FORM) ? slope_of(a, h * a.G + R - token_of(a, R) * a.G) : 0.f;
