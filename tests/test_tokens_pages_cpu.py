@@ -30,7 +30,7 @@ def test_bad_tables(ca, kw, code, msg):
     lib, err = ca.lib, lambda: ca.lib.ca_last_error().decode()
     t = _table(**kw)
     assert lib.ca_advance_pages(t, 256, -1, 0, 1024, 2048, 4096, 8192, None) == code and msg in err()
-    assert lib.ca_fork_pages(t, 256, _pool(), 1, 1024, 2048, 3072, 4096, 8192, None) == code and msg in err()
+    assert lib.ca_fork_pages(t, 256, _pool(), 1, 1024, 2048, 3584, 4096, 8192, None) == code and msg in err()
     assert lib.ca_compact_pages(t, _pool(), 1, 1024, 2048, 4096, 8192, None) == code and msg in err()
     assert lib.ca_pages_workspace(t) == 0
 
@@ -51,7 +51,7 @@ def test_workspace(ca):
 ])
 def test_bad_pools(ca, kw, code, msg):
     lib, err = ca.lib, lambda: ca.lib.ca_last_error().decode()
-    assert lib.ca_fork_pages(_table(), 256, _pool(**kw), 1, 1024, 2048, 3072, 4096, 8192, None) == code and msg in err()
+    assert lib.ca_fork_pages(_table(), 256, _pool(**kw), 1, 1024, 2048, 3584, 4096, 8192, None) == code and msg in err()
     assert lib.ca_compact_pages(_table(), _pool(**kw), 1, 1024, 2048, 4096, 8192, None) == code and msg in err()
 
 
@@ -67,8 +67,8 @@ def test_bad_results(ca):
     assert lib.ca_advance_pages(t, 256, -1, 0, 256, 2048, 4096, 8192, None) == -1 and "old one's place" in err()
     assert lib.ca_advance_pages(t, 256, -1, 0, 1024, 512, 4096, 8192, None) == -1 and "old ones' place" in err()
     assert lib.ca_advance_pages(t, 256, -1, 0, 1024, 2048, 4096, 8200, None) == -1 and "16-byte aligned" in err()
-    assert lib.ca_fork_pages(t, None, pool, 1, 1024, 2048, 3072, 4096, 8192, None) == -3 and "parents" in err()
-    assert lib.ca_fork_pages(t, 256, None, 1, 1024, 2048, 3072, 4096, 8192, None) == -3 and "without pools" in err()
+    assert lib.ca_fork_pages(t, None, pool, 1, 1024, 2048, 3584, 4096, 8192, None) == -3 and "parents" in err()
+    assert lib.ca_fork_pages(t, 256, None, 1, 1024, 2048, 3584, 4096, 8192, None) == -3 and "without pools" in err()
     assert lib.ca_fork_pages(t, 256, pool, 1, 1024, 2048, 768, 4096, 8192, None) == -1 and "lengths" in err()
 
 
