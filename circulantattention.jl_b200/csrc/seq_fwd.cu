@@ -58,14 +58,16 @@ static int encode_row_maps(FwdMaps* maps, bool bf16, const SeqArgs& a) {
     return rc;
 }
 
-// The exponents of bfloat16 weights hold capped scores without a look for their maximum up to a cap of 50 (2^73 both ways); half's do
-// not, and those take the kernel that looks.
+// bfloat16's exponents hold the weights of capped scores without a look for their maximum, and Float32's what they multiply, up to a
+// cap of 33 (kOnePassCap).  Half's do not, and larger caps leave no room for the values: those take the kernel that looks (16384 tokens,
+// window 1024, 16 and 4 heads of 128 features, scores of standard deviation 8: 266 us with one pass, 345 with two; cap 30, a few scores
+// beyond the cap, 292 and 354).
 static int run(const SeqArgs& a, const FwdMaps& maps, int dtype, bool pair, dim3 grid, cudaStream_t st) {
     switch (a.kind) {
         case kMasks: return umma_fwd<kMasks>(a, maps, dtype, pair, grid, st);
         case kSlopes: return umma_fwd<kSlopes>(a, maps, dtype, pair, grid, st);
         case kCap:
-            if (dtype == CA_BF16 && a.form.cap_out <= 73.f) return umma_fwd<kCap>(a, maps, dtype, pair, grid, st);
+            if (dtype == CA_BF16 && a.form.cap_out <= kOnePassCap) return umma_fwd<kCap>(a, maps, dtype, pair, grid, st);
             [[fallthrough]];
         case kCapSlopes: return umma_fwd<kCapSlopes>(a, maps, dtype, pair, grid, st);
         default: return umma_fwd<kNoForm>(a, maps, dtype, pair, grid, st);

@@ -11,7 +11,7 @@
 // they take the even and the odd key tiles of one row tile and are joined at the end (few rows).
 //
 // The accumulator is rescaled only where a row's maximum grew by more than 2^8 since its reference: the weights stay below
-// 2^8, and the products and sums are held in Float32.  Weights are rounded to the tensors' type before their product, once more
+// 2^8 (of small caps in bfloat16, which have a fixed reference, below 2^32), and the products and sums are held in Float32.  Weights are rounded to the tensors' type before their product, once more
 // than the result itself: errors are 1.15 to 1.6 of those of a plain implementation that keeps them in Float32.
 //
 // Bound: the exponentials and the products, 2048 cycles each for a pair of 128 x 128 tiles at 128 features; a pair takes about
@@ -49,7 +49,13 @@ template <int FORM> constexpr int kGroups = has_cap(FORM) ? 2 : 1;
 template <int FORM> constexpr int kSoftmaxWarps = 8 * kGroups<FORM>;
 template <int FORM> constexpr int kThreads = 32 * (kSoftmaxWarps<FORM> + 2);
 
-__device__ __forceinline__ float cap_reference(const SeqArgs& a) { return a.form.cap_out - 20.f; }
+// Of capped scores that are read once: the same for all rows, 2^32 below the largest weight that the cap allows.  With cap_out up to
+// kOnePassCap the smallest is 2^-64, so that neither the weights nor what they multiply leave Float32's exponents: a row's weighted
+// sum is exact (but for the roundings) from 2^-62 on, and up to 2^95 of it, whatever the scores are.  Results are read with
+// subnormal numbers taken for zeros, which is what a lower reference or a larger cap would run into first (all scores of a row near
+// -cap, a cap of 50 and 2^20 in place of 2^32: values below 0.3 came out as zeros).
+constexpr float kOnePassCap = 48.f;                 // in units of log2(e): a cap of 33
+__device__ __forceinline__ float cap_reference(const SeqArgs& a) { return a.form.cap_out - 32.f; }
 
 template <int DM> constexpr uint32_t kTileBytes = 128 * DM * 2;
 template <int DM> constexpr int kSlots = DM == 128 ? 5 : 8;
@@ -240,8 +246,8 @@ __global__ void __launch_bounds__(kThreads<FORM>, 1) umma_fwd_kernel(const __gri
         }
         const uint32_t lane_off = (uint32_t)(warp & 3) << 21;              // lane 32 * (warp % 4) in bits 16..
         const uint32_t S_at = s_col + u * 128 + lane_off, P_at = p_col + u * p_step + lane_off, O_at = o_col + u * DM + lane_off;
-        // A capped score is at most cap log2(e): with a reference of 2^20 less than that, weights of caps up to 50 fit into bfloat16
-        // (from 2^-125 on), and one pass over the scores is enough.  Scores with a slope need the maximum of the changed ones, and
+        // A capped score is at most cap log2(e): with a reference that all rows share (cap_reference) one pass over the scores is
+        // enough.  Scores with a slope need the maximum of the changed ones, and
         // return to tensor memory in units of log2(e) for the exponentials (247 us; computed twice 288).
         constexpr bool BOUNDED = FORM == kCap, KEPT = has_slopes(FORM);
         const float sl2 = has_cap(FORM) || has_slopes(FORM) ? 1.f : a.mag_log2, cap_in = fabsf(a.form.cap_in);
