@@ -1,6 +1,8 @@
 // C ABI of the attention on token sequences: argument checks and dispatch.
 #include "seq_umma.cuh"
 
+#include <float.h>
+
 namespace ca {
 
 int check_seq_dtype(int dtype) {
@@ -49,7 +51,12 @@ static int fill_form(const ca_seq_desc* d, const ca_seq_form* form, bool paged, 
     if (!form) return CA_OK;
     if (!(form->cap >= 0.f) || isinf(form->cap)) { set_error("cap must be positive, or 0 for scores as they are"); return CA_ERR_BAD_DESC; }
     if (form->cap > 0.f && !isfinite(d->scale / form->cap)) { set_error("cap=%g is too small for scale=%g", form->cap, d->scale); return CA_ERR_BAD_DESC; }
-    if (form->cap > 0.f && !isfinite(form->cap * kLog2e)) { set_error("cap=%g is too large", form->cap); return CA_ERR_BAD_DESC; }
+    // Kernels take subnormal numbers for zeros: of raw / cap that is a score of cap 2^-126 (2^-26 at the largest cap), of scale / cap all of them.
+    if (form->cap > 0x1p100f) { set_error("cap=%g is too large: up to 2^100 is supported", form->cap); return CA_ERR_BAD_DESC; }
+    if (form->cap > 0.f && fabsf(d->scale) >= FLT_MIN && fabsf(d->scale / form->cap) < FLT_MIN) {
+        set_error("cap=%g is too large for scale=%g", form->cap, d->scale);
+        return CA_ERR_BAD_DESC;
+    }
     if (!aligned(form->slopes, 4) || !aligned(form->prefix, 4) || !aligned(form->spans, 16)) { set_error("slopes, prefix or spans (16 bytes) are not aligned"); return CA_ERR_BAD_DESC; }
     if (form->spans && paged) { set_error("spans are for dense tensors"); return CA_ERR_BAD_DESC; }
     if (form->prefix && !paged) { set_error("prefix is for calls over a cache: a dense call takes spans"); return CA_ERR_BAD_DESC; }

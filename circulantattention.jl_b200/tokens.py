@@ -96,8 +96,8 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, scale=None, 
     left=None: no left end.  lengths: Int32 `(B,)`, the tokens that exist in each sequence (what lies behind them has no
     effect, whatever it holds; y and the gradients are zero there).
 
-    The score is scale * q_i . k_j, scale 1/sqrt(D) by default.  cap: it becomes cap * tanh(score / cap).  slopes: Float32
-    `(heads,)`, slopes[head] * |i - j| is taken from it after the cap; no gradient.  spans: what `token_spans` says of the
+    The score is scale * q_i . k_j, scale 1/sqrt(D) by default.  cap: it becomes cap * tanh(score / cap), cap up to
+    2^100.  slopes: Float32 `(heads,)`, slopes[head] * |i - j| is taken from it after the cap; no gradient.  spans: what `token_spans` says of the
     tokens' documents and groups takes the place of `right` and `sinks`, which are 0 then: token i sees those of its document
     from i - left to i or, if that is further, to the end of its group.
 

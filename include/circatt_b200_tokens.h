@@ -113,7 +113,7 @@ int ca_paged_window(const ca_seq_desc* d, const ca_seq_view* q, const ca_page_vi
  * prefix (calls over a cache): prefix[s] tokens of sequence s are visible to all of its tokens, whether they come later or
  * not, as far as the window's left end leaves them. */
 typedef struct ca_seq_form {
-    float cap;                /* 0: scores as they are */
+    float cap;                /* 0: scores as they are; up to 2^100 */
     const float* slopes;      /* heads_q, nullable */
     const int32_t* spans;     /* (4, N, B), 16-byte aligned, nullable */
     const int32_t* prefix;    /* (sequences), nullable */
