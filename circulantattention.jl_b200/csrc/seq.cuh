@@ -166,7 +166,7 @@ __device__ __forceinline__ Reach reach(const SeqArgs& a, const Seq& s, int pos) 
             r.lo = max(r.lo, w.x);
             r.hi = w.z;
         } else if (a.form.prefix) {
-            r.hi = max(r.hi, a.form.prefix[s.b] - 1);
+            r.hi = max(r.hi, max(0, a.form.prefix[s.b]) - 1);          // the lowest Int32 less 1 would be the highest
         }
     }
     return r;

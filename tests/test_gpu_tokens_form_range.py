@@ -103,3 +103,16 @@ def test_smallest_values(ca, cap, sign):
     v = ((1 + v.float().abs()) * v.float().sign() * 2.0 ** -61).to(torch.bfloat16)
     y = ca.window_attention(q.cuda(), k.cuda(), v.cuda(), 0, cap=cap)
     assert torch.equal(y.cpu(), v.expand_as(y))
+
+
+@types
+@pytest.mark.parametrize("new", [1, 3, 100])
+def test_negative_prefixes(ca, dtype, new):
+    """No prefix, whatever negative number says so."""
+    D, page, n = 64, 16, 150
+    kp, vp = (make(s, (D, page, 2, 10), dtype).cuda() for s in (2, 3))
+    q = make(1, (D, 4, new), dtype, 2.0).cuda()
+    where = (ints([list(range(10))]).t(), ints([0, new]), ints([n]))
+    want = ca.paged_window_attention(q, kp, vp, *where, prefix=ints([0]))
+    for prefix in (-1, -5, -2 ** 31 + 1, -2 ** 31):
+        assert torch.equal(ca.paged_window_attention(q, kp, vp, *where, prefix=ints([prefix])), want), prefix
