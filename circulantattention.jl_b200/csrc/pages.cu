@@ -359,6 +359,8 @@ int check_table(const ca_table* t, bool lengths) {
     if (!t) { set_error("table is NULL"); return CA_ERR_NULL; }
     if (t->width < 0 || t->sequences < 0 || t->pages < 0) { set_error("width=%d sequences=%d pages=%d must not be negative", t->width, t->sequences, t->pages); return CA_ERR_BAD_DESC; }
     if (t->page < 16 || t->page % 16) { set_error("page=%d: multiples of 16 tokens are supported", t->page); return CA_ERR_BAD_DESC; }
+    // 32-bit loops over them step by all threads of a cluster, and shares are rounded up
+    if (t->pages > 1 << 30 || t->sequences > 1 << 30) { set_error("sequences=%d pages=%d exceed 2^30", t->sequences, t->pages); return CA_ERR_TOO_LARGE; }
     if ((int64_t)t->width * t->page > INT32_MAX) { set_error("width=%d places of %d tokens exceed 2^31 tokens", t->width, t->page); return CA_ERR_TOO_LARGE; }
     if ((t->sequences && t->width && !t->table) || (t->pages && !t->refs) || (lengths && t->sequences && !t->lengths)) { set_error("table, refs and lengths must not be NULL"); return CA_ERR_NULL; }
     return CA_OK;
