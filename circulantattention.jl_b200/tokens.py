@@ -96,10 +96,10 @@ def window_attention(q, k, v, left, right=0, sinks=0, lengths=None, scale=None, 
     left=None: no left end.  lengths: Int32 `(B,)`, the tokens that exist in each sequence (what lies behind them has no
     effect, whatever it holds; y and the gradients are zero there).
 
-    The score is scale * q_i . k_j, scale 1/sqrt(D) by default.  cap: it becomes cap * tanh(score / cap), cap up to
-    2^100.  slopes: Float32 `(heads,)`, slopes[head] * |i - j| is taken from it after the cap; no gradient.  spans: what `token_spans` says of the
-    tokens' documents and groups takes the place of `right` and `sinks`, which are 0 then: token i sees those of its document
-    from i - left to i or, if that is further, to the end of its group.
+    The score is scale * q_i . k_j, scale 1/sqrt(D) by default.  cap: it becomes cap * tanh(score / cap), cap up to 2^100.
+    slopes: Float32 `(heads,)`, slopes[head] * |i - j| is taken from it after the cap; no gradient.  spans: what `token_spans`
+    says of the tokens' documents and groups takes the place of `right` and `sinks`, which are 0 then: token i sees those of its
+    document from i - left to i or, if that is further, to the end of its group.
 
     Infinities and NaN in keys or values that no token sees have no effect.  Where some token sees them, neighbours that do
     not may get NaN too: their weight is zero, and zero times infinity is not a number."""
@@ -127,7 +127,12 @@ def advance_pages(table, refs, starts, lengths, page, left=None, sinks=0):
     table entries hold each page; a page is free where that is not above 0.  Pages that neither the new nor later tokens see
     through a window of `left` and `sinks`, and those behind a sequence's length, go back: all of them where the length is 0 (a
     sequence that has ended).  Places of new tokens without a page get the lowest free ones, sequence by sequence, pages of
-    this call among them.  missing: Int32 `(1,)`, places that got none; tokens there are not stored.
+    this call among them.  missing: Int32 `(1,)`, places that got none; tokens there are not stored, and neither are those beyond
+    the table's width, which have no place to count: the table has to be wide enough for the lengths.
+
+    A place that has a page keeps it.  After `fork_pages` full pages belong to several sequences: one that is then made shorter, to
+    end within such a page, would write its next tokens into the others' page.  Fork it once more before they come, with its
+    parent going on as it is: the copy's last page is its own.
 
     Like the other operators on pages it gives a new state and leaves the old one as it is, and nothing waits for the host; a
     captured step copies the new table and refs over the old ones at its end."""

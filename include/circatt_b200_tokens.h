@@ -137,7 +137,8 @@ int ca_paged_window_form(const ca_seq_desc* d, const ca_seq_form* form, const ca
 /* ---------------------------------------------------------------- the pages of a cache
  * A state: the table, for each page the number of table entries that hold it (refs; a page is free if that is not above 0), and
  * the tokens of each sequence.  The operators read one and write the next into other memory; all of it is on the device and
- * nothing waits for the host.  Pages are taken from the lowest number on, for sequences and places in their order. */
+ * nothing waits for the host.  Pages are taken from the lowest number on, for sequences and places in their order.  At most 2^30
+ * sequences and pages. */
 typedef struct ca_table {
     const int32_t* table;     /* (width, sequences) */
     const int32_t* refs;      /* (pages) */
@@ -157,7 +158,11 @@ size_t ca_pages_workspace(const ca_table* t);
 /* Before a call's new tokens are stored: lengths[s] counts the starts[s+1] - starts[s] new tokens of sequence s with it.  Pages
  * that neither they nor later tokens see (a window of `left`, negative: no left end; the first `sinks` tokens), and those
  * behind the length, are given back, all of them where the length is 0; places of new tokens without a page get one.  *missing:
- * places that got none. */
+ * places of the table that got none.  Tokens beyond the table's width have no place: they are not stored and not counted there.
+ *
+ * A place that has a page keeps it, however many entries hold that page.  A sequence that has become shorter so that it ends within a
+ * page of others (ca_fork_pages shares full ones) would therefore write its next tokens into theirs: fork it before they come, with
+ * its parent going on, and the copy has a last page of its own. */
 int ca_advance_pages(const ca_table* t, const int32_t* starts, int32_t left, int32_t sinks, int32_t* table, int32_t* refs, int32_t* missing,
                      void* workspace, void* stream);
 
