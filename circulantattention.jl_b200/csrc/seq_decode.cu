@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const __grid_consta
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[n][e] = fast_exp2(c[n][e] - (e < 2 ? ma : mb));
             const uint32_t p[4] = {pack16<T>(c[0][0], c[0][1]), pack16<T>(c[0][2], c[0][3]), pack16<T>(c[1][0], c[1][1]), pack16<T>(c[1][2], c[1][3])};
-            if constexpr (FORM) {                               // the weights as they were rounded (see seq_fwd.cu)
+            if constexpr (FORM) {                               // the weights as they were rounded (see seq_fwd.cuh)
                 l[0] += (low16<T>(p[0]) + high16<T>(p[0])) + (low16<T>(p[2]) + high16<T>(p[2]));
                 l[1] += (low16<T>(p[1]) + high16<T>(p[1])) + (low16<T>(p[3]) + high16<T>(p[3]));
             } else {
